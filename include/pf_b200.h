@@ -258,6 +258,130 @@ PF_API pf_status pf_check_ordered_scan(const float* terms, int32_t rows, int32_t
                                        const float* p, uint32_t* mismatches);
 
 /* ------------------------------------------------------------------ */
+/* Paged cache (no counterpart in the reference, whose KVCache holds one */
+/* fixed three-tier buffer per layer and head)                           */
+/* ------------------------------------------------------------------ */
+/* Keys and values of many sequences in pages of page_size positions that
+ * sequences may share.  All pointers are device pointers of the current
+ * device and belong to the caller; the library keeps nothing between calls.
+ *
+ *   k, v             [n_pages][n_layers][n_kv_heads][page_size][head_dim] of `dtype`
+ *   k_scale, v_scale [n_pages][n_layers][n_kv_heads][page_size]; PF_I8 only
+ *                    (a stored row is code * scale, as KVCache::quantize_row
+ *                    makes it, src/kv_cache.cpp:19-28), else NULL
+ *   table            [max_seqs][max_pages]: the pages of each sequence in order
+ *   lens             [max_seqs]: its tokens, those of the current step included
+ *   refs             [n_pages]: sequences that hold the page; 0 = free
+ *   work             pf_paged_work_bytes() bytes, scratch of the page operations
+ *
+ * To begin with, refs and lens are zero (the table's contents do not matter).
+ * Position p of sequence b is slot p % page_size of page
+ * table[b][p / page_size].  Only full pages are ever shared: pf_paged_fork
+ * copies a last, partly filled one.  A page id outside [0, n_pages), a length
+ * outside [0, max_pages * page_size] or an offset out of order is not
+ * followed: it latches bit 1 of pf_read_device_error and its row, entry or
+ * page is left out.  k, v and work are 16-byte aligned.  Calls on one cache
+ * are ordered by the caller (one stream, or events between streams). */
+enum { PF_F32 = 0, PF_BF16 = 1, PF_F16 = 2, PF_I8 = 3 };
+
+typedef struct pf_paged_cache {
+    int32_t  dtype;       /* PF_I8, PF_BF16 or PF_F16  */
+    int32_t  n_layers;
+    int32_t  n_kv_heads;
+    int32_t  head_dim;    /* 64 or 128                 */
+    int32_t  page_size;   /* 16, 32, 64 or 128         */
+    int32_t  n_pages;
+    int32_t  max_seqs;    /* rows of table and lens    */
+    int32_t  max_pages;   /* pages a sequence may hold */
+    void*    k;
+    void*    v;
+    float*   k_scale;
+    float*   v_scale;
+    int32_t* table;
+    int32_t* lens;
+    int32_t* refs;
+    void*    work;
+} pf_paged_cache;
+
+/* Bytes of `work` for a cache of these sizes (0: the sizes are refused). */
+PF_API size_t pf_paged_work_bytes(const pf_paged_cache* c);
+
+/* Makes room for counts[i] more tokens of sequence seqs[i] (device arrays of
+ * n; the sequences distinct): takes the lowest free pages, in the list's
+ * order, and adds counts[i] to its length.  Where the pages run out, or the
+ * sequence would pass max_pages, the sequence keeps its length and pages and
+ * bit 8 is latched.  A sequence named again, or out of range, and a count
+ * below zero latch bit 1 and are left out. */
+PF_API pf_status pf_paged_reserve(const pf_paged_cache* c, const int32_t* seqs, const int32_t* counts, int32_t n,
+                                  void* stream);
+/* Gives up n sequences (device array): their length becomes 0, their table
+ * rows' pages -1, and pages that no sequence holds any more are free.  An
+ * empty sequence, or one named again, is left as it is. */
+PF_API pf_status pf_paged_free(const pf_paged_cache* c, const int32_t* seqs, int32_t n, void* stream);
+/* Gives child i the history of parent i (device arrays of n): the parent's
+ * full pages are shared, and the positions of a last, partly filled page are
+ * copied, every layer, into the lowest free page.  A parent may be named many
+ * times.  Children are empty, distinct, and no parents of the same call: one
+ * that is not latches bit 1 and is left as it is; one for which no page is
+ * free latches bit 8 and stays empty. */
+PF_API pf_status pf_paged_fork(const pf_paged_cache* c, const int32_t* parents, const int32_t* children, int32_t n,
+                               void* stream);
+/* Copies n pages, every layer, with their scales: src[i] -> dst[i] (device
+ * arrays).  No page is a destination twice, or a destination and a source. */
+PF_API pf_status pf_paged_copy(const pf_paged_cache* c, const int32_t* src, const int32_t* dst, int32_t n,
+                               void* stream);
+/* Moves the pages in use to the front of the cache: with n_live of them, the
+ * i-th one (by index) at or behind n_live goes to the i-th free page before
+ * it.  Tables and refs follow; the moved pages' old places are free. */
+PF_API pf_status pf_paged_compact(const pf_paged_cache* c, void* stream);
+
+/* Stores new keys and values of one layer.  Rows offsets[b] to offsets[b+1]
+ * (device array of n_seqs + 1, not decreasing) of k and v, each row
+ * [n_kv_heads][head_dim] of `dtype` at k_stride / v_stride elements, are the
+ * last positions of sequence b, whose length counts them already
+ * (pf_paged_reserve).  n_tokens rows are there at all; those outside
+ * [offsets[0], offsets[n_seqs]) are not read.  dtype: any of PF_F32, PF_BF16,
+ * PF_F16 for a PF_I8 cache; PF_F32 or the cache's own for the others.  A row
+ * with an infinity or NaN is stored in a PF_I8 cache with a NaN scale.  k, v
+ * and the strides' bytes are multiples of 16. */
+PF_API pf_status pf_paged_store(const pf_paged_cache* c, int32_t layer, const void* k, int64_t k_stride,
+                                const void* v, int64_t v_stride, int32_t dtype, const int32_t* offsets,
+                                int32_t n_seqs, int32_t n_tokens, void* stream);
+
+/* Attention of the `rows` newest tokens (1 to 8) of sequences 0 .. n_seqs - 1
+ * over one layer of the cache.  q and out: [n_seqs * rows][n_heads][head_dim]
+ * of `dtype`, q_stride / out_stride elements from token to token; head h reads
+ * kv head h / (n_heads / n_kv_heads).  Row r of a sequence of length n sees
+ * its first n - rows + 1 + r positions; a row that sees none gives zeros.
+ *   out = sum_j softmax_j(scale * (q . k_j)) v_j
+ * dtype: PF_F32, PF_BF16 or PF_F16 for a PF_I8 cache (PF_F32 keeps 32-bit
+ * accuracy), the cache's own for the others.  scale > 0.  `work`:
+ * pf_paged_attention_work_bytes() bytes, 16-byte aligned, zero before the
+ * first call that uses it (every call leaves its counters zero); calls that
+ * may run at the same time need one each.  q, out and the strides' bytes are
+ * multiples of 16. */
+PF_API size_t pf_paged_attention_work_bytes(const pf_paged_cache* c, int32_t n_seqs, int32_t rows, int32_t n_heads);
+PF_API pf_status pf_paged_attention(const pf_paged_cache* c, int32_t layer, const void* q, int64_t q_stride,
+                                    void* out, int64_t out_stride, int32_t dtype, int32_t n_seqs, int32_t rows,
+                                    int32_t n_heads, float scale, void* work, size_t work_bytes, void* stream);
+
+/* Causal attention over whole prompts, packed: rows offsets[b] to
+ * offsets[b+1] (device array of n_seqs + 1, not decreasing) of q
+ * [n_tokens][n_heads][head_dim], k and v [n_tokens][n_kv_heads][head_dim] are
+ * sequence b, and out[i] = sum_j softmax_j(scale * (q_i . k_j)) v_j over the
+ * sequence's rows j <= i; head h reads kv head h / (n_heads / n_kv_heads).
+ * Strides are elements from token to token (columns of a fused projection's
+ * rows will do).  Rows outside [offsets[0], offsets[n_seqs]) of out are left
+ * as they were; a sequence whose offsets are out of order or outside
+ * [0, n_tokens] latches bit 1 and is left out.  dtype PF_BF16 or PF_F16,
+ * head_dim 64 or 128, scale > 0; pointers and the strides' bytes are
+ * multiples of 16.  out overlaps none of the inputs. */
+PF_API pf_status pf_prompt_attention(const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
+                                     int64_t v_stride, void* out, int64_t out_stride, int32_t dtype,
+                                     const int32_t* offsets, int32_t n_seqs, int32_t n_tokens, int32_t n_heads,
+                                     int32_t n_kv_heads, int32_t head_dim, float scale, void* stream);
+
+/* ------------------------------------------------------------------ */
 /* Engine: batched MTP speculative decoding                             */
 /* (Engine::generate / forward_with_hidden / MTPHeads::forward,         */
 /*  src/engine.cpp:276-589, src/mtp.cpp:47-129)                         */

@@ -13,6 +13,7 @@ import numpy as np
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libpf_b200.so")
 
+PF_F32, PF_BF16, PF_F16, PF_I8 = range(4)
 PF_OK, PF_ERR_INVALID, PF_ERR_CUDA, PF_ERR_OOM, PF_ERR_NO_DEVICE, PF_ERR_DEVICE, PF_ERR_STATE = range(7)
 STATUS_NAMES = {0: "PF_OK", 1: "PF_ERR_INVALID", 2: "PF_ERR_CUDA", 3: "PF_ERR_OOM", 4: "PF_ERR_NO_DEVICE",
                 5: "PF_ERR_DEVICE", 6: "PF_ERR_STATE"}
@@ -38,6 +39,17 @@ class ModelConfigC(C.Structure):
 class SamplingConfigC(C.Structure):
     _fields_ = [("temperature", C.c_float), ("top_p", C.c_float), ("top_k", C.c_uint32),
                 ("greedy", C.c_int32)]
+
+
+class PagedCacheC(C.Structure):
+    """pf_paged_cache: a paged cache's sizes and device pointers."""
+
+    _fields_ = [
+        ("dtype", C.c_int32), ("n_layers", C.c_int32), ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32),
+        ("page_size", C.c_int32), ("n_pages", C.c_int32), ("max_seqs", C.c_int32), ("max_pages", C.c_int32),
+        ("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+        ("table", C.c_void_p), ("lens", C.c_void_p), ("refs", C.c_void_p), ("work", C.c_void_p),
+    ]
 
 
 _lib = None
@@ -74,6 +86,17 @@ def lib():
     sig("pf_gemm_packed", st, vp, vp, vp, vp, i32, vp, i32, i32, i32, vp)
     sig("pf_check_reciprocal", st, vp, vp)
     sig("pf_check_ordered_scan", st, vp, i32, i32, i32, vp, vp, vp)
+    pc = C.POINTER(PagedCacheC)
+    sig("pf_paged_work_bytes", sz, pc)
+    sig("pf_paged_reserve", st, pc, vp, vp, i32, vp)
+    sig("pf_paged_free", st, pc, vp, i32, vp)
+    sig("pf_paged_fork", st, pc, vp, vp, i32, vp)
+    sig("pf_paged_copy", st, pc, vp, vp, i32, vp)
+    sig("pf_paged_compact", st, pc, vp)
+    sig("pf_paged_store", st, pc, i32, vp, i64, vp, i64, i32, vp, i32, i32, vp)
+    sig("pf_paged_attention_work_bytes", sz, pc, i32, i32, i32)
+    sig("pf_paged_attention", st, pc, i32, vp, i64, vp, i64, i32, i32, i32, i32, f32, vp, sz, vp)
+    sig("pf_prompt_attention", st, vp, i64, vp, i64, vp, i64, vp, i64, i32, vp, i32, i32, i32, i32, i32, f32, vp)
     sig("pf_engine_create", st, C.POINTER(ModelConfigC), i32, i32, i32, C.POINTER(vp))
     sig("pf_engine_destroy", None, vp)
     sig("pf_engine_set_matrix", st, vp, i32, i32, vp, vp)

@@ -1,0 +1,56 @@
+// paged.cuh — the paged cache (pf_paged_cache) as its kernels see it.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace pf {
+
+// Checks a cache's sizes and pointers (the page operations' `work` included
+// with `need_work`); the message names the calling entry point.
+pf_status check_paged_cache(const pf_paged_cache* c, const char* where, bool need_work);
+
+// What two launches of a page operation pass on, in the cache's `work`.
+struct PageWork {
+    int* n_list;   // pages in src / dst
+    int* n_live;   // pages in use (compaction)
+    int* src;      // [n_pages]
+    int* dst;      // [n_pages]
+    int* remap;    // [n_pages] new place of a moved page
+    int* mark;     // [max_seqs] first list index that names the sequence
+    int* plan;     // [max_seqs] per list index: pages asked for before it, or its fresh page
+};
+__host__ __device__ inline PageWork page_work(const pf_paged_cache& c) {
+    int* w = reinterpret_cast<int*>(c.work);
+    PageWork p;
+    p.n_list = w;
+    p.n_live = w + 1;
+    p.src = w + 4;
+    p.dst = p.src + c.n_pages;
+    p.remap = p.dst + c.n_pages;
+    p.mark = p.remap + c.n_pages;
+    p.plan = p.mark + c.max_seqs;
+    return p;
+}
+inline size_t page_work_bytes(const pf_paged_cache& c) {
+    return (4 + 3 * (size_t)c.n_pages + 2 * (size_t)c.max_seqs) * sizeof(int);
+}
+
+__host__ __device__ inline int type_bytes(int dtype) { return dtype == PF_F32 ? 4 : (dtype == PF_I8 ? 1 : 2); }
+// Rows (page, layer, kv head, slot) are counted in 64 bits: a cache may hold more than 2^31 of them.
+__device__ __forceinline__ int64_t slot_row(const pf_paged_cache& c, int page, int layer, int g, int slot) {
+    return (((int64_t)page * c.n_layers + layer) * c.n_kv_heads + g) * c.page_size + slot;
+}
+__device__ __forceinline__ void latch(uint32_t* err, uint32_t bit) {
+    if (err) atomicOr(err, bit);
+}
+// A sequence's length, -1 (and a latched bit) where it cannot be one.
+__device__ __forceinline__ int seq_len(const pf_paged_cache& c, int b, uint32_t* err) {
+    const int n = c.lens[b];
+    if (n >= 0 && (int64_t)n <= (int64_t)c.max_pages * c.page_size) return n;
+    latch(err, ERR_BOUNDS);
+    return -1;
+}
+
+}  // namespace pf

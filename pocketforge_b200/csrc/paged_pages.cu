@@ -1,0 +1,491 @@
+// paged_pages.cu — the pages of the paged cache: reserve, free, fork, copy,
+// compact.
+//
+// Each operation that takes pages decides in one CTA of 1,024 threads which
+// ones (prefix sums over the list's needs and over the reference counts, so
+// that the answer never depends on the order in which threads arrive), and a
+// second launch on all SMs moves the bytes.  The deciding CTA reads the
+// reference counts with every thread's share in flight at once; it is bound by
+// two trips to memory and two block scans.  The copies are bound by HBM: every
+// thread has four 16-byte loads in flight.
+#include <climits>
+
+#include "paged.cuh"
+
+namespace pf {
+
+namespace {
+
+constexpr int kDecide = 1024;   // threads of the deciding CTA
+constexpr int kPerThread = 64;  // pages a thread takes at once at most (one bit each)
+constexpr int kCopy = 256;      // threads of a copying CTA
+constexpr int kVecs = 4;        // 16-byte vectors a thread has in flight
+
+// Exclusive prefix sum over the CTA's 1,024 threads, and the total.
+__device__ __forceinline__ long long block_scan(long long v, long long* total, long long* s_warp) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    long long x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    if (lane == 31) s_warp[warp] = x;
+    __syncthreads();
+    if (warp == 0) {
+        long long w = s_warp[lane];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long y = __shfl_up_sync(0xffffffffu, w, o);
+            if (lane >= o) w += y;
+        }
+        s_warp[lane] = w;
+    }
+    __syncthreads();
+    const long long before = warp ? s_warp[warp - 1] : 0;
+    *total = s_warp[31];
+    __syncthreads();  // s_warp is free for the next scan
+    return before + x - v;
+}
+
+// This thread's pages [first, first + count) of the chunk at `base`, as a mask
+// of those in use.
+struct Share {
+    int first, count;
+    unsigned long long live;
+};
+__device__ __forceinline__ int share_size(int n_pages) {
+    const int per = (n_pages + kDecide - 1) / kDecide;
+    return min(kPerThread, (per + 3) & ~3);
+}
+__device__ __forceinline__ Share share_of(const pf_paged_cache& c, int64_t base, int per) {
+    Share s;
+    const int64_t first = base + (int64_t)threadIdx.x * per;
+    s.first = (int)min(first, (int64_t)c.n_pages);
+    s.count = (int)min((int64_t)per, (int64_t)c.n_pages - s.first);
+    s.live = 0;
+    for (int i = 0; i < s.count; i++) s.live |= (unsigned long long)(c.refs[s.first + i] > 0) << i;
+    return s;
+}
+__device__ __forceinline__ unsigned long long ones(int n) { return n >= 64 ? ~0ull : (1ull << n) - 1; }
+
+// Writes the lowest free pages, `want` at most, to list[] in order; returns how many there are.
+__device__ __forceinline__ int list_free(const pf_paged_cache& c, long long want, int* list, long long* s_warp) {
+    long long found = 0;
+    const int per = share_size(c.n_pages);
+    for (int64_t base = 0; base < c.n_pages && found < want; base += (int64_t)per * kDecide) {
+        const Share s = share_of(c, base, per);
+        unsigned long long free_ = ~s.live & ones(s.count);
+        long long total;
+        long long rank = found + block_scan(__popcll(free_), &total, s_warp);
+        for (; free_ && rank < want; free_ &= free_ - 1, rank++) list[rank] = s.first + __ffsll((long long)free_) - 1;
+        found += total;
+    }
+    __syncthreads();  // list[] is read by other threads
+    return (int)min(found, want);
+}
+
+__device__ __forceinline__ bool in_range(int i, int n) { return (unsigned)i < (unsigned)n; }
+
+// mark[s] = the first index of list[] that names sequence s, for every s in it.
+__device__ __forceinline__ void mark_first(const pf_paged_cache& c, const int* list, int n, int* mark) {
+    for (int i = threadIdx.x; i < n; i += kDecide)
+        if (in_range(list[i], c.max_seqs)) mark[list[i]] = INT_MAX;
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kDecide)
+        if (in_range(list[i], c.max_seqs)) atomicMin(&mark[list[i]], i);
+    __syncthreads();
+}
+
+// Pages that entry i of a reserve asks for; -1: refused (bit latched by the caller's second look).
+__device__ __forceinline__ int reserve_need(const pf_paged_cache& c, const PageWork& w, const int* seqs,
+                                            const int* counts, int i, uint32_t* err) {
+    const int s = seqs[i];
+    if (!in_range(s, c.max_seqs) || w.mark[s] != i || counts[i] < 0) {
+        latch(err, ERR_BOUNDS);
+        return -1;
+    }
+    const int n = seq_len(c, s, err);
+    if (n < 0) return -1;
+    const int64_t pages = ((int64_t)n + counts[i] + c.page_size - 1) / c.page_size;
+    if (pages > c.max_pages) {
+        latch(err, ERR_CONTEXT);
+        return -1;
+    }
+    return (int)(pages - (n + (int64_t)c.page_size - 1) / c.page_size);
+}
+
+__global__ void __launch_bounds__(kDecide) reserve_kernel(const pf_paged_cache c, const int* seqs, const int* counts,
+                                                          int n, uint32_t* err) {
+    __shared__ long long s_warp[32];
+    const PageWork w = page_work(c);
+    mark_first(c, seqs, n, w.mark);
+    long long want = 0;
+    for (int base = 0; base < n; base += kDecide) {
+        const int i = base + threadIdx.x;
+        const int need = i < n ? reserve_need(c, w, seqs, counts, i, err) : 0;
+        long long total;
+        const long long before = want + block_scan(max(need, 0), &total, s_warp);
+        if (i < n) w.plan[i] = need < 0 ? -1 : (int)min(before, (long long)INT_MAX);
+        want += total;
+    }
+    const int found = want > 0 ? list_free(c, min(want, (long long)c.n_pages), w.src, s_warp) : 0;
+    __syncthreads();
+    // one warp an entry: its pages are w.src[before .. before + need)
+    const int lane = threadIdx.x & 31;
+    for (int i = threadIdx.x >> 5; i < n; i += kDecide / 32) {
+        const int before = w.plan[i];
+        if (before < 0) continue;
+        const int s = seqs[i], len = c.lens[s], old = (len + c.page_size - 1) / c.page_size;
+        const int need = (int)(((int64_t)len + counts[i] + c.page_size - 1) / c.page_size) - old;
+        __syncwarp();  // every lane has read the length
+        if (need && (int64_t)before + need > found) {
+            if (lane == 0) latch(err, ERR_CONTEXT);
+            continue;
+        }
+        for (int j = lane; j < need; j += 32) {
+            const int p = w.src[before + j];
+            c.table[(int64_t)s * c.max_pages + old + j] = p;
+            c.refs[p] = 1;
+        }
+        if (lane == 0) c.lens[s] = len + counts[i];
+    }
+}
+
+// One CTA a sequence; whoever takes its length first frees it, so one named
+// twice is freed once.
+__global__ void free_kernel(const pf_paged_cache c, const int* seqs, uint32_t* err) {
+    __shared__ int s_len;
+    const int s = seqs[blockIdx.x];
+    if (!in_range(s, c.max_seqs)) {
+        if (threadIdx.x == 0) latch(err, ERR_BOUNDS);
+        return;
+    }
+    if (threadIdx.x == 0) s_len = atomicExch(&c.lens[s], 0);
+    __syncthreads();
+    if (s_len < 0 || s_len > (int64_t)c.max_pages * c.page_size) {
+        if (threadIdx.x == 0) latch(err, ERR_BOUNDS);
+        return;
+    }
+    const int pages = (int)(((int64_t)s_len + c.page_size - 1) / c.page_size);
+    for (int j = threadIdx.x; j < pages; j += blockDim.x) {
+        int* at = c.table + (int64_t)s * c.max_pages + j;
+        const int p = *at;
+        *at = -1;
+        if (in_range(p, c.n_pages)) atomicSub(&c.refs[p], 1);
+        else latch(err, ERR_BOUNDS);
+    }
+}
+
+constexpr int kForkNone = -1, kForkRefused = -2;  // no partly filled page; left as it is
+
+__global__ void __launch_bounds__(kDecide) fork_decide_kernel(const pf_paged_cache c, const int* parents,
+                                                              const int* children, int n, uint32_t* err) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    __shared__ long long s_warp[32];
+    const PageWork w = page_work(c);
+    mark_first(c, children, n, w.mark);
+    for (int i = threadIdx.x; i < n; i += kDecide)  // a parent is no entry's child
+        if (in_range(parents[i], c.max_seqs)) w.mark[parents[i]] = -1;
+    __syncthreads();
+    long long want = 0;
+    for (int base = 0; base < n; base += kDecide) {
+        const int i = base + threadIdx.x;
+        int need = 0;
+        if (i < n) {
+            const int p = parents[i], k = children[i];
+            bool ok = in_range(p, c.max_seqs) && in_range(k, c.max_seqs) && w.mark[k] == i && c.lens[k] == 0;
+            int len = 0;
+            if (ok) len = seq_len(c, p, err), ok = len >= 0;
+            if (ok && len % c.page_size) {
+                need = 1;
+                ok = in_range(c.table[(int64_t)p * c.max_pages + len / c.page_size], c.n_pages);
+            }
+            if (!ok) latch(err, ERR_BOUNDS), need = 0;
+            w.plan[i] = ok ? kForkNone : kForkRefused;
+        }
+        long long total;
+        const long long before = want + block_scan(need, &total, s_warp);
+        if (need) w.plan[i] = (int)before;
+        want += total;
+    }
+    const int found = want > 0 ? list_free(c, min(want, (long long)c.n_pages), w.src, s_warp) : 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kDecide) {
+        const int rank = w.plan[i];
+        if (rank < 0) continue;
+        if (rank >= found) {
+            latch(err, ERR_CONTEXT);
+            w.plan[i] = kForkRefused;
+        } else {
+            w.plan[i] = w.src[rank];
+            c.refs[w.src[rank]] = 1;
+        }
+    }
+}
+
+// CTA (y, i): table row and reference counts of child i (y == 0), and its last
+// page's positions of eight (layer, kv head) pairs, one a warp.
+__global__ void __launch_bounds__(kCopy) fork_copy_kernel(const pf_paged_cache c, const int* parents,
+                                                          const int* children, uint32_t* err) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int i = blockIdx.y, fresh = page_work(c).plan[i];
+    if (fresh == kForkRefused) return;
+    const int p = parents[i], k = children[i], len = c.lens[p], full = len / c.page_size, rest = len % c.page_size;
+    const int* from = c.table + (int64_t)p * c.max_pages;
+    if (blockIdx.x == 0) {
+        int* to = c.table + (int64_t)k * c.max_pages;
+        for (int j = threadIdx.x; j < full; j += kCopy) {
+            const int page = from[j];
+            to[j] = page;
+            if (in_range(page, c.n_pages)) atomicAdd(&c.refs[page], 1);
+            else latch(err, ERR_BOUNDS);
+        }
+        if (threadIdx.x == 0) {
+            if (rest) to[full] = fresh;
+            c.lens[k] = len;
+        }
+    }
+    if (!rest) return;
+    const int lane = threadIdx.x & 31, pair = blockIdx.x * (kCopy / 32) + (threadIdx.x >> 5);
+    if (pair >= c.n_layers * c.n_kv_heads) return;
+    const int64_t a = slot_row(c, from[full], 0, pair, 0), b = slot_row(c, fresh, 0, pair, 0);
+    const int row = c.head_dim * type_bytes(c.dtype), vecs = rest * row / 16;
+    const uint4* ka = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(c.k) + a * row);
+    const uint4* va = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(c.v) + a * row);
+    uint4* kb = reinterpret_cast<uint4*>(reinterpret_cast<char*>(c.k) + b * row);
+    uint4* vb = reinterpret_cast<uint4*>(reinterpret_cast<char*>(c.v) + b * row);
+    float sk[4], sv[4];  // 128 slots at most
+    if (c.dtype == PF_I8) {
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+            if (lane + 32 * u < rest) sk[u] = c.k_scale[a + lane + 32 * u], sv[u] = c.v_scale[a + lane + 32 * u];
+    }
+    for (int j = lane; j < vecs; j += 32 * kVecs) {
+        uint4 x[kVecs], y[kVecs];
+#pragma unroll
+        for (int u = 0; u < kVecs; u++)
+            if (j + 32 * u < vecs) x[u] = ka[j + 32 * u], y[u] = va[j + 32 * u];
+#pragma unroll
+        for (int u = 0; u < kVecs; u++)
+            if (j + 32 * u < vecs) kb[j + 32 * u] = x[u], vb[j + 32 * u] = y[u];
+    }
+    if (c.dtype == PF_I8) {
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+            if (lane + 32 * u < rest) c.k_scale[b + lane + 32 * u] = sk[u], c.v_scale[b + lane + 32 * u] = sv[u];
+    }
+}
+
+// Copies whole pages src[i] -> dst[i], in pieces of kCopy * kVecs vectors.
+__device__ __forceinline__ void copy_pages(const pf_paged_cache& c, const int* src, const int* dst, int n,
+                                           uint32_t* err) {
+    const int64_t rows = (int64_t)c.n_layers * c.n_kv_heads * c.page_size;
+    const int64_t kv_vecs = rows * c.head_dim * type_bytes(c.dtype) / 16, sc_vecs = c.dtype == PF_I8 ? rows / 4 : 0;
+    constexpr int piece = kCopy * kVecs;
+    const int64_t kv_pieces = (kv_vecs + piece - 1) / piece, sc_pieces = (sc_vecs + piece - 1) / piece;
+    const int64_t per = 2 * (kv_pieces + sc_pieces);
+    for (int64_t u = blockIdx.x; u < per * n; u += gridDim.x) {
+        const int i = (int)(u / per), from = src[i], to = dst[i];
+        if (!in_range(from, c.n_pages) || !in_range(to, c.n_pages)) {
+            if (threadIdx.x == 0) latch(err, ERR_BOUNDS);
+            continue;
+        }
+        int64_t at = u % per;
+        uint4* base;
+        int64_t vecs;
+        if (at < 2 * kv_pieces) {
+            base = reinterpret_cast<uint4*>(at < kv_pieces ? c.k : c.v);
+            vecs = kv_vecs;
+            at %= kv_pieces;
+        } else {
+            at -= 2 * kv_pieces;
+            base = reinterpret_cast<uint4*>(at < sc_pieces ? c.k_scale : c.v_scale);
+            vecs = sc_vecs;
+            at %= sc_pieces;
+        }
+        const uint4* a = base + from * vecs;
+        uint4* b = base + to * vecs;
+        const int64_t j = at * piece + threadIdx.x;
+        uint4 x[kVecs];
+#pragma unroll
+        for (int q = 0; q < kVecs; q++)
+            if (j + q * kCopy < vecs) x[q] = a[j + q * kCopy];
+#pragma unroll
+        for (int q = 0; q < kVecs; q++)
+            if (j + q * kCopy < vecs) b[j + q * kCopy] = x[q];
+    }
+}
+
+__global__ void __launch_bounds__(kCopy) copy_kernel(const pf_paged_cache c, const int* src, const int* dst, int n,
+                                                     uint32_t* err) {
+    copy_pages(c, src, dst, n, err);
+}
+
+// n_live, the pages in use behind it (src) and the free ones before it (dst),
+// pairwise; reference counts move with them.
+__global__ void __launch_bounds__(kDecide) compact_decide_kernel(const pf_paged_cache c) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    __shared__ long long s_warp[32];
+    const PageWork w = page_work(c);
+    const int per = share_size(c.n_pages);
+    const int64_t chunk = (int64_t)per * kDecide;
+    const Share first = share_of(c, 0, per);  // all of them, up to 65,536 pages
+    long long live = 0;
+    for (int64_t base = 0; base < c.n_pages; base += chunk) {
+        const Share s = base ? share_of(c, base, per) : first;
+        long long total;
+        block_scan(__popcll(s.live), &total, s_warp);
+        live += total;
+    }
+    const int n_live = (int)live;
+    long long holes = 0, movers = 0;
+    for (int64_t base = 0; base < c.n_pages; base += chunk) {
+        const Share s = base ? share_of(c, base, per) : first;
+        // pages before n_live count if free, those behind it if in use
+        const int front = min(max(n_live - s.first, 0), s.count);
+        unsigned long long hole = ~s.live & ones(front), mover = s.live & ~ones(front);
+        long long total;
+        const long long before =
+            block_scan(((long long)__popcll(hole) << 32) | __popcll(mover), &total, s_warp);
+        long long h = holes + (before >> 32), m = movers + (before & 0xffffffffll);
+        for (; hole; hole &= hole - 1) w.dst[h++] = s.first + __ffsll((long long)hole) - 1;
+        for (; mover; mover &= mover - 1) w.src[m++] = s.first + __ffsll((long long)mover) - 1;
+        holes += total >> 32;
+        movers += total & 0xffffffffll;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < (int)movers; i += kDecide) {
+        const int a = w.src[i], b = w.dst[i];
+        c.refs[b] = c.refs[a];
+        c.refs[a] = 0;
+        w.remap[a] = b;
+    }
+    if (threadIdx.x == 0) *w.n_list = (int)movers, *w.n_live = n_live;
+}
+
+__global__ void __launch_bounds__(kCopy) compact_move_kernel(const pf_paged_cache c, uint32_t* err) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const PageWork w = page_work(c);
+    const int n = *w.n_list, n_live = *w.n_live;
+    if (n == 0) return;  // in order already
+    // tables: one warp a sequence
+    for (int s = (int)(blockIdx.x * (kCopy / 32) + (threadIdx.x >> 5)); s < c.max_seqs; s += gridDim.x * (kCopy / 32)) {
+        const int len = seq_len(c, s, err);
+        const int pages = (int)(((int64_t)max(len, 0) + c.page_size - 1) / c.page_size);
+        for (int j = threadIdx.x & 31; j < pages; j += 32) {
+            int* at = c.table + (int64_t)s * c.max_pages + j;
+            const int p = *at;
+            if (!in_range(p, c.n_pages)) latch(err, ERR_BOUNDS);
+            else if (p >= n_live) *at = w.remap[p];
+        }
+    }
+    copy_pages(c, w.src, w.dst, n, err);
+}
+
+// A launch that may begin while the one before it in the stream still runs
+// (it waits for that one's end itself, by griddepcontrol.wait).
+template <typename... P, typename... A>
+pf_status launch_after(void (*kernel)(P...), dim3 grid, int threads, cudaStream_t st, A... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    PF_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+    return PF_OK;
+}
+
+constexpr int kCopyCtas = 148 * 8;  // all SMs full of copying CTAs
+
+}  // namespace
+
+pf_status check_paged_cache(const pf_paged_cache* c, const char* where, bool need_work) {
+    PF_CHECK(c, "%s: null cache", where);
+    PF_CHECK(c->dtype == PF_I8 || c->dtype == PF_BF16 || c->dtype == PF_F16, "%s: cache dtype %d", where, c->dtype);
+    PF_CHECK(c->head_dim == 64 || c->head_dim == 128, "%s: head_dim %d is neither 64 nor 128", where, c->head_dim);
+    PF_CHECK(c->page_size == 16 || c->page_size == 32 || c->page_size == 64 || c->page_size == 128,
+             "%s: page_size %d is not 16, 32, 64 or 128", where, c->page_size);
+    PF_CHECK(c->n_layers > 0 && c->n_kv_heads > 0 && c->n_pages > 0 && c->max_seqs > 0 && c->max_pages > 0,
+             "%s: a size is not positive", where);
+    PF_CHECK((int64_t)c->n_layers * c->n_kv_heads <= 65536 && c->n_pages <= (1 << 28) && c->max_seqs <= (1 << 20) &&
+                 (int64_t)c->max_pages * c->page_size <= INT_MAX,
+             "%s: a size is too large", where);
+    PF_CHECK(c->k && c->v && c->table && c->lens && c->refs, "%s: null pointer in the cache", where);
+    PF_CHECK(c->dtype != PF_I8 || (c->k_scale && c->v_scale), "%s: an int8 cache needs scales", where);
+    PF_CHECK(!need_work || c->work, "%s: null work in the cache", where);
+    const uintptr_t all = (uintptr_t)c->k | (uintptr_t)c->v | (need_work ? (uintptr_t)c->work : 0) |
+                          (c->dtype == PF_I8 ? (uintptr_t)c->k_scale | (uintptr_t)c->v_scale : 0);
+    PF_CHECK(all % 16 == 0, "%s: k, v, scales and work must be 16-byte aligned", where);
+    return PF_OK;
+}
+
+}  // namespace pf
+
+using namespace pf;
+
+extern "C" {
+
+size_t pf_paged_work_bytes(const pf_paged_cache* c) {
+    if (!c || c->n_pages <= 0 || c->max_seqs <= 0) return 0;
+    return page_work_bytes(*c);
+}
+
+pf_status pf_paged_reserve(const pf_paged_cache* c, const int32_t* seqs, const int32_t* counts, int32_t n,
+                           void* stream) {
+    PF_TRY(check_paged_cache(c, "pf_paged_reserve", true));
+    PF_CHECK(n >= 0 && n <= c->max_seqs, "pf_paged_reserve: %d sequences of %d", n, c->max_seqs);
+    PF_TRY(require_device());
+    if (n == 0) return PF_OK;
+    PF_CHECK(seqs && counts, "pf_paged_reserve: null argument");
+    reserve_kernel<<<1, kDecide, 0, as_stream(stream)>>>(*c, seqs, counts, n, device_error_flag());
+    return launch_check("reserve");
+}
+
+pf_status pf_paged_free(const pf_paged_cache* c, const int32_t* seqs, int32_t n, void* stream) {
+    PF_TRY(check_paged_cache(c, "pf_paged_free", false));
+    PF_CHECK(n >= 0 && n <= c->max_seqs, "pf_paged_free: %d sequences of %d", n, c->max_seqs);
+    PF_TRY(require_device());
+    if (n == 0) return PF_OK;
+    PF_CHECK(seqs, "pf_paged_free: null argument");
+    free_kernel<<<n, 128, 0, as_stream(stream)>>>(*c, seqs, device_error_flag());
+    return launch_check("free");
+}
+
+pf_status pf_paged_fork(const pf_paged_cache* c, const int32_t* parents, const int32_t* children, int32_t n,
+                        void* stream) {
+    PF_TRY(check_paged_cache(c, "pf_paged_fork", true));
+    PF_CHECK(n >= 0 && n <= c->max_seqs && n <= 65535, "pf_paged_fork: %d children of %d sequences", n, c->max_seqs);
+    PF_TRY(require_device());
+    if (n == 0) return PF_OK;
+    PF_CHECK(parents && children, "pf_paged_fork: null argument");
+    uint32_t* err = device_error_flag();
+    fork_decide_kernel<<<1, kDecide, 0, as_stream(stream)>>>(*c, parents, children, n, err);
+    PF_TRY(launch_check("fork_decide"));
+    const dim3 grid(ceil_div(c->n_layers * c->n_kv_heads, kCopy / 32), n);
+    return launch_after(fork_copy_kernel, grid, kCopy, as_stream(stream), *c, parents, children, err);
+}
+
+pf_status pf_paged_copy(const pf_paged_cache* c, const int32_t* src, const int32_t* dst, int32_t n, void* stream) {
+    PF_TRY(check_paged_cache(c, "pf_paged_copy", false));
+    PF_CHECK(n >= 0 && n <= c->n_pages, "pf_paged_copy: %d pages of %d", n, c->n_pages);
+    PF_TRY(require_device());
+    if (n == 0) return PF_OK;
+    PF_CHECK(src && dst, "pf_paged_copy: null argument");
+    copy_kernel<<<kCopyCtas, kCopy, 0, as_stream(stream)>>>(*c, src, dst, n, device_error_flag());
+    return launch_check("copy");
+}
+
+pf_status pf_paged_compact(const pf_paged_cache* c, void* stream) {
+    PF_TRY(check_paged_cache(c, "pf_paged_compact", true));
+    PF_TRY(require_device());
+    compact_decide_kernel<<<1, kDecide, 0, as_stream(stream)>>>(*c);
+    PF_TRY(launch_check("compact_decide"));
+    return launch_after(compact_move_kernel, dim3(kCopyCtas), kCopy, as_stream(stream), *c, device_error_flag());
+}
+
+}  // extern "C"
