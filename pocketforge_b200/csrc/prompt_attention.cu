@@ -1,10 +1,55 @@
-// prompt_attention.cu — causal attention over packed prompts.
+// prompt_attention.cu — causal attention over packed prompts on the
+// 5th-generation tensor cores.
+//
+//   out_i = sum_{j <= i} softmax_j(scale * q_i . k_j) v_j   within a sequence
+//
+// in one pass over the keys: blocks of 128, the running row maximum m and sum
+// l in fp32, out = O / l at the end.
+//
+// A work unit is two 128-row tiles of queries that read the same keys and
+// values: two heads of one kv head at the same rows (or, with one query head a
+// kv head, two neighbouring row tiles).  Every K and V block is loaded once for
+// both.  One CTA an SM takes unit after unit (clusterlaunchcontrol: a running
+// CTA takes over the launch of the next one, so the units go to whoever is
+// free, longest first within a sequence).  Its warps:
+//   0-3, 4-7  softmax of tile 0 and 1, one row a thread: scores from TMEM,
+//             p = 2^(c s - c m) (c = scale log2 e), p as 16-bit back into TMEM,
+//             at the end O / l to memory
+//   8         unit list and TMA loads, one lane a 64-column slab
+//   9         issues the tcgen05 products S = Q K^T and O += P V
+//   10        looks through the V block on the diagonal (below)
+// The maximum that the exponents refer to rises only when a block exceeds it
+// by 2^8, so O (in TMEM) is rescaled rarely: p stays below 2^8, within fp16,
+// and the row sum takes the same p.
+//
+// Rounding: scores, maxima, sums and O are fp32.  P is rounded to the inputs'
+// 16-bit type, which the tensor core asks for (both operands of one type).
+//
+// What a row must not see: scores behind the row itself are -inf, their p is 0.
+// But 0 x inf = NaN, so V rows behind the sequence's end (another sequence's)
+// are set to 0 in shared memory, and a diagonal block with an inf or NaN among
+// its own V rows sends its unit's rows through a plain loop, one warp a row.
+//
+// Every wait is bounded (about a second): a timeout latches ERR_TIMEOUT, the
+// other roles stop waiting, and the CTA lets its copies land and frees its TMEM.
+#include <cuda.h>
+
+#include <algorithm>
+#include <mutex>
+#include <type_traits>
+
 #include "paged.cuh"
 #include "row_attention.cuh"
 
 namespace pf {
 
 namespace {
+
+constexpr int BM = 128;            // query rows a tile, keys a block
+constexpr int kSoftmaxWarps = 8;
+constexpr int kThreads = 352;      // 11 warps: 65,536 registers allow 184 a thread
+constexpr uint32_t ERR_TIMEOUT = 16u;
+constexpr int kSlots = 2;          // units in the list between the load warp and the others
 
 struct PromptParams {
     const void *q, *k, *v;
@@ -16,33 +61,224 @@ struct PromptParams {
     uint32_t* err;
 };
 
-// First and last row of sequence b; false where its offsets are not usable.
-__device__ __forceinline__ bool seq_rows(const PromptParams& p, int b, int& first, int& end) {
-    first = p.offsets[b];
-    end = p.offsets[b + 1];
-    if (first >= 0 && end >= first && end <= p.n_tokens) return true;
-    latch(p.err, ERR_BOUNDS);
-    return false;
+template <int HD>
+struct Layout {
+    static constexpr int NC = HD / 64;                // 64-column (128-byte) slabs of a row
+    static constexpr int SLAB = BM * 128;             // bytes of one
+    static constexpr int TILE = NC * SLAB;            // a Q tile, K block or V block
+    static constexpr int STAGES = HD == 64 ? 4 : 2;   // K blocks and V blocks in flight
+    static constexpr int K_OFF = 2 * TILE, V_OFF = K_OFF + STAGES * TILE, BAR_OFF = V_OFF + STAGES * TILE;
+    static constexpr int SMEM = BAR_OFF + 512 + 1024;  // barriers, unit list; alignment
+    // TMEM columns.  head_dim 64: P has its own columns, so the next scores are
+    // computed while this block's are exponentiated; at 128 the accumulators
+    // take that room and P overlays the scores it came from.
+    static constexpr bool OWN_P = HD == 64;
+    static constexpr uint32_t S = 0, P = OWN_P ? 256 : 0, P_STEP = OWN_P ? 64 : 128, O = OWN_P ? 384 : 256;
+};
+
+// ---- PTX ----
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+// False when a second has passed, or another role has given up.
+__device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint32_t* err) {
+    uint64_t t0, t;
+    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t0));
+    for (uint32_t i = 0;; i++) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((i & 63u) == 63u) {
+            if (*abort_flag) return false;
+            asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+            if (t - t0 > 1000000000ull) {
+                *abort_flag = 1;
+                latch(err, ERR_TIMEOUT);
+                return false;
+            }
+        }
+    }
+}
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint32_t* err) {
+    return mbar_try_wait(bar, parity) || mbar_wait_slow(bar, parity, abort_flag, err);
+}
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+// Operand descriptors, 128-byte swizzle (8 rows of 128 bytes = one 1,024-byte
+// atom), version 1 (sm_100), layout type 2.  K-major (Q, K): atoms 1,024 bytes
+// apart along the rows.  Rows-as-K (V): 64 columns an atom, the next 64 a slab
+// away (leading offset), the next 8 rows 1,024 bytes away (stride offset).
+__device__ __forceinline__ uint64_t desc_sw128(uint32_t addr, uint32_t lead) {
+    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// D fp32; A and B fp16 (0) or bf16 (1); B's major at bit 16; N >> 3; M >> 4.
+__host__ __device__ constexpr uint32_t idesc_f16(int bf16, int n, int b_rows_as_k) {
+    return (1u << 4) | ((uint32_t)bf16 << 7) | ((uint32_t)bf16 << 10) | ((uint32_t)b_rows_as_k << 16) |
+           ((uint32_t)(n >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_ld32(uint32_t a, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(a)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t a, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+        "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(a),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// Two fp32 in one register pair (one instruction for both on sm_100).
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(reinterpret_cast<uint64_t&>(d))
+        : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("add.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<uint64_t&>(d))
+        : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+    return d;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
 }
 
-// One warp a (row, head).
-template <typename T, int HD>
-__global__ void __launch_bounds__(256) prompt_rows_kernel(const PromptParams p) {
-    constexpr int N = HD / 32;
-    const int lane = threadIdx.x & 31, h = blockIdx.y, g = h / (p.n_heads / p.n_kv_heads);
-    const int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (i >= p.n_tokens) return;
-    int first = -1;
-    for (int b = 0; b < p.n_seqs; b++) {
-        int a, e;
-        if (seq_rows(p, b, a, e) && a <= i && i < e) first = a;
+// ---- units ----
+struct Unit {
+    int first, len;   // the sequence's first row and rows
+    int g;            // kv head
+    int tile[2];      // row tile of query tile s, -1: none
+    int head[2];
+    int bad;          // an inf or NaN in a V block on the diagonal
+    __device__ int blocks(int s) const { return tile[s] + 1; }
+    __device__ int blocks() const { return max(tile[0], tile[1]) + 1; }
+};
+
+// Walks the sequences to unit u; a whole warp, the same in every lane.
+struct UnitList {
+    int seq = 0;           // first sequence of the window of 32 looked at
+    long long before = 0;  // units before it
+    __device__ bool find(const PromptParams& p, long long u, Unit& out) {
+        if (u < before) seq = 0, before = 0;
+        const int lane = threadIdx.x & 31, group = p.n_heads / p.n_kv_heads;
+        for (; seq < p.n_seqs; seq += 32) {
+            int first = 0, len = 0;
+            if (seq + lane < p.n_seqs) {
+                first = p.offsets[seq + lane];
+                const int end = p.offsets[seq + lane + 1];
+                if (first >= 0 && end >= first && end <= p.n_tokens) len = end - first;
+                else latch(p.err, ERR_BOUNDS);
+            }
+            const long long pairs = ((long long)((len + BM - 1) / BM) * group + 1) / 2, mine = pairs * p.n_kv_heads;
+            long long upto = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long x = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += x;
+            }
+            const unsigned here = __ballot_sync(0xffffffffu, u < before + upto);
+            if (here) {
+                const int at = __ffs((int)here) - 1;
+                const long long r = u - (before + __shfl_sync(0xffffffffu, upto - mine, at));
+                out.first = __shfl_sync(0xffffffffu, first, at);
+                out.len = __shfl_sync(0xffffffffu, len, at);
+                const int pair = (int)(__shfl_sync(0xffffffffu, pairs, at) - 1 - r / p.n_kv_heads);
+                out.g = (int)(r % p.n_kv_heads);
+                const int tiles = (out.len + BM - 1) / BM;
+                for (int s = 0; s < 2; s++) {
+                    const int c = 2 * pair + s;  // (row tile, head of the group), heads fastest
+                    out.tile[s] = c < tiles * group ? c / group : -1;
+                    out.head[s] = out.g * group + c % group;
+                }
+                out.bad = 0;
+                return true;
+            }
+            before += __shfl_sync(0xffffffffu, upto, 31);
+        }
+        return false;
     }
-    if (first < 0) return;
+};
+
+// Row i of a sequence by one warp, from memory.
+template <typename T, int HD>
+__device__ __noinline__ void plain_row(const PromptParams& p, int first, int i, int h, int g) {
+    constexpr int N = HD / 32;
+    const int lane = threadIdx.x & 31;
+    const int64_t at = (int64_t)first + i;
     float q[N];
 #pragma unroll
-    for (int d = 0; d < N; d++) q[d] = (float)static_cast<const T*>(p.q)[i * p.q_stride + h * HD + lane + 32 * d] * p.scale;
+    for (int d = 0; d < N; d++) q[d] = (float)static_cast<const T*>(p.q)[at * p.q_stride + h * HD + lane + 32 * d] * p.scale;
     RowSoftmax<HD> s;
-    for (int64_t j = first; j <= i; j++) {
+    for (int64_t j = first; j <= at; j++) {
         float k[N], v[N];
 #pragma unroll
         for (int d = 0; d < N; d++) {
@@ -53,14 +289,492 @@ __global__ void __launch_bounds__(256) prompt_rows_kernel(const PromptParams p) 
     }
 #pragma unroll
     for (int d = 0; d < N; d++)
-        static_cast<T*>(p.out)[i * p.out_stride + h * HD + lane + 32 * d] = (T)(s.o[d] / s.l);
+        static_cast<T*>(p.out)[at * p.out_stride + h * HD + lane + 32 * d] = (T)(s.l == 0.0f ? 0.0f : s.o[d] / s.l);
 }
 
-template <typename T>
-pf_status launch_prompt(const PromptParams& p, int hd, cudaStream_t st) {
-    const dim3 grid(ceil_div(p.n_tokens, 8), p.n_heads);
-    if (hd == 64) prompt_rows_kernel<T, 64><<<grid, 256, 0, st>>>(p);
-    else prompt_rows_kernel<T, 128><<<grid, 256, 0, st>>>(p);
+template <typename T, int HD>
+__global__ void __launch_bounds__(kThreads, 1)
+    prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                  const __grid_constant__ CUtensorMap map_v, const PromptParams p) {
+    using Ly = Layout<HD>;
+    constexpr int ST = Ly::STAGES, NC = Ly::NC;
+    constexpr int BF = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    const uint32_t base = smem_u32(smem);
+    const uint32_t bars = base + Ly::BAR_OFF;
+    auto q_full = [&](int s) { return bars + 8u * s; };
+    auto q_empty = [&](int s) { return bars + 8u * (2 + s); };
+    auto s_full = [&](int s) { return bars + 8u * (4 + s); };
+    auto s_free = [&](int s) { return bars + 8u * (6 + s); };
+    auto p_full = [&](int s) { return bars + 8u * (8 + s); };
+    auto o_full = [&](int s) { return bars + 8u * (10 + s); };
+    auto o_free = [&](int s) { return bars + 8u * (12 + s); };
+    auto u_full = [&](int i) { return bars + 8u * (14 + i); };
+    auto u_empty = [&](int i) { return bars + 8u * (16 + i); };
+    auto u_seen = [&](int i) { return bars + 8u * (18 + i); };  // the guard is through with the unit
+    const uint32_t next_full = bars + 8u * 20;
+    auto k_full = [&](int i) { return bars + 8u * (21 + i); };
+    auto k_empty = [&](int i) { return bars + 8u * (21 + ST + i); };
+    auto v_full = [&](int i) { return bars + 8u * (21 + 2 * ST + i); };
+    auto v_empty = [&](int i) { return bars + 8u * (21 + 3 * ST + i); };
+    auto v_good = [&](int i) { return bars + 8u * (21 + 4 * ST + i); };  // looked through
+    static_assert(8 * (21 + 5 * ST) <= 336, "barriers");
+    uint8_t* tail = smem + Ly::BAR_OFF + 336;
+    const uint32_t next_at = base + Ly::BAR_OFF + 336;              // 16 bytes: the next unit's launch
+    volatile Unit* units = reinterpret_cast<volatile Unit*>(tail + 16);  // [kSlots]
+    static_assert(16 + kSlots * sizeof(Unit) + 12 <= 176, "unit list");
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tail + 16 + kSlots * sizeof(Unit));
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    int* any = reinterpret_cast<int*>(tmem_slot + 2);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    UnitList list;
+    Unit unit;
+    if (warp == 8) {
+        const bool found = list.find(p, blockIdx.x, unit);
+        if (lane == 0) {
+            *any = found;
+            for (int s = 0; s < 2; s++) {
+                mbar_init(q_full(s), NC);
+                mbar_init(q_empty(s), 1);
+                mbar_init(s_full(s), 1);
+                mbar_init(s_free(s), 4);
+                mbar_init(p_full(s), 4);
+                mbar_init(o_full(s), 1);
+                mbar_init(o_free(s), 4);
+            }
+            for (int i = 0; i < kSlots; i++) {
+                mbar_init(u_full(i), 1);
+                mbar_init(u_empty(i), kSoftmaxWarps + 2);
+                mbar_init(u_seen(i), 1);
+            }
+            mbar_init(next_full, 1);
+            for (int i = 0; i < ST; i++) {
+                mbar_init(k_full(i), NC);
+                mbar_init(k_empty(i), 1);
+                mbar_init(v_full(i), NC);
+                mbar_init(v_empty(i), 2);
+                mbar_init(v_good(i), 1);
+            }
+            *abort_flag = 0;
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+    }
+    __syncthreads();
+    if (!*any) return;  // the grid is an upper bound of the units
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    auto wait = [&](uint32_t bar, uint32_t parity) { return mbar_wait(bar, parity, abort_flag, p.err); };
+    // The unit in the list's slot, as the load warp left it.
+    auto take = [&](int i, Unit& u) {
+        volatile Unit& v = units[i];
+        u.first = v.first, u.len = v.len, u.g = v.g, u.tile[0] = v.tile[0], u.tile[1] = v.tile[1];
+        u.head[0] = v.head[0], u.head[1] = v.head[1];
+    };
+
+    if (warp == 8) {
+        // ---------------- unit list, loads ----------------
+        // Lane roles: K slabs, V slabs, then Q tile 0's and 1's slabs.  Copies issued by one lane complete one
+        // after another, hence a lane for each.
+        const int role = lane / NC, c = lane % NC;
+        uint32_t it = 0, taken[2] = {0, 0}, last_bar = 0, last_parity = 0;
+        bool more = true, ok = true;
+        for (uint32_t n = 0;; n++) {
+            const int slot = n % kSlots;
+            if (lane == 0) {
+                ok = wait(u_empty(slot), ((n / kSlots) & 1) ^ 1);
+                if (ok) {
+                    volatile Unit& v = units[slot];
+                    v.first = unit.first, v.len = more ? unit.len : 0, v.g = unit.g;
+                    v.tile[0] = unit.tile[0], v.tile[1] = unit.tile[1], v.head[0] = unit.head[0], v.head[1] = unit.head[1];
+                    v.bad = 0;
+                    mbar_arrive(u_full(slot));
+                }
+                if (ok && more) {  // ask for the next one
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    mbar_expect_tx(next_full, 16);
+                    asm volatile(
+                        "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::
+                            "r"(next_at), "r"(next_full)
+                        : "memory");
+                }
+            }
+            ok = __shfl_sync(0xffffffffu, (int)ok, 0);
+            if (!ok || !more) break;
+            const int nb = unit.blocks();
+            if (role < 2) {
+                const CUtensorMap* map = role == 0 ? &map_k : &map_v;
+                const uint32_t tiles = base + (role == 0 ? Ly::K_OFF : Ly::V_OFF) + c * Ly::SLAB;
+                for (int j = 0; j < nb && ok; j++) {
+                    const uint32_t i = it + j, st = i % ST;
+                    const uint32_t full = role == 0 ? k_full(st) : v_full(st);
+                    ok = wait(role == 0 ? k_empty(st) : v_empty(st), ((i / ST) & 1) ^ 1);
+                    if (!ok) break;
+                    mbar_expect_tx(full, Ly::SLAB);
+                    tma_load_2d(tiles + st * Ly::TILE, map, unit.g * HD + c * 64, unit.first + j * BM, full);
+                    last_bar = full, last_parity = (i / ST) & 1;
+                }
+            } else if (role < 4 && unit.tile[role - 2] >= 0) {
+                const int s = role - 2;
+                ok = wait(q_empty(s), (taken[s] & 1) ^ 1);
+                if (ok) {
+                    mbar_expect_tx(q_full(s), Ly::SLAB);
+                    tma_load_2d(base + s * Ly::TILE + c * Ly::SLAB, &map_q, unit.head[s] * HD + c * 64,
+                                unit.first + unit.tile[s] * BM, q_full(s));
+                    last_bar = q_full(s), last_parity = taken[s] & 1;
+                }
+            }
+            it += nb;
+            for (int s = 0; s < 2; s++) taken[s] += unit.tile[s] >= 0;
+            if (!__all_sync(0xffffffffu, ok)) break;
+            int got = 0;
+            uint32_t x = 0;
+            if (lane == 0) {
+                ok = wait(next_full, n & 1);
+                if (ok)
+                    asm volatile(
+                        "{\n\t.reg .pred q;\n\t.reg .b128 h;\n\t"
+                        "ld.shared.b128 h, [%2];\n\t"
+                        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 q, h;\n\t"
+                        "selp.u32 %0, 1, 0, q;\n\t"
+                        "mov.u32 %1, 0;\n\t"
+                        "@q clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n\t}"
+                        : "=r"(got), "=r"(x)
+                        : "r"(next_at)
+                        : "memory");
+            }
+            ok = __shfl_sync(0xffffffffu, (int)ok, 0);
+            if (!ok) break;
+            got = __shfl_sync(0xffffffffu, got, 0);
+            x = __shfl_sync(0xffffffffu, x, 0);
+            more = got && list.find(p, x, unit);  // the end goes through the list as a unit without rows
+        }
+        // given up: let this lane's last copy land before the shared memory is another's
+        if (*abort_flag && last_bar)
+            for (uint32_t i = 0; i < 4000000u && !mbar_try_wait(last_bar, last_parity); i++) {
+            }
+    } else if (warp == 9) {
+        // ---------------- products ----------------
+        if (lane == 0) {
+            constexpr uint32_t id_s = idesc_f16(BF, BM, 0), id_o = idesc_f16(BF, HD, 1);
+            uint32_t it = 0, taken[2] = {0, 0}, cs[2] = {0, 0};  // blocks loaded, tiles and blocks of each side
+            auto scores = [&](int s, uint32_t st) {
+                const uint32_t a = base + s * Ly::TILE, b = base + Ly::K_OFF + st * Ly::TILE;
+#pragma unroll
+                for (int kk = 0; kk < HD / 16; kk++)
+                    mma_ss(tmem + Ly::S + s * 128, desc_sw128(a + (kk / 4) * Ly::SLAB, 0) + 2 * (kk % 4),
+                           desc_sw128(b + (kk / 4) * Ly::SLAB, 0) + 2 * (kk % 4), id_s, kk > 0);
+                mma_commit(s_full(s));
+            };
+            for (uint32_t n = 0;; n++) {
+                const int slot = n % kSlots;
+                if (!wait(u_full(slot), (n / kSlots) & 1)) break;
+                Unit u;
+                take(slot, u);
+                mbar_arrive(u_empty(slot));
+                if (u.len == 0) break;
+                const int nb = u.blocks();
+                const int ns[2] = {u.blocks(0), u.blocks(1)};
+                bool ok = true;
+                // block 0's scores of both tiles
+                ok = wait(k_full(it % ST), (it / ST) & 1);
+                for (int s = 0; s < 2 && ok; s++) {
+                    if (!ns[s]) continue;
+                    ok = wait(q_full(s), taken[s] & 1);
+                    if (Ly::OWN_P) ok = ok && wait(s_free(s), (cs[s] & 1) ^ 1);
+                    if (!ok) break;
+                    tc_fence_after();
+                    scores(s, it % ST);
+                    if (ns[s] == 1) mma_commit(q_empty(s));
+                }
+                if (!ok) break;
+                mma_commit(k_empty(it % ST));
+                for (int j = 0; j < nb && ok; j++) {
+                    const uint32_t i = it + j, st = i % ST, nx = (i + 1) % ST;
+                    if (j + 1 < nb) ok = wait(k_full(nx), ((i + 1) / ST) & 1);
+                    if (Ly::OWN_P && j + 1 < nb) {
+                        for (int s = 0; s < 2 && ok; s++) {
+                            if (j + 1 >= ns[s]) continue;
+                            ok = wait(s_free(s), (cs[s] + j) & 1);
+                            if (!ok) break;
+                            tc_fence_after();
+                            scores(s, nx);
+                            if (j + 2 == ns[s]) mma_commit(q_empty(s));
+                        }
+                        if (ok) mma_commit(k_empty(nx));
+                    }
+                    ok = ok && wait(v_good(st), (i / ST) & 1);
+                    for (int s = 0; s < 2 && ok; s++) {
+                        if (j >= ns[s]) continue;
+                        if (j == 0) ok = wait(o_free(s), (taken[s] & 1) ^ 1);
+                        ok = ok && wait(p_full(s), (cs[s] + j) & 1);
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint32_t b = base + Ly::V_OFF + st * Ly::TILE;
+#pragma unroll
+                        for (int kk = 0; kk < BM / 16; kk++)
+                            mma_ts(tmem + Ly::O + s * HD, tmem + Ly::P + s * Ly::P_STEP + 8 * kk,
+                                   desc_sw128(b, Ly::SLAB) + 128 * kk, id_o, j > 0 || kk > 0);
+                        mma_commit(o_full(s));
+                        if (!Ly::OWN_P && j + 1 < ns[s]) {  // the scores go where P was, in issue order
+                            scores(s, nx);
+                            if (j + 2 == ns[s]) mma_commit(q_empty(s));
+                        }
+                    }
+                    if (!ok) break;
+                    mma_commit(v_empty(st));
+                    if (!Ly::OWN_P && j + 1 < nb) mma_commit(k_empty(nx));
+                }
+                if (!ok) break;
+                it += nb;
+                for (int s = 0; s < 2; s++) taken[s] += ns[s] > 0, cs[s] += ns[s];
+            }
+        }
+        __syncwarp();
+    } else if (warp == 10) {
+        // ---------------- V blocks on the diagonal ----------------
+        uint32_t it = 0;
+        bool ok = true;
+        for (uint32_t n = 0; ok; n++) {
+            const int slot = n % kSlots;
+            ok = __all_sync(0xffffffffu, wait(u_full(slot), (n / kSlots) & 1));
+            if (!ok) break;
+            Unit u;
+            take(slot, u);
+            if (u.len == 0) break;
+            const int nb = u.blocks();
+            bool bad = false;
+            for (int j = 0; j < nb; j++) {
+                const uint32_t i = it + j, st = i % ST;
+                ok = __all_sync(0xffffffffu, wait(v_full(st), (i / ST) & 1));
+                if (!ok) break;
+                if (j == u.tile[0] || j == u.tile[1]) {
+                    const int rows = min(BM, u.len - j * BM);
+                    constexpr uint32_t EXP = BF ? 0x7f807f80u : 0x7c007c00u, ONE = BF ? 0x00800080u : 0x04000400u;
+                    uint4* tile = reinterpret_cast<uint4*>(smem + Ly::V_OFF + st * Ly::TILE);
+                    uint32_t seen = 0;
+#pragma unroll 8
+                    for (int x = lane; x < Ly::TILE / 16; x += 32) {
+                        if ((x >> 3) % BM < rows) {  // 8 vectors a row, BM rows a slab
+                            const uint4 w = tile[x];
+                            // an all-ones exponent carries into the sign's place
+                            seen |= ((w.x & EXP) + ONE) | ((w.y & EXP) + ONE) | ((w.z & EXP) + ONE) | ((w.w & EXP) + ONE);
+                        } else {
+                            tile[x] = make_uint4(0, 0, 0, 0);
+                        }
+                    }
+                    bad |= (seen & 0x80008000u) != 0;
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                }
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(v_good(st));
+                    mbar_arrive(v_empty(st));
+                }
+            }
+            if (!ok) break;
+            bad = __any_sync(0xffffffffu, bad);
+            if (lane == 0) {
+                if (bad) units[slot].bad = 1;
+                mbar_arrive(u_seen(slot));
+                mbar_arrive(u_empty(slot));
+            }
+            it += nb;
+        }
+    } else {
+        // ---------------- softmax, output ----------------
+        const int s = warp >> 2, row = threadIdx.x & 127;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t ts = tmem + lanes + Ly::S + s * 128, tp = tmem + lanes + Ly::P + s * Ly::P_STEP,
+                       to = tmem + lanes + Ly::O + s * HD;
+        const float c = p.scale * 1.4426950408889634f;  // log2 e
+        uint32_t cs = 0;
+        for (uint32_t n = 0;; n++) {
+            const int slot = n % kSlots;
+            if (!__all_sync(0xffffffffu, wait(u_full(slot), (n / kSlots) & 1))) break;
+            Unit u;
+            take(slot, u);
+            if (u.len == 0) break;
+            const int nb = u.blocks(s);
+            float m = -INFINITY, mc = 0.0f, l = 0.0f;
+            bool ok = true;
+            for (int j = 0; j < nb; j++) {
+                ok = __all_sync(0xffffffffu, wait(s_full(s), (cs + j) & 1));
+                if (!ok) break;
+                tc_fence_after();
+                uint32_t r[128];
+#pragma unroll
+                for (int q = 0; q < 4; q++) tmem_ld32(ts + 32 * q, r + 32 * q);
+                tmem_wait_ld();
+                if (Ly::OWN_P) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(s_free(s));
+                }
+                if (j == nb - 1) {  // the diagonal
+#pragma unroll
+                    for (int q = 0; q < 128; q++)
+                        if (q > row) r[q] = 0xff800000u;
+                }
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int q = 0; q < 128; q += 8)
+#pragma unroll
+                    for (int w = 0; w < 4; w++)
+                        mx[w] = fmaxf(fmaxf(mx[w], __uint_as_float(r[q + w])), __uint_as_float(r[q + 4 + w]));
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                const bool rise = (top - m) * c > 8.0f;  // always true of the first block that has a score
+                if (__any_sync(0xffffffffu, rise)) {
+                    const float old = m;
+                    if (rise) m = top;
+                    mc = m == -INFINITY ? 0.0f : m * c;
+                    const float f = rise ? ex2((old - m) * c) : 1.0f;
+                    l *= f;
+                    if (j > 0) {
+                        ok = __all_sync(0xffffffffu, wait(o_full(s), (cs + j - 1) & 1));
+                        if (!ok) break;
+                        tc_fence_after();
+#pragma unroll
+                        for (int q = 0; q < HD / 32; q++) {
+                            uint32_t o[32];
+                            tmem_ld32(to + 32 * q, o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int w = 0; w < 32; w++) o[w] = __float_as_uint(__uint_as_float(o[w]) * f);
+                            tmem_st32(to + 32 * q, o);
+                        }
+                        tmem_wait_st();
+                        tc_fence_before();
+                    }
+                }
+                float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+                const float2 cc = make_float2(c, c), off = make_float2(-mc, -mc);
+                uint32_t pk[64];
+#pragma unroll
+                for (int q = 0; q < 128; q += 2) {
+                    float2 x = fma2(make_float2(__uint_as_float(r[q]), __uint_as_float(r[q + 1])), cc, off);
+                    x.x = ex2(x.x);
+                    x.y = ex2(x.y);
+                    sum[(q >> 1) & 1] = add2(sum[(q >> 1) & 1], x);
+                    pk[q >> 1] = pack2<T>(x.x, x.y);
+                }
+                l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+                if (Ly::OWN_P && j > 0) {  // P's columns are free once the product before is done
+                    ok = __all_sync(0xffffffffu, wait(o_full(s), (cs + j - 1) & 1));
+                    if (!ok) break;
+                    tc_fence_after();
+                }
+                tmem_st32(tp, pk);
+                tmem_st32(tp + 32, pk + 32);
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_full(s));
+            }
+            if (!ok) break;
+            if (!__all_sync(0xffffffffu, wait(u_seen(slot), (n / kSlots) & 1))) break;
+            const int bad = units[slot].bad;
+            if (nb) {
+                if (!__all_sync(0xffffffffu, wait(o_full(s), (cs + nb - 1) & 1))) break;
+                tc_fence_after();
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                const int i = u.tile[s] * BM + row;
+                T* to_row = static_cast<T*>(p.out) + ((int64_t)u.first + i) * p.out_stride + u.head[s] * HD;
+#pragma unroll
+                for (int q = 0; q < HD / 32; q++) {
+                    uint32_t o[32];
+                    tmem_ld32(to + 32 * q, o);
+                    tmem_wait_ld();
+                    if (i < u.len && !bad) {
+#pragma unroll
+                        for (int w = 0; w < 32; w += 8)
+                            *reinterpret_cast<uint4*>(to_row + 32 * q + w) =
+                                make_uint4(pack2<T>(__uint_as_float(o[w]) * inv, __uint_as_float(o[w + 1]) * inv),
+                                           pack2<T>(__uint_as_float(o[w + 2]) * inv, __uint_as_float(o[w + 3]) * inv),
+                                           pack2<T>(__uint_as_float(o[w + 4]) * inv, __uint_as_float(o[w + 5]) * inv),
+                                           pack2<T>(__uint_as_float(o[w + 6]) * inv, __uint_as_float(o[w + 7]) * inv));
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(o_free(s));
+                if (bad)
+                    for (int w = 0; w < 32; w++) {
+                        const int at = u.tile[s] * BM + (warp & 3) * 32 + w;
+                        if (at < u.len) plain_row<T, HD>(p, u.first, at, u.head[s], u.g);
+                    }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(u_empty(slot));
+            cs += nb;
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 9) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+pf_status get_encode(EncodeTiled* fn) {
+    static std::mutex mu;
+    static EncodeTiled cached = nullptr;
+    std::lock_guard<std::mutex> lk(mu);
+    if (!cached) {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        PF_CUDA(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q));
+        PF_CHECK(f && q == cudaDriverEntryPointSuccess, "cuTensorMapEncodeTiled unavailable");
+        cached = reinterpret_cast<EncodeTiled>(f);
+    }
+    *fn = cached;
+    return PF_OK;
+}
+
+// Boxes of 64 columns x 128 rows of 16-bit values; rows past the end read as zeros.
+pf_status make_map(CUtensorMap* map, const void* at, int64_t width, int64_t rows, int64_t stride) {
+    EncodeTiled enc;
+    PF_TRY(get_encode(&enc));
+    const cuuint64_t dims[2] = {(cuuint64_t)width, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)stride * 2};
+    const cuuint32_t box[2] = {64, BM}, estr[2] = {1, 1};
+    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(at), dims, strides, box, estr,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    PF_CHECK(r == CUDA_SUCCESS, "pf_prompt_attention: cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return PF_OK;
+}
+
+template <typename T, int HD>
+pf_status launch_prompt(const PromptParams& p, cudaStream_t st) {
+    using Ly = Layout<HD>;
+    CUtensorMap mq, mk, mv;
+    PF_TRY(make_map(&mq, p.q, (int64_t)p.n_heads * HD, p.n_tokens, p.q_stride));
+    PF_TRY(make_map(&mk, p.k, (int64_t)p.n_kv_heads * HD, p.n_tokens, p.k_stride));
+    PF_TRY(make_map(&mv, p.v, (int64_t)p.n_kv_heads * HD, p.n_tokens, p.v_stride));
+    // row tiles: sum ceil(len / 128) <= (sum len + 127 n_seqs) / 128, and half a pair more a sequence if the group is odd
+    const int64_t group = p.n_heads / p.n_kv_heads, tiles = ((int64_t)p.n_tokens + 127 * (int64_t)p.n_seqs) / BM;
+    const int64_t units = p.n_kv_heads * ((tiles * group + (group % 2 ? p.n_seqs : 0)) / 2);
+    PF_CHECK(units <= INT32_MAX, "pf_prompt_attention: too many row tiles");
+    if (units == 0) return PF_OK;  // not one sequence can hold a row
+    static std::atomic<uint64_t> attr{0};
+    PF_TRY(raise_smem_limit(prompt_kernel<T, HD>, Ly::SMEM, attr));
+    prompt_kernel<T, HD><<<(unsigned)units, kThreads, Ly::SMEM, st>>>(mq, mk, mv, p);
     return launch_check("prompt_attention");
 }
 
@@ -86,11 +800,15 @@ extern "C" pf_status pf_prompt_attention(const void* q, int64_t q_stride, const 
     PF_CHECK(((q_stride | k_stride | v_stride | out_stride) % 8) == 0 &&
                  (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) % 16) == 0,
              "pf_prompt_attention: pointers and strides must be multiples of 16 bytes");
+    PF_CHECK(std::max(std::max(q_stride, out_stride), std::max(k_stride, v_stride)) < (int64_t)1 << 38,
+             "pf_prompt_attention: a stride is too large");  // a tensor map's strides end at 2^40 bytes
     PF_TRY(require_device());
     if (n_seqs == 0 || n_tokens == 0) return PF_OK;
     PF_CHECK(q && k && v && out && offsets, "pf_prompt_attention: null argument");
-    PromptParams p{q, k, v, out, q_stride, k_stride, v_stride, out_stride, offsets, n_seqs, n_tokens, n_heads,
-                   n_kv_heads, scale, device_error_flag()};
-    return dtype == PF_BF16 ? launch_prompt<__nv_bfloat16>(p, head_dim, as_stream(stream))
-                            : launch_prompt<__half>(p, head_dim, as_stream(stream));
+    const PromptParams p{q, k, v, out, q_stride, k_stride, v_stride, out_stride, offsets, n_seqs, n_tokens, n_heads,
+                         n_kv_heads, scale, device_error_flag()};
+    cudaStream_t st = as_stream(stream);
+    if (dtype == PF_BF16)
+        return head_dim == 64 ? launch_prompt<__nv_bfloat16, 64>(p, st) : launch_prompt<__nv_bfloat16, 128>(p, st);
+    return head_dim == 64 ? launch_prompt<__half, 64>(p, st) : launch_prompt<__half, 128>(p, st);
 }
