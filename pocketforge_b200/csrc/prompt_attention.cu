@@ -47,7 +47,12 @@ namespace {
 
 constexpr int BM = 128;            // query rows a tile, keys a block
 constexpr int kSoftmaxWarps = 8;
-constexpr int kThreads = 352;      // 11 warps: 65,536 registers allow 184 a thread
+constexpr int kThreads = 384;      // three warpgroups, the last warp idle
+// Registers: the launch gives every thread 168 (64,512 in all).  The softmax
+// warpgroups hold a row of 128 scores and take 208 once the third one has gone
+// down to 88: 2 x 128 x 208 + 128 x 88 = 64,512.
+constexpr int kRegsSoftmax = 208, kRegsOther = 88;
+static_assert(2 * 128 * kRegsSoftmax + 128 * kRegsOther <= 384 * 168, "register split");
 constexpr uint32_t ERR_TIMEOUT = 16u;
 constexpr int kSlots = 2;          // units in the list between the load warp and the others
 
@@ -67,12 +72,16 @@ struct Layout {
     static constexpr int SLAB = BM * 128;             // bytes of one
     static constexpr int TILE = NC * SLAB;            // a Q tile, K block or V block
     static constexpr int STAGES = HD == 64 ? 4 : 2;   // K blocks and V blocks in flight
-    static constexpr int K_OFF = 2 * TILE, V_OFF = K_OFF + STAGES * TILE, BAR_OFF = V_OFF + STAGES * TILE;
+    static constexpr int K_OFF = 2 * TILE, V_OFF = K_OFF + STAGES * TILE;
+    static constexpr int OUT_OFF = V_OFF + STAGES * TILE;  // 32 rows x 128 bytes of output a softmax warp
+    static constexpr int BAR_OFF = OUT_OFF + kSoftmaxWarps * 32 * 128;
     static constexpr int SMEM = BAR_OFF + 512 + 1024;  // barriers, unit list; alignment
     // TMEM columns.  head_dim 64: P has its own columns, so the next scores are
     // computed while this block's are exponentiated; at 128 the accumulators
     // take that room and P overlays the scores it came from.
     static constexpr bool OWN_P = HD == 64;
+    // Of 16 exponentials, so many on the FMA pipe (exp2_fma).
+    static constexpr int ON_FMA = HD == 64 ? 6 : 4;
     static constexpr uint32_t S = 0, P = OWN_P ? 256 : 0, P_STEP = OWN_P ? 64 : 128, O = OWN_P ? 384 : 256;
 };
 
@@ -98,25 +107,23 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
-// False when a second has passed, or another role has given up.
-__device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint32_t* err) {
+// False when a second has passed, or another role has given up.  Inline: a call
+// would spill the row of scores that a softmax thread holds.
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint32_t* err) {
+    if (mbar_try_wait(bar, parity)) return true;
     uint64_t t0, t;
     asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t0));
-    for (uint32_t i = 0;; i++) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if ((i & 63u) == 63u) {
-            if (*abort_flag) return false;
-            asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
-            if (t - t0 > 1000000000ull) {
-                *abort_flag = 1;
-                latch(err, ERR_TIMEOUT);
-                return false;
-            }
+#pragma unroll 1
+    while (!mbar_try_wait(bar, parity)) {
+        if (*abort_flag) return false;
+        asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+        if (t - t0 > 1000000000ull) {
+            *abort_flag = 1;
+            latch(err, ERR_TIMEOUT);
+            return false;
         }
     }
-}
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint32_t* err) {
-    return mbar_try_wait(bar, parity) || mbar_wait_slow(bar, parity, abort_flag, err);
+    return true;
 }
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
     asm volatile(
@@ -149,6 +156,12 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc)
         : "memory");
 }
+// One lane of a warp that is all here.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok));
+    return ok != 0;
+}
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
@@ -167,14 +180,19 @@ __device__ __forceinline__ void tmem_ld32(uint32_t a, uint32_t* r) {
         : "r"(a)
         : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t a, const uint32_t* r) {
+__device__ __forceinline__ void tmem_ld16(uint32_t a, uint32_t* r) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
-        "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(a),
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(a)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t a, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(a),
         "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
 __device__ __forceinline__ float ex2(float x) {
@@ -196,6 +214,37 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
         : "=l"(reinterpret_cast<uint64_t&>(d))
         : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
     return d;
+}
+// 2^x of two values on the FMA pipe, for the share of the exponentials that the
+// special-function unit (16 a clock and SM, a third of what the two tiles ask
+// for) would hold up: x = n + f with n = round(x) read off the low bits of
+// x + 1.5 * 2^23, 2^f on [-1/2, 1/2] by the polynomial of least largest relative
+// error (found by exchange of its extrema; degree 3: 7.5e-5, for bf16 rounded
+// to 2^-9; degree 4: 2.7e-6, for fp16 rounded to 2^-12), n added to the
+// exponent.  x <= 8; below -125 it is taken as -125 (2^-125 in place of less).
+template <int DEGREE>
+__device__ __forceinline__ float2 exp2_fma(float2 x) {
+    x.x = fmaxf(x.x, -125.0f);
+    x.y = fmaxf(x.y, -125.0f);
+    const float2 magic = make_float2(12582912.0f, 12582912.0f), less = make_float2(-12582912.0f, -12582912.0f);
+    const float2 one = make_float2(-1.0f, -1.0f);
+    const float2 t = add2(x, magic);
+    const float2 f = fma2(add2(t, less), one, x);
+    auto both = [](float v) { return make_float2(v, v); };
+    float2 y;
+    if constexpr (DEGREE == 3) {
+        y = fma2(f, both(0.0551716685295105f), both(0.2426111251115799f));
+        y = fma2(f, y, both(0.6932609677314758f));
+        y = fma2(f, y, both(0.9999280571937561f));
+    } else {
+        y = fma2(f, both(0.009570102207362652f), both(0.05591785907745361f));
+        y = fma2(f, y, both(0.240247443318367f));
+        y = fma2(f, y, both(0.6931217908859253f));
+        y = fma2(f, y, both(0.9999992847442627f));
+    }
+    y.x = __uint_as_float(__float_as_uint(y.x) + (__float_as_uint(t.x) << 23));
+    y.y = __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(t.y) << 23));
+    return y;
 }
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi);
@@ -219,50 +268,61 @@ struct Unit {
     int tile[2];      // row tile of query tile s, -1: none
     int head[2];
     int bad;          // an inf or NaN in a V block on the diagonal
-    __device__ int blocks(int s) const { return tile[s] + 1; }
     __device__ int blocks() const { return max(tile[0], tile[1]) + 1; }
 };
 
-// Walks the sequences to unit u; a whole warp, the same in every lane.
+// Walks the sequences to unit u; a whole warp, the same in every lane.  Each
+// lane keeps one sequence of a window of 32, so the offsets are read once a window.
 struct UnitList {
-    int seq = 0;           // first sequence of the window of 32 looked at
-    long long before = 0;  // units before it
+    int seq = 0;               // first sequence of the window
+    long long before = 0;      // units before it
+    long long first_unit = 0, end_unit = -1;  // this lane's sequence, from the window's beginning; -1: not read yet
+    int first = 0, len = 0, pairs = 0;
     __device__ bool find(const PromptParams& p, long long u, Unit& out) {
-        if (u < before) seq = 0, before = 0;
+        if (u < before) seq = 0, before = 0, end_unit = -1;
         const int lane = threadIdx.x & 31, group = p.n_heads / p.n_kv_heads;
-        for (; seq < p.n_seqs; seq += 32) {
-            int first = 0, len = 0;
-            if (seq + lane < p.n_seqs) {
-                first = p.offsets[seq + lane];
-                const int end = p.offsets[seq + lane + 1];
-                if (first >= 0 && end >= first && end <= p.n_tokens) len = end - first;
-                else latch(p.err, ERR_BOUNDS);
-            }
-            const long long pairs = ((long long)((len + BM - 1) / BM) * group + 1) / 2, mine = pairs * p.n_kv_heads;
-            long long upto = mine;
+        while (seq < p.n_seqs) {
+            if (end_unit < 0) {
+                first = len = 0;
+                if (seq + lane < p.n_seqs) {
+                    first = p.offsets[seq + lane];
+                    const int end = p.offsets[seq + lane + 1];
+                    if (first >= 0 && end >= first && end <= p.n_tokens) len = end - first;
+                    else latch(p.err, ERR_BOUNDS);
+                }
+                // a bad list's sequences may overlap: 64 bits, though a good one's units fit 31
+                const long long two = ((long long)((len + BM - 1) / BM) * group + 1) / 2;
+                pairs = (int)min(two, 0x7fffffffll);
+                end_unit = two * p.n_kv_heads;
+                first_unit = end_unit;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const long long x = __shfl_up_sync(0xffffffffu, upto, o);
-                if (lane >= o) upto += x;
+                for (int o = 1; o < 32; o <<= 1) {
+                    const long long x = __shfl_up_sync(0xffffffffu, end_unit, o);
+                    if (lane >= o) end_unit += x;
+                }
+                first_unit = end_unit - first_unit;
             }
-            const unsigned here = __ballot_sync(0xffffffffu, u < before + upto);
+            const unsigned here = __ballot_sync(0xffffffffu, u < before + end_unit);
             if (here) {
                 const int at = __ffs((int)here) - 1;
-                const long long r = u - (before + __shfl_sync(0xffffffffu, upto - mine, at));
+                const int r = (int)(u - before - __shfl_sync(0xffffffffu, first_unit, at));
                 out.first = __shfl_sync(0xffffffffu, first, at);
                 out.len = __shfl_sync(0xffffffffu, len, at);
-                const int pair = (int)(__shfl_sync(0xffffffffu, pairs, at) - 1 - r / p.n_kv_heads);
-                out.g = (int)(r % p.n_kv_heads);
+                const int pair = __shfl_sync(0xffffffffu, pairs, at) - 1 - r / p.n_kv_heads;
+                out.g = r % p.n_kv_heads;
                 const int tiles = (out.len + BM - 1) / BM;
+#pragma unroll
                 for (int s = 0; s < 2; s++) {
                     const int c = 2 * pair + s;  // (row tile, head of the group), heads fastest
-                    out.tile[s] = c < tiles * group ? c / group : -1;
-                    out.head[s] = out.g * group + c % group;
+                    const int t = c / group;
+                    out.tile[s] = t < tiles ? t : -1;
+                    out.head[s] = out.g * group + c - t * group;
                 }
-                out.bad = 0;
                 return true;
             }
-            before += __shfl_sync(0xffffffffu, upto, 31);
+            before += __shfl_sync(0xffffffffu, end_unit, 31);
+            seq += 32;
+            end_unit = -1;
         }
         return false;
     }
@@ -313,17 +373,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto u_full = [&](int i) { return bars + 8u * (14 + i); };
     auto u_empty = [&](int i) { return bars + 8u * (16 + i); };
     auto u_seen = [&](int i) { return bars + 8u * (18 + i); };  // the guard is through with the unit
-    const uint32_t next_full = bars + 8u * 20;
-    auto k_full = [&](int i) { return bars + 8u * (21 + i); };
-    auto k_empty = [&](int i) { return bars + 8u * (21 + ST + i); };
-    auto v_full = [&](int i) { return bars + 8u * (21 + 2 * ST + i); };
-    auto v_empty = [&](int i) { return bars + 8u * (21 + 3 * ST + i); };
-    auto v_good = [&](int i) { return bars + 8u * (21 + 4 * ST + i); };  // looked through
-    static_assert(8 * (21 + 5 * ST) <= 336, "barriers");
-    uint8_t* tail = smem + Ly::BAR_OFF + 336;
-    const uint32_t next_at = base + Ly::BAR_OFF + 336;              // 16 bytes: the next unit's launch
+    auto p_half = [&](int s) { return bars + 8u * (20 + s); };  // p of the block's first 64 keys
+    const uint32_t next_full = bars + 8u * 22;
+    auto k_full = [&](int i) { return bars + 8u * (23 + i); };
+    auto k_empty = [&](int i) { return bars + 8u * (23 + ST + i); };
+    auto v_full = [&](int i) { return bars + 8u * (23 + 2 * ST + i); };
+    auto v_empty = [&](int i) { return bars + 8u * (23 + 3 * ST + i); };
+    auto v_good = [&](int i) { return bars + 8u * (23 + 4 * ST + i); };  // looked through
+    static_assert(8 * (23 + 5 * ST) <= 352, "barriers");
+    uint8_t* tail = smem + Ly::BAR_OFF + 352;
+    const uint32_t next_at = base + Ly::BAR_OFF + 352;              // 16 bytes: the next unit's launch
     volatile Unit* units = reinterpret_cast<volatile Unit*>(tail + 16);  // [kSlots]
-    static_assert(16 + kSlots * sizeof(Unit) + 12 <= 176, "unit list");
+    static_assert(16 + kSlots * sizeof(Unit) + 12 <= 160, "unit list");
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tail + 16 + kSlots * sizeof(Unit));
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     int* any = reinterpret_cast<int*>(tmem_slot + 2);
@@ -340,6 +401,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 mbar_init(q_empty(s), 1);
                 mbar_init(s_full(s), 1);
                 mbar_init(s_free(s), 4);
+                mbar_init(p_half(s), 4);
                 mbar_init(p_full(s), 4);
                 mbar_init(o_full(s), 1);
                 mbar_init(o_free(s), 4);
@@ -379,6 +441,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         u.head[0] = v.head[0], u.head[1] = v.head[1];
     };
 
+    if (warp >= kSoftmaxWarps) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
     if (warp == 8) {
         // ---------------- unit list, loads ----------------
         // Lane roles: K slabs, V slabs, then Q tile 0's and 1's slabs.  Copies issued by one lane complete one
@@ -421,17 +485,19 @@ __global__ void __launch_bounds__(kThreads, 1)
                     tma_load_2d(tiles + st * Ly::TILE, map, unit.g * HD + c * 64, unit.first + j * BM, full);
                     last_bar = full, last_parity = (i / ST) & 1;
                 }
-            } else if (role < 4 && unit.tile[role - 2] >= 0) {
+            } else if (role < 4 && (role == 2 ? unit.tile[0] : unit.tile[1]) >= 0) {
                 const int s = role - 2;
-                ok = wait(q_empty(s), (taken[s] & 1) ^ 1);
+                const uint32_t use = s ? taken[1] : taken[0];
+                ok = wait(q_empty(s), (use & 1) ^ 1);
                 if (ok) {
                     mbar_expect_tx(q_full(s), Ly::SLAB);
-                    tma_load_2d(base + s * Ly::TILE + c * Ly::SLAB, &map_q, unit.head[s] * HD + c * 64,
-                                unit.first + unit.tile[s] * BM, q_full(s));
-                    last_bar = q_full(s), last_parity = taken[s] & 1;
+                    tma_load_2d(base + s * Ly::TILE + c * Ly::SLAB, &map_q, (s ? unit.head[1] : unit.head[0]) * HD + c * 64,
+                                unit.first + (s ? unit.tile[1] : unit.tile[0]) * BM, q_full(s));
+                    last_bar = q_full(s), last_parity = use & 1;
                 }
             }
             it += nb;
+#pragma unroll
             for (int s = 0; s < 2; s++) taken[s] += unit.tile[s] >= 0;
             if (!__all_sync(0xffffffffu, ok)) break;
             int got = 0;
@@ -462,71 +528,80 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
     } else if (warp == 9) {
         // ---------------- products ----------------
-        if (lane == 0) {
+        // One lane, chosen by elect.sync: the compiler then knows that the operands are the warp's only ones and takes
+        // them into uniform registers.  (Under `lane == 0` each product took about 120 cycles to issue, twice what it
+        // takes to execute.)
+        if (elect_one()) {
             constexpr uint32_t id_s = idesc_f16(BF, BM, 0), id_o = idesc_f16(BF, HD, 1);
             uint32_t it = 0, taken[2] = {0, 0}, cs[2] = {0, 0};  // blocks loaded, tiles and blocks of each side
-            auto scores = [&](int s, uint32_t st) {
-                const uint32_t a = base + s * Ly::TILE, b = base + Ly::K_OFF + st * Ly::TILE;
+            // S_s = Q_s K^T from stage st
+            auto scores = [&](int s, uint32_t st, bool last) {
+                const uint64_t a = desc_sw128(base + s * Ly::TILE, 0), b = desc_sw128(base + Ly::K_OFF + st * Ly::TILE, 0);
 #pragma unroll
                 for (int kk = 0; kk < HD / 16; kk++)
-                    mma_ss(tmem + Ly::S + s * 128, desc_sw128(a + (kk / 4) * Ly::SLAB, 0) + 2 * (kk % 4),
-                           desc_sw128(b + (kk / 4) * Ly::SLAB, 0) + 2 * (kk % 4), id_s, kk > 0);
+                    mma_ss(tmem + Ly::S + s * 128, a + (kk / 4) * (Ly::SLAB >> 4) + 2 * (kk % 4),
+                           b + (kk / 4) * (Ly::SLAB >> 4) + 2 * (kk % 4), id_s, kk > 0);
                 mma_commit(s_full(s));
+                if (last) mma_commit(q_empty(s));
+            };
+            // O_s += P_s V over half of the block's keys
+            auto values = [&](int s, uint32_t st, int half, bool first) {
+                const uint64_t b = desc_sw128(base + Ly::V_OFF + st * Ly::TILE, Ly::SLAB);
+#pragma unroll
+                for (int kk = 0; kk < BM / 32; kk++)
+                    mma_ts(tmem + Ly::O + s * HD, tmem + Ly::P + s * Ly::P_STEP + 32 * half + 8 * kk,
+                           b + 128 * (BM / 32 * half + kk), id_o, !first || kk > 0);
+                if (half) mma_commit(o_full(s));
             };
             for (uint32_t n = 0;; n++) {
                 const int slot = n % kSlots;
                 if (!wait(u_full(slot), (n / kSlots) & 1)) break;
-                Unit u;
-                take(slot, u);
+                const int len = units[slot].len;
+                const int ns[2] = {units[slot].tile[0] + 1, units[slot].tile[1] + 1};
                 mbar_arrive(u_empty(slot));
-                if (u.len == 0) break;
-                const int nb = u.blocks();
-                const int ns[2] = {u.blocks(0), u.blocks(1)};
-                bool ok = true;
+                if (len == 0) break;
+                const int nb = max(ns[0], ns[1]);
                 // block 0's scores of both tiles
-                ok = wait(k_full(it % ST), (it / ST) & 1);
-                for (int s = 0; s < 2 && ok; s++) {
-                    if (!ns[s]) continue;
+                bool ok = wait(k_full(it % ST), (it / ST) & 1);
+#pragma unroll
+                for (int s = 0; s < 2; s++) {
+                    if (!ok || !ns[s]) continue;
                     ok = wait(q_full(s), taken[s] & 1);
                     if (Ly::OWN_P) ok = ok && wait(s_free(s), (cs[s] & 1) ^ 1);
-                    if (!ok) break;
+                    if (!ok) continue;
                     tc_fence_after();
-                    scores(s, it % ST);
-                    if (ns[s] == 1) mma_commit(q_empty(s));
+                    scores(s, it % ST, ns[s] == 1);
                 }
                 if (!ok) break;
                 mma_commit(k_empty(it % ST));
-                for (int j = 0; j < nb && ok; j++) {
+                for (int j = 0; j < nb; j++) {
                     const uint32_t i = it + j, st = i % ST, nx = (i + 1) % ST;
                     if (j + 1 < nb) ok = wait(k_full(nx), ((i + 1) / ST) & 1);
                     if (Ly::OWN_P && j + 1 < nb) {
-                        for (int s = 0; s < 2 && ok; s++) {
-                            if (j + 1 >= ns[s]) continue;
+#pragma unroll
+                        for (int s = 0; s < 2; s++) {
+                            if (!ok || j + 1 >= ns[s]) continue;
                             ok = wait(s_free(s), (cs[s] + j) & 1);
-                            if (!ok) break;
+                            if (!ok) continue;
                             tc_fence_after();
-                            scores(s, nx);
-                            if (j + 2 == ns[s]) mma_commit(q_empty(s));
+                            scores(s, nx, j + 2 == ns[s]);
                         }
                         if (ok) mma_commit(k_empty(nx));
                     }
                     ok = ok && wait(v_good(st), (i / ST) & 1);
-                    for (int s = 0; s < 2 && ok; s++) {
-                        if (j >= ns[s]) continue;
-                        if (j == 0) ok = wait(o_free(s), (taken[s] & 1) ^ 1);
-                        ok = ok && wait(p_full(s), (cs[s] + j) & 1);
-                        if (!ok) break;
-                        tc_fence_after();
-                        const uint32_t b = base + Ly::V_OFF + st * Ly::TILE;
 #pragma unroll
-                        for (int kk = 0; kk < BM / 16; kk++)
-                            mma_ts(tmem + Ly::O + s * HD, tmem + Ly::P + s * Ly::P_STEP + 8 * kk,
-                                   desc_sw128(b, Ly::SLAB) + 128 * kk, id_o, j > 0 || kk > 0);
-                        mma_commit(o_full(s));
-                        if (!Ly::OWN_P && j + 1 < ns[s]) {  // the scores go where P was, in issue order
-                            scores(s, nx);
-                            if (j + 2 == ns[s]) mma_commit(q_empty(s));
-                        }
+                    for (int s = 0; s < 2; s++) {
+                        if (!ok || j >= ns[s]) continue;
+                        if (j == 0) ok = wait(o_free(s), (taken[s] & 1) ^ 1);
+                        ok = ok && wait(p_half(s), (cs[s] + j) & 1);
+                        if (!ok) continue;
+                        tc_fence_after();
+                        values(s, st, 0, j == 0);
+                        ok = wait(p_full(s), (cs[s] + j) & 1);
+                        if (!ok) continue;
+                        tc_fence_after();
+                        values(s, st, 1, false);
+                        if (!Ly::OWN_P && j + 1 < ns[s]) scores(s, nx, j + 2 == ns[s]);  // over P, in issue order
                     }
                     if (!ok) break;
                     mma_commit(v_empty(st));
@@ -534,6 +609,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 if (!ok) break;
                 it += nb;
+#pragma unroll
                 for (int s = 0; s < 2; s++) taken[s] += ns[s] > 0, cs[s] += ns[s];
             }
         }
@@ -588,8 +664,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             it += nb;
         }
+    }
     } else {
         // ---------------- softmax, output ----------------
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
         const int s = warp >> 2, row = threadIdx.x & 127;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t ts = tmem + lanes + Ly::S + s * 128, tp = tmem + lanes + Ly::P + s * Ly::P_STEP,
@@ -602,7 +680,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             Unit u;
             take(slot, u);
             if (u.len == 0) break;
-            const int nb = u.blocks(s);
+            const int tile = s ? u.tile[1] : u.tile[0], head = s ? u.head[1] : u.head[0], nb = tile + 1;
             float m = -INFINITY, mc = 0.0f, l = 0.0f;
             bool ok = true;
             for (int j = 0; j < nb; j++) {
@@ -618,18 +696,26 @@ __global__ void __launch_bounds__(kThreads, 1)
                     __syncwarp();
                     if (lane == 0) mbar_arrive(s_free(s));
                 }
-                if (j == nb - 1) {  // the diagonal
+                // On the diagonal a warp's rows see no key behind its own 32: it works on its first `parts` quarters only.
+                const bool diagonal = j == nb - 1;
+                const int parts = diagonal ? (warp & 3) + 1 : 4;
+                if (diagonal) {
 #pragma unroll
                     for (int q = 0; q < 128; q++)
                         if (q > row) r[q] = 0xff800000u;
                 }
-                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                float top = -INFINITY;
 #pragma unroll
-                for (int q = 0; q < 128; q += 8)
+                for (int h = 0; h < 4; h++) {
+                    if (h >= parts) break;
+                    float mx[4] = {top, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int w = 0; w < 4; w++)
-                        mx[w] = fmaxf(fmaxf(mx[w], __uint_as_float(r[q + w])), __uint_as_float(r[q + 4 + w]));
-                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                    for (int q = 32 * h; q < 32 * h + 32; q += 8)
+#pragma unroll
+                        for (int w = 0; w < 4; w++)
+                            mx[w] = fmaxf(fmaxf(mx[w], __uint_as_float(r[q + w])), __uint_as_float(r[q + 4 + w]));
+                    top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                }
                 const bool rise = (top - m) * c > 8.0f;  // always true of the first block that has a score
                 if (__any_sync(0xffffffffu, rise)) {
                     const float old = m;
@@ -642,41 +728,59 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (!ok) break;
                         tc_fence_after();
 #pragma unroll
-                        for (int q = 0; q < HD / 32; q++) {
-                            uint32_t o[32];
-                            tmem_ld32(to + 32 * q, o);
+                        for (int q = 0; q < HD / 16; q++) {
+                            uint32_t o[16];
+                            tmem_ld16(to + 16 * q, o);
                             tmem_wait_ld();
 #pragma unroll
-                            for (int w = 0; w < 32; w++) o[w] = __float_as_uint(__uint_as_float(o[w]) * f);
-                            tmem_st32(to + 32 * q, o);
+                            for (int w = 0; w < 16; w++) o[w] = __float_as_uint(__uint_as_float(o[w]) * f);
+                            tmem_st16(to + 16 * q, o);
                         }
-                        tmem_wait_st();
-                        tc_fence_before();
                     }
                 }
-                float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-                const float2 cc = make_float2(c, c), off = make_float2(-mc, -mc);
-                uint32_t pk[64];
-#pragma unroll
-                for (int q = 0; q < 128; q += 2) {
-                    float2 x = fma2(make_float2(__uint_as_float(r[q]), __uint_as_float(r[q + 1])), cc, off);
-                    x.x = ex2(x.x);
-                    x.y = ex2(x.y);
-                    sum[(q >> 1) & 1] = add2(sum[(q >> 1) & 1], x);
-                    pk[q >> 1] = pack2<T>(x.x, x.y);
-                }
-                l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 if (Ly::OWN_P && j > 0) {  // P's columns are free once the product before is done
                     ok = __all_sync(0xffffffffu, wait(o_full(s), (cs + j - 1) & 1));
                     if (!ok) break;
                     tc_fence_after();
                 }
-                tmem_st32(tp, pk);
-                tmem_st32(tp + 32, pk + 32);
-                tmem_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(p_full(s));
+                float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+                const float2 cc = make_float2(c, c), off = make_float2(-mc, -mc);
+#pragma unroll
+                for (int h = 0; h < 4; h++) {
+                    uint32_t pk[16];
+                    if (!diagonal) {
+#pragma unroll
+                        for (int q = 0; q < 16; q++) {
+                            const float2 x = fma2(make_float2(__uint_as_float(r[32 * h + 2 * q]),
+                                                              __uint_as_float(r[32 * h + 2 * q + 1])), cc, off);
+                            // spread evenly: q in steps of 16 / ON_FMA
+                            const bool fma = (q + 1) * Ly::ON_FMA / 16 > q * Ly::ON_FMA / 16;
+                            const float2 y = fma ? exp2_fma<BF ? 3 : 4>(x) : make_float2(ex2(x.x), ex2(x.y));
+                            sum[q & 1] = add2(sum[q & 1], y);
+                            pk[q] = pack2<T>(y.x, y.y);
+                        }
+                    } else if (h < parts) {  // a masked score's p is 0 to the last bit here
+#pragma unroll
+                        for (int q = 0; q < 16; q++) {
+                            const float2 x = fma2(make_float2(__uint_as_float(r[32 * h + 2 * q]),
+                                                              __uint_as_float(r[32 * h + 2 * q + 1])), cc, off);
+                            const float2 y = make_float2(ex2(x.x), ex2(x.y));
+                            sum[q & 1] = add2(sum[q & 1], y);
+                            pk[q] = pack2<T>(y.x, y.y);
+                        }
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < 16; q++) pk[q] = 0;
+                    }
+                    tmem_st16(tp + 16 * h, pk);
+                    if (h & 1) {
+                        tmem_wait_st();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(h == 1 ? p_half(s) : p_full(s));
+                    }
+                }
+                l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
             }
             if (!ok) break;
             if (!__all_sync(0xffffffffu, wait(u_seen(slot), (n / kSlots) & 1))) break;
@@ -685,30 +789,42 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!__all_sync(0xffffffffu, wait(o_full(s), (cs + nb - 1) & 1))) break;
                 tc_fence_after();
                 const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-                const int i = u.tile[s] * BM + row;
-                T* to_row = static_cast<T*>(p.out) + ((int64_t)u.first + i) * p.out_stride + u.head[s] * HD;
+                const int i = tile * BM + row;
+                const int rows = bad ? 0 : min(32, u.len - (i - lane));  // of this warp's 32
+                T* to_row = static_cast<T*>(p.out) + ((int64_t)u.first + i - lane) * p.out_stride + head * HD;
+                uint4* stage = reinterpret_cast<uint4*>(smem + Ly::OUT_OFF + warp * 4096);
 #pragma unroll
-                for (int q = 0; q < HD / 32; q++) {
-                    uint32_t o[32];
-                    tmem_ld32(to + 32 * q, o);
+                for (int q = 0; q < HD / 64; q++) {
+                    uint32_t o[64];
+                    tmem_ld32(to + 64 * q, o);
+                    tmem_ld32(to + 64 * q + 32, o + 32);
                     tmem_wait_ld();
-                    if (i < u.len && !bad) {
+                    // a row's 128 bytes by its own thread, chunks permuted by the row against bank conflicts; then
+                    // eight lanes store one row
 #pragma unroll
-                        for (int w = 0; w < 32; w += 8)
-                            *reinterpret_cast<uint4*>(to_row + 32 * q + w) =
-                                make_uint4(pack2<T>(__uint_as_float(o[w]) * inv, __uint_as_float(o[w + 1]) * inv),
-                                           pack2<T>(__uint_as_float(o[w + 2]) * inv, __uint_as_float(o[w + 3]) * inv),
-                                           pack2<T>(__uint_as_float(o[w + 4]) * inv, __uint_as_float(o[w + 5]) * inv),
-                                           pack2<T>(__uint_as_float(o[w + 6]) * inv, __uint_as_float(o[w + 7]) * inv));
+                    for (int w = 0; w < 8; w++)
+                        stage[lane * 8 + (w ^ (lane & 7))] =
+                            make_uint4(pack2<T>(__uint_as_float(o[8 * w]) * inv, __uint_as_float(o[8 * w + 1]) * inv),
+                                       pack2<T>(__uint_as_float(o[8 * w + 2]) * inv, __uint_as_float(o[8 * w + 3]) * inv),
+                                       pack2<T>(__uint_as_float(o[8 * w + 4]) * inv, __uint_as_float(o[8 * w + 5]) * inv),
+                                       pack2<T>(__uint_as_float(o[8 * w + 6]) * inv, __uint_as_float(o[8 * w + 7]) * inv));
+                    __syncwarp();
+#pragma unroll
+                    for (int w = 0; w < 8; w++) {
+                        const int to_r = 4 * w + (lane >> 3);
+                        if (to_r < rows)
+                            *reinterpret_cast<uint4*>(to_row + to_r * p.out_stride + 64 * q + 8 * (lane & 7)) =
+                                stage[to_r * 8 + ((lane & 7) ^ (to_r & 7))];
                     }
+                    __syncwarp();
                 }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(o_free(s));
                 if (bad)
                     for (int w = 0; w < 32; w++) {
-                        const int at = u.tile[s] * BM + (warp & 3) * 32 + w;
-                        if (at < u.len) plain_row<T, HD>(p, u.first, at, u.head[s], u.g);
+                        const int at = tile * BM + (warp & 3) * 32 + w;
+                        if (at < u.len) plain_row<T, HD>(p, u.first, at, head, u.g);
                     }
             }
             __syncwarp();
