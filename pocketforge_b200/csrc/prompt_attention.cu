@@ -49,9 +49,9 @@ constexpr int BM = 128;            // query rows a tile, keys a block
 constexpr int kSoftmaxWarps = 8;
 constexpr int kThreads = 384;      // three warpgroups, the last warp idle
 // Registers: the launch gives every thread 168 (64,512 in all).  The softmax
-// warpgroups hold a row of 128 scores and take 208 once the third one has gone
-// down to 88: 2 x 128 x 208 + 128 x 88 = 64,512.
-constexpr int kRegsSoftmax = 208, kRegsOther = 88;
+// warpgroups hold a row of 128 scores and take 200 once the third one has gone
+// down to 104: 2 x 128 x 200 + 128 x 104 = 64,512.
+constexpr int kRegsSoftmax = 200, kRegsOther = 104;
 static_assert(2 * 128 * kRegsSoftmax + 128 * kRegsOther <= 384 * 168, "register split");
 constexpr uint32_t ERR_TIMEOUT = 16u;
 constexpr int kSlots = 2;          // units in the list between the load warp and the others
@@ -61,7 +61,7 @@ struct PromptParams {
     void* out;
     int64_t q_stride, k_stride, v_stride, out_stride;
     const int* offsets;
-    int n_seqs, n_tokens, n_heads, n_kv_heads;
+    int n_seqs, n_tokens, n_heads, n_kv_heads, group;  // group = n_heads / n_kv_heads
     float scale;
     uint32_t* err;
 };
@@ -80,8 +80,6 @@ struct Layout {
     // computed while this block's are exponentiated; at 128 the accumulators
     // take that room and P overlays the scores it came from.
     static constexpr bool OWN_P = HD == 64;
-    // Of 16 exponentials, so many on the FMA pipe (exp2_fma).
-    static constexpr int ON_FMA = HD == 64 ? 6 : 4;
     static constexpr uint32_t S = 0, P = OWN_P ? 256 : 0, P_STEP = OWN_P ? 64 : 128, O = OWN_P ? 384 : 256;
 };
 
@@ -93,37 +91,41 @@ __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+// Predicated, not branched around: the code on both sides stays one block to schedule.
+__device__ __forceinline__ void mbar_arrive_if(uint32_t bar, bool on) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %1, 0;\n\t@p mbarrier.arrive.shared::cta.b64 _, [%0];\n\t}" ::"r"(bar),
+        "r"((int)on)
+        : "memory");
+}
 __device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
+// Sleeps in hardware for up to the hint's 10 ms (a short default would have the waiting warps poll the issue slots away).
 __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(ok)
-        : "r"(bar), "r"(parity)
+        : "r"(bar), "r"(parity), "r"(10000000u)
         : "memory");
     return ok != 0;
 }
-// False when a second has passed, or another role has given up.  Inline: a call
-// would spill the row of scores that a softmax thread holds.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint32_t* err) {
-    if (mbar_try_wait(bar, parity)) return true;
+// False when a second has passed, or another role has given up.
+__device__ __forceinline__ bool mbar_spin(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
     uint64_t t0, t;
     asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t0));
 #pragma unroll 1
-    while (!mbar_try_wait(bar, parity)) {
-        if (*abort_flag) return false;
+    do {
+        if (mbar_try_wait(bar, parity)) return true;
         asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
-        if (t - t0 > 1000000000ull) {
-            *abort_flag = 1;
-            latch(err, ERR_TIMEOUT);
-            return false;
-        }
-    }
-    return true;
+    } while (!*abort_flag && t - t0 < 1000000000ull);
+    return false;
+}
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+    return mbar_try_wait(bar, parity) || mbar_spin(bar, parity, abort_flag);
 }
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
     asm volatile(
@@ -215,37 +217,6 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
         : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
     return d;
 }
-// 2^x of two values on the FMA pipe, for the share of the exponentials that the
-// special-function unit (16 a clock and SM, a third of what the two tiles ask
-// for) would hold up: x = n + f with n = round(x) read off the low bits of
-// x + 1.5 * 2^23, 2^f on [-1/2, 1/2] by the polynomial of least largest relative
-// error (found by exchange of its extrema; degree 3: 7.5e-5, for bf16 rounded
-// to 2^-9; degree 4: 2.7e-6, for fp16 rounded to 2^-12), n added to the
-// exponent.  x <= 8; below -125 it is taken as -125 (2^-125 in place of less).
-template <int DEGREE>
-__device__ __forceinline__ float2 exp2_fma(float2 x) {
-    x.x = fmaxf(x.x, -125.0f);
-    x.y = fmaxf(x.y, -125.0f);
-    const float2 magic = make_float2(12582912.0f, 12582912.0f), less = make_float2(-12582912.0f, -12582912.0f);
-    const float2 one = make_float2(-1.0f, -1.0f);
-    const float2 t = add2(x, magic);
-    const float2 f = fma2(add2(t, less), one, x);
-    auto both = [](float v) { return make_float2(v, v); };
-    float2 y;
-    if constexpr (DEGREE == 3) {
-        y = fma2(f, both(0.0551716685295105f), both(0.2426111251115799f));
-        y = fma2(f, y, both(0.6932609677314758f));
-        y = fma2(f, y, both(0.9999280571937561f));
-    } else {
-        y = fma2(f, both(0.009570102207362652f), both(0.05591785907745361f));
-        y = fma2(f, y, both(0.240247443318367f));
-        y = fma2(f, y, both(0.6931217908859253f));
-        y = fma2(f, y, both(0.9999992847442627f));
-    }
-    y.x = __uint_as_float(__float_as_uint(y.x) + (__float_as_uint(t.x) << 23));
-    y.y = __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(t.y) << 23));
-    return y;
-}
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi);
 template <>
@@ -259,6 +230,31 @@ __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
     uint32_t r;
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
+}
+
+// Largest of r[0 .. N).
+template <int N>
+__device__ __forceinline__ float row_max(const uint32_t* r) {
+    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int q = 0; q < N; q += 8)
+#pragma unroll
+        for (int w = 0; w < 4; w++)
+            mx[w] = fmaxf(fmaxf(mx[w], __uint_as_float(r[q + w])), __uint_as_float(r[q + 4 + w]));
+    return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+}
+// 16 pairs of scores to p = 2^(c s + off), rounded and packed; sum takes the unrounded ones.
+template <typename T>
+__device__ __forceinline__ void exponentials(const uint32_t* r, float c, float off, float2 (&sum)[2], uint32_t* pk) {
+#pragma unroll
+    for (int q = 0; q < 16; q++) {
+        float2 x = fma2(make_float2(__uint_as_float(r[2 * q]), __uint_as_float(r[2 * q + 1])), make_float2(c, c),
+                        make_float2(off, off));
+        x.x = ex2(x.x);
+        x.y = ex2(x.y);
+        sum[q & 1] = add2(sum[q & 1], x);
+        pk[q] = pack2<T>(x.x, x.y);
+    }
 }
 
 // ---- units ----
@@ -280,7 +276,7 @@ struct UnitList {
     int first = 0, len = 0, pairs = 0;
     __device__ bool find(const PromptParams& p, long long u, Unit& out) {
         if (u < before) seq = 0, before = 0, end_unit = -1;
-        const int lane = threadIdx.x & 31, group = p.n_heads / p.n_kv_heads;
+        const int lane = threadIdx.x & 31, group = p.group;
         while (seq < p.n_seqs) {
             if (end_unit < 0) {
                 first = len = 0;
@@ -295,7 +291,7 @@ struct UnitList {
                 pairs = (int)min(two, 0x7fffffffll);
                 end_unit = two * p.n_kv_heads;
                 first_unit = end_unit;
-#pragma unroll
+#pragma unroll 1
                 for (int o = 1; o < 32; o <<= 1) {
                     const long long x = __shfl_up_sync(0xffffffffu, end_unit, o);
                     if (lane >= o) end_unit += x;
@@ -308,16 +304,16 @@ struct UnitList {
                 const int r = (int)(u - before - __shfl_sync(0xffffffffu, first_unit, at));
                 out.first = __shfl_sync(0xffffffffu, first, at);
                 out.len = __shfl_sync(0xffffffffu, len, at);
-                const int pair = __shfl_sync(0xffffffffu, pairs, at) - 1 - r / p.n_kv_heads;
-                out.g = r % p.n_kv_heads;
+                const int q = r / p.n_kv_heads, c = 2 * (__shfl_sync(0xffffffffu, pairs, at) - 1 - q);
+                out.g = r - q * p.n_kv_heads;
                 const int tiles = (out.len + BM - 1) / BM;
-#pragma unroll
-                for (int s = 0; s < 2; s++) {
-                    const int c = 2 * pair + s;  // (row tile, head of the group), heads fastest
-                    const int t = c / group;
-                    out.tile[s] = t < tiles ? t : -1;
-                    out.head[s] = out.g * group + c - t * group;
-                }
+                // tiles c and c + 1 of (row tile, head of the group), heads fastest
+                const int t = c / group, h = c - t * group;
+                const bool wraps = h + 1 == group;
+                out.tile[0] = t;
+                out.tile[1] = t + wraps < tiles ? t + wraps : -1;
+                out.head[0] = out.g * group + h;
+                out.head[1] = out.g * group + (wraps ? 0 : h + 1);
                 return true;
             }
             before += __shfl_sync(0xffffffffu, end_unit, 31);
@@ -433,7 +429,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    auto wait = [&](uint32_t bar, uint32_t parity) { return mbar_wait(bar, parity, abort_flag, p.err); };
+    auto wait = [&](uint32_t bar, uint32_t parity) { return mbar_wait(bar, parity, abort_flag); };
+    auto give_up = [&]() {  // a wait ran out, here or (again) elsewhere
+        *abort_flag = 1;
+        latch(p.err, ERR_TIMEOUT);
+    };
     // The unit in the list's slot, as the load warp left it.
     auto take = [&](int i, Unit& u) {
         volatile Unit& v = units[i];
@@ -476,6 +476,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (role < 2) {
                 const CUtensorMap* map = role == 0 ? &map_k : &map_v;
                 const uint32_t tiles = base + (role == 0 ? Ly::K_OFF : Ly::V_OFF) + c * Ly::SLAB;
+#pragma unroll 1
                 for (int j = 0; j < nb && ok; j++) {
                     const uint32_t i = it + j, st = i % ST;
                     const uint32_t full = role == 0 ? k_full(st) : v_full(st);
@@ -522,9 +523,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             x = __shfl_sync(0xffffffffu, x, 0);
             more = got && list.find(p, x, unit);  // the end goes through the list as a unit without rows
         }
+        if (!ok) give_up();
         // given up: let this lane's last copy land before the shared memory is another's
         if (*abort_flag && last_bar)
-            for (uint32_t i = 0; i < 4000000u && !mbar_try_wait(last_bar, last_parity); i++) {
+            for (uint32_t i = 0; i < 1000u && !mbar_try_wait(last_bar, last_parity); i++) {
             }
     } else if (warp == 9) {
         // ---------------- products ----------------
@@ -533,7 +535,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // takes to execute.)
         if (elect_one()) {
             constexpr uint32_t id_s = idesc_f16(BF, BM, 0), id_o = idesc_f16(BF, HD, 1);
-            uint32_t it = 0, taken[2] = {0, 0}, cs[2] = {0, 0};  // blocks loaded, tiles and blocks of each side
+            uint32_t it = 0, taken0 = 0, taken1 = 0, cs0 = 0, cs1 = 0;  // blocks loaded, tiles and blocks of each side
             // S_s = Q_s K^T from stage st
             auto scores = [&](int s, uint32_t st, bool last) {
                 const uint64_t a = desc_sw128(base + s * Ly::TILE, 0), b = desc_sw128(base + Ly::K_OFF + st * Ly::TILE, 0);
@@ -553,65 +555,62 @@ __global__ void __launch_bounds__(kThreads, 1)
                            b + 128 * (BM / 32 * half + kk), id_o, !first || kk > 0);
                 if (half) mma_commit(o_full(s));
             };
-            for (uint32_t n = 0;; n++) {
+            bool ok = true;
+            for (uint32_t n = 0; ok; n++) {
                 const int slot = n % kSlots;
-                if (!wait(u_full(slot), (n / kSlots) & 1)) break;
-                const int len = units[slot].len;
-                const int ns[2] = {units[slot].tile[0] + 1, units[slot].tile[1] + 1};
+                ok = wait(u_full(slot), (n / kSlots) & 1);
+                if (!ok) break;
+                const int len = units[slot].len, n0 = units[slot].tile[0] + 1, n1 = units[slot].tile[1] + 1;
                 mbar_arrive(u_empty(slot));
                 if (len == 0) break;
-                const int nb = max(ns[0], ns[1]);
-                // block 0's scores of both tiles
-                bool ok = wait(k_full(it % ST), (it / ST) & 1);
-#pragma unroll
-                for (int s = 0; s < 2; s++) {
-                    if (!ok || !ns[s]) continue;
-                    ok = wait(q_full(s), taken[s] & 1);
-                    if (Ly::OWN_P) ok = ok && wait(s_free(s), (cs[s] & 1) ^ 1);
-                    if (!ok) continue;
-                    tc_fence_after();
-                    scores(s, it % ST, ns[s] == 1);
-                }
-                if (!ok) break;
-                mma_commit(k_empty(it % ST));
-                for (int j = 0; j < nb; j++) {
+                const int nb = max(n0, n1);
+                // Step j: the scores of block j + 1 (head_dim 64: as soon as softmax has read those of block j; 128: once
+                // block j's p, which lies in their place, has been multiplied), then block j's values.
+#pragma unroll 1
+                for (int j = -1; j < nb && ok; j++) {
                     const uint32_t i = it + j, st = i % ST, nx = (i + 1) % ST;
-                    if (j + 1 < nb) ok = wait(k_full(nx), ((i + 1) / ST) & 1);
-                    if (Ly::OWN_P && j + 1 < nb) {
-#pragma unroll
-                        for (int s = 0; s < 2; s++) {
-                            if (!ok || j + 1 >= ns[s]) continue;
-                            ok = wait(s_free(s), (cs[s] + j) & 1);
-                            if (!ok) continue;
+                    const bool more = j + 1 < nb;
+                    if (more) ok = wait(k_full(nx), ((i + 1) / ST) & 1);
+                    if (more && (Ly::OWN_P || j < 0)) {
+#pragma unroll 1
+                        for (int s = 0; s < 2 && ok; s++) {
+                            const int ns = s ? n1 : n0;
+                            const uint32_t done = (s ? cs1 : cs0) + j + 1;  // this side's blocks before
+                            if (j + 1 >= ns) continue;
+                            if (j < 0) ok = wait(q_full(s), (s ? taken1 : taken0) & 1);
+                            if (Ly::OWN_P) ok = ok && wait(s_free(s), (done & 1) ^ 1);
+                            if (!ok) break;
                             tc_fence_after();
-                            scores(s, nx, j + 2 == ns[s]);
+                            scores(s, nx, j + 2 == ns);
                         }
                         if (ok) mma_commit(k_empty(nx));
                     }
+                    if (j < 0) continue;
                     ok = ok && wait(v_good(st), (i / ST) & 1);
-#pragma unroll
-                    for (int s = 0; s < 2; s++) {
-                        if (!ok || j >= ns[s]) continue;
-                        if (j == 0) ok = wait(o_free(s), (taken[s] & 1) ^ 1);
-                        ok = ok && wait(p_half(s), (cs[s] + j) & 1);
-                        if (!ok) continue;
+#pragma unroll 1
+                    for (int s = 0; s < 2 && ok; s++) {
+                        const int ns = s ? n1 : n0;
+                        const uint32_t done = (s ? cs1 : cs0) + j;
+                        if (j >= ns) continue;
+                        if (j == 0) ok = wait(o_free(s), ((s ? taken1 : taken0) & 1) ^ 1);
+                        ok = ok && wait(p_half(s), done & 1);
+                        if (!ok) break;
                         tc_fence_after();
                         values(s, st, 0, j == 0);
-                        ok = wait(p_full(s), (cs[s] + j) & 1);
-                        if (!ok) continue;
+                        ok = wait(p_full(s), done & 1);
+                        if (!ok) break;
                         tc_fence_after();
                         values(s, st, 1, false);
-                        if (!Ly::OWN_P && j + 1 < ns[s]) scores(s, nx, j + 2 == ns[s]);  // over P, in issue order
+                        if (!Ly::OWN_P && j + 1 < ns) scores(s, nx, j + 2 == ns);  // in issue order
                     }
                     if (!ok) break;
                     mma_commit(v_empty(st));
-                    if (!Ly::OWN_P && j + 1 < nb) mma_commit(k_empty(nx));
+                    if (!Ly::OWN_P && more) mma_commit(k_empty(nx));
                 }
-                if (!ok) break;
                 it += nb;
-#pragma unroll
-                for (int s = 0; s < 2; s++) taken[s] += ns[s] > 0, cs[s] += ns[s];
+                taken0 += n0 > 0, taken1 += n1 > 0, cs0 += n0, cs1 += n1;
             }
+            if (!ok) give_up();
         }
         __syncwarp();
     } else if (warp == 10) {
@@ -627,6 +626,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (u.len == 0) break;
             const int nb = u.blocks();
             bool bad = false;
+#pragma unroll 1
             for (int j = 0; j < nb; j++) {
                 const uint32_t i = it + j, st = i % ST;
                 ok = __all_sync(0xffffffffu, wait(v_full(st), (i / ST) & 1));
@@ -636,7 +636,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     constexpr uint32_t EXP = BF ? 0x7f807f80u : 0x7c007c00u, ONE = BF ? 0x00800080u : 0x04000400u;
                     uint4* tile = reinterpret_cast<uint4*>(smem + Ly::V_OFF + st * Ly::TILE);
                     uint32_t seen = 0;
-#pragma unroll 8
+#pragma unroll 4
                     for (int x = lane; x < Ly::TILE / 16; x += 32) {
                         if ((x >> 3) % BM < rows) {  // 8 vectors a row, BM rows a slab
                             const uint4 w = tile[x];
@@ -664,29 +664,58 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             it += nb;
         }
+        if (!ok) give_up();
     }
     } else {
         // ---------------- softmax, output ----------------
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
-        const int s = warp >> 2, row = threadIdx.x & 127;
+        const int s = warp >> 2;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t ts = tmem + lanes + Ly::S + s * 128, tp = tmem + lanes + Ly::P + s * Ly::P_STEP,
                        to = tmem + lanes + Ly::O + s * HD;
         const float c = p.scale * 1.4426950408889634f;  // log2 e
-        uint32_t cs = 0;
-        for (uint32_t n = 0;; n++) {
+        uint32_t cs = 0;  // blocks of this side
+        float m = -INFINITY, off = 0.0f, l = 0.0f;  // maximum that exponents refer to, -c m, row sum
+        auto wait_all = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
+        // A higher maximum: l and, where there is one, O scaled down to it.
+        auto raise = [&](float to_m, bool scale_o) {
+            const float f = to_m == m ? 1.0f : ex2((m - to_m) * c);
+            m = to_m;
+            off = m == -INFINITY ? 0.0f : -m * c;
+            l *= f;
+            if (!scale_o) return;
+#pragma unroll 1
+            for (int q = 0; q < HD; q += 16) {
+                uint32_t o[16];
+                tmem_ld16(to + q, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int w = 0; w < 16; w++) o[w] = __float_as_uint(__uint_as_float(o[w]) * f);
+                tmem_st16(to + q, o);
+            }
+        };
+        // This warp's p of half a block is in TMEM.
+        auto publish = [&](uint32_t bar) {
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            mbar_arrive_if(bar, lane == 0);
+        };
+        bool ok = true;
+        for (uint32_t n = 0; ok; n++) {
             const int slot = n % kSlots;
-            if (!__all_sync(0xffffffffu, wait(u_full(slot), (n / kSlots) & 1))) break;
-            Unit u;
-            take(slot, u);
-            if (u.len == 0) break;
-            const int tile = s ? u.tile[1] : u.tile[0], head = s ? u.head[1] : u.head[0], nb = tile + 1;
-            float m = -INFINITY, mc = 0.0f, l = 0.0f;
-            bool ok = true;
+            ok = wait_all(u_full(slot), (n / kSlots) & 1);
+            if (!ok) break;
+            const int first = units[slot].first, len = units[slot].len, tile = units[slot].tile[s],
+                      head = units[slot].head[s], nb = tile + 1;
+            if (len == 0) break;
+            m = -INFINITY, off = 0.0f, l = 0.0f;
+#pragma unroll 1
             for (int j = 0; j < nb; j++) {
-                ok = __all_sync(0xffffffffu, wait(s_full(s), (cs + j) & 1));
+                ok = wait_all(s_full(s), (cs + j) & 1);
                 if (!ok) break;
                 tc_fence_after();
+                float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
                 uint32_t r[128];
 #pragma unroll
                 for (int q = 0; q < 4; q++) tmem_ld32(ts + 32 * q, r + 32 * q);
@@ -694,143 +723,93 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (Ly::OWN_P) {
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(s_free(s));
+                    mbar_arrive_if(s_free(s), lane == 0);
                 }
-                // On the diagonal a warp's rows see no key behind its own 32: it works on its first `parts` quarters only.
-                const bool diagonal = j == nb - 1;
-                const int parts = diagonal ? (warp & 3) + 1 : 4;
-                if (diagonal) {
+                if (j == nb - 1) {  // the diagonal: row i sees its first i + 1 keys
+                    const int row = threadIdx.x & 127;
 #pragma unroll
-                    for (int q = 0; q < 128; q++)
-                        if (q > row) r[q] = 0xff800000u;
-                }
-                float top = -INFINITY;
+                    for (int h = 0; h < 4; h++) {
+                        const int n_seen = row + 1 - 32 * h;
+                        const uint32_t seen = n_seen >= 32 ? 0xffffffffu : n_seen <= 0 ? 0u : (1u << n_seen) - 1;
 #pragma unroll
-                for (int h = 0; h < 4; h++) {
-                    if (h >= parts) break;
-                    float mx[4] = {top, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                    for (int q = 32 * h; q < 32 * h + 32; q += 8)
-#pragma unroll
-                        for (int w = 0; w < 4; w++)
-                            mx[w] = fmaxf(fmaxf(mx[w], __uint_as_float(r[q + w])), __uint_as_float(r[q + 4 + w]));
-                    top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                }
-                const bool rise = (top - m) * c > 8.0f;  // always true of the first block that has a score
-                if (__any_sync(0xffffffffu, rise)) {
-                    const float old = m;
-                    if (rise) m = top;
-                    mc = m == -INFINITY ? 0.0f : m * c;
-                    const float f = rise ? ex2((old - m) * c) : 1.0f;
-                    l *= f;
-                    if (j > 0) {
-                        ok = __all_sync(0xffffffffu, wait(o_full(s), (cs + j - 1) & 1));
-                        if (!ok) break;
-                        tc_fence_after();
-#pragma unroll
-                        for (int q = 0; q < HD / 16; q++) {
-                            uint32_t o[16];
-                            tmem_ld16(to + 16 * q, o);
-                            tmem_wait_ld();
-#pragma unroll
-                            for (int w = 0; w < 16; w++) o[w] = __float_as_uint(__uint_as_float(o[w]) * f);
-                            tmem_st16(to + 16 * q, o);
-                        }
+                        for (int q = 0; q < 32; q++)
+                            if (!(seen & (1u << q))) r[32 * h + q] = 0xff800000u;
                     }
                 }
-                if (Ly::OWN_P && j > 0) {  // P's columns are free once the product before is done
-                    ok = __all_sync(0xffffffffu, wait(o_full(s), (cs + j - 1) & 1));
+                const float top = row_max<128>(r);
+                const bool rise = (top - m) * c > 8.0f;  // true of a first block that has a score
+                const bool any_rise = __any_sync(0xffffffffu, rise);
+                // P's columns (head_dim 64) and O are free once the product before is done
+                if (j > 0 && (Ly::OWN_P || any_rise)) {
+                    ok = wait_all(o_full(s), (cs + j - 1) & 1);
                     if (!ok) break;
                     tc_fence_after();
                 }
-                float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-                const float2 cc = make_float2(c, c), off = make_float2(-mc, -mc);
-#pragma unroll
-                for (int h = 0; h < 4; h++) {
-                    uint32_t pk[16];
-                    if (!diagonal) {
-#pragma unroll
-                        for (int q = 0; q < 16; q++) {
-                            const float2 x = fma2(make_float2(__uint_as_float(r[32 * h + 2 * q]),
-                                                              __uint_as_float(r[32 * h + 2 * q + 1])), cc, off);
-                            // spread evenly: q in steps of 16 / ON_FMA
-                            const bool fma = (q + 1) * Ly::ON_FMA / 16 > q * Ly::ON_FMA / 16;
-                            const float2 y = fma ? exp2_fma<BF ? 3 : 4>(x) : make_float2(ex2(x.x), ex2(x.y));
-                            sum[q & 1] = add2(sum[q & 1], y);
-                            pk[q] = pack2<T>(y.x, y.y);
-                        }
-                    } else if (h < parts) {  // a masked score's p is 0 to the last bit here
-#pragma unroll
-                        for (int q = 0; q < 16; q++) {
-                            const float2 x = fma2(make_float2(__uint_as_float(r[32 * h + 2 * q]),
-                                                              __uint_as_float(r[32 * h + 2 * q + 1])), cc, off);
-                            const float2 y = make_float2(ex2(x.x), ex2(x.y));
-                            sum[q & 1] = add2(sum[q & 1], y);
-                            pk[q] = pack2<T>(y.x, y.y);
-                        }
-                    } else {
-#pragma unroll
-                        for (int q = 0; q < 16; q++) pk[q] = 0;
-                    }
-                    tmem_st16(tp + 16 * h, pk);
-                    if (h & 1) {
-                        tmem_wait_st();
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(h == 1 ? p_half(s) : p_full(s));
-                    }
-                }
+                if (any_rise) raise(rise ? top : m, j > 0);
+                uint32_t pk[32];
+                exponentials<T>(r, c, off, sum, pk);
+                tmem_st16(tp, pk);
+                exponentials<T>(r + 32, c, off, sum, pk + 16);
+                tmem_st16(tp + 16, pk + 16);
+                exponentials<T>(r + 64, c, off, sum, pk);
+                publish(p_half(s));  // stored while the third quarter was computed
+                tmem_st16(tp + 32, pk);
+                exponentials<T>(r + 96, c, off, sum, pk + 16);
+                tmem_st16(tp + 48, pk + 16);
+                publish(p_full(s));
                 l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
             }
+            ok = ok && wait_all(u_seen(slot), (n / kSlots) & 1);
             if (!ok) break;
-            if (!__all_sync(0xffffffffu, wait(u_seen(slot), (n / kSlots) & 1))) break;
-            const int bad = units[slot].bad;
             if (nb) {
-                if (!__all_sync(0xffffffffu, wait(o_full(s), (cs + nb - 1) & 1))) break;
+                const int bad = units[slot].bad;
+                ok = wait_all(o_full(s), (cs + nb - 1) & 1);
+                if (!ok) break;
                 tc_fence_after();
                 const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-                const int i = tile * BM + row;
-                const int rows = bad ? 0 : min(32, u.len - (i - lane));  // of this warp's 32
-                T* to_row = static_cast<T*>(p.out) + ((int64_t)u.first + i - lane) * p.out_stride + head * HD;
+                const int i = tile * BM + (warp & 3) * 32;        // this warp's first row
+                const int rows = bad ? 0 : min(32, len - i);
+                T* out = static_cast<T*>(p.out) + ((int64_t)first + i) * p.out_stride + head * HD;
                 uint4* stage = reinterpret_cast<uint4*>(smem + Ly::OUT_OFF + warp * 4096);
-#pragma unroll
-                for (int q = 0; q < HD / 64; q++) {
-                    uint32_t o[64];
-                    tmem_ld32(to + 64 * q, o);
-                    tmem_ld32(to + 64 * q + 32, o + 32);
-                    tmem_wait_ld();
+#pragma unroll 1
+                for (int q = 0; q < HD; q += 64) {
                     // a row's 128 bytes by its own thread, chunks permuted by the row against bank conflicts; then
                     // eight lanes store one row
+#pragma unroll 1
+                    for (int w = 0; w < 8; w += 4) {
+                        uint32_t o[32];
+                        tmem_ld32(to + q + 8 * w, o);
+                        tmem_wait_ld();
 #pragma unroll
-                    for (int w = 0; w < 8; w++)
-                        stage[lane * 8 + (w ^ (lane & 7))] =
-                            make_uint4(pack2<T>(__uint_as_float(o[8 * w]) * inv, __uint_as_float(o[8 * w + 1]) * inv),
-                                       pack2<T>(__uint_as_float(o[8 * w + 2]) * inv, __uint_as_float(o[8 * w + 3]) * inv),
-                                       pack2<T>(__uint_as_float(o[8 * w + 4]) * inv, __uint_as_float(o[8 * w + 5]) * inv),
-                                       pack2<T>(__uint_as_float(o[8 * w + 6]) * inv, __uint_as_float(o[8 * w + 7]) * inv));
+                        for (int x = 0; x < 4; x++) {
+                            uint32_t y[4];
+#pragma unroll
+                            for (int e = 0; e < 4; e++)
+                                y[e] = pack2<T>(__uint_as_float(o[8 * x + 2 * e]) * inv, __uint_as_float(o[8 * x + 2 * e + 1]) * inv);
+                            stage[lane * 8 + ((w + x) ^ (lane & 7))] = make_uint4(y[0], y[1], y[2], y[3]);
+                        }
+                    }
                     __syncwarp();
 #pragma unroll
                     for (int w = 0; w < 8; w++) {
-                        const int to_r = 4 * w + (lane >> 3);
-                        if (to_r < rows)
-                            *reinterpret_cast<uint4*>(to_row + to_r * p.out_stride + 64 * q + 8 * (lane & 7)) =
-                                stage[to_r * 8 + ((lane & 7) ^ (to_r & 7))];
+                        const int r = 4 * w + (lane >> 3);
+                        if (r < rows)
+                            *reinterpret_cast<uint4*>(out + r * p.out_stride + q + 8 * (lane & 7)) =
+                                stage[r * 8 + ((lane & 7) ^ (r & 7))];
                     }
                     __syncwarp();
                 }
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(o_free(s));
+                mbar_arrive_if(o_free(s), lane == 0);
                 if (bad)
-                    for (int w = 0; w < 32; w++) {
-                        const int at = tile * BM + (warp & 3) * 32 + w;
-                        if (at < u.len) plain_row<T, HD>(p, u.first, at, head, u.g);
-                    }
+                    for (int w = 0; w < 32 && i + w < len; w++) plain_row<T, HD>(p, first, i + w, head, head / p.group);
             }
             __syncwarp();
-            if (lane == 0) mbar_arrive(u_empty(slot));
+            mbar_arrive_if(u_empty(slot), lane == 0);
             cs += nb;
         }
+        if (!ok) give_up();
     }
     tc_fence_before();
     __syncthreads();
@@ -922,7 +901,7 @@ extern "C" pf_status pf_prompt_attention(const void* q, int64_t q_stride, const 
     if (n_seqs == 0 || n_tokens == 0) return PF_OK;
     PF_CHECK(q && k && v && out && offsets, "pf_prompt_attention: null argument");
     const PromptParams p{q, k, v, out, q_stride, k_stride, v_stride, out_stride, offsets, n_seqs, n_tokens, n_heads,
-                         n_kv_heads, scale, device_error_flag()};
+                         n_kv_heads, n_heads / n_kv_heads, scale, device_error_flag()};
     cudaStream_t st = as_stream(stream);
     if (dtype == PF_BF16)
         return head_dim == 64 ? launch_prompt<__nv_bfloat16, 64>(p, st) : launch_prompt<__nv_bfloat16, 128>(p, st);
