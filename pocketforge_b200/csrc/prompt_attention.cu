@@ -72,7 +72,8 @@ struct Layout {
     static constexpr int SLAB = BM * 128;             // bytes of one
     static constexpr int TILE = NC * SLAB;            // a Q tile, K block or V block
     static constexpr int STAGES = HD == 64 ? 4 : 2;   // K blocks and V blocks in flight
-    static constexpr int K_OFF = 2 * TILE, V_OFF = K_OFF + STAGES * TILE;
+    static constexpr int QB = HD == 64 ? 2 : 1;       // buffers of each Q tile: the next unit's, where there is room
+    static constexpr int K_OFF = 2 * QB * TILE, V_OFF = K_OFF + STAGES * TILE;
     static constexpr int OUT_OFF = V_OFF + STAGES * TILE;  // 32 rows x 128 bytes of output a softmax warp
     static constexpr int BAR_OFF = OUT_OFF + kSoftmaxWarps * 32 * 128;
     static constexpr int SMEM = BAR_OFF + 512 + 1024;  // barriers, unit list; alignment
@@ -243,7 +244,9 @@ __device__ __forceinline__ float row_max(const uint32_t* r) {
             mx[w] = fmaxf(fmaxf(mx[w], __uint_as_float(r[q + w])), __uint_as_float(r[q + 4 + w]));
     return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
 }
-// 16 pairs of scores to p = 2^(c s + off), rounded and packed; sum takes the unrounded ones.
+// 16 pairs of scores to p = 2^(c s + off), rounded and packed; sum takes the unrounded ones.  All on the
+// special-function unit: a share of 1/8 or 1/4 by a polynomial on the FMA pipe measured the same to 2% slower (8192
+// tokens 498, 504, 509 us), which the more instructions' power accounts for.
 template <typename T>
 __device__ __forceinline__ void exponentials(const uint32_t* r, float c, float off, float2 (&sum)[2], uint32_t* pk) {
 #pragma unroll
@@ -359,28 +362,30 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     const uint32_t base = smem_u32(smem);
     const uint32_t bars = base + Ly::BAR_OFF;
-    auto q_full = [&](int s) { return bars + 8u * s; };
-    auto q_empty = [&](int s) { return bars + 8u * (2 + s); };
-    auto s_full = [&](int s) { return bars + 8u * (4 + s); };
-    auto s_free = [&](int s) { return bars + 8u * (6 + s); };
-    auto p_full = [&](int s) { return bars + 8u * (8 + s); };
-    auto o_full = [&](int s) { return bars + 8u * (10 + s); };
-    auto o_free = [&](int s) { return bars + 8u * (12 + s); };
-    auto u_full = [&](int i) { return bars + 8u * (14 + i); };
-    auto u_empty = [&](int i) { return bars + 8u * (16 + i); };
-    auto u_seen = [&](int i) { return bars + 8u * (18 + i); };  // the guard is through with the unit
-    auto p_half = [&](int s) { return bars + 8u * (20 + s); };  // p of the block's first 64 keys
-    const uint32_t next_full = bars + 8u * 22;
-    auto k_full = [&](int i) { return bars + 8u * (23 + i); };
-    auto k_empty = [&](int i) { return bars + 8u * (23 + ST + i); };
-    auto v_full = [&](int i) { return bars + 8u * (23 + 2 * ST + i); };
-    auto v_empty = [&](int i) { return bars + 8u * (23 + 3 * ST + i); };
-    auto v_good = [&](int i) { return bars + 8u * (23 + 4 * ST + i); };  // looked through
-    static_assert(8 * (23 + 5 * ST) <= 352, "barriers");
-    uint8_t* tail = smem + Ly::BAR_OFF + 352;
-    const uint32_t next_at = base + Ly::BAR_OFF + 352;              // 16 bytes: the next unit's launch
+    constexpr int QB = Ly::QB;
+    auto s_full = [&](int s) { return bars + 8u * (0 + s); };
+    auto s_free = [&](int s) { return bars + 8u * (2 + s); };
+    auto p_half = [&](int s) { return bars + 8u * (4 + s); };  // p of the block's first 64 keys
+    auto p_full = [&](int s) { return bars + 8u * (6 + s); };
+    auto o_full = [&](int s) { return bars + 8u * (8 + s); };
+    auto o_free = [&](int s) { return bars + 8u * (10 + s); };
+    auto u_full = [&](int i) { return bars + 8u * (12 + i); };
+    auto u_empty = [&](int i) { return bars + 8u * (14 + i); };
+    auto u_seen = [&](int i) { return bars + 8u * (16 + i); };  // the guard is through with the unit
+    const uint32_t next_full = bars + 8u * 18;
+    auto q_full = [&](int s, uint32_t use) { return bars + 8u * (19 + s * QB + use % QB); };
+    auto q_empty = [&](int s, uint32_t use) { return bars + 8u * (19 + 2 * QB + s * QB + use % QB); };
+    auto k_full = [&](int i) { return bars + 8u * (19 + 4 * QB + i); };
+    auto k_empty = [&](int i) { return bars + 8u * (19 + 4 * QB + ST + i); };
+    auto v_full = [&](int i) { return bars + 8u * (19 + 4 * QB + 2 * ST + i); };
+    auto v_empty = [&](int i) { return bars + 8u * (19 + 4 * QB + 3 * ST + i); };
+    auto v_good = [&](int i) { return bars + 8u * (19 + 4 * QB + 4 * ST + i); };  // looked through
+    auto q_tile = [&](int s, uint32_t use) { return base + (uint32_t)((s * QB + use % QB) * Ly::TILE); };
+    static_assert(8 * (19 + 4 * QB + 5 * ST) <= 384, "barriers");
+    uint8_t* tail = smem + Ly::BAR_OFF + 384;
+    const uint32_t next_at = base + Ly::BAR_OFF + 384;                   // 16 bytes: the next unit's launch
     volatile Unit* units = reinterpret_cast<volatile Unit*>(tail + 16);  // [kSlots]
-    static_assert(16 + kSlots * sizeof(Unit) + 12 <= 160, "unit list");
+    static_assert(16 + kSlots * sizeof(Unit) + 12 <= 128, "unit list");
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tail + 16 + kSlots * sizeof(Unit));
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     int* any = reinterpret_cast<int*>(tmem_slot + 2);
@@ -393,8 +398,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) {
             *any = found;
             for (int s = 0; s < 2; s++) {
-                mbar_init(q_full(s), NC);
-                mbar_init(q_empty(s), 1);
+                for (int i = 0; i < QB; i++) {
+                    mbar_init(q_full(s, i), NC);
+                    mbar_init(q_empty(s, i), 1);
+                }
                 mbar_init(s_full(s), 1);
                 mbar_init(s_free(s), 4);
                 mbar_init(p_half(s), 4);
@@ -489,12 +496,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             } else if (role < 4 && (role == 2 ? unit.tile[0] : unit.tile[1]) >= 0) {
                 const int s = role - 2;
                 const uint32_t use = s ? taken[1] : taken[0];
-                ok = wait(q_empty(s), (use & 1) ^ 1);
+                ok = wait(q_empty(s, use), ((use / QB) & 1) ^ 1);
                 if (ok) {
-                    mbar_expect_tx(q_full(s), Ly::SLAB);
-                    tma_load_2d(base + s * Ly::TILE + c * Ly::SLAB, &map_q, (s ? unit.head[1] : unit.head[0]) * HD + c * 64,
-                                unit.first + (s ? unit.tile[1] : unit.tile[0]) * BM, q_full(s));
-                    last_bar = q_full(s), last_parity = use & 1;
+                    last_bar = q_full(s, use), last_parity = (use / QB) & 1;
+                    mbar_expect_tx(last_bar, Ly::SLAB);
+                    tma_load_2d(q_tile(s, use) + c * Ly::SLAB, &map_q, (s ? unit.head[1] : unit.head[0]) * HD + c * 64,
+                                unit.first + (s ? unit.tile[1] : unit.tile[0]) * BM, last_bar);
                 }
             }
             it += nb;
@@ -535,80 +542,91 @@ __global__ void __launch_bounds__(kThreads, 1)
         // takes to execute.)
         if (elect_one()) {
             constexpr uint32_t id_s = idesc_f16(BF, BM, 0), id_o = idesc_f16(BF, HD, 1);
-            uint32_t it = 0, taken0 = 0, taken1 = 0, cs0 = 0, cs1 = 0;  // blocks loaded, tiles and blocks of each side
-            // S_s = Q_s K^T from stage st
-            auto scores = [&](int s, uint32_t st, bool last) {
-                const uint64_t a = desc_sw128(base + s * Ly::TILE, 0), b = desc_sw128(base + Ly::K_OFF + st * Ly::TILE, 0);
+            // The units' blocks are one stream.  head_dim 64: block k + 1's scores go before block k's values, as soon as
+            // softmax has read the scores of block k.  128: after them, side by side, since block k's p lies in their
+            // place (products of one CTA execute in issue order).
+            struct Block {
+                int j, n0, n1;                  // block of its unit, and the unit's blocks on either side
+                __device__ bool has(int s) const { return j < (s ? n1 : n0); }
+                __device__ bool last(int s) const { return j + 1 == (s ? n1 : n0); }
+            };
+            uint32_t n = 0, k_it = 0, v_it = 0;               // units, blocks of K and of V taken
+            uint32_t sc0 = 0, sc1 = 0, vc0 = 0, vc1 = 0;      // scores and values of either side so far
+            uint32_t tq0 = 0, tq1 = 0, tv0 = 0, tv1 = 0;      // tiles of either side begun, for the scores and the values
+            bool ok = true, more = true;
+            Block next{-1, 0, 0}, now{0, 0, 0};
+            // The stream's next block into `next`; false at its end.
+            auto advance = [&]() {
+                if (++next.j < max(next.n0, next.n1)) return true;
+                const int slot = n % kSlots;
+                ok = wait(u_full(slot), (n / kSlots) & 1);
+                if (!ok) return false;
+                n++;
+                const int len = units[slot].len;
+                next.j = 0, next.n0 = units[slot].tile[0] + 1, next.n1 = units[slot].tile[1] + 1;
+                mbar_arrive(u_empty(slot));
+                return len != 0;
+            };
+            // S_s = Q_s K^T of block `next`
+            auto scores = [&](int s) {
+                const uint32_t use = s ? tq1 : tq0, st = k_it % ST, done = s ? sc1 : sc0;
+                if (next.j == 0) ok = ok && wait(q_full(s, use), (use / QB) & 1);
+                if (Ly::OWN_P) ok = ok && wait(s_free(s), (done & 1) ^ 1);
+                if (!ok) return;
+                tc_fence_after();
+                const uint64_t a = desc_sw128(q_tile(s, use), 0), b = desc_sw128(base + Ly::K_OFF + st * Ly::TILE, 0);
 #pragma unroll
                 for (int kk = 0; kk < HD / 16; kk++)
                     mma_ss(tmem + Ly::S + s * 128, a + (kk / 4) * (Ly::SLAB >> 4) + 2 * (kk % 4),
                            b + (kk / 4) * (Ly::SLAB >> 4) + 2 * (kk % 4), id_s, kk > 0);
                 mma_commit(s_full(s));
-                if (last) mma_commit(q_empty(s));
+                if (next.last(s)) {
+                    mma_commit(q_empty(s, use));
+                    s ? tq1++ : tq0++;
+                }
+                s ? sc1++ : sc0++;
             };
-            // O_s += P_s V over half of the block's keys
-            auto values = [&](int s, uint32_t st, int half, bool first) {
+            // O_s += P_s V of block `now`, its keys in two halves
+            auto values = [&](int s) {
+                const uint32_t done = s ? vc1 : vc0, st = v_it % ST;
+                if (now.j == 0) ok = ok && wait(o_free(s), ((s ? tv1 : tv0) & 1) ^ 1);
                 const uint64_t b = desc_sw128(base + Ly::V_OFF + st * Ly::TILE, Ly::SLAB);
 #pragma unroll
-                for (int kk = 0; kk < BM / 32; kk++)
-                    mma_ts(tmem + Ly::O + s * HD, tmem + Ly::P + s * Ly::P_STEP + 32 * half + 8 * kk,
-                           b + 128 * (BM / 32 * half + kk), id_o, !first || kk > 0);
-                if (half) mma_commit(o_full(s));
-            };
-            bool ok = true;
-            for (uint32_t n = 0; ok; n++) {
-                const int slot = n % kSlots;
-                ok = wait(u_full(slot), (n / kSlots) & 1);
-                if (!ok) break;
-                const int len = units[slot].len, n0 = units[slot].tile[0] + 1, n1 = units[slot].tile[1] + 1;
-                mbar_arrive(u_empty(slot));
-                if (len == 0) break;
-                const int nb = max(n0, n1);
-                // Step j: the scores of block j + 1 (head_dim 64: as soon as softmax has read those of block j; 128: once
-                // block j's p, which lies in their place, has been multiplied), then block j's values.
-#pragma unroll 1
-                for (int j = -1; j < nb && ok; j++) {
-                    const uint32_t i = it + j, st = i % ST, nx = (i + 1) % ST;
-                    const bool more = j + 1 < nb;
-                    if (more) ok = wait(k_full(nx), ((i + 1) / ST) & 1);
-                    if (more && (Ly::OWN_P || j < 0)) {
-#pragma unroll 1
-                        for (int s = 0; s < 2 && ok; s++) {
-                            const int ns = s ? n1 : n0;
-                            const uint32_t done = (s ? cs1 : cs0) + j + 1;  // this side's blocks before
-                            if (j + 1 >= ns) continue;
-                            if (j < 0) ok = wait(q_full(s), (s ? taken1 : taken0) & 1);
-                            if (Ly::OWN_P) ok = ok && wait(s_free(s), (done & 1) ^ 1);
-                            if (!ok) break;
-                            tc_fence_after();
-                            scores(s, nx, j + 2 == ns);
-                        }
-                        if (ok) mma_commit(k_empty(nx));
-                    }
-                    if (j < 0) continue;
-                    ok = ok && wait(v_good(st), (i / ST) & 1);
-#pragma unroll 1
-                    for (int s = 0; s < 2 && ok; s++) {
-                        const int ns = s ? n1 : n0;
-                        const uint32_t done = (s ? cs1 : cs0) + j;
-                        if (j >= ns) continue;
-                        if (j == 0) ok = wait(o_free(s), ((s ? taken1 : taken0) & 1) ^ 1);
-                        ok = ok && wait(p_half(s), done & 1);
-                        if (!ok) break;
-                        tc_fence_after();
-                        values(s, st, 0, j == 0);
-                        ok = wait(p_full(s), done & 1);
-                        if (!ok) break;
-                        tc_fence_after();
-                        values(s, st, 1, false);
-                        if (!Ly::OWN_P && j + 1 < ns) scores(s, nx, j + 2 == ns);  // in issue order
-                    }
-                    if (!ok) break;
-                    mma_commit(v_empty(st));
-                    if (!Ly::OWN_P && more) mma_commit(k_empty(nx));
+                for (int half = 0; half < 2; half++) {
+                    ok = ok && wait(half ? p_full(s) : p_half(s), done & 1);
+                    if (!ok) return;
+                    tc_fence_after();
+#pragma unroll
+                    for (int kk = BM / 32 * half; kk < BM / 32 * (half + 1); kk++)
+                        mma_ts(tmem + Ly::O + s * HD, tmem + Ly::P + s * Ly::P_STEP + 8 * kk, b + 128 * kk, id_o,
+                               now.j > 0 || kk > 0);
                 }
-                it += nb;
-                taken0 += n0 > 0, taken1 += n1 > 0, cs0 += n0, cs1 += n1;
+                mma_commit(o_full(s));
+                if (now.last(s)) s ? tv1++ : tv0++;
+                s ? vc1++ : vc0++;
+            };
+            for (bool begun = false; more || begun; begun = true) {
+                // head_dim 64: scores of the next block of both sides, then values of this one; 128: side by side
+                if (begun) now = next;
+                more = more && advance();
+                if (!ok) break;
+                if (more) ok = wait(k_full(k_it % ST), (k_it / ST) & 1);
+                if (more && Ly::OWN_P) {
+#pragma unroll 1
+                    for (int s = 0; s < 2; s++)
+                        if (next.has(s)) scores(s);
+                    mma_commit(k_empty(k_it % ST)), k_it++;
+                }
+                if (begun) ok = ok && wait(v_good(v_it % ST), (v_it / ST) & 1);
+#pragma unroll 1
+                for (int s = 0; s < 2; s++) {
+                    if (begun && now.has(s)) values(s);
+                    if (more && !Ly::OWN_P && next.has(s)) scores(s);
+                }
+                if (!ok) break;
+                if (begun) mma_commit(v_empty(v_it % ST)), v_it++;
+                if (!more) break;
+                if (!Ly::OWN_P) mma_commit(k_empty(k_it % ST)), k_it++;
             }
             if (!ok) give_up();
         }
@@ -717,24 +735,26 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tc_fence_after();
                 float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
                 uint32_t r[128];
+                // r holds the block's quarters in order; on the diagonal from the warp's own quarter on, so that the one to mask
+                // by lane has fixed registers
+                const uint32_t turn = j == nb - 1 ? warp & 3 : 0;
 #pragma unroll
-                for (int q = 0; q < 4; q++) tmem_ld32(ts + 32 * q, r + 32 * q);
+                for (int q = 0; q < 4; q++) tmem_ld32(ts + 32 * ((turn + q) & 3), r + 32 * q);
                 tmem_wait_ld();
                 if (Ly::OWN_P) {
                     tc_fence_before();
                     __syncwarp();
                     mbar_arrive_if(s_free(s), lane == 0);
                 }
-                if (j == nb - 1) {  // the diagonal: row i sees its first i + 1 keys
-                    const int row = threadIdx.x & 127;
+                const bool diagonal = j == nb - 1;
+                if (diagonal) {  // row i sees its first i + 1 keys
+                    // r[0 .. 31] are the quarter where this warp's rows end (below); the quarters behind it are not seen at all.
 #pragma unroll
-                    for (int h = 0; h < 4; h++) {
-                        const int n_seen = row + 1 - 32 * h;
-                        const uint32_t seen = n_seen >= 32 ? 0xffffffffu : n_seen <= 0 ? 0u : (1u << n_seen) - 1;
+                    for (int q = 0; q < 32; q++)
+                        if (q > lane) r[q] = 0xff800000u;
 #pragma unroll
-                        for (int q = 0; q < 32; q++)
-                            if (!(seen & (1u << q))) r[32 * h + q] = 0xff800000u;
-                    }
+                    for (int q = 32; q < 128; q++)
+                        if ((warp & 3) + q / 32 < 4) r[q] = 0xff800000u;
                 }
                 const float top = row_max<128>(r);
                 const bool rise = (top - m) * c > 8.0f;  // true of a first block that has a score
@@ -746,17 +766,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                     tc_fence_after();
                 }
                 if (any_rise) raise(rise ? top : m, j > 0);
-                uint32_t pk[32];
-                exponentials<T>(r, c, off, sum, pk);
-                tmem_st16(tp, pk);
-                exponentials<T>(r + 32, c, off, sum, pk + 16);
-                tmem_st16(tp + 16, pk + 16);
-                exponentials<T>(r + 64, c, off, sum, pk);
-                publish(p_half(s));  // stored while the third quarter was computed
-                tmem_st16(tp + 32, pk);
-                exponentials<T>(r + 96, c, off, sum, pk + 16);
-                tmem_st16(tp + 48, pk + 16);
+                uint32_t pk[2][16];
+                exponentials<T>(r, c, off, sum, pk[0]);
+                tmem_st16(tp + 16 * turn, pk[0]);
+                exponentials<T>(r + 32, c, off, sum, pk[1]);
+                tmem_st16(tp + 16 * ((turn + 1) & 3), pk[1]);
+                exponentials<T>(r + 64, c, off, sum, pk[0]);
+                if (!diagonal) publish(p_half(s));  // its stores went on while this quarter was computed
+                tmem_st16(tp + 16 * ((turn + 2) & 3), pk[0]);
+                exponentials<T>(r + 96, c, off, sum, pk[1]);
+                tmem_st16(tp + 16 * ((turn + 3) & 3), pk[1]);
                 publish(p_full(s));
+                if (diagonal) mbar_arrive_if(p_half(s), lane == 0);
                 l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
             }
             ok = ok && wait_all(u_seen(slot), (n / kSlots) & 1);
@@ -773,21 +794,24 @@ __global__ void __launch_bounds__(kThreads, 1)
                 uint4* stage = reinterpret_cast<uint4*>(smem + Ly::OUT_OFF + warp * 4096);
 #pragma unroll 1
                 for (int q = 0; q < HD; q += 64) {
+                    uint32_t o[64];
+                    tmem_ld32(to + q, o);
+                    tmem_ld32(to + q + 32, o + 32);
+                    tmem_wait_ld();
+                    if (q + 64 == HD) {
+                        tc_fence_before();
+                        __syncwarp();
+                        mbar_arrive_if(o_free(s), lane == 0);
+                    }
                     // a row's 128 bytes by its own thread, chunks permuted by the row against bank conflicts; then
                     // eight lanes store one row
-#pragma unroll 1
-                    for (int w = 0; w < 8; w += 4) {
-                        uint32_t o[32];
-                        tmem_ld32(to + q + 8 * w, o);
-                        tmem_wait_ld();
 #pragma unroll
-                        for (int x = 0; x < 4; x++) {
-                            uint32_t y[4];
+                    for (int x = 0; x < 8; x++) {
+                        uint32_t y[4];
 #pragma unroll
-                            for (int e = 0; e < 4; e++)
-                                y[e] = pack2<T>(__uint_as_float(o[8 * x + 2 * e]) * inv, __uint_as_float(o[8 * x + 2 * e + 1]) * inv);
-                            stage[lane * 8 + ((w + x) ^ (lane & 7))] = make_uint4(y[0], y[1], y[2], y[3]);
-                        }
+                        for (int e = 0; e < 4; e++)
+                            y[e] = pack2<T>(__uint_as_float(o[8 * x + 2 * e]) * inv, __uint_as_float(o[8 * x + 2 * e + 1]) * inv);
+                        stage[lane * 8 + (x ^ (lane & 7))] = make_uint4(y[0], y[1], y[2], y[3]);
                     }
                     __syncwarp();
 #pragma unroll
@@ -799,9 +823,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     __syncwarp();
                 }
-                tc_fence_before();
-                __syncwarp();
-                mbar_arrive_if(o_free(s), lane == 0);
                 if (bad)
                     for (int w = 0; w < 32 && i + w < len; w++) plain_row<T, HD>(p, first, i + w, head, head / p.group);
             }
