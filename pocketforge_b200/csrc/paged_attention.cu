@@ -1,61 +1,652 @@
-// paged_attention.cu — attention of the newest tokens over the paged cache.
+// paged_attention.cu — attention of the newest tokens over the paged cache,
+// split over the cache's length and joined.
+//
+//   out = sum_j softmax_j(scale * q . k_j) v_j   over the positions a row sees
+//
+// Bound by HBM: every key and value is read once for all the query rows of its
+// kv head (the group's heads times the newest tokens), so the work is laid out
+// as one list of 128-entry chunks over all (sequence, kv head, row group)
+// segments and cut into equal runs, one a CTA, however long or short the
+// sequences are.  A segment that lies in several runs is joined by the CTA that
+// comes to its end last, in the order of the runs (the answer does not depend
+// on who that is).
+//
+// A CTA has four warps; each takes every fourth 32-entry block of the run, with
+// its own ring of blocks in flight (cp.async, no barrier between warps) and its
+// own running softmax, and the four are put together at a segment's end.  The
+// products are 16x8x16 tensor-core ones with the entries (S^T = K Q^T) and the
+// dims (O^T = V^T P^T) as the 16 and the query rows as the 8, so a few rows
+// waste little; which entry or dim stands where in an operand is free as long
+// as both operands agree, and is chosen so that every thread reads 16 (int8
+// head_dim 64 values: 8) bytes of a stored row at a time, in banks apart.  The
+// transposition that V needs is a byte permutation of two entries' words.
+//
+// Accuracy.  int8 codes are exact in fp16, and fp32 queries are split into two
+// fp16 planes (22 bits) after a power of two takes the row's largest value to
+// 2^13..2^14.  Over an int8 cache weights are two fp16 planes as well; they take
+// the entry's scale, and a power of two that keeps a block's largest below 2^15.
+// Over a 16-bit cache weights are rounded to its type (both operands of a
+// product have one type), an error like the output's own rounding; a second
+// plane would turn an inf among the values into NaN.  A block's products
+// start from zero and are added to O in fp32 with rounding, as the tensor cores
+// cut sums off instead, which would add up over a long cache.
+//
+// A row sees nothing behind its own position: those entries' weights are 0 by
+// selection, entries behind the sequence's end are zeros in shared memory, and
+// a 16-bit cache's last block is multiplied once for each new token with the
+// values it may not see set to 0 (0 x inf would be NaN).
+#include <algorithm>
+#include <climits>
+#include <type_traits>
+
 #include "paged.cuh"
-#include "row_attention.cuh"
 
 namespace pf {
 
 namespace {
+
+constexpr int kWarps = 4;
+constexpr int kBlock = 32;                  // entries a warp takes at a time
+constexpr int kChunk = kWarps * kBlock;     // entries the CTA takes at a time
+constexpr int kMaxCtas = 1024;              // counters at the start of `work`
 
 struct PagedParams {
     pf_paged_cache c;
     const void* q;
     void* out;
     int64_t q_stride, out_stride;
-    int layer, n_seqs, rows, n_heads;
+    int layer, n_seqs, rows, n_heads, dtype;
+    int group, cols, row_groups, page_shift;  // heads a kv head; rows x group; tiles of them; log2 page_size
     float scale;
+    int* count;    // [kMaxCtas] parts of the segment that begins in a CTA's run, arrived so far
+    float* part;   // [CTA][2][columns a row group][head_dim + 2]
     uint32_t* err;
 };
 
-// One warp a (sequence, row, head).
-template <typename QT, typename CT, int HD>
-__global__ void __launch_bounds__(32) paged_rows_kernel(const PagedParams p) {
-    constexpr int N = HD / 32;
-    const pf_paged_cache& c = p.c;
-    const int lane = threadIdx.x, h = blockIdx.y, g = h / (p.n_heads / c.n_kv_heads);
-    const int64_t i = blockIdx.x;
-    const int b = (int)(i / p.rows), r = (int)(i % p.rows);
-    const int n = seq_len(c, b, p.err) - p.rows + 1 + r;
-    float q[N];
-#pragma unroll
-    for (int d = 0; d < N; d++) q[d] = (float)static_cast<const QT*>(p.q)[i * p.q_stride + h * HD + lane + 32 * d] * p.scale;
-    RowSoftmax<HD> s;
-    for (int j = 0; j < n; j++) {
-        const int page = c.table[(int64_t)b * c.max_pages + j / c.page_size];
-        if ((unsigned)page >= (unsigned)c.n_pages) {
-            latch(p.err, ERR_BOUNDS);
-            continue;
-        }
-        const int64_t row = slot_row(c, page, p.layer, g, j % c.page_size);
-        const float ks = sizeof(CT) == 1 ? c.k_scale[row] : 1.0f, vs = sizeof(CT) == 1 ? c.v_scale[row] : 1.0f;
-        float k[N], v[N];
-#pragma unroll
-        for (int d = 0; d < N; d++) {
-            k[d] = (float)static_cast<const CT*>(c.k)[row * HD + lane + 32 * d] * ks;
-            v[d] = (float)static_cast<const CT*>(c.v)[row * HD + lane + 32 * d] * vs;
-        }
-        s.add(warp_dot(q, k), v);
-    }
-#pragma unroll
-    for (int d = 0; d < N; d++)
-        static_cast<QT*>(p.out)[i * p.out_stride + h * HD + lane + 32 * d] = (QT)(s.l == 0.0f ? 0.0f : s.o[d] / s.l);
+template <typename CT, int HD>
+struct Ring {
+    static constexpr int RB = HD * (int)sizeof(CT);                 // bytes of a stored row
+    static constexpr int SCALES = sizeof(CT) == 1 ? 2 * kBlock * 4 : 0;
+    static constexpr int BYTES = 2 * kBlock * RB + SCALES;          // keys, values, scales of a block
+    static constexpr int STAGES = RB == 64 ? 4 : 3;
+    static constexpr int SMEM = kWarps * STAGES * BYTES;
+    static constexpr int CTAS = RB == 64 ? 3 : (RB == 128 ? 2 : 1);  // that fit an SM
+};
+
+// Where 16-byte piece c of row r lies: rows read together in other banks.
+template <int RB>
+__device__ __forceinline__ int key_at(int r, int c) {
+    return RB == 64 ? r * RB + c * 16 : r * RB + (c ^ ((r & 1) << 2)) * 16;
+}
+template <int RB>
+__device__ __forceinline__ int value_row(int r) {
+    return RB == 64 ? (r & ~3) | ((r & 1) << 1) | ((r >> 1) & 1) : r;
+}
+template <int RB>
+__device__ __forceinline__ int value_at(int r, int c) {
+    const int at = value_row<RB>(r);
+    return RB == 64 ? at * RB + (c ^ (((at >> 2) & 1) << 1)) * 16 : at * RB + (c ^ (((r >> 1) & 3) << 1)) * 16;
 }
 
-template <typename QT, typename CT>
-pf_status launch_paged(const PagedParams& p, cudaStream_t st) {
-    const dim3 grid(p.n_seqs * p.rows, p.n_heads);
-    if (p.c.head_dim == 64) paged_rows_kernel<QT, CT, 64><<<grid, 32, 0, st>>>(p);
-    else paged_rows_kernel<QT, CT, 128><<<grid, 32, 0, st>>>(p);
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool on) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src, bool on) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(on ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+template <bool BF>
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                    uint32_t b1) {
+    if constexpr (BF)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+// Two bytes (already +128) of x in halves: 0x6400 + u is 1024 + u in fp16.
+__device__ __forceinline__ uint32_t bytes_to_half2(uint32_t x, uint32_t sel) {
+    const uint32_t h = __byte_perm(x, 0x64646464u, sel);
+    const __half2 y = __hsub2(reinterpret_cast<const __half2&>(h), __half2half2(__ushort_as_half(0x6480)));  // 1152
+    return reinterpret_cast<const uint32_t&>(y);
+}
+template <bool BF>
+__device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    uint32_t r;
+    if constexpr (BF) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+template <bool BF>
+__device__ __forceinline__ float2 unpack(uint32_t x) {
+    if constexpr (BF) return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+    else return __half22float2(reinterpret_cast<const __half2&>(x));
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// 2^k for k in [-126, 127], as a float.
+__device__ __forceinline__ float power_of_two(int k) { return __int_as_float((k + 127) << 23); }
+// floor(log2 x) of a finite x > 0 (-127 for subnormal ones).
+__device__ __forceinline__ int exponent_of(float x) { return (__float_as_int(x) >> 23) - 127; }
+
+__device__ __forceinline__ float load_q(const void* q, int64_t i, int dtype) {
+    if (dtype == PF_F32) return static_cast<const float*>(q)[i];
+    if (dtype == PF_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(q)[i]);
+    return __half2float(static_cast<const __half*>(q)[i]);
+}
+__device__ __forceinline__ void store_out(void* out, int64_t i, int dtype, float x) {
+    if (dtype == PF_F32) static_cast<float*>(out)[i] = x;
+    else if (dtype == PF_BF16) static_cast<__nv_bfloat16*>(out)[i] = __float2bfloat16_rn(x);
+    else static_cast<__half*>(out)[i] = __float2half_rn(x);
+}
+
+// A sequence's length as it counts here, and its chunks (one even if it is empty: its rows are zeros).
+__device__ __forceinline__ int length_of(const PagedParams& p, int b, uint32_t* err) { return max(seq_len(p.c, b, err), 0); }
+__device__ __forceinline__ int chunks_of(int len) { return max((len + kChunk - 1) / kChunk, 1); }
+
+// Output rows: column x of kv head g is head g * group + x % group of token x / group.
+__device__ __forceinline__ int64_t row_of(const PagedParams& p, int b, int x) { return (int64_t)b * p.rows + x / p.group; }
+
+template <typename CT, int HD, int NT, int PLANES>
+__global__ void __launch_bounds__(kWarps * 32, Ring<CT, HD>::CTAS) paged_kernel(const PagedParams p) {
+    using R = Ring<CT, HD>;
+    constexpr int RB = R::RB, ST = R::STAGES;
+    constexpr bool I8 = sizeof(CT) == 1, BF = std::is_same<CT, __nv_bfloat16>::value;
+    constexpr int KS = HD / 16;        // products along the dims of a score
+    constexpr int MT = HD / 16;        // 16-dim tiles of the output
+    constexpr int COLS = 8 * NT;
+    constexpr int VP = I8 ? 2 : 1;     // planes of a weight
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ long long s_sum[kWarps], s_before;
+    __shared__ int s_seq, s_last;
+    const pf_paged_cache& c = p.c;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, t = lane & 3;
+    const int segs = c.n_kv_heads * p.row_groups;  // of one sequence
+
+    // ---- this CTA's run of chunks ----
+    long long mine = 0;
+    for (int b = threadIdx.x; b < p.n_seqs; b += kWarps * 32)
+        mine += chunks_of(length_of(p, b, blockIdx.x == 0 ? p.err : nullptr));
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    if (lane == 0) s_sum[warp] = mine;
+    __syncthreads();
+    const long long total = (s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3]) * segs;
+    const long long per = (total + gridDim.x - 1) / gridDim.x, begin = per * blockIdx.x, end = min(begin + per, total);
+    if (begin >= end) return;
+    if (warp == 0) {  // the sequence that the run begins in
+        long long before = 0;
+        for (int b0 = 0;; b0 += 32) {
+            const int b = b0 + lane;
+            const long long n = b < p.n_seqs ? (long long)chunks_of(length_of(p, b, nullptr)) * segs : 0;
+            long long upto = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long x = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += x;
+            }
+            const unsigned here = __ballot_sync(0xffffffffu, begin < before + upto);
+            if (here) {
+                const int at = __ffs((int)here) - 1;
+                if (lane == at) s_seq = b, s_before = before + upto - n;
+                break;
+            }
+            before += __shfl_sync(0xffffffffu, upto, 31);
+        }
+    }
+    __syncthreads();
+    int seq = s_seq;
+    long long seq_begin = s_before;
+
+    uint8_t* ring = smem + warp * ST * R::BYTES;
+    const uint32_t ring_u32 = (uint32_t)__cvta_generic_to_shared(ring);
+    const int64_t page_bytes = (int64_t)c.n_layers * c.n_kv_heads * c.page_size * RB;
+    const int64_t page_slots = (int64_t)c.n_layers * c.n_kv_heads * c.page_size;
+
+    for (long long w = begin; w < end;) {
+        const int len = length_of(p, seq, nullptr), chunks = chunks_of(len);
+        const int seg = (int)((w - seq_begin) / chunks), g = seg / p.row_groups, rg = seg - g * p.row_groups;
+        const long long seg_begin = seq_begin + (long long)seg * chunks;
+        const int ch0 = (int)(w - seg_begin), ch1 = (int)min((long long)chunks, ch0 + (end - w));
+        const int x0 = rg * COLS, cols = min(COLS, p.cols - x0);  // this row group's columns
+        const int sees_all = len - p.rows + 1;                    // entries that the first new token sees
+
+        // ---- queries ----
+        uint32_t q[NT][PLANES][KS][2];
+        float cf[NT][2];  // score units -> log2 units, for this thread's columns 2t, 2t + 1
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            const int x = 8 * nt + gr;
+            const bool on = x < cols;
+            const int64_t at = on ? row_of(p, seq, x0 + x) * p.q_stride + (g * p.group + (x0 + x) % p.group) * HD : 0;
+            float f = 1.0f;
+            if constexpr (I8) {
+                // piece j of the row's 16-byte ones that this thread reads: dims 64 j + 16 t ..
+                float v[HD / 4];
+                float big = 0.0f;
+#pragma unroll
+                for (int j = 0; j < HD / 64; j++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        v[16 * j + i] = on ? load_q(p.q, at + 64 * j + 16 * t + i, p.dtype) : 0.0f;
+                        big = fmaxf(big, fabsf(v[16 * j + i]));
+                    }
+                big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+                big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+                if (big > 0.0f && big < __int_as_float(0x7f800000))
+                    f = power_of_two(min(max(13 - exponent_of(big), -100), 100));
+#pragma unroll
+                for (int i = 0; i < HD / 4; i += 2) {
+                    const float a = v[i] * f, b = v[i + 1] * f;
+                    const uint32_t hi = pack<false>(a, b);
+                    q[nt][0][i / 4][i / 2 % 2] = hi;
+                    if constexpr (PLANES == 2) {
+                        const float2 h = unpack<false>(hi);
+                        q[nt][1][i / 4][i / 2 % 2] = pack<false>(a - h.x, b - h.y);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < HD / 32; j++) {
+                    uint4 v = make_uint4(0, 0, 0, 0);
+                    if (on) v = *reinterpret_cast<const uint4*>(static_cast<const CT*>(p.q) + at + 32 * j + 8 * t);
+                    q[nt][0][2 * j][0] = v.x, q[nt][0][2 * j][1] = v.y;
+                    q[nt][0][2 * j + 1][0] = v.z, q[nt][0][2 * j + 1][1] = v.w;
+                }
+            }
+            const float all = p.scale * 1.4426950408889634f / f;  // f is a power of two
+            cf[nt][0] = __shfl_sync(0xffffffffu, all, 8 * t);
+            cf[nt][1] = __shfl_sync(0xffffffffu, all, 8 * t + 4);
+        }
+        // Entries that this thread's two columns of each tile see.
+        int sees[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const int x = 8 * nt + 2 * t + i;
+                sees[nt][i] = x < cols ? sees_all + (x0 + x) / p.group : 0;
+            }
+
+        // ---- the ring: block k of this warp is entries first(k) .. + 31 ----
+        const int n_blocks = ch1 - ch0;
+        auto first_entry = [&](int k) { return ((ch0 + k) * kWarps + warp) * kBlock; };
+        const int* table = c.table + (int64_t)seq * c.max_pages;
+        // Page of the block's 16-entry half; -1: none of it is there.
+        auto page_of = [&](int k, int half) {
+            const int e = first_entry(k) + 16 * half;
+            if (k >= n_blocks || e >= len) return -1;
+            const int page = table[e >> p.page_shift];
+            if ((unsigned)page < (unsigned)c.n_pages) return page;
+            latch(p.err, ERR_BOUNDS);
+            return -1;
+        };
+        auto issue = [&](int k, int page0, int page1) {
+            const int e0 = first_entry(k);
+            const uint32_t to = ring_u32 + (k % ST) * R::BYTES;
+            const int64_t row0 = ((int64_t)p.layer * c.n_kv_heads + g) * c.page_size;
+            constexpr int PR = RB / 16;          // pieces of a row
+            constexpr int STEP = 32 / PR;        // rows a pass (16: RB = 256 has two)
+#pragma unroll
+            for (int r0 = 0; r0 < kBlock; r0 += STEP) {
+                const int r = r0 + lane / PR, piece = lane % PR, e = e0 + r;
+                const int page = r0 < 16 ? page0 : page1;
+                const bool on = page >= 0 && e < len;
+                const int64_t from = (on ? page : 0) * page_bytes + (row0 + (e & (c.page_size - 1))) * RB + piece * 16;
+                copy16(to + key_at<RB>(r, piece), static_cast<const uint8_t*>(c.k) + from, on);
+                copy16(to + kBlock * RB + value_at<RB>(r, piece), static_cast<const uint8_t*>(c.v) + from, on);
+            }
+            if constexpr (I8) {
+                const int e = e0 + lane, page = lane < 16 ? page0 : page1;
+                const bool on = page >= 0 && e < len;
+                const int64_t from = (on ? page : 0) * page_slots + row0 + (e & (c.page_size - 1));
+                copy4(to + 2 * kBlock * RB + 4 * lane, c.k_scale + from, on);
+                copy4(to + 2 * kBlock * RB + 4 * (kBlock + lane), c.v_scale + from, on);
+            }
+        };
+        int page0 = page_of(0, 0), page1 = page_of(0, 1);
+#pragma unroll
+        for (int k = 0; k < ST - 1; k++) {
+            const int n0 = page_of(k + 1, 0), n1 = page_of(k + 1, 1);
+            if (k < n_blocks) issue(k, page0, page1);
+            copy_commit();
+            page0 = n0, page1 = n1;
+        }
+
+        // ---- running softmax ----
+        float o[MT][NT][4], m[NT][2], l[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            m[nt][0] = m[nt][1] = -INFINITY;
+            l[nt][0] = l[nt][1] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < MT; i++) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.0f;
+        }
+        for (int k = 0; k < n_blocks; k++) {
+            {
+                const int n0 = page_of(k + ST, 0), n1 = page_of(k + ST, 1);
+                __syncwarp();  // every lane is through with the block whose place is filled now
+                if (k + ST - 1 < n_blocks) issue(k + ST - 1, page0, page1);
+                copy_commit();
+                page0 = n0, page1 = n1;
+            }
+            copy_wait<ST - 1>();
+            __syncwarp();
+            const int e0 = first_entry(k);
+            if (e0 >= len) break;  // the sequence ends in another warp's block
+            const uint8_t* kb = ring + (k % ST) * R::BYTES;
+            const uint8_t* vb = kb + kBlock * RB;
+            const float* scales = reinterpret_cast<const float*>(vb + kBlock * RB);
+
+            // scores of 2 x 16 entries: rows gr, gr + 8 of each, in log2 units
+            float s[2][NT][4];
+#pragma unroll
+            for (int mt = 0; mt < 2; mt++) {
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) s[mt][nt][0] = s[mt][nt][1] = s[mt][nt][2] = s[mt][nt][3] = 0.0f;
+                const int r0 = 16 * mt + gr, r1 = r0 + 8;
+#pragma unroll
+                for (int j = 0; j < RB / 64; j++) {  // pieces t, t + 4, ...
+                    const uint4 a = *reinterpret_cast<const uint4*>(kb + key_at<RB>(r0, 4 * j + t));
+                    const uint4 b = *reinterpret_cast<const uint4*>(kb + key_at<RB>(r1, 4 * j + t));
+                    const uint32_t wa[4] = {a.x, a.y, a.z, a.w}, wb[4] = {b.x, b.y, b.z, b.w};
+                    if constexpr (I8) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const uint32_t ua = wa[i] ^ 0x80808080u, ub = wb[i] ^ 0x80808080u;
+                            const uint32_t a0 = bytes_to_half2(ua, 0x4140), a2 = bytes_to_half2(ua, 0x4342);
+                            const uint32_t a1 = bytes_to_half2(ub, 0x4140), a3 = bytes_to_half2(ub, 0x4342);
+#pragma unroll
+                            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                                for (int pl = 0; pl < PLANES; pl++)
+                                    mma<false>(s[mt][nt], a0, a1, a2, a3, q[nt][pl][4 * j + i][0], q[nt][pl][4 * j + i][1]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 2; i++)
+#pragma unroll
+                            for (int nt = 0; nt < NT; nt++)
+                                mma<BF>(s[mt][nt], wa[2 * i], wb[2 * i], wa[2 * i + 1], wb[2 * i + 1],
+                                        q[nt][0][2 * j + i][0], q[nt][0][2 * j + i][1]);
+                    }
+                }
+            }
+            // scales, mask; does any score lie 2^8 above its column's maximum?
+            const bool tail = e0 + kBlock > sees_all;  // some entry is not seen by every column
+            bool rise = false;
+#pragma unroll
+            for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const int r = 16 * mt + 8 * h + gr;
+                    const float ks = I8 ? scales[r] : 1.0f;
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                        for (int i = 0; i < 2; i++) {
+                            float& x = s[mt][nt][2 * h + i];
+                            x = I8 ? x * (ks * cf[nt][i]) : x * cf[nt][i];
+                            if (tail && e0 + r >= sees[nt][i]) x = -INFINITY;
+                            rise |= x - m[nt][i] > 8.0f;
+                        }
+                }
+            if (__any_sync(0xffffffffu, rise)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        float top = fmaxf(fmaxf(s[0][nt][i], s[0][nt][2 + i]), fmaxf(s[1][nt][i], s[1][nt][2 + i]));
+#pragma unroll
+                        for (int x = 4; x <= 16; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+                        if (top - m[nt][i] > 8.0f) {  // no other column has a say: a row stays the same whatever its neighbours are
+                            const float f = exp2_approx(m[nt][i] - top);
+                            m[nt][i] = top;
+                            l[nt][i] *= f;
+#pragma unroll
+                            for (int d = 0; d < MT; d++) o[d][nt][i] *= f, o[d][nt][2 + i] *= f;
+                        }
+                    }
+            }
+            // weights
+            float vscale = 1.0f, back = 1.0f;
+            if constexpr (I8) {
+                float big = scales[kBlock + lane];
+                big = fabsf(big) < __int_as_float(0x7f800000) ? fabsf(big) : 0.0f;  // inf and NaN make their own way
+#pragma unroll
+                for (int x = 16; x >= 1; x >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, x));
+                const int up = min(max(6 - exponent_of(big), -100), 100);  // p <= 2^8, so p v_scale 2^up < 2^15
+                vscale = power_of_two(up), back = power_of_two(-up);
+            }
+            uint32_t pw[2][NT][VP][2];  // [entries 16 mt ..][column tile][plane][first, second 8 entries], transposed
+#pragma unroll
+            for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const int r = 16 * mt + 8 * h + gr;
+                    const float vs = I8 ? scales[kBlock + r] * vscale : 1.0f;
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) {
+                        float y[2];
+#pragma unroll
+                        for (int i = 0; i < 2; i++) {
+                            const float x = s[mt][nt][2 * h + i];
+                            const float e = exp2_approx(x - (m[nt][i] == -INFINITY ? 0.0f : m[nt][i]));
+                            l[nt][i] += e;
+                            y[i] = I8 ? e * vs : e;
+                            if (tail && e0 + r >= sees[nt][i]) y[i] = 0.0f;  // whatever the entry's scale is
+                        }
+                        const uint32_t hi = pack<BF>(y[0], y[1]);
+                        pw[mt][nt][0][h] = transpose8x8(hi);
+                        if constexpr (VP == 2) {  // an inf or NaN stays in the first plane
+                            const float2 got = unpack<BF>(hi);
+                            const float inf = __int_as_float(0x7f800000);
+                            pw[mt][nt][1][h] = transpose8x8(pack<BF>(fabsf(got.x) < inf ? y[0] - got.x : 0.0f,
+                                                                     fabsf(got.y) < inf ? y[1] - got.y : 0.0f));
+                        }
+                    }
+                }
+            // values
+            const int passes = !I8 && tail && p.rows > 1 ? p.rows : 1;
+            for (int pass = 0; pass < passes; pass++) {
+                // one pass for all, or one a new token with what it may not see set to 0
+                const int upto = passes == 1 ? INT_MAX : sees_all + pass - e0;
+                constexpr int VB = RB == 64 ? 8 : 16;  // bytes of a row this thread reads at a time
+                constexpr int W = VB / 4, GROUPS = RB / 8 / VB, PER = MT / GROUPS;
+#pragma unroll
+                for (int gi = 0; gi < GROUPS; gi++) {
+                    uint32_t v[2][4][W];  // entries 16 mt + 2t, 2t + 1, 2t + 8, 2t + 9
+#pragma unroll
+                    for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const int r = 16 * mt + 2 * t + (e & 1) + 8 * (e >> 1);
+                            if constexpr (W == 2) {
+                                const uint2 x = *reinterpret_cast<const uint2*>(vb + value_at<RB>(r, gr >> 1) + 8 * (gr & 1));
+                                v[mt][e][0] = x.x ^ 0x80808080u, v[mt][e][1] = x.y ^ 0x80808080u;
+                            } else {
+                                uint4 x = *reinterpret_cast<const uint4*>(vb + value_at<RB>(r, 8 * gi + gr));
+                                if (!I8 && r >= upto) x = make_uint4(0, 0, 0, 0);
+                                const uint32_t flip = I8 ? 0x80808080u : 0u;
+                                v[mt][e][0] = x.x ^ flip, v[mt][e][1] = x.y ^ flip, v[mt][e][2] = x.z ^ flip, v[mt][e][3] = x.w ^ flip;
+                            }
+                        }
+#pragma unroll
+                    for (int i = 0; i < PER; i++) {
+                        float acc[NT][4];
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.0f;
+#pragma unroll
+                        for (int mt = 0; mt < 2; mt++) {
+                            uint32_t a0, a1, a2, a3;
+                            if constexpr (I8) {
+                                // word i / 2: four dims; its first two (i even) or last two, of two entries each
+                                const uint32_t sel = i & 1 ? 0x7362 : 0x5140;
+                                const uint32_t x = __byte_perm(v[mt][0][i / 2], v[mt][1][i / 2], sel);
+                                const uint32_t y = __byte_perm(v[mt][2][i / 2], v[mt][3][i / 2], sel);
+                                a0 = bytes_to_half2(x, 0x4140), a1 = bytes_to_half2(x, 0x4342);
+                                a2 = bytes_to_half2(y, 0x4140), a3 = bytes_to_half2(y, 0x4342);
+                            } else {
+                                a0 = __byte_perm(v[mt][0][i], v[mt][1][i], 0x5410), a1 = __byte_perm(v[mt][0][i], v[mt][1][i], 0x7632);
+                                a2 = __byte_perm(v[mt][2][i], v[mt][3][i], 0x5410), a3 = __byte_perm(v[mt][2][i], v[mt][3][i], 0x7632);
+                            }
+#pragma unroll
+                            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                                for (int pl = 0; pl < VP; pl++)
+                                    mma<BF>(acc[nt], a0, a1, a2, a3, pw[mt][nt][pl][0], pw[mt][nt][pl][1]);
+                        }
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                if (!I8 && passes > 1 && sees[nt][e & 1] != upto + e0) continue;  // another token's pass
+                                float& to = o[gi * PER + i][nt][e];
+                                to = I8 ? fmaf(acc[nt][e], back, to) : to + acc[nt][e];
+                            }
+                    }
+                }
+            }
+        }
+        copy_wait<0>();
+
+        // ---- the four warps' shares together ----
+        // smem: [warp][column][HD + 2], a row's last two its maximum and sum
+        constexpr int PITCH = HD + 2;
+        float* shared = reinterpret_cast<float*>(smem);
+        static_assert(kWarps * COLS * PITCH * 4 <= R::SMEM, "the shares fit the ring");
+        __syncthreads();  // the rings are empty
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                float sum = l[nt][i];
+#pragma unroll
+                for (int x = 4; x <= 16; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+                float* to = shared + (warp * COLS + 8 * nt + 2 * t + i) * PITCH;
+                if (gr == 0) to[HD] = m[nt][i], to[HD + 1] = sum;
+#pragma unroll
+                for (int d = 0; d < MT; d++) {
+                    // tile d's rows gr and gr + 8 are two neighbouring dims
+                    constexpr int VB = RB == 64 ? 8 : 16, PER = MT / (RB / 8 / VB), DIMS = VB / (int)sizeof(CT);
+                    const int dim = d / PER * (HD / (MT / PER)) + gr * DIMS + 2 * (d % PER);
+                    *reinterpret_cast<float2*>(to + dim) = make_float2(o[d][nt][i], o[d][nt][2 + i]);
+                }
+            }
+        __syncthreads();
+        const bool whole = ch0 == 0 && ch1 == chunks;
+        const int slot = ch0 == 0 ? 1 : 0;  // a CTA's run begins inside a segment once, and ends inside one once
+        float* part = p.part + ((int64_t)blockIdx.x * 2 + slot) * COLS * PITCH;
+        for (int i = threadIdx.x; i < cols * (HD / 2); i += kWarps * 32) {
+            const int x = i / (HD / 2), d = i % (HD / 2) * 2;
+            float top = -INFINITY;
+#pragma unroll
+            for (int s = 0; s < kWarps; s++) top = fmaxf(top, shared[(s * COLS + x) * PITCH + HD]);
+            float sum = 0.0f;
+            float2 v = make_float2(0.0f, 0.0f);
+#pragma unroll
+            for (int s = 0; s < kWarps; s++) {
+                const float* from = shared + (s * COLS + x) * PITCH;
+                const float f = from[HD] == -INFINITY ? 0.0f : exp2_approx(from[HD] - top);
+                // a warp without an entry has zeros; one whose sum is NaN has no maximum that says so
+                sum += from[HD + 1] * (from[HD] == -INFINITY ? 1.0f : f);
+                const float2 y = *reinterpret_cast<const float2*>(from + d);
+                v.x += y.x * (from[HD] == -INFINITY ? 1.0f : f), v.y += y.y * (from[HD] == -INFINITY ? 1.0f : f);
+            }
+            if (whole) {
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                const int64_t to = row_of(p, seq, x0 + x) * p.out_stride + (g * p.group + (x0 + x) % p.group) * HD + d;
+                store_out(p.out, to, p.dtype, v.x * inv);
+                store_out(p.out, to + 1, p.dtype, v.y * inv);
+            } else {
+                float* to = part + x * PITCH;
+                __stcg(reinterpret_cast<float2*>(to + d), v);
+                if (d == 0) __stcg(reinterpret_cast<float2*>(to + HD), make_float2(top, sum));
+            }
+        }
+        if (!whole) {
+            // ---- the segment's parts together, by the last to come ----
+            const int from = (int)(seg_begin / per), upto = (int)((seg_begin + chunks - 1) / per);  // CTAs it lies in
+            __threadfence();
+            __syncthreads();
+            if (threadIdx.x == 0) s_last = atomicAdd(&p.count[from], 1) == upto - from;
+            __syncthreads();
+            if (s_last) {
+                __threadfence();
+                if (threadIdx.x == 0) p.count[from] = 0;  // as it was found
+                for (int i = threadIdx.x; i < cols * (HD / 2); i += kWarps * 32) {
+                    const int x = i / (HD / 2), d = i % (HD / 2) * 2;
+                    float top = -INFINITY, sum = 0.0f;
+                    float2 v = make_float2(0.0f, 0.0f);
+#pragma unroll 4
+                    for (int cta = from; cta <= upto; cta++) {
+                        const float* a = p.part + (((int64_t)cta * 2 + (cta == from)) * COLS + x) * PITCH;
+                        const float2 ms = __ldcg(reinterpret_cast<const float2*>(a + HD));
+                        const float2 y = __ldcg(reinterpret_cast<const float2*>(a + d));
+                        const float m2 = fmaxf(top, ms.x);
+                        const float f0 = top == m2 ? 1.0f : exp2_approx(top - m2);
+                        const float f1 = ms.x == m2 || ms.x == -INFINITY ? 1.0f : exp2_approx(ms.x - m2);
+                        top = m2;
+                        sum = sum * f0 + ms.y * f1;
+                        v.x = v.x * f0 + y.x * f1, v.y = v.y * f0 + y.y * f1;
+                    }
+                    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                    const int64_t to = row_of(p, seq, x0 + x) * p.out_stride + (g * p.group + (x0 + x) % p.group) * HD + d;
+                    store_out(p.out, to, p.dtype, v.x * inv);
+                    store_out(p.out, to + 1, p.dtype, v.y * inv);
+                }
+            }
+        }
+        __syncthreads();  // the ring may be filled again
+        w = seg_begin + ch1;
+        if (seg == segs - 1 && ch1 == chunks) seq++, seq_begin = w;
+    }
+}
+
+// Column tiles of 8 that a CTA takes: as many as the rows need, up to what the registers hold.
+int tiles_for(int cols, int head_dim) { return std::min(ceil_div(cols, 8), head_dim == 64 ? 4 : 2); }
+
+int cta_limit(const pf_paged_cache& c) {
+    const int row = c.head_dim * type_bytes(c.dtype);
+    return 148 * (row == 64 ? 3 : (row == 128 ? 2 : 1));
+}
+
+template <typename CT, int HD, int NT, int PLANES>
+pf_status launch_tiles(PagedParams& p, cudaStream_t st) {
+    using R = Ring<CT, HD>;
+    p.row_groups = ceil_div(p.cols, 8 * NT);
+    const int64_t most = (int64_t)p.n_seqs * p.c.n_kv_heads * p.row_groups *
+                         std::max<int64_t>(((int64_t)p.c.max_pages * p.c.page_size + kChunk - 1) / kChunk, 1);
+    const int grid = (int)std::min<int64_t>(most, cta_limit(p.c));
+    static std::atomic<uint64_t> attr{0};
+    PF_TRY(raise_smem_limit(paged_kernel<CT, HD, NT, PLANES>, R::SMEM, attr));
+    paged_kernel<CT, HD, NT, PLANES><<<grid, kWarps * 32, R::SMEM, st>>>(p);
     return launch_check("paged_attention");
+}
+
+template <typename CT, int PLANES>
+pf_status launch_paged(PagedParams& p, cudaStream_t st) {
+    const int nt = tiles_for(p.cols, p.c.head_dim);
+    if (p.c.head_dim == 128) return nt == 1 ? launch_tiles<CT, 128, 1, PLANES>(p, st) : launch_tiles<CT, 128, 2, PLANES>(p, st);
+    if (nt == 1) return launch_tiles<CT, 64, 1, PLANES>(p, st);
+    if (nt == 2) return launch_tiles<CT, 64, 2, PLANES>(p, st);
+    return nt == 3 ? launch_tiles<CT, 64, 3, PLANES>(p, st) : launch_tiles<CT, 64, 4, PLANES>(p, st);
 }
 
 }  // namespace
@@ -68,7 +659,11 @@ extern "C" {
 
 size_t pf_paged_attention_work_bytes(const pf_paged_cache* c, int32_t n_seqs, int32_t rows, int32_t n_heads) {
     if (!c || n_seqs < 0 || rows < 1 || rows > 8 || n_heads < 1 || c->n_kv_heads < 1 || n_heads % c->n_kv_heads) return 0;
-    return 16;
+    if (c->head_dim != 64 && c->head_dim != 128) return 0;
+    const int cols = n_heads / c->n_kv_heads * rows;
+    // counters, then two parts a CTA
+    return kMaxCtas * sizeof(int) +
+           (size_t)cta_limit(*c) * 2 * 8 * tiles_for(cols, c->head_dim) * (c->head_dim + 2) * sizeof(float);
 }
 
 pf_status pf_paged_attention(const pf_paged_cache* c, int32_t layer, const void* q, int64_t q_stride, void* out,
@@ -93,13 +688,19 @@ pf_status pf_paged_attention(const pf_paged_cache* c, int32_t layer, const void*
     PF_TRY(require_device());
     if (n_seqs == 0) return PF_OK;
     PF_CHECK(q && out && work, "pf_paged_attention: null argument");
-    PagedParams p{*c, q, out, q_stride, out_stride, layer, n_seqs, rows, n_heads, scale, device_error_flag()};
+    PagedParams p{};
+    p.c = *c, p.q = q, p.out = out, p.q_stride = q_stride, p.out_stride = out_stride;
+    p.layer = layer, p.n_seqs = n_seqs, p.rows = rows, p.n_heads = n_heads, p.dtype = dtype;
+    p.group = n_heads / c->n_kv_heads, p.cols = p.group * rows;
+    p.page_shift = c->page_size == 16 ? 4 : c->page_size == 32 ? 5 : c->page_size == 64 ? 6 : 7;
+    p.scale = scale;
+    p.count = static_cast<int*>(work);
+    p.part = reinterpret_cast<float*>(static_cast<char*>(work) + kMaxCtas * sizeof(int));
+    p.err = device_error_flag();
     cudaStream_t st = as_stream(stream);
-    if (c->dtype == PF_BF16) return launch_paged<__nv_bfloat16, __nv_bfloat16>(p, st);
-    if (c->dtype == PF_F16) return launch_paged<__half, __half>(p, st);
-    if (dtype == PF_F32) return launch_paged<float, int8_t>(p, st);
-    if (dtype == PF_BF16) return launch_paged<__nv_bfloat16, int8_t>(p, st);
-    return launch_paged<__half, int8_t>(p, st);
+    if (c->dtype == PF_BF16) return launch_paged<__nv_bfloat16, 1>(p, st);
+    if (c->dtype == PF_F16) return launch_paged<__half, 1>(p, st);
+    return dtype == PF_F32 ? launch_paged<int8_t, 2>(p, st) : launch_paged<int8_t, 1>(p, st);
 }
 
 }  // extern "C"
