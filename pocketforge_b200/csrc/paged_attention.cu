@@ -4,16 +4,19 @@
 //   out = sum_j softmax_j(scale * q . k_j) v_j   over the positions a row sees
 //
 // Bound by HBM: every key and value is read once for all the query rows of its
-// kv head (the group's heads times the newest tokens), so the work is laid out
-// as one list of 128-entry chunks over all (sequence, kv head, row group)
-// segments and cut into equal runs, one a CTA, however long or short the
-// sequences are.  A segment that lies in several runs is joined by the CTA that
-// comes to its end last, in the order of the runs (the answer does not depend
-// on who that is).
+// kv head (the group's heads times the newest tokens).  A (sequence, kv head,
+// row group) is a segment of 128-entry chunks, cut into equal pieces of at most
+// P chunks, P being all chunks over the CTAs that fit the GPU: where there are
+// segments enough none is cut, and a few long ones are spread over every SM.
+// One CTA a piece; the pieces of a cut segment are joined by the CTA that ends
+// last, in their order (the answer does not depend on who that is).  (One run
+// of exactly total / CTAs chunks each, wherever it began and ended, balanced
+// better and measured twice as slow on 64 sequences of 512 to 1024: nearly
+// every CTA had two segments to begin, end and join.)
 //
-// A CTA has four warps; each takes every fourth 32-entry block of the run, with
-// its own ring of blocks in flight (cp.async, no barrier between warps) and its
-// own running softmax, and the four are put together at a segment's end.  The
+// A CTA has four warps; each takes every fourth 32-entry block of the piece,
+// with its own ring of blocks in flight (cp.async, no barrier between warps) and
+// its own running softmax, and the four are put together at the end.  The
 // products are 16x8x16 tensor-core ones with the entries (S^T = K Q^T) and the
 // dims (O^T = V^T P^T) as the 16 and the query rows as the 8, so a few rows
 // waste little; which entry or dim stands where in an operand is free as long
@@ -58,8 +61,9 @@ struct PagedParams {
     int layer, n_seqs, rows, n_heads, dtype;
     int group, cols, row_groups, page_shift;  // heads a kv head; rows x group; tiles of them; log2 page_size
     float scale;
-    int* count;    // [kMaxCtas] parts of the segment that begins in a CTA's run, arrived so far
-    float* part;   // [CTA][2][columns a row group][head_dim + 2]
+    int ctas;      // that fit the GPU
+    int* count;    // [kMaxCtas] pieces of a cut segment that have ended
+    float* part;   // [piece of a cut segment][columns a row group][head_dim + 2]
     uint32_t* err;
 };
 
@@ -112,6 +116,19 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
             : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
             : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// The same from zero.
+template <bool BF>
+__device__ __forceinline__ void mma_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                          uint32_t b1) {
+    if constexpr (BF)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     uint32_t y;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -130,6 +147,12 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
+// The same to fp16 with an inf taken down to the largest value.
+__device__ __forceinline__ uint32_t pack_finite(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
 template <bool BF>
 __device__ __forceinline__ float2 unpack(uint32_t x) {
     if constexpr (BF) return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
@@ -145,23 +168,41 @@ __device__ __forceinline__ float power_of_two(int k) { return __int_as_float((k 
 // floor(log2 x) of a finite x > 0 (-127 for subnormal ones).
 __device__ __forceinline__ int exponent_of(float x) { return (__float_as_int(x) >> 23) - 127; }
 
-__device__ __forceinline__ float load_q(const void* q, int64_t i, int dtype) {
-    if (dtype == PF_F32) return static_cast<const float*>(q)[i];
-    if (dtype == PF_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(q)[i]);
-    return __half2float(static_cast<const __half*>(q)[i]);
+// 16 values from element i on (16-byte aligned): fp32 (two planes) or a 16-bit type.
+template <int PLANES>
+__device__ __forceinline__ void load16(const void* q, int64_t i, int dtype, bool on, float* v) {
+    if constexpr (PLANES == 2) {
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const float4 x = on ? reinterpret_cast<const float4*>(static_cast<const float*>(q) + i)[k] : make_float4(0.f, 0.f, 0.f, 0.f);
+            v[4 * k] = x.x, v[4 * k + 1] = x.y, v[4 * k + 2] = x.z, v[4 * k + 3] = x.w;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const uint4 x = on ? reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(q) + i)[k] : make_uint4(0, 0, 0, 0);
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float2 y = dtype == PF_BF16 ? unpack<true>(w[e]) : unpack<false>(w[e]);
+                v[8 * k + 2 * e] = y.x, v[8 * k + 2 * e + 1] = y.y;
+            }
+        }
+    }
 }
-__device__ __forceinline__ void store_out(void* out, int64_t i, int dtype, float x) {
-    if (dtype == PF_F32) static_cast<float*>(out)[i] = x;
-    else if (dtype == PF_BF16) static_cast<__nv_bfloat16*>(out)[i] = __float2bfloat16_rn(x);
-    else static_cast<__half*>(out)[i] = __float2half_rn(x);
-}
-
 // A sequence's length as it counts here, and its chunks (one even if it is empty: its rows are zeros).
 __device__ __forceinline__ int length_of(const PagedParams& p, int b, uint32_t* err) { return max(seq_len(p.c, b, err), 0); }
 __device__ __forceinline__ int chunks_of(int len) { return max((len + kChunk - 1) / kChunk, 1); }
 
-// Output rows: column x of kv head g is head g * group + x % group of token x / group.
-__device__ __forceinline__ int64_t row_of(const PagedParams& p, int b, int x) { return (int64_t)b * p.rows + x / p.group; }
+// Dims d, d + 1 of column x of kv head g: head g * group + x % group of token x / group.
+__device__ __forceinline__ void store_out(const PagedParams& p, int seq, int g, int x, int d, int hd, float2 v) {
+    const int token = x / p.group, head = g * p.group + x - token * p.group;
+    const int64_t at = ((int64_t)seq * p.rows + token) * p.out_stride + head * hd + d;
+    if (p.dtype == PF_F32) *reinterpret_cast<float2*>(static_cast<float*>(p.out) + at) = v;
+    else
+        *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + at) =
+            p.dtype == PF_BF16 ? pack<true>(v.x, v.y) : pack<false>(v.x, v.y);
+}
 
 template <typename CT, int HD, int NT, int PLANES>
 __global__ void __launch_bounds__(kWarps * 32, Ring<CT, HD>::CTAS) paged_kernel(const PagedParams p) {
@@ -174,12 +215,12 @@ __global__ void __launch_bounds__(kWarps * 32, Ring<CT, HD>::CTAS) paged_kernel(
     constexpr int VP = I8 ? 2 : 1;     // planes of a weight
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ long long s_sum[kWarps], s_before;
-    __shared__ int s_seq, s_last;
+    __shared__ int s_seq, s_piece, s_last;
     const pf_paged_cache& c = p.c;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, t = lane & 3;
     const int segs = c.n_kv_heads * p.row_groups;  // of one sequence
 
-    // ---- this CTA's run of chunks ----
+    // ---- this CTA's piece ----
     long long mine = 0;
     for (int b = threadIdx.x; b < p.n_seqs; b += kWarps * 32)
         mine += chunks_of(length_of(p, b, blockIdx.x == 0 ? p.err : nullptr));
@@ -188,117 +229,66 @@ __global__ void __launch_bounds__(kWarps * 32, Ring<CT, HD>::CTAS) paged_kernel(
     if (lane == 0) s_sum[warp] = mine;
     __syncthreads();
     const long long total = (s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3]) * segs;
-    const long long per = (total + gridDim.x - 1) / gridDim.x, begin = per * blockIdx.x, end = min(begin + per, total);
-    if (begin >= end) return;
-    if (warp == 0) {  // the sequence that the run begins in
-        long long before = 0;
-        for (int b0 = 0;; b0 += 32) {
+    // chunks a piece: with more segments than CTAs that fit, only what is twice as long is cut
+    const long long share = (total + p.ctas - 1) / p.ctas;
+    const int most = (int)min((long long)p.n_seqs * segs >= p.ctas ? 2 * share : share, (long long)INT_MAX);
+    if (warp == 0) {  // the sequence that it belongs to
+        long long pieces = 0, chunks = 0;
+        int found = -1;
+        for (int b0 = 0; b0 < p.n_seqs && found < 0; b0 += 32) {
             const int b = b0 + lane;
-            const long long n = b < p.n_seqs ? (long long)chunks_of(length_of(p, b, nullptr)) * segs : 0;
-            long long upto = n;
+            const int n = b < p.n_seqs ? chunks_of(length_of(p, b, nullptr)) : 0;
+            const long long my_pieces = (long long)((n + most - 1) / most) * segs, my_chunks = (long long)n * segs;
+            long long upto = my_pieces, upto_chunks = my_chunks;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const long long x = __shfl_up_sync(0xffffffffu, upto, o);
-                if (lane >= o) upto += x;
+                const long long x = __shfl_up_sync(0xffffffffu, upto, o), y = __shfl_up_sync(0xffffffffu, upto_chunks, o);
+                if (lane >= o) upto += x, upto_chunks += y;
             }
-            const unsigned here = __ballot_sync(0xffffffffu, begin < before + upto);
+            const unsigned here = __ballot_sync(0xffffffffu, blockIdx.x < pieces + upto);
             if (here) {
                 const int at = __ffs((int)here) - 1;
-                if (lane == at) s_seq = b, s_before = before + upto - n;
-                break;
+                if (lane == at) s_piece = (int)(blockIdx.x - (pieces + upto - my_pieces)), s_before = chunks + upto_chunks - my_chunks;
+                found = b0 + at;
             }
-            before += __shfl_sync(0xffffffffu, upto, 31);
+            pieces += __shfl_sync(0xffffffffu, upto, 31);
+            chunks += __shfl_sync(0xffffffffu, upto_chunks, 31);
         }
+        if (lane == 0) s_seq = found;
     }
     __syncthreads();
-    int seq = s_seq;
-    long long seq_begin = s_before;
+    const int seq = s_seq;
+    if (seq < 0) return;  // the grid is an upper bound
 
     uint8_t* ring = smem + warp * ST * R::BYTES;
     const uint32_t ring_u32 = (uint32_t)__cvta_generic_to_shared(ring);
     const int64_t page_bytes = (int64_t)c.n_layers * c.n_kv_heads * c.page_size * RB;
     const int64_t page_slots = (int64_t)c.n_layers * c.n_kv_heads * c.page_size;
-
-    for (long long w = begin; w < end;) {
-        const int len = length_of(p, seq, nullptr), chunks = chunks_of(len);
-        const int seg = (int)((w - seq_begin) / chunks), g = seg / p.row_groups, rg = seg - g * p.row_groups;
-        const long long seg_begin = seq_begin + (long long)seg * chunks;
-        const int ch0 = (int)(w - seg_begin), ch1 = (int)min((long long)chunks, ch0 + (end - w));
-        const int x0 = rg * COLS, cols = min(COLS, p.cols - x0);  // this row group's columns
-        const int sees_all = len - p.rows + 1;                    // entries that the first new token sees
-
-        // ---- queries ----
-        uint32_t q[NT][PLANES][KS][2];
-        float cf[NT][2];  // score units -> log2 units, for this thread's columns 2t, 2t + 1
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-            const int x = 8 * nt + gr;
-            const bool on = x < cols;
-            const int64_t at = on ? row_of(p, seq, x0 + x) * p.q_stride + (g * p.group + (x0 + x) % p.group) * HD : 0;
-            float f = 1.0f;
-            if constexpr (I8) {
-                // piece j of the row's 16-byte ones that this thread reads: dims 64 j + 16 t ..
-                float v[HD / 4];
-                float big = 0.0f;
-#pragma unroll
-                for (int j = 0; j < HD / 64; j++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        v[16 * j + i] = on ? load_q(p.q, at + 64 * j + 16 * t + i, p.dtype) : 0.0f;
-                        big = fmaxf(big, fabsf(v[16 * j + i]));
-                    }
-                big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
-                big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-                if (big > 0.0f && big < __int_as_float(0x7f800000))
-                    f = power_of_two(min(max(13 - exponent_of(big), -100), 100));
-#pragma unroll
-                for (int i = 0; i < HD / 4; i += 2) {
-                    const float a = v[i] * f, b = v[i + 1] * f;
-                    const uint32_t hi = pack<false>(a, b);
-                    q[nt][0][i / 4][i / 2 % 2] = hi;
-                    if constexpr (PLANES == 2) {
-                        const float2 h = unpack<false>(hi);
-                        q[nt][1][i / 4][i / 2 % 2] = pack<false>(a - h.x, b - h.y);
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < HD / 32; j++) {
-                    uint4 v = make_uint4(0, 0, 0, 0);
-                    if (on) v = *reinterpret_cast<const uint4*>(static_cast<const CT*>(p.q) + at + 32 * j + 8 * t);
-                    q[nt][0][2 * j][0] = v.x, q[nt][0][2 * j][1] = v.y;
-                    q[nt][0][2 * j + 1][0] = v.z, q[nt][0][2 * j + 1][1] = v.w;
-                }
-            }
-            const float all = p.scale * 1.4426950408889634f / f;  // f is a power of two
-            cf[nt][0] = __shfl_sync(0xffffffffu, all, 8 * t);
-            cf[nt][1] = __shfl_sync(0xffffffffu, all, 8 * t + 4);
-        }
-        // Entries that this thread's two columns of each tile see.
-        int sees[NT][2];
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const int x = 8 * nt + 2 * t + i;
-                sees[nt][i] = x < cols ? sees_all + (x0 + x) / p.group : 0;
-            }
+    const int len = length_of(p, seq, nullptr), chunks = chunks_of(len), cuts = (chunks + most - 1) / most;
+    const int seg = s_piece / cuts, piece = s_piece - seg * cuts, g = seg / p.row_groups, rg = seg - g * p.row_groups;
+    const long long seg_begin = s_before + (long long)seg * chunks;
+    const int ch0 = (int)((long long)chunks * piece / cuts), ch1 = (int)((long long)chunks * (piece + 1) / cuts);
+    const int x0 = rg * COLS, cols = min(COLS, p.cols - x0);  // this row group's columns
+    const int sees_all = len - p.rows + 1;                    // entries that the first new token sees
 
         // ---- the ring: block k of this warp is entries first(k) .. + 31 ----
         const int n_blocks = ch1 - ch0;
         auto first_entry = [&](int k) { return ((ch0 + k) * kWarps + warp) * kBlock; };
         const int* table = c.table + (int64_t)seq * c.max_pages;
-        // Page of the block's 16-entry half; -1: none of it is there.
+        // The table's entry for the block's 16-entry half (not looked at before the block is asked for: it is on its way);
+        // -1: none of the half is there.
         auto page_of = [&](int k, int half) {
             const int e = first_entry(k) + 16 * half;
-            if (k >= n_blocks || e >= len) return -1;
-            const int page = table[e >> p.page_shift];
+            return k < n_blocks && e < len ? table[e >> p.page_shift] : -1;
+        };
+        auto checked = [&](int page, int e) {
             if ((unsigned)page < (unsigned)c.n_pages) return page;
-            latch(p.err, ERR_BOUNDS);
+            if (e < len) latch(p.err, ERR_BOUNDS);
             return -1;
         };
         auto issue = [&](int k, int page0, int page1) {
             const int e0 = first_entry(k);
+            page0 = checked(page0, e0), page1 = checked(page1, e0 + 16);
             const uint32_t to = ring_u32 + (k % ST) * R::BYTES;
             const int64_t row0 = ((int64_t)p.layer * c.n_kv_heads + g) * c.page_size;
             constexpr int PR = RB / 16;          // pieces of a row
@@ -329,11 +319,72 @@ __global__ void __launch_bounds__(kWarps * 32, Ring<CT, HD>::CTAS) paged_kernel(
             page0 = n0, page1 = n1;
         }
 
+        // ---- queries ----
+        uint32_t q[NT][PLANES][KS][2];
+        float unit = p.scale * 1.4426950408889634f;  // score units -> log2 units (log2 e)
+        if constexpr (I8) {
+            // One power of two for all columns: what a smaller row loses at fp16's lower end is as small beside the largest
+            // row's scores as that row's own loss.
+            float v[NT][HD / 4], big = 0.0f;
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                const int x = 8 * nt + gr, token = (x0 + x) / p.group, head = g * p.group + x0 + x - token * p.group;
+                const int64_t at = ((int64_t)seq * p.rows + token) * p.q_stride + head * HD + 16 * t;
+                // piece j of the row's 16-byte ones that this thread reads: dims 64 j + 16 t ..
+#pragma unroll
+                for (int j = 0; j < HD / 64; j++) load16<PLANES>(p.q, at + 64 * j, p.dtype, x < cols, v[nt] + 16 * j);
+#pragma unroll
+                for (int i = 0; i < HD / 4; i++)
+                    if (fabsf(v[nt][i]) < __int_as_float(0x7f800000)) big = fmaxf(big, fabsf(v[nt][i]));
+            }
+#pragma unroll
+            for (int x = 16; x >= 1; x >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, x));
+            const int up = big > 0.0f ? min(max(13 - exponent_of(big), -100), 100) : 0;
+            const float f = power_of_two(up);
+            unit *= power_of_two(-up);
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int i = 0; i < HD / 4; i += 2) {
+                    const float a = v[nt][i] * f, b = v[nt][i + 1] * f;
+                    const uint32_t hi = pack<false>(a, b);
+                    q[nt][0][i / 4][i / 2 % 2] = hi;
+                    if constexpr (PLANES == 2) {
+                        const float2 h = unpack<false>(hi);
+                        q[nt][1][i / 4][i / 2 % 2] = pack<false>(a - h.x, b - h.y);
+                    }
+                }
+        } else {
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                const int x = 8 * nt + gr, token = (x0 + x) / p.group, head = g * p.group + x0 + x - token * p.group;
+                const int64_t at = ((int64_t)seq * p.rows + token) * p.q_stride + head * HD + 8 * t;
+#pragma unroll
+                for (int j = 0; j < HD / 32; j++) {
+                    uint4 v = make_uint4(0, 0, 0, 0);
+                    if (x < cols) v = *reinterpret_cast<const uint4*>(static_cast<const CT*>(p.q) + at + 32 * j);
+                    q[nt][0][2 * j][0] = v.x, q[nt][0][2 * j][1] = v.y;
+                    q[nt][0][2 * j + 1][0] = v.z, q[nt][0][2 * j + 1][1] = v.w;
+                }
+            }
+        }
+        // Entries that this thread's two columns of each tile see.
+        int sees[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const int x = 8 * nt + 2 * t + i;
+                sees[nt][i] = x < cols ? sees_all + (x0 + x) / p.group : 0;
+            }
+
         // ---- running softmax ----
-        float o[MT][NT][4], m[NT][2], l[NT][2];
+        // Maxima as their negatives, 0 as long as there is none (`above`, the exponent that calls for a new one, is -inf then).
+        float o[MT][NT][4], minus_m[NT][2], above[NT][2], l[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-            m[nt][0] = m[nt][1] = -INFINITY;
+            minus_m[nt][0] = minus_m[nt][1] = 0.0f;
+            above[nt][0] = above[nt][1] = -INFINITY;
             l[nt][0] = l[nt][1] = 0.0f;
 #pragma unroll
             for (int i = 0; i < MT; i++) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.0f;
@@ -358,8 +409,6 @@ __global__ void __launch_bounds__(kWarps * 32, Ring<CT, HD>::CTAS) paged_kernel(
             float s[2][NT][4];
 #pragma unroll
             for (int mt = 0; mt < 2; mt++) {
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++) s[mt][nt][0] = s[mt][nt][1] = s[mt][nt][2] = s[mt][nt][3] = 0.0f;
                 const int r0 = 16 * mt + gr, r1 = r0 + 8;
 #pragma unroll
                 for (int j = 0; j < RB / 64; j++) {  // pieces t, t + 4, ...
@@ -375,49 +424,68 @@ __global__ void __launch_bounds__(kWarps * 32, Ring<CT, HD>::CTAS) paged_kernel(
 #pragma unroll
                             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                                for (int pl = 0; pl < PLANES; pl++)
-                                    mma<false>(s[mt][nt], a0, a1, a2, a3, q[nt][pl][4 * j + i][0], q[nt][pl][4 * j + i][1]);
+                                for (int pl = 0; pl < PLANES; pl++) {
+                                    const uint32_t(&b)[2] = q[nt][pl][4 * j + i];
+                                    if (i + j + pl == 0) mma_first<false>(s[mt][nt], a0, a1, a2, a3, b[0], b[1]);
+                                    else mma<false>(s[mt][nt], a0, a1, a2, a3, b[0], b[1]);
+                                }
                         }
                     } else {
 #pragma unroll
                         for (int i = 0; i < 2; i++)
 #pragma unroll
-                            for (int nt = 0; nt < NT; nt++)
-                                mma<BF>(s[mt][nt], wa[2 * i], wb[2 * i], wa[2 * i + 1], wb[2 * i + 1],
-                                        q[nt][0][2 * j + i][0], q[nt][0][2 * j + i][1]);
+                            for (int nt = 0; nt < NT; nt++) {
+                                const uint32_t(&b)[2] = q[nt][0][2 * j + i];
+                                if (i + j == 0) mma_first<BF>(s[mt][nt], wa[0], wb[0], wa[1], wb[1], b[0], b[1]);
+                                else mma<BF>(s[mt][nt], wa[2 * i], wb[2 * i], wa[2 * i + 1], wb[2 * i + 1], b[0], b[1]);
+                            }
                     }
                 }
             }
-            // scales, mask; does any score lie 2^8 above its column's maximum?
+            // exponents against the maxima so far; does any lie 2^8 above?
             const bool tail = e0 + kBlock > sees_all;  // some entry is not seen by every column
             bool rise = false;
+            float ks[2][2];
 #pragma unroll
             for (int mt = 0; mt < 2; mt++)
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const int r = 16 * mt + 8 * h + gr;
-                    const float ks = I8 ? scales[r] : 1.0f;
+                for (int h = 0; h < 2; h++) ks[mt][h] = I8 ? scales[16 * mt + 8 * h + gr] * unit : unit;
+            if (tail) {
+#pragma unroll
+                for (int mt = 0; mt < 2; mt++)
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                        for (int i = 0; i < 2; i++) {
-                            float& x = s[mt][nt][2 * h + i];
-                            x = I8 ? x * (ks * cf[nt][i]) : x * cf[nt][i];
-                            if (tail && e0 + r >= sees[nt][i]) x = -INFINITY;
-                            rise |= x - m[nt][i] > 8.0f;
+                        for (int i = 0; i < 4; i++) {  // ks may be inf or NaN here: the factor goes in before the mask
+                            const bool seen = e0 + 16 * mt + 8 * (i >> 1) + gr < sees[nt][i & 1];
+                            s[mt][nt][i] = seen ? s[mt][nt][i] * ks[mt][i >> 1] : -INFINITY;
                         }
-                }
+                ks[0][0] = ks[0][1] = ks[1][0] = ks[1][1] = 1.0f;
+            }
+#pragma unroll
+            for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        // (fma(-inf, 1, 0) where there is no maximum yet)
+                        rise |= fmaf(s[mt][nt][i], ks[mt][i >> 1], minus_m[nt][i & 1]) > above[nt][i & 1];
+                    }
             if (__any_sync(0xffffffffu, rise)) {
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                     for (int i = 0; i < 2; i++) {
-                        float top = fmaxf(fmaxf(s[0][nt][i], s[0][nt][2 + i]), fmaxf(s[1][nt][i], s[1][nt][2 + i]));
+                        float top = fmaxf(fmaxf(s[0][nt][i] * ks[0][0], s[0][nt][2 + i] * ks[0][1]),
+                                          fmaxf(s[1][nt][i] * ks[1][0], s[1][nt][2 + i] * ks[1][1]));
 #pragma unroll
                         for (int x = 4; x <= 16; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-                        if (top - m[nt][i] > 8.0f) {  // no other column has a say: a row stays the same whatever its neighbours are
-                            const float f = exp2_approx(m[nt][i] - top);
-                            m[nt][i] = top;
+                        // no other column has a say: a row stays the same whatever its neighbours are
+                        const bool none = above[nt][i] == -INFINITY;
+                        if (none ? top > -INFINITY : top + minus_m[nt][i] > 8.0f) {
+                            const float f = none ? 0.0f : exp2_approx(-minus_m[nt][i] - top);
+                            minus_m[nt][i] = -top;
+                            above[nt][i] = 8.0f;
                             l[nt][i] *= f;
 #pragma unroll
                             for (int d = 0; d < MT; d++) o[d][nt][i] *= f, o[d][nt][2 + i] *= f;
@@ -441,24 +509,24 @@ __global__ void __launch_bounds__(kWarps * 32, Ring<CT, HD>::CTAS) paged_kernel(
                 for (int h = 0; h < 2; h++) {
                     const int r = 16 * mt + 8 * h + gr;
                     const float vs = I8 ? scales[kBlock + r] * vscale : 1.0f;
+                    const bool vs_ok = fabsf(vs) < __int_as_float(0x7f800000);
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++) {
                         float y[2];
 #pragma unroll
                         for (int i = 0; i < 2; i++) {
-                            const float x = s[mt][nt][2 * h + i];
-                            const float e = exp2_approx(x - (m[nt][i] == -INFINITY ? 0.0f : m[nt][i]));
+                            const float e = exp2_approx(fmaf(s[mt][nt][2 * h + i], ks[mt][h], minus_m[nt][i]));
                             l[nt][i] += e;
                             y[i] = I8 ? e * vs : e;
-                            if (tail && e0 + r >= sees[nt][i]) y[i] = 0.0f;  // whatever the entry's scale is
+                            if (I8 && tail && !vs_ok && e0 + r >= sees[nt][i]) y[i] = 0.0f;  // 0 whatever its scale is
                         }
-                        const uint32_t hi = pack<BF>(y[0], y[1]);
-                        pw[mt][nt][0][h] = transpose8x8(hi);
-                        if constexpr (VP == 2) {  // an inf or NaN stays in the first plane
-                            const float2 got = unpack<BF>(hi);
-                            const float inf = __int_as_float(0x7f800000);
-                            pw[mt][nt][1][h] = transpose8x8(pack<BF>(fabsf(got.x) < inf ? y[0] - got.x : 0.0f,
-                                                                     fabsf(got.y) < inf ? y[1] - got.y : 0.0f));
+                        if constexpr (VP == 2) {  // (an inf is the largest value and an inf)
+                            const uint32_t hi = pack_finite(y[0], y[1]);
+                            const float2 got = unpack<false>(hi);
+                            pw[mt][nt][0][h] = transpose8x8(hi);
+                            pw[mt][nt][1][h] = transpose8x8(pack<false>(y[0] - got.x, y[1] - got.y));
+                        } else {
+                            pw[mt][nt][0][h] = transpose8x8(pack<BF>(y[0], y[1]));
                         }
                     }
                 }
@@ -491,8 +559,6 @@ __global__ void __launch_bounds__(kWarps * 32, Ring<CT, HD>::CTAS) paged_kernel(
                     for (int i = 0; i < PER; i++) {
                         float acc[NT][4];
 #pragma unroll
-                        for (int nt = 0; nt < NT; nt++) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.0f;
-#pragma unroll
                         for (int mt = 0; mt < 2; mt++) {
                             uint32_t a0, a1, a2, a3;
                             if constexpr (I8) {
@@ -509,8 +575,10 @@ __global__ void __launch_bounds__(kWarps * 32, Ring<CT, HD>::CTAS) paged_kernel(
 #pragma unroll
                             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                                for (int pl = 0; pl < VP; pl++)
-                                    mma<BF>(acc[nt], a0, a1, a2, a3, pw[mt][nt][pl][0], pw[mt][nt][pl][1]);
+                                for (int pl = 0; pl < VP; pl++) {
+                                    if (mt == 0 && pl == 0) mma_first<BF>(acc[nt], a0, a1, a2, a3, pw[0][nt][0][0], pw[0][nt][0][1]);
+                                    else mma<BF>(acc[nt], a0, a1, a2, a3, pw[mt][nt][pl][0], pw[mt][nt][pl][1]);
+                                }
                         }
 #pragma unroll
                         for (int nt = 0; nt < NT; nt++)
@@ -540,7 +608,7 @@ __global__ void __launch_bounds__(kWarps * 32, Ring<CT, HD>::CTAS) paged_kernel(
 #pragma unroll
                 for (int x = 4; x <= 16; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
                 float* to = shared + (warp * COLS + 8 * nt + 2 * t + i) * PITCH;
-                if (gr == 0) to[HD] = m[nt][i], to[HD + 1] = sum;
+                if (gr == 0) to[HD] = above[nt][i] == -INFINITY ? -INFINITY : -minus_m[nt][i], to[HD + 1] = sum;
 #pragma unroll
                 for (int d = 0; d < MT; d++) {
                     // tile d's rows gr and gr + 8 are two neighbouring dims
@@ -550,9 +618,10 @@ __global__ void __launch_bounds__(kWarps * 32, Ring<CT, HD>::CTAS) paged_kernel(
                 }
             }
         __syncthreads();
-        const bool whole = ch0 == 0 && ch1 == chunks;
-        const int slot = ch0 == 0 ? 1 : 0;  // a CTA's run begins inside a segment once, and ends inside one once
-        float* part = p.part + ((int64_t)blockIdx.x * 2 + slot) * COLS * PITCH;
+        // A cut segment is longer than P = `most` chunks, so no two have one seg_begin / P, and its pieces fit twice that
+        // many places.
+        const int64_t place = seg_begin / most;
+        float* part = p.part + (2 * place + piece) * COLS * PITCH;
         for (int i = threadIdx.x; i < cols * (HD / 2); i += kWarps * 32) {
             const int x = i / (HD / 2), d = i % (HD / 2) * 2;
             float top = -INFINITY;
@@ -569,54 +638,44 @@ __global__ void __launch_bounds__(kWarps * 32, Ring<CT, HD>::CTAS) paged_kernel(
                 const float2 y = *reinterpret_cast<const float2*>(from + d);
                 v.x += y.x * (from[HD] == -INFINITY ? 1.0f : f), v.y += y.y * (from[HD] == -INFINITY ? 1.0f : f);
             }
-            if (whole) {
+            if (cuts == 1) {
                 const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-                const int64_t to = row_of(p, seq, x0 + x) * p.out_stride + (g * p.group + (x0 + x) % p.group) * HD + d;
-                store_out(p.out, to, p.dtype, v.x * inv);
-                store_out(p.out, to + 1, p.dtype, v.y * inv);
+                store_out(p, seq, g, x0 + x, d, HD, make_float2(v.x * inv, v.y * inv));
             } else {
                 float* to = part + x * PITCH;
                 __stcg(reinterpret_cast<float2*>(to + d), v);
                 if (d == 0) __stcg(reinterpret_cast<float2*>(to + HD), make_float2(top, sum));
             }
         }
-        if (!whole) {
-            // ---- the segment's parts together, by the last to come ----
-            const int from = (int)(seg_begin / per), upto = (int)((seg_begin + chunks - 1) / per);  // CTAs it lies in
+        if (cuts > 1) {
+            // ---- the segment's pieces together, by the last to come ----
             __threadfence();
             __syncthreads();
-            if (threadIdx.x == 0) s_last = atomicAdd(&p.count[from], 1) == upto - from;
+            if (threadIdx.x == 0) s_last = atomicAdd(&p.count[place], 1) == cuts - 1;
             __syncthreads();
-            if (s_last) {
-                __threadfence();
-                if (threadIdx.x == 0) p.count[from] = 0;  // as it was found
-                for (int i = threadIdx.x; i < cols * (HD / 2); i += kWarps * 32) {
-                    const int x = i / (HD / 2), d = i % (HD / 2) * 2;
-                    float top = -INFINITY, sum = 0.0f;
-                    float2 v = make_float2(0.0f, 0.0f);
+            if (!s_last) return;
+            __threadfence();
+            if (threadIdx.x == 0) p.count[place] = 0;  // as it was found
+            for (int i = threadIdx.x; i < cols * (HD / 2); i += kWarps * 32) {
+                const int x = i / (HD / 2), d = i % (HD / 2) * 2;
+                float top = -INFINITY, sum = 0.0f;
+                float2 v = make_float2(0.0f, 0.0f);
 #pragma unroll 4
-                    for (int cta = from; cta <= upto; cta++) {
-                        const float* a = p.part + (((int64_t)cta * 2 + (cta == from)) * COLS + x) * PITCH;
-                        const float2 ms = __ldcg(reinterpret_cast<const float2*>(a + HD));
-                        const float2 y = __ldcg(reinterpret_cast<const float2*>(a + d));
-                        const float m2 = fmaxf(top, ms.x);
-                        const float f0 = top == m2 ? 1.0f : exp2_approx(top - m2);
-                        const float f1 = ms.x == m2 || ms.x == -INFINITY ? 1.0f : exp2_approx(ms.x - m2);
-                        top = m2;
-                        sum = sum * f0 + ms.y * f1;
-                        v.x = v.x * f0 + y.x * f1, v.y = v.y * f0 + y.y * f1;
-                    }
-                    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-                    const int64_t to = row_of(p, seq, x0 + x) * p.out_stride + (g * p.group + (x0 + x) % p.group) * HD + d;
-                    store_out(p.out, to, p.dtype, v.x * inv);
-                    store_out(p.out, to + 1, p.dtype, v.y * inv);
+                for (int k = 0; k < cuts; k++) {
+                    const float* a = p.part + ((2 * place + k) * COLS + x) * PITCH;
+                    const float2 ms = __ldcg(reinterpret_cast<const float2*>(a + HD));
+                    const float2 y = __ldcg(reinterpret_cast<const float2*>(a + d));
+                    const float m2 = fmaxf(top, ms.x);
+                    const float f0 = top == m2 ? 1.0f : exp2_approx(top - m2);
+                    const float f1 = ms.x == m2 || ms.x == -INFINITY ? 1.0f : exp2_approx(ms.x - m2);
+                    top = m2;
+                    sum = sum * f0 + ms.y * f1;
+                    v.x = v.x * f0 + y.x * f1, v.y = v.y * f0 + y.y * f1;
                 }
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                store_out(p, seq, g, x0 + x, d, HD, make_float2(v.x * inv, v.y * inv));
             }
         }
-        __syncthreads();  // the ring may be filled again
-        w = seg_begin + ch1;
-        if (seg == segs - 1 && ch1 == chunks) seq++, seq_begin = w;
-    }
 }
 
 // Column tiles of 8 that a CTA takes: as many as the rows need, up to what the registers hold.
@@ -631,12 +690,15 @@ template <typename CT, int HD, int NT, int PLANES>
 pf_status launch_tiles(PagedParams& p, cudaStream_t st) {
     using R = Ring<CT, HD>;
     p.row_groups = ceil_div(p.cols, 8 * NT);
-    const int64_t most = (int64_t)p.n_seqs * p.c.n_kv_heads * p.row_groups *
-                         std::max<int64_t>(((int64_t)p.c.max_pages * p.c.page_size + kChunk - 1) / kChunk, 1);
-    const int grid = (int)std::min<int64_t>(most, cta_limit(p.c));
+    p.ctas = cta_limit(p.c);
+    // segments, and with pieces of total / CTAs chunks no more than that many cuts
+    const int64_t segments = (int64_t)p.n_seqs * p.c.n_kv_heads * p.row_groups;
+    const int64_t chunks = std::max<int64_t>(((int64_t)p.c.max_pages * p.c.page_size + kChunk - 1) / kChunk, 1);
+    const int64_t grid = std::min(segments * chunks, segments + p.ctas);
+    PF_CHECK(grid <= INT32_MAX, "pf_paged_attention: too many rows");
     static std::atomic<uint64_t> attr{0};
     PF_TRY(raise_smem_limit(paged_kernel<CT, HD, NT, PLANES>, R::SMEM, attr));
-    paged_kernel<CT, HD, NT, PLANES><<<grid, kWarps * 32, R::SMEM, st>>>(p);
+    paged_kernel<CT, HD, NT, PLANES><<<(unsigned)grid, kWarps * 32, R::SMEM, st>>>(p);
     return launch_check("paged_attention");
 }
 
@@ -661,9 +723,9 @@ size_t pf_paged_attention_work_bytes(const pf_paged_cache* c, int32_t n_seqs, in
     if (!c || n_seqs < 0 || rows < 1 || rows > 8 || n_heads < 1 || c->n_kv_heads < 1 || n_heads % c->n_kv_heads) return 0;
     if (c->head_dim != 64 && c->head_dim != 128) return 0;
     const int cols = n_heads / c->n_kv_heads * rows;
-    // counters, then two parts a CTA
+    // counters, then the pieces of cut segments
     return kMaxCtas * sizeof(int) +
-           (size_t)cta_limit(*c) * 2 * 8 * tiles_for(cols, c->head_dim) * (c->head_dim + 2) * sizeof(float);
+           (size_t)(cta_limit(*c) + 1) * 2 * 8 * tiles_for(cols, c->head_dim) * (c->head_dim + 2) * sizeof(float);
 }
 
 pf_status pf_paged_attention(const pf_paged_cache* c, int32_t layer, const void* q, int64_t q_stride, void* out,
