@@ -48,10 +48,7 @@ namespace pf {
 
 namespace {
 
-constexpr int kWarps = 4;
-constexpr int kBlock = 32;                  // entries a warp takes at a time
-constexpr int kChunk = kWarps * kBlock;     // entries the CTA takes at a time
-constexpr int kMaxCtas = 1024;              // counters at the start of `work`
+constexpr int kCounters = 2048;  // at the start of `work`: seg_begin / P is at most twice the CTAs that fit
 
 struct PagedParams {
     pf_paged_cache c;
@@ -62,7 +59,7 @@ struct PagedParams {
     int group, cols, row_groups, page_shift;  // heads a kv head; rows x group; tiles of them; log2 page_size
     float scale;
     int ctas;      // that fit the GPU
-    int* count;    // [kMaxCtas] pieces of a cut segment that have ended
+    int* count;    // [kCounters] pieces of a cut segment that have ended
     float* part;   // [piece of a cut segment][columns a row group][head_dim + 2]
     uint32_t* err;
 };
@@ -70,11 +67,14 @@ struct PagedParams {
 template <typename CT, int HD>
 struct Ring {
     static constexpr int RB = HD * (int)sizeof(CT);                 // bytes of a stored row
-    static constexpr int SCALES = sizeof(CT) == 1 ? 2 * kBlock * 4 : 0;
-    static constexpr int BYTES = 2 * kBlock * RB + SCALES;          // keys, values, scales of a block
+    static constexpr int WARPS = RB == 64 ? 3 : 4;
+    static constexpr int BLOCK = RB == 256 ? 16 : 32;               // entries a warp takes at a time
+    static constexpr int CHUNK = WARPS * BLOCK;                     // entries the CTA takes at a time
+    static constexpr int SCALES = sizeof(CT) == 1 ? 2 * BLOCK * 4 : 0;
+    static constexpr int BYTES = 2 * BLOCK * RB + SCALES;           // keys, values, scales of a block
     static constexpr int STAGES = RB == 64 ? 4 : 3;
-    static constexpr int SMEM = kWarps * STAGES * BYTES;
-    static constexpr int CTAS = RB == 64 ? 3 : (RB == 128 ? 2 : 1);  // that fit an SM
+    static constexpr int SMEM = WARPS * STAGES * BYTES;
+    static constexpr int CTAS = RB == 64 ? 4 : 2;                   // that fit an SM
 };
 
 // Where 16-byte piece c of row r lies: rows read together in other banks.
@@ -192,11 +192,22 @@ __device__ __forceinline__ void load16(const void* q, int64_t i, int dtype, bool
 }
 // A sequence's length as it counts here, and its chunks (one even if it is empty: its rows are zeros).
 __device__ __forceinline__ int length_of(const PagedParams& p, int b, uint32_t* err) { return max(seq_len(p.c, b, err), 0); }
-__device__ __forceinline__ int chunks_of(int len) { return max((len + kChunk - 1) / kChunk, 1); }
+template <int CHUNK>
+__device__ __forceinline__ int chunks_of(int len) {
+    return max((len + CHUNK - 1) / CHUNK, 1);
+}
+
+// x / group for a column x of at most eight tokens.
+__device__ __forceinline__ int token_of(int x, int group) {
+    int t = 0;
+#pragma unroll
+    for (int k = 1; k < 8; k++) t += x >= k * group;
+    return t;
+}
 
 // Dims d, d + 1 of column x of kv head g: head g * group + x % group of token x / group.
 __device__ __forceinline__ void store_out(const PagedParams& p, int seq, int g, int x, int d, int hd, float2 v) {
-    const int token = x / p.group, head = g * p.group + x - token * p.group;
+    const int token = token_of(x, p.group), head = g * p.group + x - token * p.group;
     const int64_t at = ((int64_t)seq * p.rows + token) * p.out_stride + head * hd + d;
     if (p.dtype == PF_F32) *reinterpret_cast<float2*>(static_cast<float*>(p.out) + at) = v;
     else
@@ -205,72 +216,76 @@ __device__ __forceinline__ void store_out(const PagedParams& p, int seq, int g, 
 }
 
 template <typename CT, int HD, int NT, int PLANES>
-__global__ void __launch_bounds__(kWarps * 32, Ring<CT, HD>::CTAS) paged_kernel(const PagedParams p) {
+__global__ void __launch_bounds__(Ring<CT, HD>::WARPS * 32, Ring<CT, HD>::CTAS) paged_kernel(const PagedParams p) {
     using R = Ring<CT, HD>;
-    constexpr int RB = R::RB, ST = R::STAGES;
+    constexpr int RB = R::RB, ST = R::STAGES, kWarps = R::WARPS, kBlock = R::BLOCK, HALVES = kBlock / 16;
     constexpr bool I8 = sizeof(CT) == 1, BF = std::is_same<CT, __nv_bfloat16>::value;
     constexpr int KS = HD / 16;        // products along the dims of a score
     constexpr int MT = HD / 16;        // 16-dim tiles of the output
     constexpr int COLS = 8 * NT;
     constexpr int VP = I8 ? 2 : 1;     // planes of a weight
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ long long s_sum[kWarps], s_before;
-    __shared__ int s_seq, s_piece, s_last;
+    __shared__ int s_sum[kWarps], s_before, s_seq, s_piece, s_len, s_last;
     const pf_paged_cache& c = p.c;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, t = lane & 3;
     const int segs = c.n_kv_heads * p.row_groups;  // of one sequence
 
-    // ---- this CTA's piece ----
-    long long mine = 0;
+    // ---- this CTA's piece ----  (the host has seen to it that all chunks count in 31 bits)
+    int mine = 0;
     for (int b = threadIdx.x; b < p.n_seqs; b += kWarps * 32)
-        mine += chunks_of(length_of(p, b, blockIdx.x == 0 ? p.err : nullptr));
-#pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+        mine += chunks_of<R::CHUNK>(length_of(p, b, blockIdx.x == 0 ? p.err : nullptr));
+    mine = __reduce_add_sync(0xffffffffu, mine);
     if (lane == 0) s_sum[warp] = mine;
     __syncthreads();
-    const long long total = (s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3]) * segs;
-    // chunks a piece: with more segments than CTAs that fit, only what is twice as long is cut
-    const long long share = (total + p.ctas - 1) / p.ctas;
-    const int most = (int)min((long long)p.n_seqs * segs >= p.ctas ? 2 * share : share, (long long)INT_MAX);
+    int total = 0;
+#pragma unroll
+    for (int i = 0; i < kWarps; i++) total += s_sum[i];
+    total *= segs;
+    // Chunks a piece.  With nearly as many segments as CTAs fit, only what is twice as long as the share is cut; with fewer,
+    // half a share, so that the pieces that come last are small; with very few, a share (the joining would grow).
+    const int segments = p.n_seqs * segs, share = (total + p.ctas - 1) / p.ctas;
+    const int most = 4 * segments >= 3 * p.ctas ? 2 * share : (16 * segments >= p.ctas ? (share + 1) / 2 : share);
     if (warp == 0) {  // the sequence that it belongs to
-        long long pieces = 0, chunks = 0;
-        int found = -1;
+        int pieces = 0, before = 0, found = -1;
         for (int b0 = 0; b0 < p.n_seqs && found < 0; b0 += 32) {
-            const int b = b0 + lane;
-            const int n = b < p.n_seqs ? chunks_of(length_of(p, b, nullptr)) : 0;
-            const long long my_pieces = (long long)((n + most - 1) / most) * segs, my_chunks = (long long)n * segs;
-            long long upto = my_pieces, upto_chunks = my_chunks;
+            const int b = b0 + lane, len = b < p.n_seqs ? length_of(p, b, nullptr) : 0;
+            const int n = b < p.n_seqs ? chunks_of<R::CHUNK>(len) : 0;
+            const int my_pieces = (n <= most ? min(n, 1) : (n + most - 1) / most) * segs, my_chunks = n * segs;
+            int upto = my_pieces, upto_chunks = my_chunks;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const long long x = __shfl_up_sync(0xffffffffu, upto, o), y = __shfl_up_sync(0xffffffffu, upto_chunks, o);
+                const int x = __shfl_up_sync(0xffffffffu, upto, o), y = __shfl_up_sync(0xffffffffu, upto_chunks, o);
                 if (lane >= o) upto += x, upto_chunks += y;
             }
-            const unsigned here = __ballot_sync(0xffffffffu, blockIdx.x < pieces + upto);
+            const unsigned here = __ballot_sync(0xffffffffu, (int)blockIdx.x < pieces + upto);
             if (here) {
                 const int at = __ffs((int)here) - 1;
-                if (lane == at) s_piece = (int)(blockIdx.x - (pieces + upto - my_pieces)), s_before = chunks + upto_chunks - my_chunks;
+                if (lane == at) {
+                    s_piece = (int)blockIdx.x - (pieces + upto - my_pieces);
+                    s_before = before + upto_chunks - my_chunks;
+                    s_len = len;
+                }
                 found = b0 + at;
             }
             pieces += __shfl_sync(0xffffffffu, upto, 31);
-            chunks += __shfl_sync(0xffffffffu, upto_chunks, 31);
+            before += __shfl_sync(0xffffffffu, upto_chunks, 31);
         }
         if (lane == 0) s_seq = found;
     }
     __syncthreads();
     const int seq = s_seq;
     if (seq < 0) return;  // the grid is an upper bound
-
-    uint8_t* ring = smem + warp * ST * R::BYTES;
-    const uint32_t ring_u32 = (uint32_t)__cvta_generic_to_shared(ring);
-    const int64_t page_bytes = (int64_t)c.n_layers * c.n_kv_heads * c.page_size * RB;
-    const int64_t page_slots = (int64_t)c.n_layers * c.n_kv_heads * c.page_size;
-    const int len = length_of(p, seq, nullptr), chunks = chunks_of(len), cuts = (chunks + most - 1) / most;
+    const int len = s_len, chunks = chunks_of<R::CHUNK>(len), cuts = chunks <= most ? 1 : (chunks + most - 1) / most;
     const int seg = s_piece / cuts, piece = s_piece - seg * cuts, g = seg / p.row_groups, rg = seg - g * p.row_groups;
-    const long long seg_begin = s_before + (long long)seg * chunks;
-    const int ch0 = (int)((long long)chunks * piece / cuts), ch1 = (int)((long long)chunks * (piece + 1) / cuts);
+    const int seg_begin = s_before + seg * chunks;
+    const int ch0 = cuts == 1 ? 0 : (int)((int64_t)chunks * piece / cuts);
+    const int ch1 = cuts == 1 ? chunks : (int)((int64_t)chunks * (piece + 1) / cuts);
     const int x0 = rg * COLS, cols = min(COLS, p.cols - x0);  // this row group's columns
     const int sees_all = len - p.rows + 1;                    // entries that the first new token sees
 
+    uint8_t* ring = smem + warp * ST * R::BYTES;
+    const uint32_t ring_u32 = (uint32_t)__cvta_generic_to_shared(ring);
+    const int64_t page_slots = (int64_t)c.n_layers * c.n_kv_heads * c.page_size;
         // ---- the ring: block k of this warp is entries first(k) .. + 31 ----
         const int n_blocks = ch1 - ch0;
         auto first_entry = [&](int k) { return ((ch0 + k) * kWarps + warp) * kBlock; };
@@ -286,34 +301,45 @@ __global__ void __launch_bounds__(kWarps * 32, Ring<CT, HD>::CTAS) paged_kernel(
             if (e < len) latch(p.err, ERR_BOUNDS);
             return -1;
         };
+        // A half's 16 rows lie behind one another in their page: a pass of 32 lanes is 512 bytes of them, and only its base
+        // depends on the block.
+        constexpr int PR = RB / 16, STEP = 32 / PR;  // pieces of a row, rows a pass
+        const int lane_row = lane / PR, lane_piece = lane % PR;
+        const uint32_t key_to = key_at<RB>(lane_row, lane_piece);
+        constexpr int VARIANTS = RB == 64 ? 1 : (RB == 128 ? 2 : 4);  // of the values' permutation among passes
+        uint32_t value_to[VARIANTS];
+#pragma unroll
+        for (int i = 0; i < VARIANTS; i++)
+            value_to[i] = kBlock * RB + value_at<RB>(i * STEP + lane_row, lane_piece) - i * STEP * RB;
+        const int64_t unit_row = ((int64_t)p.layer * c.n_kv_heads + g) * c.page_size;
         auto issue = [&](int k, int page0, int page1) {
             const int e0 = first_entry(k);
-            page0 = checked(page0, e0), page1 = checked(page1, e0 + 16);
             const uint32_t to = ring_u32 + (k % ST) * R::BYTES;
-            const int64_t row0 = ((int64_t)p.layer * c.n_kv_heads + g) * c.page_size;
-            constexpr int PR = RB / 16;          // pieces of a row
-            constexpr int STEP = 32 / PR;        // rows a pass (16: RB = 256 has two)
 #pragma unroll
-            for (int r0 = 0; r0 < kBlock; r0 += STEP) {
-                const int r = r0 + lane / PR, piece = lane % PR, e = e0 + r;
-                const int page = r0 < 16 ? page0 : page1;
-                const bool on = page >= 0 && e < len;
-                const int64_t from = (on ? page : 0) * page_bytes + (row0 + (e & (c.page_size - 1))) * RB + piece * 16;
-                copy16(to + key_at<RB>(r, piece), static_cast<const uint8_t*>(c.k) + from, on);
-                copy16(to + kBlock * RB + value_at<RB>(r, piece), static_cast<const uint8_t*>(c.v) + from, on);
-            }
-            if constexpr (I8) {
-                const int e = e0 + lane, page = lane < 16 ? page0 : page1;
-                const bool on = page >= 0 && e < len;
-                const int64_t from = (on ? page : 0) * page_slots + row0 + (e & (c.page_size - 1));
-                copy4(to + 2 * kBlock * RB + 4 * lane, c.k_scale + from, on);
-                copy4(to + 2 * kBlock * RB + 4 * (kBlock + lane), c.v_scale + from, on);
+            for (int half = 0; half < HALVES; half++) {
+                const int e = e0 + 16 * half, page = checked(half ? page1 : page0, e);
+                const int rows = page < 0 ? 0 : min(len - e, 16);  // of the half's 16; the others are filled with zeros
+                const int64_t row = (int64_t)max(page, 0) * page_slots + unit_row + (e & (c.page_size - 1));
+                const uint8_t* from_k = static_cast<const uint8_t*>(c.k) + row * RB + lane * 16;
+                const uint8_t* from_v = static_cast<const uint8_t*>(c.v) + row * RB + lane * 16;
+#pragma unroll
+                for (int i = 0; i < 16 / STEP; i++) {
+                    const int pass = half * (16 / STEP) + i;
+                    const bool on = i * STEP + lane_row < rows;
+                    copy16(to + key_to + pass * 512, from_k + i * 512, on);
+                    copy16(to + value_to[pass % VARIANTS] + pass * 512, from_v + i * 512, on);
+                }
+                if constexpr (I8) {  // lanes 0-15 the keys' scales, 16-31 the values'
+                    const float* from = (lane < 16 ? c.k_scale : c.v_scale) + row + (lane & 15);
+                    copy4(to + 2 * kBlock * RB + (lane < 16 ? 0 : 4 * kBlock) + 64 * half + 4 * (lane & 15), from,
+                          (lane & 15) < rows);
+                }
             }
         };
-        int page0 = page_of(0, 0), page1 = page_of(0, 1);
+        int page0 = page_of(0, 0), page1 = HALVES == 2 ? page_of(0, 1) : -1;
 #pragma unroll
         for (int k = 0; k < ST - 1; k++) {
-            const int n0 = page_of(k + 1, 0), n1 = page_of(k + 1, 1);
+            const int n0 = page_of(k + 1, 0), n1 = HALVES == 2 ? page_of(k + 1, 1) : -1;
             if (k < n_blocks) issue(k, page0, page1);
             copy_commit();
             page0 = n0, page1 = n1;
@@ -328,7 +354,7 @@ __global__ void __launch_bounds__(kWarps * 32, Ring<CT, HD>::CTAS) paged_kernel(
             float v[NT][HD / 4], big = 0.0f;
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
-                const int x = 8 * nt + gr, token = (x0 + x) / p.group, head = g * p.group + x0 + x - token * p.group;
+                const int x = 8 * nt + gr, token = token_of(x0 + x, p.group), head = g * p.group + x0 + x - token * p.group;
                 const int64_t at = ((int64_t)seq * p.rows + token) * p.q_stride + head * HD + 16 * t;
                 // piece j of the row's 16-byte ones that this thread reads: dims 64 j + 16 t ..
 #pragma unroll
@@ -357,7 +383,7 @@ __global__ void __launch_bounds__(kWarps * 32, Ring<CT, HD>::CTAS) paged_kernel(
         } else {
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
-                const int x = 8 * nt + gr, token = (x0 + x) / p.group, head = g * p.group + x0 + x - token * p.group;
+                const int x = 8 * nt + gr, token = token_of(x0 + x, p.group), head = g * p.group + x0 + x - token * p.group;
                 const int64_t at = ((int64_t)seq * p.rows + token) * p.q_stride + head * HD + 8 * t;
 #pragma unroll
                 for (int j = 0; j < HD / 32; j++) {
@@ -375,7 +401,7 @@ __global__ void __launch_bounds__(kWarps * 32, Ring<CT, HD>::CTAS) paged_kernel(
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 const int x = 8 * nt + 2 * t + i;
-                sees[nt][i] = x < cols ? sees_all + (x0 + x) / p.group : 0;
+                sees[nt][i] = x < cols ? sees_all + token_of(x0 + x, p.group) : 0;
             }
 
         // ---- running softmax ----
@@ -391,7 +417,7 @@ __global__ void __launch_bounds__(kWarps * 32, Ring<CT, HD>::CTAS) paged_kernel(
         }
         for (int k = 0; k < n_blocks; k++) {
             {
-                const int n0 = page_of(k + ST, 0), n1 = page_of(k + ST, 1);
+                const int n0 = page_of(k + ST, 0), n1 = HALVES == 2 ? page_of(k + ST, 1) : -1;
                 __syncwarp();  // every lane is through with the block whose place is filled now
                 if (k + ST - 1 < n_blocks) issue(k + ST - 1, page0, page1);
                 copy_commit();
@@ -405,10 +431,10 @@ __global__ void __launch_bounds__(kWarps * 32, Ring<CT, HD>::CTAS) paged_kernel(
             const uint8_t* vb = kb + kBlock * RB;
             const float* scales = reinterpret_cast<const float*>(vb + kBlock * RB);
 
-            // scores of 2 x 16 entries: rows gr, gr + 8 of each, in log2 units
-            float s[2][NT][4];
+            // scores of 16 entries each: rows gr, gr + 8
+            float s[HALVES][NT][4];
 #pragma unroll
-            for (int mt = 0; mt < 2; mt++) {
+            for (int mt = 0; mt < HALVES; mt++) {
                 const int r0 = 16 * mt + gr, r1 = r0 + 8;
 #pragma unroll
                 for (int j = 0; j < RB / 64; j++) {  // pieces t, t + 4, ...
@@ -445,14 +471,14 @@ __global__ void __launch_bounds__(kWarps * 32, Ring<CT, HD>::CTAS) paged_kernel(
             // exponents against the maxima so far; does any lie 2^8 above?
             const bool tail = e0 + kBlock > sees_all;  // some entry is not seen by every column
             bool rise = false;
-            float ks[2][2];
+            float ks[HALVES][2];
 #pragma unroll
-            for (int mt = 0; mt < 2; mt++)
+            for (int mt = 0; mt < HALVES; mt++)
 #pragma unroll
                 for (int h = 0; h < 2; h++) ks[mt][h] = I8 ? scales[16 * mt + 8 * h + gr] * unit : unit;
             if (tail) {
 #pragma unroll
-                for (int mt = 0; mt < 2; mt++)
+                for (int mt = 0; mt < HALVES; mt++)
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -460,10 +486,11 @@ __global__ void __launch_bounds__(kWarps * 32, Ring<CT, HD>::CTAS) paged_kernel(
                             const bool seen = e0 + 16 * mt + 8 * (i >> 1) + gr < sees[nt][i & 1];
                             s[mt][nt][i] = seen ? s[mt][nt][i] * ks[mt][i >> 1] : -INFINITY;
                         }
-                ks[0][0] = ks[0][1] = ks[1][0] = ks[1][1] = 1.0f;
+#pragma unroll
+                for (int mt = 0; mt < HALVES; mt++) ks[mt][0] = ks[mt][1] = 1.0f;
             }
 #pragma unroll
-            for (int mt = 0; mt < 2; mt++)
+            for (int mt = 0; mt < HALVES; mt++)
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -476,8 +503,10 @@ __global__ void __launch_bounds__(kWarps * 32, Ring<CT, HD>::CTAS) paged_kernel(
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                     for (int i = 0; i < 2; i++) {
-                        float top = fmaxf(fmaxf(s[0][nt][i] * ks[0][0], s[0][nt][2 + i] * ks[0][1]),
-                                          fmaxf(s[1][nt][i] * ks[1][0], s[1][nt][2 + i] * ks[1][1]));
+                        float top = -INFINITY;
+#pragma unroll
+                        for (int mt = 0; mt < HALVES; mt++)
+                            top = fmaxf(top, fmaxf(s[mt][nt][i] * ks[mt][0], s[mt][nt][2 + i] * ks[mt][1]));
 #pragma unroll
                         for (int x = 4; x <= 16; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
                         // no other column has a say: a row stays the same whatever its neighbours are
@@ -487,24 +516,25 @@ __global__ void __launch_bounds__(kWarps * 32, Ring<CT, HD>::CTAS) paged_kernel(
                             minus_m[nt][i] = -top;
                             above[nt][i] = 8.0f;
                             l[nt][i] *= f;
+                            if (!none)
 #pragma unroll
-                            for (int d = 0; d < MT; d++) o[d][nt][i] *= f, o[d][nt][2 + i] *= f;
+                                for (int d = 0; d < MT; d++) o[d][nt][i] *= f, o[d][nt][2 + i] *= f;
                         }
                     }
             }
             // weights
             float vscale = 1.0f, back = 1.0f;
             if constexpr (I8) {
-                float big = scales[kBlock + lane];
+                float big = scales[kBlock + lane % kBlock];
                 big = fabsf(big) < __int_as_float(0x7f800000) ? fabsf(big) : 0.0f;  // inf and NaN make their own way
 #pragma unroll
                 for (int x = 16; x >= 1; x >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, x));
                 const int up = min(max(6 - exponent_of(big), -100), 100);  // p <= 2^8, so p v_scale 2^up < 2^15
                 vscale = power_of_two(up), back = power_of_two(-up);
             }
-            uint32_t pw[2][NT][VP][2];  // [entries 16 mt ..][column tile][plane][first, second 8 entries], transposed
+            uint32_t pw[HALVES][NT][VP][2];  // [entries 16 mt ..][column tile][plane][first, second 8 entries], transposed
 #pragma unroll
-            for (int mt = 0; mt < 2; mt++)
+            for (int mt = 0; mt < HALVES; mt++)
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
                     const int r = 16 * mt + 8 * h + gr;
@@ -539,9 +569,9 @@ __global__ void __launch_bounds__(kWarps * 32, Ring<CT, HD>::CTAS) paged_kernel(
                 constexpr int W = VB / 4, GROUPS = RB / 8 / VB, PER = MT / GROUPS;
 #pragma unroll
                 for (int gi = 0; gi < GROUPS; gi++) {
-                    uint32_t v[2][4][W];  // entries 16 mt + 2t, 2t + 1, 2t + 8, 2t + 9
+                    uint32_t v[HALVES][4][W];  // entries 16 mt + 2t, 2t + 1, 2t + 8, 2t + 9
 #pragma unroll
-                    for (int mt = 0; mt < 2; mt++)
+                    for (int mt = 0; mt < HALVES; mt++)
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
                             const int r = 16 * mt + 2 * t + (e & 1) + 8 * (e >> 1);
@@ -559,7 +589,7 @@ __global__ void __launch_bounds__(kWarps * 32, Ring<CT, HD>::CTAS) paged_kernel(
                     for (int i = 0; i < PER; i++) {
                         float acc[NT][4];
 #pragma unroll
-                        for (int mt = 0; mt < 2; mt++) {
+                        for (int mt = 0; mt < HALVES; mt++) {
                             uint32_t a0, a1, a2, a3;
                             if constexpr (I8) {
                                 // word i / 2: four dims; its first two (i even) or last two, of two entries each
@@ -620,32 +650,36 @@ __global__ void __launch_bounds__(kWarps * 32, Ring<CT, HD>::CTAS) paged_kernel(
         __syncthreads();
         // A cut segment is longer than P = `most` chunks, so no two have one seg_begin / P, and its pieces fit twice that
         // many places.
-        const int64_t place = seg_begin / most;
-        float* part = p.part + (2 * place + piece) * COLS * PITCH;
+        const int place = seg_begin / most;
+        float* part = p.part + (int64_t)(2 * place + piece) * COLS * PITCH;
+        if (threadIdx.x < cols) {  // a column's factors, in the place of the warps' maxima
+            float* at = shared + threadIdx.x * PITCH + HD;
+            float top = -INFINITY, sum = 0.0f, f[kWarps];
+#pragma unroll
+            for (int s = 0; s < kWarps; s++) top = fmaxf(top, at[s * COLS * PITCH]);
+#pragma unroll
+            for (int s = 0; s < kWarps; s++) {
+                const float m = at[s * COLS * PITCH];
+                f[s] = m == -INFINITY ? 1.0f : exp2_approx(m - top);  // no maximum: its shares are zeros, or NaN
+                sum += at[s * COLS * PITCH + 1] * f[s];
+            }
+            if (cuts > 1) __stcg(reinterpret_cast<float2*>(part + threadIdx.x * PITCH + HD), make_float2(top, sum));
+            const float inv = cuts > 1 ? 1.0f : (sum == 0.0f ? 0.0f : 1.0f / sum);
+#pragma unroll
+            for (int s = 0; s < kWarps; s++) at[s * COLS * PITCH] = f[s] * inv;
+        }
+        __syncthreads();
         for (int i = threadIdx.x; i < cols * (HD / 2); i += kWarps * 32) {
             const int x = i / (HD / 2), d = i % (HD / 2) * 2;
-            float top = -INFINITY;
-#pragma unroll
-            for (int s = 0; s < kWarps; s++) top = fmaxf(top, shared[(s * COLS + x) * PITCH + HD]);
-            float sum = 0.0f;
             float2 v = make_float2(0.0f, 0.0f);
 #pragma unroll
             for (int s = 0; s < kWarps; s++) {
                 const float* from = shared + (s * COLS + x) * PITCH;
-                const float f = from[HD] == -INFINITY ? 0.0f : exp2_approx(from[HD] - top);
-                // a warp without an entry has zeros; one whose sum is NaN has no maximum that says so
-                sum += from[HD + 1] * (from[HD] == -INFINITY ? 1.0f : f);
                 const float2 y = *reinterpret_cast<const float2*>(from + d);
-                v.x += y.x * (from[HD] == -INFINITY ? 1.0f : f), v.y += y.y * (from[HD] == -INFINITY ? 1.0f : f);
+                v.x += y.x * from[HD], v.y += y.y * from[HD];
             }
-            if (cuts == 1) {
-                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-                store_out(p, seq, g, x0 + x, d, HD, make_float2(v.x * inv, v.y * inv));
-            } else {
-                float* to = part + x * PITCH;
-                __stcg(reinterpret_cast<float2*>(to + d), v);
-                if (d == 0) __stcg(reinterpret_cast<float2*>(to + HD), make_float2(top, sum));
-            }
+            if (cuts == 1) store_out(p, seq, g, x0 + x, d, HD, v);
+            else __stcg(reinterpret_cast<float2*>(part + x * PITCH + d), v);
         }
         if (cuts > 1) {
             // ---- the segment's pieces together, by the last to come ----
@@ -662,7 +696,7 @@ __global__ void __launch_bounds__(kWarps * 32, Ring<CT, HD>::CTAS) paged_kernel(
                 float2 v = make_float2(0.0f, 0.0f);
 #pragma unroll 4
                 for (int k = 0; k < cuts; k++) {
-                    const float* a = p.part + ((2 * place + k) * COLS + x) * PITCH;
+                    const float* a = p.part + ((int64_t)(2 * place + k) * COLS + x) * PITCH;
                     const float2 ms = __ldcg(reinterpret_cast<const float2*>(a + HD));
                     const float2 y = __ldcg(reinterpret_cast<const float2*>(a + d));
                     const float m2 = fmaxf(top, ms.x);
@@ -683,7 +717,7 @@ int tiles_for(int cols, int head_dim) { return std::min(ceil_div(cols, 8), head_
 
 int cta_limit(const pf_paged_cache& c) {
     const int row = c.head_dim * type_bytes(c.dtype);
-    return 148 * (row == 64 ? 3 : (row == 128 ? 2 : 1));
+    return 148 * (row == 64 ? 4 : 2);  // Ring::CTAS
 }
 
 template <typename CT, int HD, int NT, int PLANES>
@@ -691,14 +725,14 @@ pf_status launch_tiles(PagedParams& p, cudaStream_t st) {
     using R = Ring<CT, HD>;
     p.row_groups = ceil_div(p.cols, 8 * NT);
     p.ctas = cta_limit(p.c);
-    // segments, and with pieces of total / CTAs chunks no more than that many cuts
+    // segments, and with pieces of half of total / CTAs chunks no more than twice that many cuts
     const int64_t segments = (int64_t)p.n_seqs * p.c.n_kv_heads * p.row_groups;
-    const int64_t chunks = std::max<int64_t>(((int64_t)p.c.max_pages * p.c.page_size + kChunk - 1) / kChunk, 1);
-    const int64_t grid = std::min(segments * chunks, segments + p.ctas);
-    PF_CHECK(grid <= INT32_MAX, "pf_paged_attention: too many rows");
+    const int64_t chunks = std::max<int64_t>(((int64_t)p.c.max_pages * p.c.page_size + R::CHUNK - 1) / R::CHUNK, 1);
+    const int64_t grid = std::min(segments * chunks, segments + 2 * p.ctas);
+    PF_CHECK(2 * segments * chunks <= INT32_MAX, "pf_paged_attention: too many positions for one call");
     static std::atomic<uint64_t> attr{0};
     PF_TRY(raise_smem_limit(paged_kernel<CT, HD, NT, PLANES>, R::SMEM, attr));
-    paged_kernel<CT, HD, NT, PLANES><<<(unsigned)grid, kWarps * 32, R::SMEM, st>>>(p);
+    paged_kernel<CT, HD, NT, PLANES><<<(unsigned)grid, R::WARPS * 32, R::SMEM, st>>>(p);
     return launch_check("paged_attention");
 }
 
@@ -724,8 +758,8 @@ size_t pf_paged_attention_work_bytes(const pf_paged_cache* c, int32_t n_seqs, in
     if (c->head_dim != 64 && c->head_dim != 128) return 0;
     const int cols = n_heads / c->n_kv_heads * rows;
     // counters, then the pieces of cut segments
-    return kMaxCtas * sizeof(int) +
-           (size_t)(cta_limit(*c) + 1) * 2 * 8 * tiles_for(cols, c->head_dim) * (c->head_dim + 2) * sizeof(float);
+    return kCounters * sizeof(int) +
+           (size_t)(2 * cta_limit(*c) + 1) * 2 * 8 * tiles_for(cols, c->head_dim) * (c->head_dim + 2) * sizeof(float);
 }
 
 pf_status pf_paged_attention(const pf_paged_cache* c, int32_t layer, const void* q, int64_t q_stride, void* out,
@@ -757,7 +791,7 @@ pf_status pf_paged_attention(const pf_paged_cache* c, int32_t layer, const void*
     p.page_shift = c->page_size == 16 ? 4 : c->page_size == 32 ? 5 : c->page_size == 64 ? 6 : 7;
     p.scale = scale;
     p.count = static_cast<int*>(work);
-    p.part = reinterpret_cast<float*>(static_cast<char*>(work) + kMaxCtas * sizeof(int));
+    p.part = reinterpret_cast<float*>(static_cast<char*>(work) + kCounters * sizeof(int));
     p.err = device_error_flag();
     cudaStream_t st = as_stream(stream);
     if (c->dtype == PF_BF16) return launch_paged<__nv_bfloat16, 1>(p, st);
