@@ -48,7 +48,8 @@ namespace pf {
 
 namespace {
 
-constexpr int kCounters = 2048;  // at the start of `work`: seg_begin / P is at most twice the CTAs that fit
+constexpr int kMaxCuts = 64;     // pieces of a segment: as many as one CTA joins in about a microsecond
+constexpr int kCounters = 1024;  // at the start of `work`: seg_begin / P is below the CTAs that fit
 
 struct PagedParams {
     pf_paged_cache c;
@@ -60,9 +61,13 @@ struct PagedParams {
     float scale;
     int ctas;      // that fit the GPU
     int* count;    // [kCounters] pieces of a cut segment that have ended
-    float* part;   // [piece of a cut segment][columns a row group][head_dim + 2]
+    float* part;   // [piece of a cut segment][columns a row group][head_dim + 4]
     uint32_t* err;
 };
+
+// CTAs that fit an SM, by the bytes of a stored row.  (More of them with shorter rings, where one column tile leaves the
+// registers, measured no faster: the warps that there are keep the loads going.)
+__host__ __device__ constexpr int ctas_per_sm(int row_bytes) { return row_bytes == 64 ? 4 : 2; }
 
 template <typename CT, int HD>
 struct Ring {
@@ -72,9 +77,9 @@ struct Ring {
     static constexpr int CHUNK = WARPS * BLOCK;                     // entries the CTA takes at a time
     static constexpr int SCALES = sizeof(CT) == 1 ? 2 * BLOCK * 4 : 0;
     static constexpr int BYTES = 2 * BLOCK * RB + SCALES;           // keys, values, scales of a block
+    static constexpr int CTAS = ctas_per_sm(RB);
     static constexpr int STAGES = RB == 64 ? 4 : 3;
     static constexpr int SMEM = WARPS * STAGES * BYTES;
-    static constexpr int CTAS = RB == 64 ? 4 : 2;                   // that fit an SM
 };
 
 // Where 16-byte piece c of row r lies: rows read together in other banks.
@@ -197,6 +202,14 @@ __device__ __forceinline__ int chunks_of(int len) {
     return max((len + CHUNK - 1) / CHUNK, 1);
 }
 
+// Pieces of at most `most` chunks that n are cut into (inv = 1 / most; n is exact in fp32), kMaxCuts at most.
+__device__ __forceinline__ int cuts_of(int n, int most, float inv) {
+    int k = (int)((float)n * inv);
+    k += (k + 1) * most <= n;
+    k -= k * most > n;                 // n / most
+    return min(k + (k * most < n), kMaxCuts);
+}
+
 // x / group for a column x of at most eight tokens.
 __device__ __forceinline__ int token_of(int x, int group) {
     int t = 0;
@@ -225,32 +238,36 @@ __global__ void __launch_bounds__(Ring<CT, HD>::WARPS * 32, Ring<CT, HD>::CTAS) 
     constexpr int COLS = 8 * NT;
     constexpr int VP = I8 ? 2 : 1;     // planes of a weight
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ int s_sum[kWarps], s_before, s_seq, s_piece, s_len, s_last;
+    __shared__ int s_before, s_seq, s_piece, s_len, s_cuts, s_most, s_last;
     const pf_paged_cache& c = p.c;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, t = lane & 3;
     const int segs = c.n_kv_heads * p.row_groups;  // of one sequence
 
     // ---- this CTA's piece ----  (the host has seen to it that all chunks count in 31 bits)
-    int mine = 0;
-    for (int b = threadIdx.x; b < p.n_seqs; b += kWarps * 32)
-        mine += chunks_of<R::CHUNK>(length_of(p, b, blockIdx.x == 0 ? p.err : nullptr));
-    mine = __reduce_add_sync(0xffffffffu, mine);
-    if (lane == 0) s_sum[warp] = mine;
-    __syncthreads();
-    int total = 0;
-#pragma unroll
-    for (int i = 0; i < kWarps; i++) total += s_sum[i];
-    total *= segs;
-    // Chunks a piece.  With nearly as many segments as CTAs fit, only what is twice as long as the share is cut; with fewer,
-    // half a share, so that the pieces that come last are small; with very few, a share (the joining would grow).
-    const int segments = p.n_seqs * segs, share = (total + p.ctas - 1) / p.ctas;
-    const int most = 4 * segments >= 3 * p.ctas ? 2 * share : (16 * segments >= p.ctas ? (share + 1) / 2 : share);
-    if (warp == 0) {  // the sequence that it belongs to
+    if (warp == 0) {
+        int total = 0;
+        for (int b = lane; b < p.n_seqs; b += 32) total += chunks_of<R::CHUNK>(length_of(p, b, blockIdx.x == 0 ? p.err : nullptr));
+        total = __reduce_add_sync(0xffffffffu, total) * segs;
+        // Chunks a piece.  With nearly as many segments as CTAs fit, only what is twice as long as the share is cut.  With
+        // fewer, the least with which all pieces are there at once (a second, nearly empty round of CTAs costs more than
+        // pieces that are a little longer): each lane tries one between the share and twice that.
+        const int share = (total + p.ctas - 1) / p.ctas;
+        int most = 2 * share;
+        if (4 * p.n_seqs * segs < 3 * p.ctas) {
+            const int mine = share + lane * ((share + 31) / 32);
+            const float inv = 1.0f / (float)mine;
+            int pieces = 0;
+#pragma unroll 4
+            for (int b = 0; b < p.n_seqs; b++) pieces += cuts_of(chunks_of<R::CHUNK>(length_of(p, b, nullptr)), mine, inv);
+            const unsigned fits = __ballot_sync(0xffffffffu, pieces * segs <= p.ctas);
+            most = __shfl_sync(0xffffffffu, mine, fits ? __ffs((int)fits) - 1 : 31);
+        }
+        const float inv_most = 1.0f / (float)most;
         int pieces = 0, before = 0, found = -1;
         for (int b0 = 0; b0 < p.n_seqs && found < 0; b0 += 32) {
             const int b = b0 + lane, len = b < p.n_seqs ? length_of(p, b, nullptr) : 0;
             const int n = b < p.n_seqs ? chunks_of<R::CHUNK>(len) : 0;
-            const int my_pieces = (n <= most ? min(n, 1) : (n + most - 1) / most) * segs, my_chunks = n * segs;
+            const int cuts = n ? cuts_of(n, most, inv_most) : 0, my_pieces = cuts * segs, my_chunks = n * segs;
             int upto = my_pieces, upto_chunks = my_chunks;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -264,6 +281,8 @@ __global__ void __launch_bounds__(Ring<CT, HD>::WARPS * 32, Ring<CT, HD>::CTAS) 
                     s_piece = (int)blockIdx.x - (pieces + upto - my_pieces);
                     s_before = before + upto_chunks - my_chunks;
                     s_len = len;
+                    s_cuts = cuts;
+                    s_most = most;
                 }
                 found = b0 + at;
             }
@@ -275,7 +294,7 @@ __global__ void __launch_bounds__(Ring<CT, HD>::WARPS * 32, Ring<CT, HD>::CTAS) 
     __syncthreads();
     const int seq = s_seq;
     if (seq < 0) return;  // the grid is an upper bound
-    const int len = s_len, chunks = chunks_of<R::CHUNK>(len), cuts = chunks <= most ? 1 : (chunks + most - 1) / most;
+    const int len = s_len, chunks = chunks_of<R::CHUNK>(len), cuts = s_cuts, most = s_most;
     const int seg = s_piece / cuts, piece = s_piece - seg * cuts, g = seg / p.row_groups, rg = seg - g * p.row_groups;
     const int seg_begin = s_before + seg * chunks;
     const int ch0 = cuts == 1 ? 0 : (int)((int64_t)chunks * piece / cuts);
@@ -415,6 +434,7 @@ __global__ void __launch_bounds__(Ring<CT, HD>::WARPS * 32, Ring<CT, HD>::CTAS) 
 #pragma unroll
             for (int i = 0; i < MT; i++) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.0f;
         }
+        float vscale = 1.0f, back = 1.0f;
         for (int k = 0; k < n_blocks; k++) {
             {
                 const int n0 = page_of(k + ST, 0), n1 = HALVES == 2 ? page_of(k + ST, 1) : -1;
@@ -523,14 +543,15 @@ __global__ void __launch_bounds__(Ring<CT, HD>::WARPS * 32, Ring<CT, HD>::CTAS) 
                     }
             }
             // weights
-            float vscale = 1.0f, back = 1.0f;
+            // int8: 2^up takes the block's largest finite scale to 1 .. 2^7, so that p v_scale 2^up < 2^15 (p <= 2^8); the one
+            // before is kept while it does.
             if constexpr (I8) {
-                float big = scales[kBlock + lane % kBlock];
-                big = fabsf(big) < __int_as_float(0x7f800000) ? fabsf(big) : 0.0f;  // inf and NaN make their own way
-#pragma unroll
-                for (int x = 16; x >= 1; x >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, x));
-                const int up = min(max(6 - exponent_of(big), -100), 100);  // p <= 2^8, so p v_scale 2^up < 2^15
-                vscale = power_of_two(up), back = power_of_two(-up);
+                const float inf = __int_as_float(0x7f800000), vs = fabsf(scales[kBlock + lane]), x = vs * vscale;
+                if (__any_sync(0xffffffffu, x >= 128.0f && vs < inf) || !__any_sync(0xffffffffu, x >= 1.0f && x < inf)) {
+                    const unsigned big = __reduce_max_sync(0xffffffffu, vs < inf ? __float_as_uint(vs) : 0u);
+                    const int up = min(max(6 - exponent_of(__uint_as_float(big)), -100), 100);
+                    vscale = power_of_two(up), back = power_of_two(-up);
+                }
             }
             uint32_t pw[HALVES][NT][VP][2];  // [entries 16 mt ..][column tile][plane][first, second 8 entries], transposed
 #pragma unroll
@@ -626,9 +647,9 @@ __global__ void __launch_bounds__(Ring<CT, HD>::WARPS * 32, Ring<CT, HD>::CTAS) 
 
         // ---- the four warps' shares together ----
         // smem: [warp][column][HD + 2], a row's last two its maximum and sum
-        constexpr int PITCH = HD + 2;
+        constexpr int PITCH = HD + 2, PART = HD + 4;  // here, and in `part` (16-byte loads)
         float* shared = reinterpret_cast<float*>(smem);
-        static_assert(kWarps * COLS * PITCH * 4 <= R::SMEM, "the shares fit the ring");
+        static_assert(kWarps * COLS * PITCH * 4 <= R::SMEM && COLS * kMaxCuts * 4 <= R::SMEM, "the shares fit the ring");
         __syncthreads();  // the rings are empty
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
@@ -651,7 +672,7 @@ __global__ void __launch_bounds__(Ring<CT, HD>::WARPS * 32, Ring<CT, HD>::CTAS) 
         // A cut segment is longer than P = `most` chunks, so no two have one seg_begin / P, and its pieces fit twice that
         // many places.
         const int place = seg_begin / most;
-        float* part = p.part + (int64_t)(2 * place + piece) * COLS * PITCH;
+        float* part = p.part + (int64_t)(2 * place + piece) * COLS * PART;
         if (threadIdx.x < cols) {  // a column's factors, in the place of the warps' maxima
             float* at = shared + threadIdx.x * PITCH + HD;
             float top = -INFINITY, sum = 0.0f, f[kWarps];
@@ -663,7 +684,7 @@ __global__ void __launch_bounds__(Ring<CT, HD>::WARPS * 32, Ring<CT, HD>::CTAS) 
                 f[s] = m == -INFINITY ? 1.0f : exp2_approx(m - top);  // no maximum: its shares are zeros, or NaN
                 sum += at[s * COLS * PITCH + 1] * f[s];
             }
-            if (cuts > 1) __stcg(reinterpret_cast<float2*>(part + threadIdx.x * PITCH + HD), make_float2(top, sum));
+            if (cuts > 1) __stcg(reinterpret_cast<float2*>(part + threadIdx.x * PART + HD), make_float2(top, sum));
             const float inv = cuts > 1 ? 1.0f : (sum == 0.0f ? 0.0f : 1.0f / sum);
 #pragma unroll
             for (int s = 0; s < kWarps; s++) at[s * COLS * PITCH] = f[s] * inv;
@@ -679,7 +700,7 @@ __global__ void __launch_bounds__(Ring<CT, HD>::WARPS * 32, Ring<CT, HD>::CTAS) 
                 v.x += y.x * from[HD], v.y += y.y * from[HD];
             }
             if (cuts == 1) store_out(p, seq, g, x0 + x, d, HD, v);
-            else __stcg(reinterpret_cast<float2*>(part + x * PITCH + d), v);
+            else __stcg(reinterpret_cast<float2*>(part + x * PART + d), v);
         }
         if (cuts > 1) {
             // ---- the segment's pieces together, by the last to come ----
@@ -690,24 +711,43 @@ __global__ void __launch_bounds__(Ring<CT, HD>::WARPS * 32, Ring<CT, HD>::CTAS) 
             if (!s_last) return;
             __threadfence();
             if (threadIdx.x == 0) p.count[place] = 0;  // as it was found
-            for (int i = threadIdx.x; i < cols * (HD / 2); i += kWarps * 32) {
-                const int x = i / (HD / 2), d = i % (HD / 2) * 2;
+            const float* parts = p.part + (int64_t)2 * place * COLS * PART;
+            float* factor = shared;  // [column][kMaxCuts]
+            for (int x = warp; x < cols; x += kWarps) {  // two pieces a lane
+                float2 ms[2];
                 float top = -INFINITY, sum = 0.0f;
-                float2 v = make_float2(0.0f, 0.0f);
-#pragma unroll 4
-                for (int k = 0; k < cuts; k++) {
-                    const float* a = p.part + ((int64_t)(2 * place + k) * COLS + x) * PITCH;
-                    const float2 ms = __ldcg(reinterpret_cast<const float2*>(a + HD));
-                    const float2 y = __ldcg(reinterpret_cast<const float2*>(a + d));
-                    const float m2 = fmaxf(top, ms.x);
-                    const float f0 = top == m2 ? 1.0f : exp2_approx(top - m2);
-                    const float f1 = ms.x == m2 || ms.x == -INFINITY ? 1.0f : exp2_approx(ms.x - m2);
-                    top = m2;
-                    sum = sum * f0 + ms.y * f1;
-                    v.x = v.x * f0 + y.x * f1, v.y = v.y * f0 + y.y * f1;
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const int k = lane + 32 * i;
+                    ms[i] = k < cuts ? __ldcg(reinterpret_cast<const float2*>(parts + ((int64_t)k * COLS + x) * PART + HD))
+                                     : make_float2(-INFINITY, 0.0f);
+                    top = fmaxf(top, ms[i].x);
                 }
+#pragma unroll
+                for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    ms[i].x = ms[i].x == -INFINITY ? 1.0f : exp2_approx(ms[i].x - top);
+                    sum += ms[i].y * ms[i].x;
+                }
+#pragma unroll
+                for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
                 const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-                store_out(p, seq, g, x0 + x, d, HD, make_float2(v.x * inv, v.y * inv));
+#pragma unroll
+                for (int i = 0; i < 2; i++) factor[x * kMaxCuts + lane + 32 * i] = ms[i].x * inv;
+            }
+            __syncthreads();
+            for (int i = threadIdx.x; i < cols * (HD / 4); i += kWarps * 32) {
+                const int x = i / (HD / 4), d = i % (HD / 4) * 4;
+                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+                for (int k = 0; k < cuts; k++) {
+                    const float4 y = __ldcg(reinterpret_cast<const float4*>(parts + ((int64_t)k * COLS + x) * PART + d));
+                    const float f = factor[x * kMaxCuts + k];
+                    v.x += y.x * f, v.y += y.y * f, v.z += y.z * f, v.w += y.w * f;
+                }
+                store_out(p, seq, g, x0 + x, d, HD, make_float2(v.x, v.y));
+                store_out(p, seq, g, x0 + x, d + 2, HD, make_float2(v.z, v.w));
             }
         }
 }
@@ -715,20 +755,17 @@ __global__ void __launch_bounds__(Ring<CT, HD>::WARPS * 32, Ring<CT, HD>::CTAS) 
 // Column tiles of 8 that a CTA takes: as many as the rows need, up to what the registers hold.
 int tiles_for(int cols, int head_dim) { return std::min(ceil_div(cols, 8), head_dim == 64 ? 4 : 2); }
 
-int cta_limit(const pf_paged_cache& c) {
-    const int row = c.head_dim * type_bytes(c.dtype);
-    return 148 * (row == 64 ? 4 : 2);  // Ring::CTAS
-}
+int cta_limit(const pf_paged_cache& c) { return 148 * ctas_per_sm(c.head_dim * type_bytes(c.dtype)); }
 
 template <typename CT, int HD, int NT, int PLANES>
 pf_status launch_tiles(PagedParams& p, cudaStream_t st) {
     using R = Ring<CT, HD>;
     p.row_groups = ceil_div(p.cols, 8 * NT);
     p.ctas = cta_limit(p.c);
-    // segments, and with pieces of half of total / CTAs chunks no more than twice that many cuts
+    // segments, and with pieces of total / CTAs chunks or more no more than that many cuts
     const int64_t segments = (int64_t)p.n_seqs * p.c.n_kv_heads * p.row_groups;
     const int64_t chunks = std::max<int64_t>(((int64_t)p.c.max_pages * p.c.page_size + R::CHUNK - 1) / R::CHUNK, 1);
-    const int64_t grid = std::min(segments * chunks, segments + 2 * p.ctas);
+    const int64_t grid = std::min(segments * chunks, segments + p.ctas);
     PF_CHECK(2 * segments * chunks <= INT32_MAX, "pf_paged_attention: too many positions for one call");
     static std::atomic<uint64_t> attr{0};
     PF_TRY(raise_smem_limit(paged_kernel<CT, HD, NT, PLANES>, R::SMEM, attr));
@@ -756,10 +793,9 @@ extern "C" {
 size_t pf_paged_attention_work_bytes(const pf_paged_cache* c, int32_t n_seqs, int32_t rows, int32_t n_heads) {
     if (!c || n_seqs < 0 || rows < 1 || rows > 8 || n_heads < 1 || c->n_kv_heads < 1 || n_heads % c->n_kv_heads) return 0;
     if (c->head_dim != 64 && c->head_dim != 128) return 0;
-    const int cols = n_heads / c->n_kv_heads * rows;
+    const int nt = tiles_for(n_heads / c->n_kv_heads * rows, c->head_dim);
     // counters, then the pieces of cut segments
-    return kCounters * sizeof(int) +
-           (size_t)(2 * cta_limit(*c) + 1) * 2 * 8 * tiles_for(cols, c->head_dim) * (c->head_dim + 2) * sizeof(float);
+    return kCounters * sizeof(int) + (size_t)(cta_limit(*c) + 1) * 2 * 8 * nt * (c->head_dim + 4) * sizeof(float);
 }
 
 pf_status pf_paged_attention(const pf_paged_cache* c, int32_t layer, const void* q, int64_t q_stride, void* out,
