@@ -340,7 +340,7 @@ PF_API pf_status pf_paged_compact(const pf_paged_cache* c, void* stream);
  * [n_kv_heads][head_dim] of `dtype` at k_stride / v_stride elements, are the
  * last positions of sequence b, whose length counts them already
  * (pf_paged_reserve).  n_tokens rows are there at all; those outside
- * [offsets[0], offsets[n_seqs]) are not read.  dtype: any of PF_F32, PF_BF16,
+ * [offsets[0], offsets[n_seqs]) are left out.  dtype: any of PF_F32, PF_BF16,
  * PF_F16 for a PF_I8 cache; PF_F32 or the cache's own for the others.  A row
  * with an infinity or NaN is stored in a PF_I8 cache with a NaN scale.  k, v
  * and the strides' bytes are multiples of 16. */

@@ -1,12 +1,16 @@
 // paged_store.cu — new keys and values into the pages of the paged cache.
 //
 // A row (token, kv head) is read once and written once: bound by HBM for a
-// prompt, by two trips to memory for a step.  A CTA takes kTokens tokens; its
-// warps first find each one's sequence (a 32-way search of the offsets: two
-// rounds up to 1,024 sequences) and leave its place in shared memory, then
-// every group of LPR lanes moves one row's key and value, 16 bytes a lane of
-// each (fp32, head_dim 64: 16 lanes), the row's largest value found by
-// shuffles.
+// prompt, by the chain of trips to memory (offsets, length, table, row) for a
+// step.  A CTA takes TOKENS tokens, as few as still fill the GPU; its warps
+// first find each one's sequence (a 32-way search of the offsets: two rounds up
+// to 1,024 sequences) and leave its place in shared memory, while the first
+// rows are on their way.  Every group of head_dim / 8 lanes moves one row's key
+// and value, 8 elements a lane of each, kAhead rows in flight, the row's largest
+// value found by shuffles.  Quantising fp32 rows is as much work as moving them:
+// the four quotients of a row (key and value, scale and multiplier) are made by
+// four lanes, one each, and a code is rounded by adding 1.5 * 2^23 (to the
+// nearest, ties to even) and putting the ties right.
 //
 // int8 rows are KVCache::quantize_row's (src/kv_cache.cpp:19-28): scale =
 // amax / 127, code = round(x * (127 / amax)) with halves away from zero, each
@@ -20,7 +24,8 @@ namespace pf {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kTokens = 16;  // tokens a CTA takes
+constexpr int kAhead = 2;  // rows a group of lanes has in flight
+constexpr int kElems = 8;  // elements a lane
 
 // Number of entries of off[0 .. n) that are <= x (they do not decrease), by a whole warp.
 __device__ __forceinline__ int count_le(const int* off, int n, int x) {
@@ -36,106 +41,166 @@ __device__ __forceinline__ int count_le(const int* off, int n, int x) {
     return lo;
 }
 
-template <typename T>
-__device__ __forceinline__ float to_float(T x) {
-    return (float)x;
+// A lane's 8 elements.
+template <typename ST>
+struct alignas(16) Piece {
+    ST e[kElems];
+};
+
+// The largest magnitude of a row, inf if one is inf or NaN, in every lane of it.
+template <typename ST, int LPR>
+__device__ __forceinline__ float largest(const Piece<ST>& x, unsigned mask) {
+    float big = 0.0f;
+    bool bad = false;
+#pragma unroll
+    for (int j = 0; j < kElems; j++) {
+        const float a = fabsf((float)x.e[j]);
+        bad |= !(a <= 3.402823466e38f);
+        big = fmaxf(big, a);
+    }
+    if (bad) big = __int_as_float(0x7f800000);
+#pragma unroll
+    for (int o = LPR / 2; o >= 1; o >>= 1) big = fmaxf(big, __shfl_xor_sync(mask, big, o));
+    return big;
 }
 
+// round(x * mul) with halves away from zero, for |x * mul| <= 127 and a little, as four bytes.
+__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d, float mul) {
+    const float v[4] = {a, b, c, d};
+    int r[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float y = __fmul_rn(v[i], mul), m = fabsf(y), t = __fadd_rn(m, 12582912.0f);
+        // m - round(m) is exact; 1/2 means a tie that went down to an even number
+        const int n = __float_as_int(t) - __float_as_int(12582912.0f) + (__fsub_rn(m, __fsub_rn(t, 12582912.0f)) == 0.5f);
+        r[i] = y < 0.0f ? -n : n;
+    }
+    uint32_t hi, all;
+    asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, 0;" : "=r"(hi) : "r"(r[3]), "r"(r[2]));
+    asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, %3;" : "=r"(all) : "r"(r[1]), "r"(r[0]), "r"(hi));
+    return all;
+}
+
+// One row's key and value into the cache.
 template <typename ST, typename CT, int HD>
+__device__ __forceinline__ void put(const pf_paged_cache& c, int64_t row, const Piece<ST>& k, const Piece<ST>& v, int part,
+                                    unsigned mask) {
+    constexpr int LPR = HD / kElems;
+    CT* to_k = static_cast<CT*>(c.k) + row * HD + part * kElems;
+    CT* to_v = static_cast<CT*>(c.v) + row * HD + part * kElems;
+    if constexpr (sizeof(CT) == 1) {
+        const float big_k = largest<ST, LPR>(k, mask), big_v = largest<ST, LPR>(v, mask);
+        const float inf = __int_as_float(0x7f800000);
+        // lane 0: k's scale, 1: v's, 2: k's multiplier, 3: v's.  127 / big is no number below 127 / FLT_MAX: such a row is
+        // multiplied by 2^64 first.
+        const float big = part & 1 ? big_v : big_k, up = big < 1e-36f ? 18446744073709551616.0f : 1.0f;
+        float q = big == 0.0f ? 1.0f : (part & 2 ? __fdiv_rn(127.0f, big * up) : __fdiv_rn(big, 127.0f));
+        if (!(part & 2) && big == inf) q = __int_as_float(0x7fffffff);
+        if (part < 2) (part ? c.v_scale : c.k_scale)[row] = q;
+        const int first = (threadIdx.x & 31) & ~(LPR - 1);
+        const float mul_k = __shfl_sync(mask, q, first + 2), mul_v = __shfl_sync(mask, q, first + 3);
+        auto codes = [&](const Piece<ST>& x, float big, float mul, CT* to) {
+            uint2 w = make_uint2(0, 0);
+            const float up = big < 1e-36f ? 18446744073709551616.0f : 1.0f;
+            if (big < inf) {
+                w.x = codes4((float)x.e[0] * up, (float)x.e[1] * up, (float)x.e[2] * up, (float)x.e[3] * up, mul);
+                w.y = codes4((float)x.e[4] * up, (float)x.e[5] * up, (float)x.e[6] * up, (float)x.e[7] * up, mul);
+            }
+            *reinterpret_cast<uint2*>(to) = w;
+        };
+        codes(k, big_k, mul_k, to_k);
+        codes(v, big_v, mul_v, to_v);
+    } else {
+        Piece<CT> a, b;
+#pragma unroll
+        for (int j = 0; j < kElems; j++) a.e[j] = (CT)(float)k.e[j], b.e[j] = (CT)(float)v.e[j];  // to the nearest
+        *reinterpret_cast<uint4*>(to_k) = *reinterpret_cast<const uint4*>(&a);
+        *reinterpret_cast<uint4*>(to_v) = *reinterpret_cast<const uint4*>(&b);
+    }
+}
+
+template <typename ST, typename CT, int HD, int TOKENS>
 __global__ void __launch_bounds__(kThreads) store_kernel(const pf_paged_cache c, int layer, const ST* __restrict__ k,
                                                          int64_t k_stride, const ST* __restrict__ v, int64_t v_stride,
                                                          const int* __restrict__ offsets, int n_seqs, int n_tokens,
                                                          uint32_t* err) {
-    constexpr int EPT = 16 / sizeof(ST);  // elements a lane
-    constexpr int LPR = HD / EPT;         // lanes a row
-    __shared__ int s_page[kTokens], s_slot[kTokens];
-    const int t0 = blockIdx.x * kTokens, lane = threadIdx.x & 31;
-    for (int i = threadIdx.x >> 5; i < kTokens; i += kThreads / 32) {
-        const int t = t0 + i;
+    constexpr int LPR = HD / kElems, GROUPS = kThreads / LPR;  // lanes a row, rows the CTA has in hand at once
+    __shared__ int s_page[TOKENS], s_slot[TOKENS];
+    const int t0 = blockIdx.x * TOKENS, lane = threadIdx.x & 31, G = c.n_kv_heads, part = threadIdx.x % LPR;
+    const int tokens = min(TOKENS, n_tokens - t0), rows = tokens * G;
+    // the lanes of a row, which are all here or all not
+    const unsigned mask = (LPR == 32 ? 0xffffffffu : ((1u << (LPR & 31)) - 1u)) << (lane & ~(LPR - 1));
+    int u = threadIdx.x / LPR, i = u / G, g = u - i * G;  // row u: token i of the CTA, kv head g
+    Piece<ST> x[kAhead], y[kAhead];
+    auto load = [&](int i, int g, Piece<ST>& a, Piece<ST>& b) {
+        const uint4* from_k = reinterpret_cast<const uint4*>(k + (t0 + i) * k_stride + g * HD + part * kElems);
+        const uint4* from_v = reinterpret_cast<const uint4*>(v + (t0 + i) * v_stride + g * HD + part * kElems);
+#pragma unroll
+        for (int j = 0; j < (int)sizeof(Piece<ST>) / 16; j++) {
+            reinterpret_cast<uint4*>(&a)[j] = from_k[j];
+            reinterpret_cast<uint4*>(&b)[j] = from_v[j];
+        }
+    };
+    auto next = [&](int& i, int& g) {  // GROUPS rows on
+        g += GROUPS;
+        while (g >= G) g -= G, i++;
+    };
+    auto load_all = [&](int u, int i, int g) {
+#pragma unroll
+        for (int a = 0; a < kAhead; a++) {
+            if (u + a * GROUPS < rows) load(i, g, x[a], y[a]);
+            next(i, g);
+        }
+    };
+    load_all(u, i, g);
+    for (int w = threadIdx.x >> 5; w < tokens; w += kThreads / 32) {
+        const int t = t0 + w, b = count_le(offsets, n_seqs + 1, t) - 1;
         int page = -1, slot = 0;
-        if (t < n_tokens) {
-            const int b = count_le(offsets, n_seqs + 1, t) - 1;
-            if (b >= 0 && b < n_seqs) {
-                const int n = seq_len(c, b, lane == 0 ? err : nullptr);
-                const int64_t pos = (int64_t)n - ((int64_t)offsets[b + 1] - t);
-                if (n >= 0 && pos >= 0 && pos < n) {
-                    page = c.table[(int64_t)b * c.max_pages + pos / c.page_size];
-                    slot = (int)(pos % c.page_size);
-                }
-                if ((unsigned)page >= (unsigned)c.n_pages) {
-                    page = -1;
-                    if (lane == 0) latch(err, ERR_BOUNDS);
-                }
+        if (b >= 0 && b < n_seqs) {
+            const int n = seq_len(c, b, lane == 0 ? err : nullptr);
+            const int64_t pos = (int64_t)n - ((int64_t)offsets[b + 1] - t);
+            if (n >= 0 && pos >= 0 && pos < n) {
+                page = c.table[(int64_t)b * c.max_pages + pos / c.page_size];
+                slot = (int)(pos % c.page_size);
+            }
+            if ((unsigned)page >= (unsigned)c.n_pages) {
+                page = -1;
+                if (lane == 0) latch(err, ERR_BOUNDS);
             }
         }
-        if (lane == 0) s_page[i] = page, s_slot[i] = slot;
+        if (lane == 0) s_page[w] = page, s_slot[w] = slot;
     }
     __syncthreads();
-    const int G = c.n_kv_heads, part = threadIdx.x % LPR;
-    for (int u = threadIdx.x / LPR; u < kTokens * G; u += kThreads / LPR) {  // uniform over the lanes of a row
-        const int i = u / G, g = u % G, page = s_page[i];
-        if (page < 0) continue;
-        union {
-            uint4 w;
-            ST e[EPT];
-        } x[2];
-        x[0].w = *reinterpret_cast<const uint4*>(k + (t0 + i) * k_stride + g * HD + part * EPT);
-        x[1].w = *reinterpret_cast<const uint4*>(v + (t0 + i) * v_stride + g * HD + part * EPT);
-        const int64_t row = slot_row(c, page, layer, g, s_slot[i]);
-        // the lanes of this row, all here
-        const unsigned mask = (LPR == 32 ? 0xffffffffu : ((1u << (LPR & 31)) - 1u)) << (lane & ~(LPR - 1));
+    while (u < rows) {
 #pragma unroll
-        for (int w = 0; w < 2; w++) {
-            CT* to = reinterpret_cast<CT*>(w ? c.v : c.k) + row * HD + part * EPT;
-            union {
-                CT e[EPT];
-                uint32_t w32[EPT * sizeof(CT) / 4 > 0 ? EPT * sizeof(CT) / 4 : 1];
-            } y;
-            if constexpr (sizeof(CT) == 1) {
-                float big = 0.0f;
-                bool bad = false;
-#pragma unroll
-                for (int j = 0; j < EPT; j++) {
-                    const float a = fabsf(to_float(x[w].e[j]));
-                    bad |= !(a <= 3.402823466e38f);
-                    big = fmaxf(big, a);
-                }
-                if (bad) big = __int_as_float(0x7f800000);
-#pragma unroll
-                for (int o = LPR / 2; o >= 1; o >>= 1) big = fmaxf(big, __shfl_xor_sync(mask, big, o));
-                bad = big > 3.402823466e38f;
-                const float scale = bad ? __int_as_float(0x7fffffff) : (big == 0.0f ? 1.0f : __fdiv_rn(big, 127.0f));
-                const float mul = big == 0.0f ? 1.0f : __fdiv_rn(127.0f, big);
-#pragma unroll
-                for (int j = 0; j < EPT; j++)
-                    y.e[j] = bad ? (CT)0 : (CT)(int)roundf(__fmul_rn(to_float(x[w].e[j]), mul));
-                if (part == 0) (w ? c.v_scale : c.k_scale)[row] = scale;
-            } else {
-#pragma unroll
-                for (int j = 0; j < EPT; j++) y.e[j] = (CT)to_float(x[w].e[j]);  // rounded to the nearest
-            }
-            constexpr int WORDS = EPT * sizeof(CT) / 4;
-            if constexpr (WORDS == 4)
-                *reinterpret_cast<uint4*>(to) = make_uint4(y.w32[0], y.w32[1], y.w32[2], y.w32[3]);
-            else if constexpr (WORDS == 2)
-                *reinterpret_cast<uint2*>(to) = make_uint2(y.w32[0], y.w32[1]);
-            else
-                *reinterpret_cast<uint32_t*>(to) = y.w32[0];
+        for (int a = 0; a < kAhead; a++) {
+            if (u < rows && s_page[i] >= 0)
+                put<ST, CT, HD>(c, slot_row(c, s_page[i], layer, g, s_slot[i]), x[a], y[a], part, mask);
+            u += GROUPS;
+            next(i, g);
         }
+        if (u < rows) load_all(u, i, g);
     }
+}
+
+template <typename ST, typename CT, int HD>
+pf_status launch_store(const pf_paged_cache& c, int layer, const void* k, int64_t ks, const void* v, int64_t vs,
+                       const int* offsets, int n_seqs, int n_tokens, cudaStream_t st) {
+    uint32_t* err = device_error_flag();
+    const ST *kp = static_cast<const ST*>(k), *vp = static_cast<const ST*>(v);
+    // 16 tokens a CTA share one round of searches; below four CTAs an SM the chain of a single round is what counts
+    if (n_tokens >= 16 * 4 * 148)
+        store_kernel<ST, CT, HD, 16><<<ceil_div(n_tokens, 16), kThreads, 0, st>>>(c, layer, kp, ks, vp, vs, offsets, n_seqs, n_tokens, err);
+    else
+        store_kernel<ST, CT, HD, 2><<<ceil_div(n_tokens, 2), kThreads, 0, st>>>(c, layer, kp, ks, vp, vs, offsets, n_seqs, n_tokens, err);
+    return launch_check("paged_store");
 }
 
 template <typename ST, typename CT>
 pf_status launch_store(const pf_paged_cache& c, int layer, const void* k, int64_t ks, const void* v, int64_t vs,
                        const int* offsets, int n_seqs, int n_tokens, cudaStream_t st) {
-    const int grid = ceil_div(n_tokens, kTokens);
-    uint32_t* err = device_error_flag();
-    const ST *kp = static_cast<const ST*>(k), *vp = static_cast<const ST*>(v);
-    if (c.head_dim == 64)
-        store_kernel<ST, CT, 64><<<grid, kThreads, 0, st>>>(c, layer, kp, ks, vp, vs, offsets, n_seqs, n_tokens, err);
-    else
-        store_kernel<ST, CT, 128><<<grid, kThreads, 0, st>>>(c, layer, kp, ks, vp, vs, offsets, n_seqs, n_tokens, err);
-    return launch_check("paged_store");
+    return c.head_dim == 64 ? launch_store<ST, CT, 64>(c, layer, k, ks, v, vs, offsets, n_seqs, n_tokens, st)
+                            : launch_store<ST, CT, 128>(c, layer, k, ks, v, vs, offsets, n_seqs, n_tokens, st);
 }
 
 }  // namespace
