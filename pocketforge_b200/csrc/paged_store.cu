@@ -6,8 +6,9 @@
 // first find each one's sequence (a 32-way search of the offsets: two rounds up
 // to 1,024 sequences) and leave its place in shared memory, while the first
 // rows are on their way.  Every group of head_dim / 8 lanes moves one row's key
-// and value, 8 elements a lane of each, kAhead rows in flight, the row's largest
-// value found by shuffles.  Quantising fp32 rows is as much work as moving them:
+// and value, 8 elements a lane of each (two contiguous runs of 4 if they are fp32), the
+// row's largest value found by shuffles.  One row in flight a lane and more CTAs
+// an SM: two or four rows in flight measured 5% and 35% slower on 64 prompts.  Quantising fp32 rows is as much work as moving them:
 // the four quotients of a row (key and value, scale and multiplier) are made by
 // four lanes, one each, and a code is rounded by adding 1.5 * 2^23 (to the
 // nearest, ties to even) and putting the ties right.
@@ -24,7 +25,6 @@ namespace pf {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kAhead = 2;  // rows a group of lanes has in flight
 constexpr int kElems = 8;  // elements a lane
 
 // Number of entries of off[0 .. n) that are <= x (they do not decrease), by a whole warp.
@@ -41,9 +41,10 @@ __device__ __forceinline__ int count_le(const int* off, int n, int x) {
     return lo;
 }
 
-// A lane's 8 elements.
+// A lane's 8 elements: 8 at 8 * part, or (fp32) 4 at 4 * part of either half of the row, so that a group's loads are runs.
 template <typename ST>
 struct alignas(16) Piece {
+    static constexpr int RUNS = sizeof(ST) / 2, RUN = kElems / RUNS;
     ST e[kElems];
 };
 
@@ -86,8 +87,9 @@ template <typename ST, typename CT, int HD>
 __device__ __forceinline__ void put(const pf_paged_cache& c, int64_t row, const Piece<ST>& k, const Piece<ST>& v, int part,
                                     unsigned mask) {
     constexpr int LPR = HD / kElems;
-    CT* to_k = static_cast<CT*>(c.k) + row * HD + part * kElems;
-    CT* to_v = static_cast<CT*>(c.v) + row * HD + part * kElems;
+    constexpr int RUNS = Piece<ST>::RUNS, RUN = Piece<ST>::RUN;
+    CT* to_k = static_cast<CT*>(c.k) + row * HD + part * RUN;
+    CT* to_v = static_cast<CT*>(c.v) + row * HD + part * RUN;
     if constexpr (sizeof(CT) == 1) {
         const float big_k = largest<ST, LPR>(k, mask), big_v = largest<ST, LPR>(v, mask);
         const float inf = __int_as_float(0x7f800000);
@@ -106,7 +108,8 @@ __device__ __forceinline__ void put(const pf_paged_cache& c, int64_t row, const 
                 w.x = codes4((float)x.e[0] * up, (float)x.e[1] * up, (float)x.e[2] * up, (float)x.e[3] * up, mul);
                 w.y = codes4((float)x.e[4] * up, (float)x.e[5] * up, (float)x.e[6] * up, (float)x.e[7] * up, mul);
             }
-            *reinterpret_cast<uint2*>(to) = w;
+            if constexpr (RUNS == 1) *reinterpret_cast<uint2*>(to) = w;
+            else *reinterpret_cast<uint32_t*>(to) = w.x, *reinterpret_cast<uint32_t*>(to + HD / 2) = w.y;
         };
         codes(k, big_k, mul_k, to_k);
         codes(v, big_v, mul_v, to_v);
@@ -114,8 +117,16 @@ __device__ __forceinline__ void put(const pf_paged_cache& c, int64_t row, const 
         Piece<CT> a, b;
 #pragma unroll
         for (int j = 0; j < kElems; j++) a.e[j] = (CT)(float)k.e[j], b.e[j] = (CT)(float)v.e[j];  // to the nearest
-        *reinterpret_cast<uint4*>(to_k) = *reinterpret_cast<const uint4*>(&a);
-        *reinterpret_cast<uint4*>(to_v) = *reinterpret_cast<const uint4*>(&b);
+        if constexpr (RUNS == 1) {
+            *reinterpret_cast<uint4*>(to_k) = *reinterpret_cast<const uint4*>(&a);
+            *reinterpret_cast<uint4*>(to_v) = *reinterpret_cast<const uint4*>(&b);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                *reinterpret_cast<uint2*>(to_k + j * HD / 2) = reinterpret_cast<const uint2*>(&a)[j];
+                *reinterpret_cast<uint2*>(to_v + j * HD / 2) = reinterpret_cast<const uint2*>(&b)[j];
+            }
+        }
     }
 }
 
@@ -131,55 +142,45 @@ __global__ void __launch_bounds__(kThreads) store_kernel(const pf_paged_cache c,
     // the lanes of a row, which are all here or all not
     const unsigned mask = (LPR == 32 ? 0xffffffffu : ((1u << (LPR & 31)) - 1u)) << (lane & ~(LPR - 1));
     int u = threadIdx.x / LPR, i = u / G, g = u - i * G;  // row u: token i of the CTA, kv head g
-    Piece<ST> x[kAhead], y[kAhead];
-    auto load = [&](int i, int g, Piece<ST>& a, Piece<ST>& b) {
-        const uint4* from_k = reinterpret_cast<const uint4*>(k + (t0 + i) * k_stride + g * HD + part * kElems);
-        const uint4* from_v = reinterpret_cast<const uint4*>(v + (t0 + i) * v_stride + g * HD + part * kElems);
+    Piece<ST> x, y;
+    auto load = [&]() {
+        using P = Piece<ST>;
+        const ST* from_k = k + (t0 + i) * k_stride + g * HD + part * P::RUN;
+        const ST* from_v = v + (t0 + i) * v_stride + g * HD + part * P::RUN;
 #pragma unroll
-        for (int j = 0; j < (int)sizeof(Piece<ST>) / 16; j++) {
-            reinterpret_cast<uint4*>(&a)[j] = from_k[j];
-            reinterpret_cast<uint4*>(&b)[j] = from_v[j];
+        for (int j = 0; j < P::RUNS; j++) {
+            reinterpret_cast<uint4*>(&x)[j] = *reinterpret_cast<const uint4*>(from_k + j * HD / 2);
+            reinterpret_cast<uint4*>(&y)[j] = *reinterpret_cast<const uint4*>(from_v + j * HD / 2);
         }
     };
-    auto next = [&](int& i, int& g) {  // GROUPS rows on
-        g += GROUPS;
-        while (g >= G) g -= G, i++;
-    };
-    auto load_all = [&](int u, int i, int g) {
-#pragma unroll
-        for (int a = 0; a < kAhead; a++) {
-            if (u + a * GROUPS < rows) load(i, g, x[a], y[a]);
-            next(i, g);
-        }
-    };
-    load_all(u, i, g);
-    for (int w = threadIdx.x >> 5; w < tokens; w += kThreads / 32) {
-        const int t = t0 + w, b = count_le(offsets, n_seqs + 1, t) - 1;
-        int page = -1, slot = 0;
-        if (b >= 0 && b < n_seqs) {
-            const int n = seq_len(c, b, lane == 0 ? err : nullptr);
-            const int64_t pos = (int64_t)n - ((int64_t)offsets[b + 1] - t);
-            if (n >= 0 && pos >= 0 && pos < n) {
-                page = c.table[(int64_t)b * c.max_pages + pos / c.page_size];
-                slot = (int)(pos % c.page_size);
+    if (u < rows) load();
+    if (threadIdx.x < 32) {  // one search for the first token; the others' sequences are close behind
+        int b = count_le(offsets, n_seqs + 1, t0) - 1;
+        if (lane < tokens) {
+            const int t = t0 + lane;
+            while (b < n_seqs && offsets[b + 1] <= t) b++;  // (b = -1: offsets[0] > t0)
+            int page = -1, slot = 0;
+            if (b >= 0 && b < n_seqs) {
+                const int n = seq_len(c, b, err);
+                const int64_t pos = (int64_t)n - ((int64_t)offsets[b + 1] - t);
+                if (n >= 0 && pos >= 0 && pos < n) {
+                    page = c.table[(int64_t)b * c.max_pages + pos / c.page_size];
+                    slot = (int)(pos % c.page_size);
+                }
+                if ((unsigned)page >= (unsigned)c.n_pages) {
+                    page = -1;
+                    latch(err, ERR_BOUNDS);
+                }
             }
-            if ((unsigned)page >= (unsigned)c.n_pages) {
-                page = -1;
-                if (lane == 0) latch(err, ERR_BOUNDS);
-            }
+            s_page[lane] = page, s_slot[lane] = slot;
         }
-        if (lane == 0) s_page[w] = page, s_slot[w] = slot;
     }
     __syncthreads();
     while (u < rows) {
-#pragma unroll
-        for (int a = 0; a < kAhead; a++) {
-            if (u < rows && s_page[i] >= 0)
-                put<ST, CT, HD>(c, slot_row(c, s_page[i], layer, g, s_slot[i]), x[a], y[a], part, mask);
-            u += GROUPS;
-            next(i, g);
-        }
-        if (u < rows) load_all(u, i, g);
+        if (s_page[i] >= 0) put<ST, CT, HD>(c, slot_row(c, s_page[i], layer, g, s_slot[i]), x, y, part, mask);
+        u += GROUPS;
+        for (g += GROUPS; g >= G; g -= G) i++;
+        if (u < rows) load();
     }
 }
 
