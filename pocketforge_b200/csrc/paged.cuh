@@ -19,22 +19,22 @@ struct PageWork {
     int* dst;      // [n_pages]
     int* remap;    // [n_pages] new place of a moved page
     int* mark;     // [max_seqs] first list index that names the sequence
-    int* plan;     // [max_seqs] per list index: pages asked for before it, or its fresh page
+    int4* plan;    // [max_seqs] per list index: pages asked for before it; of a fork, {fresh page, parent's page, length}
 };
 __host__ __device__ inline PageWork page_work(const pf_paged_cache& c) {
     int* w = reinterpret_cast<int*>(c.work);
     PageWork p;
     p.n_list = w;
     p.n_live = w + 1;
-    p.src = w + 4;
+    p.plan = reinterpret_cast<int4*>(w + 4);
+    p.src = w + 4 + 4 * (int64_t)c.max_seqs;
     p.dst = p.src + c.n_pages;
     p.remap = p.dst + c.n_pages;
     p.mark = p.remap + c.n_pages;
-    p.plan = p.mark + c.max_seqs;
     return p;
 }
 inline size_t page_work_bytes(const pf_paged_cache& c) {
-    return (4 + 3 * (size_t)c.n_pages + 2 * (size_t)c.max_seqs) * sizeof(int);
+    return (4 + 3 * (size_t)c.n_pages + 5 * (size_t)c.max_seqs) * sizeof(int);
 }
 
 __host__ __device__ inline int type_bytes(int dtype) { return dtype == PF_F32 ? 4 : (dtype == PF_I8 ? 1 : 2); }
@@ -51,6 +51,30 @@ __device__ __forceinline__ int seq_len(const pf_paged_cache& c, int b, uint32_t*
     if (n >= 0 && (int64_t)n <= (int64_t)c.max_pages * c.page_size) return n;
     latch(err, ERR_BOUNDS);
     return -1;
+}
+
+// A launch that may begin while the one before it in the stream still runs: the
+// kernel waits for that one's end itself (after_previous) before it reads or
+// writes anything, so only the way to its first instruction overlaps.
+template <typename... P, typename... A>
+pf_status launch_after(const char* what, void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st,
+                       A... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    PF_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+    return launch_check(what);
+}
+__device__ __forceinline__ void after_previous() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
 }  // namespace pf

@@ -243,6 +243,7 @@ __global__ void __launch_bounds__(Ring<CT, HD>::WARPS * 32, Ring<CT, HD>::CTAS) 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, t = lane & 3;
     const int segs = c.n_kv_heads * p.row_groups;  // of one sequence
 
+    after_previous();
     // ---- this CTA's piece ----  (the host has seen to it that all chunks count in 31 bits)
     if (warp == 0) {
         int total = 0;
@@ -769,8 +770,7 @@ pf_status launch_tiles(PagedParams& p, cudaStream_t st) {
     PF_CHECK(2 * segments * chunks <= INT32_MAX, "pf_paged_attention: too many positions for one call");
     static std::atomic<uint64_t> attr{0};
     PF_TRY(raise_smem_limit(paged_kernel<CT, HD, NT, PLANES>, R::SMEM, attr));
-    paged_kernel<CT, HD, NT, PLANES><<<(unsigned)grid, R::WARPS * 32, R::SMEM, st>>>(p);
-    return launch_check("paged_attention");
+    return launch_after("paged_attention", paged_kernel<CT, HD, NT, PLANES>, dim3((unsigned)grid), R::WARPS * 32, R::SMEM, st, p);
 }
 
 template <typename CT, int PLANES>

@@ -64,6 +64,7 @@ __device__ __forceinline__ Share share_of(const pf_paged_cache& c, int64_t base,
     s.first = (int)min(first, (int64_t)c.n_pages);
     s.count = (int)min((int64_t)per, (int64_t)c.n_pages - s.first);
     s.live = 0;
+#pragma unroll 8
     for (int i = 0; i < s.count; i++) s.live |= (unsigned long long)(c.refs[s.first + i] > 0) << i;
     return s;
 }
@@ -117,6 +118,7 @@ __device__ __forceinline__ int reserve_need(const pf_paged_cache& c, const PageW
 
 __global__ void __launch_bounds__(kDecide) reserve_kernel(const pf_paged_cache c, const int* seqs, const int* counts,
                                                           int n, uint32_t* err) {
+    after_previous();
     __shared__ long long s_warp[32];
     const PageWork w = page_work(c);
     mark_first(c, seqs, n, w.mark);
@@ -126,7 +128,7 @@ __global__ void __launch_bounds__(kDecide) reserve_kernel(const pf_paged_cache c
         const int need = i < n ? reserve_need(c, w, seqs, counts, i, err) : 0;
         long long total;
         const long long before = want + block_scan(max(need, 0), &total, s_warp);
-        if (i < n) w.plan[i] = need < 0 ? -1 : (int)min(before, (long long)INT_MAX);
+        if (i < n) w.plan[i].x = need < 0 ? -1 : (int)min(before, (long long)INT_MAX);
         want += total;
     }
     const int found = want > 0 ? list_free(c, min(want, (long long)c.n_pages), w.src, s_warp) : 0;
@@ -134,7 +136,7 @@ __global__ void __launch_bounds__(kDecide) reserve_kernel(const pf_paged_cache c
     // one warp an entry: its pages are w.src[before .. before + need)
     const int lane = threadIdx.x & 31;
     for (int i = threadIdx.x >> 5; i < n; i += kDecide / 32) {
-        const int before = w.plan[i];
+        const int before = w.plan[i].x;
         if (before < 0) continue;
         const int s = seqs[i], len = c.lens[s], old = (len + c.page_size - 1) / c.page_size;
         const int need = (int)(((int64_t)len + counts[i] + c.page_size - 1) / c.page_size) - old;
@@ -155,6 +157,7 @@ __global__ void __launch_bounds__(kDecide) reserve_kernel(const pf_paged_cache c
 // One CTA a sequence; whoever takes its length first frees it, so one named
 // twice is freed once.
 __global__ void free_kernel(const pf_paged_cache c, const int* seqs, uint32_t* err) {
+    after_previous();
     __shared__ int s_len;
     const int s = seqs[blockIdx.x];
     if (!in_range(s, c.max_seqs)) {
@@ -181,7 +184,7 @@ constexpr int kForkNone = -1, kForkRefused = -2;  // no partly filled page; left
 
 __global__ void __launch_bounds__(kDecide) fork_decide_kernel(const pf_paged_cache c, const int* parents,
                                                               const int* children, int n, uint32_t* err) {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    after_previous();
     __shared__ long long s_warp[32];
     const PageWork w = page_work(c);
     mark_first(c, children, n, w.mark);
@@ -192,34 +195,37 @@ __global__ void __launch_bounds__(kDecide) fork_decide_kernel(const pf_paged_cac
     for (int base = 0; base < n; base += kDecide) {
         const int i = base + threadIdx.x;
         int need = 0;
+        int4 plan = make_int4(kForkRefused, -1, 0, 0);
         if (i < n) {
             const int p = parents[i], k = children[i];
             bool ok = in_range(p, c.max_seqs) && in_range(k, c.max_seqs) && w.mark[k] == i && c.lens[k] == 0;
-            int len = 0;
-            if (ok) len = seq_len(c, p, err), ok = len >= 0;
-            if (ok && len % c.page_size) {
-                need = 1;
-                ok = in_range(c.table[(int64_t)p * c.max_pages + len / c.page_size], c.n_pages);
+            if (ok) plan.z = seq_len(c, p, err), ok = plan.z >= 0;
+            if (ok && plan.z % c.page_size) {
+                plan.y = c.table[(int64_t)p * c.max_pages + plan.z / c.page_size];
+                ok = in_range(plan.y, c.n_pages);
+                need = ok;
             }
-            if (!ok) latch(err, ERR_BOUNDS), need = 0;
-            w.plan[i] = ok ? kForkNone : kForkRefused;
+            if (ok) plan.x = kForkNone;
+            else latch(err, ERR_BOUNDS);
         }
         long long total;
         const long long before = want + block_scan(need, &total, s_warp);
-        if (need) w.plan[i] = (int)before;
+        if (need) plan.x = (int)before;
+        if (i < n) w.plan[i] = plan;
         want += total;
     }
     const int found = want > 0 ? list_free(c, min(want, (long long)c.n_pages), w.src, s_warp) : 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < n; i += kDecide) {
-        const int rank = w.plan[i];
+    for (int i = threadIdx.x; i < n; i += kDecide) {  // (each thread its own)
+        const int rank = w.plan[i].x;
         if (rank < 0) continue;
         if (rank >= found) {
             latch(err, ERR_CONTEXT);
-            w.plan[i] = kForkRefused;
+            w.plan[i].x = kForkRefused;
         } else {
-            w.plan[i] = w.src[rank];
-            c.refs[w.src[rank]] = 1;
+            const int page = w.src[rank];
+            w.plan[i].x = page;
+            c.refs[page] = 1;
         }
     }
 }
@@ -228,12 +234,14 @@ __global__ void __launch_bounds__(kDecide) fork_decide_kernel(const pf_paged_cac
 // page's positions of eight (layer, kv head) pairs, one a warp.
 __global__ void __launch_bounds__(kCopy) fork_copy_kernel(const pf_paged_cache c, const int* parents,
                                                           const int* children, uint32_t* err) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int i = blockIdx.y, fresh = page_work(c).plan[i];
+    after_previous();
+    const int i = blockIdx.y;
+    const int4 plan = page_work(c).plan[i];
+    const int fresh = plan.x, len = plan.z, full = len / c.page_size, rest = len % c.page_size;
     if (fresh == kForkRefused) return;
-    const int p = parents[i], k = children[i], len = c.lens[p], full = len / c.page_size, rest = len % c.page_size;
-    const int* from = c.table + (int64_t)p * c.max_pages;
     if (blockIdx.x == 0) {
+        const int p = parents[i], k = children[i];
+        const int* from = c.table + (int64_t)p * c.max_pages;
         int* to = c.table + (int64_t)k * c.max_pages;
         for (int j = threadIdx.x; j < full; j += kCopy) {
             const int page = from[j];
@@ -249,7 +257,7 @@ __global__ void __launch_bounds__(kCopy) fork_copy_kernel(const pf_paged_cache c
     if (!rest) return;
     const int lane = threadIdx.x & 31, pair = blockIdx.x * (kCopy / 32) + (threadIdx.x >> 5);
     if (pair >= c.n_layers * c.n_kv_heads) return;
-    const int64_t a = slot_row(c, from[full], 0, pair, 0), b = slot_row(c, fresh, 0, pair, 0);
+    const int64_t a = slot_row(c, plan.y, 0, pair, 0), b = slot_row(c, fresh, 0, pair, 0);
     const int row = c.head_dim * type_bytes(c.dtype), vecs = rest * row / 16;
     const uint4* ka = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(c.k) + a * row);
     const uint4* va = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(c.v) + a * row);
@@ -319,13 +327,14 @@ __device__ __forceinline__ void copy_pages(const pf_paged_cache& c, const int* s
 
 __global__ void __launch_bounds__(kCopy) copy_kernel(const pf_paged_cache c, const int* src, const int* dst, int n,
                                                      uint32_t* err) {
+    after_previous();
     copy_pages(c, src, dst, n, err);
 }
 
 // n_live, the pages in use behind it (src) and the free ones before it (dst),
 // pairwise; reference counts move with them.
 __global__ void __launch_bounds__(kDecide) compact_decide_kernel(const pf_paged_cache c) {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    after_previous();
     __shared__ long long s_warp[32];
     const PageWork w = page_work(c);
     const int per = share_size(c.n_pages);
@@ -365,7 +374,7 @@ __global__ void __launch_bounds__(kDecide) compact_decide_kernel(const pf_paged_
 }
 
 __global__ void __launch_bounds__(kCopy) compact_move_kernel(const pf_paged_cache c, uint32_t* err) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    after_previous();
     const PageWork w = page_work(c);
     const int n = *w.n_list, n_live = *w.n_live;
     if (n == 0) return;  // in order already
@@ -381,23 +390,6 @@ __global__ void __launch_bounds__(kCopy) compact_move_kernel(const pf_paged_cach
         }
     }
     copy_pages(c, w.src, w.dst, n, err);
-}
-
-// A launch that may begin while the one before it in the stream still runs
-// (it waits for that one's end itself, by griddepcontrol.wait).
-template <typename... P, typename... A>
-pf_status launch_after(void (*kernel)(P...), dim3 grid, int threads, cudaStream_t st, A... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(threads);
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    PF_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
-    return PF_OK;
 }
 
 constexpr int kCopyCtas = 148 * 8;  // all SMs full of copying CTAs
@@ -442,8 +434,7 @@ pf_status pf_paged_reserve(const pf_paged_cache* c, const int32_t* seqs, const i
     PF_TRY(require_device());
     if (n == 0) return PF_OK;
     PF_CHECK(seqs && counts, "pf_paged_reserve: null argument");
-    reserve_kernel<<<1, kDecide, 0, as_stream(stream)>>>(*c, seqs, counts, n, device_error_flag());
-    return launch_check("reserve");
+    return launch_after("reserve", reserve_kernel, dim3(1), kDecide, 0, as_stream(stream), *c, seqs, counts, n, device_error_flag());
 }
 
 pf_status pf_paged_free(const pf_paged_cache* c, const int32_t* seqs, int32_t n, void* stream) {
@@ -452,8 +443,7 @@ pf_status pf_paged_free(const pf_paged_cache* c, const int32_t* seqs, int32_t n,
     PF_TRY(require_device());
     if (n == 0) return PF_OK;
     PF_CHECK(seqs, "pf_paged_free: null argument");
-    free_kernel<<<n, 128, 0, as_stream(stream)>>>(*c, seqs, device_error_flag());
-    return launch_check("free");
+    return launch_after("free", free_kernel, dim3(n), 128, 0, as_stream(stream), *c, seqs, device_error_flag());
 }
 
 pf_status pf_paged_fork(const pf_paged_cache* c, const int32_t* parents, const int32_t* children, int32_t n,
@@ -464,10 +454,9 @@ pf_status pf_paged_fork(const pf_paged_cache* c, const int32_t* parents, const i
     if (n == 0) return PF_OK;
     PF_CHECK(parents && children, "pf_paged_fork: null argument");
     uint32_t* err = device_error_flag();
-    fork_decide_kernel<<<1, kDecide, 0, as_stream(stream)>>>(*c, parents, children, n, err);
-    PF_TRY(launch_check("fork_decide"));
+    PF_TRY(launch_after("fork_decide", fork_decide_kernel, dim3(1), kDecide, 0, as_stream(stream), *c, parents, children, n, err));
     const dim3 grid(ceil_div(c->n_layers * c->n_kv_heads, kCopy / 32), n);
-    return launch_after(fork_copy_kernel, grid, kCopy, as_stream(stream), *c, parents, children, err);
+    return launch_after("fork_copy", fork_copy_kernel, grid, kCopy, 0, as_stream(stream), *c, parents, children, err);
 }
 
 pf_status pf_paged_copy(const pf_paged_cache* c, const int32_t* src, const int32_t* dst, int32_t n, void* stream) {
@@ -476,16 +465,14 @@ pf_status pf_paged_copy(const pf_paged_cache* c, const int32_t* src, const int32
     PF_TRY(require_device());
     if (n == 0) return PF_OK;
     PF_CHECK(src && dst, "pf_paged_copy: null argument");
-    copy_kernel<<<kCopyCtas, kCopy, 0, as_stream(stream)>>>(*c, src, dst, n, device_error_flag());
-    return launch_check("copy");
+    return launch_after("copy", copy_kernel, dim3(kCopyCtas), kCopy, 0, as_stream(stream), *c, src, dst, n, device_error_flag());
 }
 
 pf_status pf_paged_compact(const pf_paged_cache* c, void* stream) {
     PF_TRY(check_paged_cache(c, "pf_paged_compact", true));
     PF_TRY(require_device());
-    compact_decide_kernel<<<1, kDecide, 0, as_stream(stream)>>>(*c);
-    PF_TRY(launch_check("compact_decide"));
-    return launch_after(compact_move_kernel, dim3(kCopyCtas), kCopy, as_stream(stream), *c, device_error_flag());
+    PF_TRY(launch_after("compact_decide", compact_decide_kernel, dim3(1), kDecide, 0, as_stream(stream), *c));
+    return launch_after("compact_move", compact_move_kernel, dim3(kCopyCtas), kCopy, 0, as_stream(stream), *c, device_error_flag());
 }
 
 }  // extern "C"

@@ -137,6 +137,7 @@ __global__ void __launch_bounds__(kThreads) store_kernel(const pf_paged_cache c,
                                                          uint32_t* err) {
     constexpr int LPR = HD / kElems, GROUPS = kThreads / LPR;  // lanes a row, rows the CTA has in hand at once
     __shared__ int s_page[TOKENS], s_slot[TOKENS];
+    after_previous();
     const int t0 = blockIdx.x * TOKENS, lane = threadIdx.x & 31, G = c.n_kv_heads, part = threadIdx.x % LPR;
     const int tokens = min(TOKENS, n_tokens - t0), rows = tokens * G;
     // the lanes of a row, which are all here or all not
@@ -191,10 +192,10 @@ pf_status launch_store(const pf_paged_cache& c, int layer, const void* k, int64_
     const ST *kp = static_cast<const ST*>(k), *vp = static_cast<const ST*>(v);
     // 16 tokens a CTA share one round of searches; below four CTAs an SM the chain of a single round is what counts
     if (n_tokens >= 16 * 4 * 148)
-        store_kernel<ST, CT, HD, 16><<<ceil_div(n_tokens, 16), kThreads, 0, st>>>(c, layer, kp, ks, vp, vs, offsets, n_seqs, n_tokens, err);
-    else
-        store_kernel<ST, CT, HD, 2><<<ceil_div(n_tokens, 2), kThreads, 0, st>>>(c, layer, kp, ks, vp, vs, offsets, n_seqs, n_tokens, err);
-    return launch_check("paged_store");
+        return launch_after("paged_store", store_kernel<ST, CT, HD, 16>, dim3(ceil_div(n_tokens, 16)), kThreads, 0, st, c, layer, kp, ks,
+                            vp, vs, offsets, n_seqs, n_tokens, err);
+    return launch_after("paged_store", store_kernel<ST, CT, HD, 2>, dim3(ceil_div(n_tokens, 2)), kThreads, 0, st, c, layer, kp, ks, vp,
+                        vs, offsets, n_seqs, n_tokens, err);
 }
 
 template <typename ST, typename CT>

@@ -393,6 +393,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     UnitList list;
     Unit unit;
+    after_previous();
     if (warp == 8) {
         const bool found = list.find(p, blockIdx.x, unit);
         if (lane == 0) {
@@ -890,8 +891,7 @@ pf_status launch_prompt(const PromptParams& p, cudaStream_t st) {
     if (units == 0) return PF_OK;  // not one sequence can hold a row
     static std::atomic<uint64_t> attr{0};
     PF_TRY(raise_smem_limit(prompt_kernel<T, HD>, Ly::SMEM, attr));
-    prompt_kernel<T, HD><<<(unsigned)units, kThreads, Ly::SMEM, st>>>(mq, mk, mv, p);
-    return launch_check("prompt_attention");
+    return launch_after("prompt_attention", prompt_kernel<T, HD>, dim3((unsigned)units), kThreads, Ly::SMEM, st, mq, mk, mv, p);
 }
 
 }  // namespace
