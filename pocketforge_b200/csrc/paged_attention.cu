@@ -452,41 +452,43 @@ __global__ void __launch_bounds__(Ring<CT, HD>::WARPS * 32, Ring<CT, HD>::CTAS) 
             const uint8_t* vb = kb + kBlock * RB;
             const float* scales = reinterpret_cast<const float*>(vb + kBlock * RB);
 
-            // scores of 16 entries each: rows gr, gr + 8
+            // Scores of 16 entries each: rows gr, gr + 8.  All tiles take one product before any takes its next, so that
+            // a product does not wait for the one before it.
             float s[HALVES][NT][4];
 #pragma unroll
-            for (int mt = 0; mt < HALVES; mt++) {
-                const int r0 = 16 * mt + gr, r1 = r0 + 8;
+            for (int j = 0; j < RB / 64; j++) {  // pieces t, t + 4, ...
+                uint32_t w[HALVES][2][4];
 #pragma unroll
-                for (int j = 0; j < RB / 64; j++) {  // pieces t, t + 4, ...
-                    const uint4 a = *reinterpret_cast<const uint4*>(kb + key_at<RB>(r0, 4 * j + t));
-                    const uint4 b = *reinterpret_cast<const uint4*>(kb + key_at<RB>(r1, 4 * j + t));
-                    const uint32_t wa[4] = {a.x, a.y, a.z, a.w}, wb[4] = {b.x, b.y, b.z, b.w};
-                    if constexpr (I8) {
+                for (int mt = 0; mt < HALVES; mt++)
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const uint32_t ua = wa[i] ^ 0x80808080u, ub = wb[i] ^ 0x80808080u;
-                            const uint32_t a0 = bytes_to_half2(ua, 0x4140), a2 = bytes_to_half2(ua, 0x4342);
-                            const uint32_t a1 = bytes_to_half2(ub, 0x4140), a3 = bytes_to_half2(ub, 0x4342);
+                    for (int h = 0; h < 2; h++) {
+                        const uint4 x = *reinterpret_cast<const uint4*>(kb + key_at<RB>(16 * mt + 8 * h + gr, 4 * j + t));
+                        w[mt][h][0] = x.x, w[mt][h][1] = x.y, w[mt][h][2] = x.z, w[mt][h][3] = x.w;
+                    }
 #pragma unroll
-                            for (int nt = 0; nt < NT; nt++)
+                for (int i = 0; i < (I8 ? 4 : 2); i++) {
+                    uint32_t f[HALVES][4];
 #pragma unroll
-                                for (int pl = 0; pl < PLANES; pl++) {
-                                    const uint32_t(&b)[2] = q[nt][pl][4 * j + i];
-                                    if (i + j + pl == 0) mma_first<false>(s[mt][nt], a0, a1, a2, a3, b[0], b[1]);
-                                    else mma<false>(s[mt][nt], a0, a1, a2, a3, b[0], b[1]);
-                                }
+                    for (int mt = 0; mt < HALVES; mt++) {
+                        if constexpr (I8) {
+                            const uint32_t ua = w[mt][0][i] ^ 0x80808080u, ub = w[mt][1][i] ^ 0x80808080u;
+                            f[mt][0] = bytes_to_half2(ua, 0x4140), f[mt][2] = bytes_to_half2(ua, 0x4342);
+                            f[mt][1] = bytes_to_half2(ub, 0x4140), f[mt][3] = bytes_to_half2(ub, 0x4342);
+                        } else {
+                            f[mt][0] = w[mt][0][2 * i], f[mt][1] = w[mt][1][2 * i];
+                            f[mt][2] = w[mt][0][2 * i + 1], f[mt][3] = w[mt][1][2 * i + 1];
                         }
-                    } else {
+                    }
 #pragma unroll
-                        for (int i = 0; i < 2; i++)
+                    for (int pl = 0; pl < PLANES; pl++)
+#pragma unroll
+                        for (int mt = 0; mt < HALVES; mt++)
 #pragma unroll
                             for (int nt = 0; nt < NT; nt++) {
-                                const uint32_t(&b)[2] = q[nt][0][2 * j + i];
-                                if (i + j == 0) mma_first<BF>(s[mt][nt], wa[0], wb[0], wa[1], wb[1], b[0], b[1]);
-                                else mma<BF>(s[mt][nt], wa[2 * i], wb[2 * i], wa[2 * i + 1], wb[2 * i + 1], b[0], b[1]);
+                                const uint32_t(&b)[2] = q[nt][pl][(I8 ? 4 : 2) * j + i];
+                                if (i + j + pl == 0) mma_first<BF>(s[mt][nt], f[mt][0], f[mt][1], f[mt][2], f[mt][3], b[0], b[1]);
+                                else mma<BF>(s[mt][nt], f[mt][0], f[mt][1], f[mt][2], f[mt][3], b[0], b[1]);
                             }
-                    }
                 }
             }
             // exponents against the maxima so far; does any lie 2^8 above?
@@ -608,38 +610,48 @@ __global__ void __launch_bounds__(Ring<CT, HD>::WARPS * 32, Ring<CT, HD>::CTAS) 
                             }
                         }
 #pragma unroll
-                    for (int i = 0; i < PER; i++) {
-                        float acc[NT][4];
+                    for (int i = 0; i < PER; i += 2) {  // two dim tiles at once, for the same reason
+                        float acc[2][NT][4];
 #pragma unroll
                         for (int mt = 0; mt < HALVES; mt++) {
-                            uint32_t a0, a1, a2, a3;
-                            if constexpr (I8) {
-                                // word i / 2: four dims; its first two (i even) or last two, of two entries each
-                                const uint32_t sel = i & 1 ? 0x7362 : 0x5140;
-                                const uint32_t x = __byte_perm(v[mt][0][i / 2], v[mt][1][i / 2], sel);
-                                const uint32_t y = __byte_perm(v[mt][2][i / 2], v[mt][3][i / 2], sel);
-                                a0 = bytes_to_half2(x, 0x4140), a1 = bytes_to_half2(x, 0x4342);
-                                a2 = bytes_to_half2(y, 0x4140), a3 = bytes_to_half2(y, 0x4342);
-                            } else {
-                                a0 = __byte_perm(v[mt][0][i], v[mt][1][i], 0x5410), a1 = __byte_perm(v[mt][0][i], v[mt][1][i], 0x7632);
-                                a2 = __byte_perm(v[mt][2][i], v[mt][3][i], 0x5410), a3 = __byte_perm(v[mt][2][i], v[mt][3][i], 0x7632);
+                            uint32_t f[2][4];
+#pragma unroll
+                            for (int y = 0; y < 2; y++) {
+                                if constexpr (I8) {
+                                    // word i / 2: four dims; its first two or last two, of two entries each
+                                    const uint32_t sel = y ? 0x7362 : 0x5140;
+                                    const uint32_t a = __byte_perm(v[mt][0][i / 2], v[mt][1][i / 2], sel);
+                                    const uint32_t b = __byte_perm(v[mt][2][i / 2], v[mt][3][i / 2], sel);
+                                    f[y][0] = bytes_to_half2(a, 0x4140), f[y][1] = bytes_to_half2(a, 0x4342);
+                                    f[y][2] = bytes_to_half2(b, 0x4140), f[y][3] = bytes_to_half2(b, 0x4342);
+                                } else {
+                                    f[y][0] = __byte_perm(v[mt][0][i + y], v[mt][1][i + y], 0x5410);
+                                    f[y][1] = __byte_perm(v[mt][0][i + y], v[mt][1][i + y], 0x7632);
+                                    f[y][2] = __byte_perm(v[mt][2][i + y], v[mt][3][i + y], 0x5410);
+                                    f[y][3] = __byte_perm(v[mt][2][i + y], v[mt][3][i + y], 0x7632);
+                                }
                             }
+#pragma unroll
+                            for (int pl = 0; pl < VP; pl++)
+#pragma unroll
+                                for (int y = 0; y < 2; y++)
+#pragma unroll
+                                    for (int nt = 0; nt < NT; nt++) {
+                                        const uint32_t b0 = pw[mt][nt][pl][0], b1 = pw[mt][nt][pl][1];
+                                        if (mt + pl == 0) mma_first<BF>(acc[y][nt], f[y][0], f[y][1], f[y][2], f[y][3], b0, b1);
+                                        else mma<BF>(acc[y][nt], f[y][0], f[y][1], f[y][2], f[y][3], b0, b1);
+                                    }
+                        }
+#pragma unroll
+                        for (int y = 0; y < 2; y++)
 #pragma unroll
                             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                                for (int pl = 0; pl < VP; pl++) {
-                                    if (mt == 0 && pl == 0) mma_first<BF>(acc[nt], a0, a1, a2, a3, pw[0][nt][0][0], pw[0][nt][0][1]);
-                                    else mma<BF>(acc[nt], a0, a1, a2, a3, pw[mt][nt][pl][0], pw[mt][nt][pl][1]);
+                                for (int e = 0; e < 4; e++) {
+                                    if (!I8 && passes > 1 && sees[nt][e & 1] != upto + e0) continue;  // another token's pass
+                                    float& to = o[gi * PER + i + y][nt][e];
+                                    to = I8 ? fmaf(acc[y][nt][e], back, to) : to + acc[y][nt][e];
                                 }
-                        }
-#pragma unroll
-                        for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                if (!I8 && passes > 1 && sees[nt][e & 1] != upto + e0) continue;  // another token's pass
-                                float& to = o[gi * PER + i][nt][e];
-                                to = I8 ? fmaf(acc[nt][e], back, to) : to + acc[nt][e];
-                            }
                     }
                 }
             }
