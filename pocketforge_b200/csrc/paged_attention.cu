@@ -306,6 +306,26 @@ __global__ void __launch_bounds__(Ring<CT, HD>::WARPS * 32, Ring<CT, HD>::CTAS) 
     uint8_t* ring = smem + warp * ST * R::BYTES;
     const uint32_t ring_u32 = (uint32_t)__cvta_generic_to_shared(ring);
     const int64_t page_slots = (int64_t)c.n_layers * c.n_kv_heads * c.page_size;
+        // ---- queries, on their way while the ring is set up ----
+        // int8: piece j of the row's 16-byte ones that this thread reads is dims 64 j + 16 t ..; 16-bit: 32 j + 8 t ..
+        float raw[NT][I8 ? HD / 4 : HD / 8];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            const int x = 8 * nt + gr, token = token_of(x0 + x, p.group), head = g * p.group + x0 + x - token * p.group;
+            const int64_t at = ((int64_t)seq * p.rows + token) * p.q_stride + head * HD;
+            if constexpr (I8) {
+#pragma unroll
+                for (int j = 0; j < HD / 64; j++) load16<PLANES>(p.q, at + 64 * j + 16 * t, p.dtype, x < cols, raw[nt] + 16 * j);
+            } else {
+#pragma unroll
+                for (int j = 0; j < HD / 32; j++) {
+                    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);  // bits
+                    if (x < cols) v = *reinterpret_cast<const float4*>(static_cast<const CT*>(p.q) + at + 32 * j + 8 * t);
+                    raw[nt][4 * j] = v.x, raw[nt][4 * j + 1] = v.y, raw[nt][4 * j + 2] = v.z, raw[nt][4 * j + 3] = v.w;
+                }
+            }
+        }
+
         // ---- the ring: block k of this warp is entries first(k) .. + 31 ----
         const int n_blocks = ch1 - ch0;
         auto first_entry = [&](int k) { return ((ch0 + k) * kWarps + warp) * kBlock; };
@@ -365,34 +385,25 @@ __global__ void __launch_bounds__(Ring<CT, HD>::WARPS * 32, Ring<CT, HD>::CTAS) 
             page0 = n0, page1 = n1;
         }
 
-        // ---- queries ----
+        // ---- queries into operands ----
         uint32_t q[NT][PLANES][KS][2];
-        float unit = p.scale * 1.4426950408889634f;  // score units -> log2 units (log2 e)
-        if constexpr (I8) {
-            // One power of two for all columns: what a smaller row loses at fp16's lower end is as small beside the largest
-            // row's scores as that row's own loss.
-            float v[NT][HD / 4], big = 0.0f;
+        float unit[NT][2];  // score units -> log2 units (log2 e) of this thread's columns 2t, 2t + 1
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                const int x = 8 * nt + gr, token = token_of(x0 + x, p.group), head = g * p.group + x0 + x - token * p.group;
-                const int64_t at = ((int64_t)seq * p.rows + token) * p.q_stride + head * HD + 16 * t;
-                // piece j of the row's 16-byte ones that this thread reads: dims 64 j + 16 t ..
+        for (int nt = 0; nt < NT; nt++) {
+            float all = p.scale * 1.4426950408889634f;
+            if constexpr (I8) {
+                float big = 0.0f;
 #pragma unroll
-                for (int j = 0; j < HD / 64; j++) load16<PLANES>(p.q, at + 64 * j, p.dtype, x < cols, v[nt] + 16 * j);
-#pragma unroll
-                for (int i = 0; i < HD / 4; i++)
-                    if (fabsf(v[nt][i]) < __int_as_float(0x7f800000)) big = fmaxf(big, fabsf(v[nt][i]));
-            }
-#pragma unroll
-            for (int x = 16; x >= 1; x >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, x));
-            const int up = big > 0.0f ? min(max(13 - exponent_of(big), -100), 100) : 0;
-            const float f = power_of_two(up);
-            unit *= power_of_two(-up);
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++)
+                for (int i = 0; i < HD / 4; i++) big = fmaxf(big, fabsf(raw[nt][i]));
+                big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+                big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+                const bool finite = big > 0.0f && big < __int_as_float(0x7f800000);
+                const int up = finite ? min(max(13 - exponent_of(big), -100), 100) : 0;
+                const float f = power_of_two(up);
+                all *= power_of_two(-up);
 #pragma unroll
                 for (int i = 0; i < HD / 4; i += 2) {
-                    const float a = v[nt][i] * f, b = v[nt][i + 1] * f;
+                    const float a = raw[nt][i] * f, b = raw[nt][i + 1] * f;
                     const uint32_t hi = pack<false>(a, b);
                     q[nt][0][i / 4][i / 2 % 2] = hi;
                     if constexpr (PLANES == 2) {
@@ -400,19 +411,12 @@ __global__ void __launch_bounds__(Ring<CT, HD>::WARPS * 32, Ring<CT, HD>::CTAS) 
                         q[nt][1][i / 4][i / 2 % 2] = pack<false>(a - h.x, b - h.y);
                     }
                 }
-        } else {
+            } else {
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                const int x = 8 * nt + gr, token = token_of(x0 + x, p.group), head = g * p.group + x0 + x - token * p.group;
-                const int64_t at = ((int64_t)seq * p.rows + token) * p.q_stride + head * HD + 8 * t;
-#pragma unroll
-                for (int j = 0; j < HD / 32; j++) {
-                    uint4 v = make_uint4(0, 0, 0, 0);
-                    if (x < cols) v = *reinterpret_cast<const uint4*>(static_cast<const CT*>(p.q) + at + 32 * j);
-                    q[nt][0][2 * j][0] = v.x, q[nt][0][2 * j][1] = v.y;
-                    q[nt][0][2 * j + 1][0] = v.z, q[nt][0][2 * j + 1][1] = v.w;
-                }
+                for (int i = 0; i < HD / 8; i++) q[nt][0][i / 2][i % 2] = __float_as_uint(raw[nt][i]);
             }
+            unit[nt][0] = __shfl_sync(0xffffffffu, all, 8 * t);
+            unit[nt][1] = __shfl_sync(0xffffffffu, all, 8 * t + 4);
         }
         // Entries that this thread's two columns of each tile see.
         int sees[NT][2];
@@ -498,7 +502,13 @@ __global__ void __launch_bounds__(Ring<CT, HD>::WARPS * 32, Ring<CT, HD>::CTAS) 
 #pragma unroll
             for (int mt = 0; mt < HALVES; mt++)
 #pragma unroll
-                for (int h = 0; h < 2; h++) ks[mt][h] = I8 ? scales[16 * mt + 8 * h + gr] * unit : unit;
+                for (int h = 0; h < 2; h++) ks[mt][h] = I8 ? scales[16 * mt + 8 * h + gr] : 1.0f;
+#pragma unroll
+            for (int mt = 0; mt < HALVES; mt++)
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) s[mt][nt][i] *= unit[nt][i & 1];
             if (tail) {
 #pragma unroll
                 for (int mt = 0; mt < HALVES; mt++)

@@ -409,6 +409,30 @@ def test_attention_scores_of_all_sizes():
             attend(c, t, 2, 3, 4, by=by)
 
 
+@pytest.mark.parametrize("cache,t", [(I8, F32), (I8, BF16), (BF16, BF16), (F16, F16)])
+def test_attention_rows_of_unlike_sizes(cache, t):
+    """A head whose queries are large, small or no numbers leaves the heads beside it as they are."""
+    c = Cache(cache, 1, 1, 64, 16, 40, 2, 30).place([400, 21])
+    q = randn((4, 8 * 64), TYPES[t], 3)
+    plain, out = torch.empty_like(q), torch.empty_like(q)
+    c.attend(0, q, plain, t, 2, 2, 8, 0.125)
+    q.view(4, 8, 64)[:, 1] *= 1e-4
+    q.view(4, 8, 64)[:, 2] *= 3e3
+    q.view(4, 8, 64)[:, 4, 9] = math.inf
+    q.view(4, 8, 64)[:, 5, 3] = math.nan
+    q.view(4, 8, 64)[:, 7] = 0
+    if t != F16:
+        q.view(4, 8, 64)[:, 6] *= 1e18
+    c.attend(0, q, out, t, 2, 2, 8, 0.125)
+    torch.cuda.synchronize()
+    a, b = out.view(4, 8, 64), plain.view(4, 8, 64)
+    assert torch.equal(a[:, [0, 3]], b[:, [0, 3]])
+    assert torch.isnan(a[:, 5]).all()
+    few = [0, 1, 3, 7]
+    want = c.attention(0, torch.nan_to_num(q, 0, 0, 0), 2, 2, 8, 0.125)
+    check(a[:, few].contiguous(), tuple(x[:, few] for x in want), TYPES[t])
+
+
 @pytest.mark.parametrize("cache,t", [(I8, F32), (BF16, BF16), (F16, F16)])
 @pytest.mark.parametrize("rows", [1, 4])
 def test_attention_does_not_read_behind_the_end(cache, t, rows):
