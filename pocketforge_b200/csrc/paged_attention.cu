@@ -3,20 +3,36 @@
 //
 //   out = sum_j softmax_j(scale * q . k_j) v_j   over the positions a row sees
 //
-// Bound by HBM: every key and value is read once for all the query rows of its
-// kv head (the group's heads times the newest tokens).  A (sequence, kv head,
-// row group) is a segment of 128-entry chunks, cut into equal pieces of at most
-// P chunks, P being all chunks over the CTAs that fit the GPU: where there are
-// segments enough none is cut, and a few long ones are spread over every SM.
-// One CTA a piece; the pieces of a cut segment are joined by the CTA that ends
-// last, in their order (the answer does not depend on who that is).  (One run
-// of exactly total / CTAs chunks each, wherever it began and ended, balanced
-// better and measured twice as slow on 64 sequences of 512 to 1024: nearly
-// every CTA had two segments to begin, end and join.)
+// Every key and value is read once for all the query rows of its kv head (the
+// group's heads times the newest tokens).  A (sequence, kv head, row group) is a
+// segment of chunks (the warps' blocks side by side: 64 to 128 entries), cut into
+// equal pieces of at most P chunks, one CTA a piece: where there are nearly as
+// many segments as CTAs fit the GPU none is cut unless it is far longer than the
+// others, and a few long ones are spread over every SM in one round.  The pieces
+// of a cut segment are joined by the CTA that ends last, in their order (the
+// answer does not depend on who that is).  Measured otherwise: one run of exactly
+// total / CTAs chunks each, wherever it began and ended, 70 against 57 us on 64
+// sequences of 512 to 1,024 with 5 rows (nearly every CTA had two segments to
+// begin, end and join); pieces of half a share, 166 against 125 us on 8 contexts
+// of 3,000 to 65,536 (a second round of CTAs, mostly empty); no limit to a
+// segment's pieces, 115 against 21 us for one kv head's 30,000 entries (joining
+// 235 of them).
 //
-// A CTA has four warps; each takes every fourth 32-entry block of the piece,
-// with its own ring of blocks in flight (cp.async, no barrier between warps) and
-// its own running softmax, and the four are put together at the end.  The
+// What bounds it (B200, measured): HBM for 16-bit caches (8 contexts of up to
+// 65,536 entries, head_dim 128: 713 MB in 124 us, 5.7 TB/s, 88% of the measured
+// copy rate); instruction issue for int8 ones, whose codes take one and a half
+// instructions each on the way to an operand (16 contexts of 8,000, one fp32 row:
+// 139 MB in 37.6 us, 57%); the chain of trips to memory before the first block
+// and the joining for one short context (777 entries: 8.5 us).  64 sequences with
+// 5 fp32 rows, 41 us for 55 MB: 20 rows make 24 columns and two planes of each,
+// 1,150 instructions a warp and 32 entries, issued at 0.4 a clock by the 12 warps
+// that the registers allow, a quarter of a CTA's time before its first block.
+//
+// A CTA's three (64-byte rows) or four warps take blocks of 32 entries (256-byte
+// rows: 16) in turn, each with its own ring of them in flight (cp.async, no
+// barrier between warps) and its own running softmax, and are put together at the
+// end.  Three warps let 64-byte rows have four CTAs an SM: 592, so that the 512
+// segments of 64 sequences and 8 kv heads run at once (55 to 45 us).  The
 // products are 16x8x16 tensor-core ones with the entries (S^T = K Q^T) and the
 // dims (O^T = V^T P^T) as the 16 and the query rows as the 8, so a few rows
 // waste little; which entry or dim stands where in an operand is free as long
@@ -306,473 +322,473 @@ __global__ void __launch_bounds__(Ring<CT, HD>::WARPS * 32, Ring<CT, HD>::CTAS) 
     uint8_t* ring = smem + warp * ST * R::BYTES;
     const uint32_t ring_u32 = (uint32_t)__cvta_generic_to_shared(ring);
     const int64_t page_slots = (int64_t)c.n_layers * c.n_kv_heads * c.page_size;
-        // ---- queries, on their way while the ring is set up ----
-        // int8: piece j of the row's 16-byte ones that this thread reads is dims 64 j + 16 t ..; 16-bit: 32 j + 8 t ..
-        float raw[NT][I8 ? HD / 4 : HD / 8];
+    // ---- queries, on their way while the ring is set up ----
+    // int8: piece j of the row's 16-byte ones that this thread reads is dims 64 j + 16 t ..; 16-bit: 32 j + 8 t ..
+    float raw[NT][I8 ? HD / 4 : HD / 8];
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-            const int x = 8 * nt + gr, token = token_of(x0 + x, p.group), head = g * p.group + x0 + x - token * p.group;
-            const int64_t at = ((int64_t)seq * p.rows + token) * p.q_stride + head * HD;
-            if constexpr (I8) {
+    for (int nt = 0; nt < NT; nt++) {
+        const int x = 8 * nt + gr, token = token_of(x0 + x, p.group), head = g * p.group + x0 + x - token * p.group;
+        const int64_t at = ((int64_t)seq * p.rows + token) * p.q_stride + head * HD;
+        if constexpr (I8) {
 #pragma unroll
-                for (int j = 0; j < HD / 64; j++) load16<PLANES>(p.q, at + 64 * j + 16 * t, p.dtype, x < cols, raw[nt] + 16 * j);
-            } else {
+            for (int j = 0; j < HD / 64; j++) load16<PLANES>(p.q, at + 64 * j + 16 * t, p.dtype, x < cols, raw[nt] + 16 * j);
+        } else {
 #pragma unroll
-                for (int j = 0; j < HD / 32; j++) {
-                    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);  // bits
-                    if (x < cols) v = *reinterpret_cast<const float4*>(static_cast<const CT*>(p.q) + at + 32 * j + 8 * t);
-                    raw[nt][4 * j] = v.x, raw[nt][4 * j + 1] = v.y, raw[nt][4 * j + 2] = v.z, raw[nt][4 * j + 3] = v.w;
-                }
+            for (int j = 0; j < HD / 32; j++) {
+                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);  // bits
+                if (x < cols) v = *reinterpret_cast<const float4*>(static_cast<const CT*>(p.q) + at + 32 * j + 8 * t);
+                raw[nt][4 * j] = v.x, raw[nt][4 * j + 1] = v.y, raw[nt][4 * j + 2] = v.z, raw[nt][4 * j + 3] = v.w;
             }
         }
+    }
 
-        // ---- the ring: block k of this warp is entries first(k) .. + 31 ----
-        const int n_blocks = ch1 - ch0;
-        auto first_entry = [&](int k) { return ((ch0 + k) * kWarps + warp) * kBlock; };
-        const int* table = c.table + (int64_t)seq * c.max_pages;
-        // The table's entry for the block's 16-entry half (not looked at before the block is asked for: it is on its way);
-        // -1: none of the half is there.
-        auto page_of = [&](int k, int half) {
-            const int e = first_entry(k) + 16 * half;
-            return k < n_blocks && e < len ? table[e >> p.page_shift] : -1;
-        };
-        auto checked = [&](int page, int e) {
-            if ((unsigned)page < (unsigned)c.n_pages) return page;
-            if (e < len) latch(p.err, ERR_BOUNDS);
-            return -1;
-        };
-        // A half's 16 rows lie behind one another in their page: a pass of 32 lanes is 512 bytes of them, and only its base
-        // depends on the block.
-        constexpr int PR = RB / 16, STEP = 32 / PR;  // pieces of a row, rows a pass
-        const int lane_row = lane / PR, lane_piece = lane % PR;
-        const uint32_t key_to = key_at<RB>(lane_row, lane_piece);
-        constexpr int VARIANTS = RB == 64 ? 1 : (RB == 128 ? 2 : 4);  // of the values' permutation among passes
-        uint32_t value_to[VARIANTS];
+    // ---- the ring: block k of this warp is entries first(k) .. + 31 ----
+    const int n_blocks = ch1 - ch0;
+    auto first_entry = [&](int k) { return ((ch0 + k) * kWarps + warp) * kBlock; };
+    const int* table = c.table + (int64_t)seq * c.max_pages;
+    // The table's entry for the block's 16-entry half (not looked at before the block is asked for: it is on its way);
+    // -1: none of the half is there.
+    auto page_of = [&](int k, int half) {
+        const int e = first_entry(k) + 16 * half;
+        return k < n_blocks && e < len ? table[e >> p.page_shift] : -1;
+    };
+    auto checked = [&](int page, int e) {
+        if ((unsigned)page < (unsigned)c.n_pages) return page;
+        if (e < len) latch(p.err, ERR_BOUNDS);
+        return -1;
+    };
+    // A half's 16 rows lie behind one another in their page: a pass of 32 lanes is 512 bytes of them, and only its base
+    // depends on the block.
+    constexpr int PR = RB / 16, STEP = 32 / PR;  // pieces of a row, rows a pass
+    const int lane_row = lane / PR, lane_piece = lane % PR;
+    const uint32_t key_to = key_at<RB>(lane_row, lane_piece);
+    constexpr int VARIANTS = RB == 64 ? 1 : (RB == 128 ? 2 : 4);  // of the values' permutation among passes
+    uint32_t value_to[VARIANTS];
 #pragma unroll
-        for (int i = 0; i < VARIANTS; i++)
-            value_to[i] = kBlock * RB + value_at<RB>(i * STEP + lane_row, lane_piece) - i * STEP * RB;
-        const int64_t unit_row = ((int64_t)p.layer * c.n_kv_heads + g) * c.page_size;
-        auto issue = [&](int k, int page0, int page1) {
-            const int e0 = first_entry(k);
-            const uint32_t to = ring_u32 + (k % ST) * R::BYTES;
+    for (int i = 0; i < VARIANTS; i++)
+        value_to[i] = kBlock * RB + value_at<RB>(i * STEP + lane_row, lane_piece) - i * STEP * RB;
+    const int64_t unit_row = ((int64_t)p.layer * c.n_kv_heads + g) * c.page_size;
+    auto issue = [&](int k, int page0, int page1) {
+        const int e0 = first_entry(k);
+        const uint32_t to = ring_u32 + (k % ST) * R::BYTES;
 #pragma unroll
-            for (int half = 0; half < HALVES; half++) {
-                const int e = e0 + 16 * half, page = checked(half ? page1 : page0, e);
-                const int rows = page < 0 ? 0 : min(len - e, 16);  // of the half's 16; the others are filled with zeros
-                const int64_t row = (int64_t)max(page, 0) * page_slots + unit_row + (e & (c.page_size - 1));
-                const uint8_t* from_k = static_cast<const uint8_t*>(c.k) + row * RB + lane * 16;
-                const uint8_t* from_v = static_cast<const uint8_t*>(c.v) + row * RB + lane * 16;
+        for (int half = 0; half < HALVES; half++) {
+            const int e = e0 + 16 * half, page = checked(half ? page1 : page0, e);
+            const int rows = page < 0 ? 0 : min(len - e, 16);  // of the half's 16; the others are filled with zeros
+            const int64_t row = (int64_t)max(page, 0) * page_slots + unit_row + (e & (c.page_size - 1));
+            const uint8_t* from_k = static_cast<const uint8_t*>(c.k) + row * RB + lane * 16;
+            const uint8_t* from_v = static_cast<const uint8_t*>(c.v) + row * RB + lane * 16;
 #pragma unroll
-                for (int i = 0; i < 16 / STEP; i++) {
-                    const int pass = half * (16 / STEP) + i;
-                    const bool on = i * STEP + lane_row < rows;
-                    copy16(to + key_to + pass * 512, from_k + i * 512, on);
-                    copy16(to + value_to[pass % VARIANTS] + pass * 512, from_v + i * 512, on);
-                }
-                if constexpr (I8) {  // lanes 0-15 the keys' scales, 16-31 the values'
-                    const float* from = (lane < 16 ? c.k_scale : c.v_scale) + row + (lane & 15);
-                    copy4(to + 2 * kBlock * RB + (lane < 16 ? 0 : 4 * kBlock) + 64 * half + 4 * (lane & 15), from,
-                          (lane & 15) < rows);
+            for (int i = 0; i < 16 / STEP; i++) {
+                const int pass = half * (16 / STEP) + i;
+                const bool on = i * STEP + lane_row < rows;
+                copy16(to + key_to + pass * 512, from_k + i * 512, on);
+                copy16(to + value_to[pass % VARIANTS] + pass * 512, from_v + i * 512, on);
+            }
+            if constexpr (I8) {  // lanes 0-15 the keys' scales, 16-31 the values'
+                const float* from = (lane < 16 ? c.k_scale : c.v_scale) + row + (lane & 15);
+                copy4(to + 2 * kBlock * RB + (lane < 16 ? 0 : 4 * kBlock) + 64 * half + 4 * (lane & 15), from,
+                      (lane & 15) < rows);
+            }
+        }
+    };
+    int page0 = page_of(0, 0), page1 = HALVES == 2 ? page_of(0, 1) : -1;
+#pragma unroll
+    for (int k = 0; k < ST - 1; k++) {
+        const int n0 = page_of(k + 1, 0), n1 = HALVES == 2 ? page_of(k + 1, 1) : -1;
+        if (k < n_blocks) issue(k, page0, page1);
+        copy_commit();
+        page0 = n0, page1 = n1;
+    }
+
+    // ---- queries into operands ----
+    uint32_t q[NT][PLANES][KS][2];
+    float unit[NT][2];  // score units -> log2 units (log2 e) of this thread's columns 2t, 2t + 1
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        float all = p.scale * 1.4426950408889634f;
+        if constexpr (I8) {
+            float big = 0.0f;
+#pragma unroll
+            for (int i = 0; i < HD / 4; i++) big = fmaxf(big, fabsf(raw[nt][i]));
+            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+            const bool finite = big > 0.0f && big < __int_as_float(0x7f800000);
+            const int up = finite ? min(max(13 - exponent_of(big), -100), 100) : 0;
+            const float f = power_of_two(up);
+            all *= power_of_two(-up);
+#pragma unroll
+            for (int i = 0; i < HD / 4; i += 2) {
+                const float a = raw[nt][i] * f, b = raw[nt][i + 1] * f;
+                const uint32_t hi = pack<false>(a, b);
+                q[nt][0][i / 4][i / 2 % 2] = hi;
+                if constexpr (PLANES == 2) {
+                    const float2 h = unpack<false>(hi);
+                    q[nt][1][i / 4][i / 2 % 2] = pack<false>(a - h.x, b - h.y);
                 }
             }
-        };
-        int page0 = page_of(0, 0), page1 = HALVES == 2 ? page_of(0, 1) : -1;
+        } else {
 #pragma unroll
-        for (int k = 0; k < ST - 1; k++) {
-            const int n0 = page_of(k + 1, 0), n1 = HALVES == 2 ? page_of(k + 1, 1) : -1;
-            if (k < n_blocks) issue(k, page0, page1);
+            for (int i = 0; i < HD / 8; i++) q[nt][0][i / 2][i % 2] = __float_as_uint(raw[nt][i]);
+        }
+        unit[nt][0] = __shfl_sync(0xffffffffu, all, 8 * t);
+        unit[nt][1] = __shfl_sync(0xffffffffu, all, 8 * t + 4);
+    }
+    // Entries that this thread's two columns of each tile see.
+    int sees[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const int x = 8 * nt + 2 * t + i;
+            sees[nt][i] = x < cols ? sees_all + token_of(x0 + x, p.group) : 0;
+        }
+
+    // ---- running softmax ----
+    // Maxima as their negatives, 0 as long as there is none (`above`, the exponent that calls for a new one, is -inf then).
+    float o[MT][NT][4], minus_m[NT][2], above[NT][2], l[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        minus_m[nt][0] = minus_m[nt][1] = 0.0f;
+        above[nt][0] = above[nt][1] = -INFINITY;
+        l[nt][0] = l[nt][1] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < MT; i++) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.0f;
+    }
+    float vscale = 1.0f, back = 1.0f;
+    for (int k = 0; k < n_blocks; k++) {
+        {
+            const int n0 = page_of(k + ST, 0), n1 = HALVES == 2 ? page_of(k + ST, 1) : -1;
+            __syncwarp();  // every lane is through with the block whose place is filled now
+            if (k + ST - 1 < n_blocks) issue(k + ST - 1, page0, page1);
             copy_commit();
             page0 = n0, page1 = n1;
         }
+        copy_wait<ST - 1>();
+        __syncwarp();
+        const int e0 = first_entry(k);
+        if (e0 >= len) break;  // the sequence ends in another warp's block
+        const uint8_t* kb = ring + (k % ST) * R::BYTES;
+        const uint8_t* vb = kb + kBlock * RB;
+        const float* scales = reinterpret_cast<const float*>(vb + kBlock * RB);
 
-        // ---- queries into operands ----
-        uint32_t q[NT][PLANES][KS][2];
-        float unit[NT][2];  // score units -> log2 units (log2 e) of this thread's columns 2t, 2t + 1
+        // Scores of 16 entries each: rows gr, gr + 8.  All tiles take one product before any takes its next, so that
+        // a product does not wait for the one before it.
+        float s[HALVES][NT][4];
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-            float all = p.scale * 1.4426950408889634f;
-            if constexpr (I8) {
-                float big = 0.0f;
-#pragma unroll
-                for (int i = 0; i < HD / 4; i++) big = fmaxf(big, fabsf(raw[nt][i]));
-                big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
-                big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-                const bool finite = big > 0.0f && big < __int_as_float(0x7f800000);
-                const int up = finite ? min(max(13 - exponent_of(big), -100), 100) : 0;
-                const float f = power_of_two(up);
-                all *= power_of_two(-up);
-#pragma unroll
-                for (int i = 0; i < HD / 4; i += 2) {
-                    const float a = raw[nt][i] * f, b = raw[nt][i + 1] * f;
-                    const uint32_t hi = pack<false>(a, b);
-                    q[nt][0][i / 4][i / 2 % 2] = hi;
-                    if constexpr (PLANES == 2) {
-                        const float2 h = unpack<false>(hi);
-                        q[nt][1][i / 4][i / 2 % 2] = pack<false>(a - h.x, b - h.y);
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < HD / 8; i++) q[nt][0][i / 2][i % 2] = __float_as_uint(raw[nt][i]);
-            }
-            unit[nt][0] = __shfl_sync(0xffffffffu, all, 8 * t);
-            unit[nt][1] = __shfl_sync(0xffffffffu, all, 8 * t + 4);
-        }
-        // Entries that this thread's two columns of each tile see.
-        int sees[NT][2];
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const int x = 8 * nt + 2 * t + i;
-                sees[nt][i] = x < cols ? sees_all + token_of(x0 + x, p.group) : 0;
-            }
-
-        // ---- running softmax ----
-        // Maxima as their negatives, 0 as long as there is none (`above`, the exponent that calls for a new one, is -inf then).
-        float o[MT][NT][4], minus_m[NT][2], above[NT][2], l[NT][2];
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-            minus_m[nt][0] = minus_m[nt][1] = 0.0f;
-            above[nt][0] = above[nt][1] = -INFINITY;
-            l[nt][0] = l[nt][1] = 0.0f;
-#pragma unroll
-            for (int i = 0; i < MT; i++) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.0f;
-        }
-        float vscale = 1.0f, back = 1.0f;
-        for (int k = 0; k < n_blocks; k++) {
-            {
-                const int n0 = page_of(k + ST, 0), n1 = HALVES == 2 ? page_of(k + ST, 1) : -1;
-                __syncwarp();  // every lane is through with the block whose place is filled now
-                if (k + ST - 1 < n_blocks) issue(k + ST - 1, page0, page1);
-                copy_commit();
-                page0 = n0, page1 = n1;
-            }
-            copy_wait<ST - 1>();
-            __syncwarp();
-            const int e0 = first_entry(k);
-            if (e0 >= len) break;  // the sequence ends in another warp's block
-            const uint8_t* kb = ring + (k % ST) * R::BYTES;
-            const uint8_t* vb = kb + kBlock * RB;
-            const float* scales = reinterpret_cast<const float*>(vb + kBlock * RB);
-
-            // Scores of 16 entries each: rows gr, gr + 8.  All tiles take one product before any takes its next, so that
-            // a product does not wait for the one before it.
-            float s[HALVES][NT][4];
-#pragma unroll
-            for (int j = 0; j < RB / 64; j++) {  // pieces t, t + 4, ...
-                uint32_t w[HALVES][2][4];
-#pragma unroll
-                for (int mt = 0; mt < HALVES; mt++)
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const uint4 x = *reinterpret_cast<const uint4*>(kb + key_at<RB>(16 * mt + 8 * h + gr, 4 * j + t));
-                        w[mt][h][0] = x.x, w[mt][h][1] = x.y, w[mt][h][2] = x.z, w[mt][h][3] = x.w;
-                    }
-#pragma unroll
-                for (int i = 0; i < (I8 ? 4 : 2); i++) {
-                    uint32_t f[HALVES][4];
-#pragma unroll
-                    for (int mt = 0; mt < HALVES; mt++) {
-                        if constexpr (I8) {
-                            const uint32_t ua = w[mt][0][i] ^ 0x80808080u, ub = w[mt][1][i] ^ 0x80808080u;
-                            f[mt][0] = bytes_to_half2(ua, 0x4140), f[mt][2] = bytes_to_half2(ua, 0x4342);
-                            f[mt][1] = bytes_to_half2(ub, 0x4140), f[mt][3] = bytes_to_half2(ub, 0x4342);
-                        } else {
-                            f[mt][0] = w[mt][0][2 * i], f[mt][1] = w[mt][1][2 * i];
-                            f[mt][2] = w[mt][0][2 * i + 1], f[mt][3] = w[mt][1][2 * i + 1];
-                        }
-                    }
-#pragma unroll
-                    for (int pl = 0; pl < PLANES; pl++)
-#pragma unroll
-                        for (int mt = 0; mt < HALVES; mt++)
-#pragma unroll
-                            for (int nt = 0; nt < NT; nt++) {
-                                const uint32_t(&b)[2] = q[nt][pl][(I8 ? 4 : 2) * j + i];
-                                if (i + j + pl == 0) mma_first<BF>(s[mt][nt], f[mt][0], f[mt][1], f[mt][2], f[mt][3], b[0], b[1]);
-                                else mma<BF>(s[mt][nt], f[mt][0], f[mt][1], f[mt][2], f[mt][3], b[0], b[1]);
-                            }
-                }
-            }
-            // exponents against the maxima so far; does any lie 2^8 above?
-            const bool tail = e0 + kBlock > sees_all;  // some entry is not seen by every column
-            bool rise = false;
-            float ks[HALVES][2];
-#pragma unroll
-            for (int mt = 0; mt < HALVES; mt++)
-#pragma unroll
-                for (int h = 0; h < 2; h++) ks[mt][h] = I8 ? scales[16 * mt + 8 * h + gr] : 1.0f;
-#pragma unroll
-            for (int mt = 0; mt < HALVES; mt++)
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) s[mt][nt][i] *= unit[nt][i & 1];
-            if (tail) {
-#pragma unroll
-                for (int mt = 0; mt < HALVES; mt++)
-#pragma unroll
-                    for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {  // ks may be inf or NaN here: the factor goes in before the mask
-                            const bool seen = e0 + 16 * mt + 8 * (i >> 1) + gr < sees[nt][i & 1];
-                            s[mt][nt][i] = seen ? s[mt][nt][i] * ks[mt][i >> 1] : -INFINITY;
-                        }
-#pragma unroll
-                for (int mt = 0; mt < HALVES; mt++) ks[mt][0] = ks[mt][1] = 1.0f;
-            }
-#pragma unroll
-            for (int mt = 0; mt < HALVES; mt++)
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        // (fma(-inf, 1, 0) where there is no maximum yet)
-                        rise |= fmaf(s[mt][nt][i], ks[mt][i >> 1], minus_m[nt][i & 1]) > above[nt][i & 1];
-                    }
-            if (__any_sync(0xffffffffu, rise)) {
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        float top = -INFINITY;
-#pragma unroll
-                        for (int mt = 0; mt < HALVES; mt++)
-                            top = fmaxf(top, fmaxf(s[mt][nt][i] * ks[mt][0], s[mt][nt][2 + i] * ks[mt][1]));
-#pragma unroll
-                        for (int x = 4; x <= 16; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-                        // no other column has a say: a row stays the same whatever its neighbours are
-                        const bool none = above[nt][i] == -INFINITY;
-                        if (none ? top > -INFINITY : top + minus_m[nt][i] > 8.0f) {
-                            const float f = none ? 0.0f : exp2_approx(-minus_m[nt][i] - top);
-                            minus_m[nt][i] = -top;
-                            above[nt][i] = 8.0f;
-                            l[nt][i] *= f;
-                            if (!none)
-#pragma unroll
-                                for (int d = 0; d < MT; d++) o[d][nt][i] *= f, o[d][nt][2 + i] *= f;
-                        }
-                    }
-            }
-            // weights
-            // int8: 2^up takes the block's largest finite scale to 1 .. 2^7, so that p v_scale 2^up < 2^15 (p <= 2^8); the one
-            // before is kept while it does.
-            if constexpr (I8) {
-                const float inf = __int_as_float(0x7f800000), vs = fabsf(scales[kBlock + lane]), x = vs * vscale;
-                if (__any_sync(0xffffffffu, x >= 128.0f && vs < inf) || !__any_sync(0xffffffffu, x >= 1.0f && x < inf)) {
-                    const unsigned big = __reduce_max_sync(0xffffffffu, vs < inf ? __float_as_uint(vs) : 0u);
-                    const int up = min(max(6 - exponent_of(__uint_as_float(big)), -100), 100);
-                    vscale = power_of_two(up), back = power_of_two(-up);
-                }
-            }
-            uint32_t pw[HALVES][NT][VP][2];  // [entries 16 mt ..][column tile][plane][first, second 8 entries], transposed
+        for (int j = 0; j < RB / 64; j++) {  // pieces t, t + 4, ...
+            uint32_t w[HALVES][2][4];
 #pragma unroll
             for (int mt = 0; mt < HALVES; mt++)
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    const int r = 16 * mt + 8 * h + gr;
-                    const float vs = I8 ? scales[kBlock + r] * vscale : 1.0f;
-                    const bool vs_ok = fabsf(vs) < __int_as_float(0x7f800000);
+                    const uint4 x = *reinterpret_cast<const uint4*>(kb + key_at<RB>(16 * mt + 8 * h + gr, 4 * j + t));
+                    w[mt][h][0] = x.x, w[mt][h][1] = x.y, w[mt][h][2] = x.z, w[mt][h][3] = x.w;
+                }
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++) {
-                        float y[2];
+            for (int i = 0; i < (I8 ? 4 : 2); i++) {
+                uint32_t f[HALVES][4];
 #pragma unroll
-                        for (int i = 0; i < 2; i++) {
-                            const float e = exp2_approx(fmaf(s[mt][nt][2 * h + i], ks[mt][h], minus_m[nt][i]));
-                            l[nt][i] += e;
-                            y[i] = I8 ? e * vs : e;
-                            if (I8 && tail && !vs_ok && e0 + r >= sees[nt][i]) y[i] = 0.0f;  // 0 whatever its scale is
-                        }
-                        if constexpr (VP == 2) {  // (an inf is the largest value and an inf)
-                            const uint32_t hi = pack_finite(y[0], y[1]);
-                            const float2 got = unpack<false>(hi);
-                            pw[mt][nt][0][h] = transpose8x8(hi);
-                            pw[mt][nt][1][h] = transpose8x8(pack<false>(y[0] - got.x, y[1] - got.y));
-                        } else {
-                            pw[mt][nt][0][h] = transpose8x8(pack<BF>(y[0], y[1]));
-                        }
+                for (int mt = 0; mt < HALVES; mt++) {
+                    if constexpr (I8) {
+                        const uint32_t ua = w[mt][0][i] ^ 0x80808080u, ub = w[mt][1][i] ^ 0x80808080u;
+                        f[mt][0] = bytes_to_half2(ua, 0x4140), f[mt][2] = bytes_to_half2(ua, 0x4342);
+                        f[mt][1] = bytes_to_half2(ub, 0x4140), f[mt][3] = bytes_to_half2(ub, 0x4342);
+                    } else {
+                        f[mt][0] = w[mt][0][2 * i], f[mt][1] = w[mt][1][2 * i];
+                        f[mt][2] = w[mt][0][2 * i + 1], f[mt][3] = w[mt][1][2 * i + 1];
                     }
                 }
-            // values
-            const int passes = !I8 && tail && p.rows > 1 ? p.rows : 1;
-            for (int pass = 0; pass < passes; pass++) {
-                // one pass for all, or one a new token with what it may not see set to 0
-                const int upto = passes == 1 ? INT_MAX : sees_all + pass - e0;
-                constexpr int VB = RB == 64 ? 8 : 16;  // bytes of a row this thread reads at a time
-                constexpr int W = VB / 4, GROUPS = RB / 8 / VB, PER = MT / GROUPS;
 #pragma unroll
-                for (int gi = 0; gi < GROUPS; gi++) {
-                    uint32_t v[HALVES][4][W];  // entries 16 mt + 2t, 2t + 1, 2t + 8, 2t + 9
+                for (int pl = 0; pl < PLANES; pl++)
 #pragma unroll
                     for (int mt = 0; mt < HALVES; mt++)
 #pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            const int r = 16 * mt + 2 * t + (e & 1) + 8 * (e >> 1);
-                            if constexpr (W == 2) {
-                                const uint2 x = *reinterpret_cast<const uint2*>(vb + value_at<RB>(r, gr >> 1) + 8 * (gr & 1));
-                                v[mt][e][0] = x.x ^ 0x80808080u, v[mt][e][1] = x.y ^ 0x80808080u;
-                            } else {
-                                uint4 x = *reinterpret_cast<const uint4*>(vb + value_at<RB>(r, 8 * gi + gr));
-                                if (!I8 && r >= upto) x = make_uint4(0, 0, 0, 0);
-                                const uint32_t flip = I8 ? 0x80808080u : 0u;
-                                v[mt][e][0] = x.x ^ flip, v[mt][e][1] = x.y ^ flip, v[mt][e][2] = x.z ^ flip, v[mt][e][3] = x.w ^ flip;
-                            }
+                        for (int nt = 0; nt < NT; nt++) {
+                            const uint32_t(&b)[2] = q[nt][pl][(I8 ? 4 : 2) * j + i];
+                            if (i + j + pl == 0) mma_first<BF>(s[mt][nt], f[mt][0], f[mt][1], f[mt][2], f[mt][3], b[0], b[1]);
+                            else mma<BF>(s[mt][nt], f[mt][0], f[mt][1], f[mt][2], f[mt][3], b[0], b[1]);
                         }
+            }
+        }
+        // exponents against the maxima so far; does any lie 2^8 above?
+        const bool tail = e0 + kBlock > sees_all;  // some entry is not seen by every column
+        bool rise = false;
+        float ks[HALVES][2];
 #pragma unroll
-                    for (int i = 0; i < PER; i += 2) {  // two dim tiles at once, for the same reason
-                        float acc[2][NT][4];
+        for (int mt = 0; mt < HALVES; mt++)
 #pragma unroll
-                        for (int mt = 0; mt < HALVES; mt++) {
-                            uint32_t f[2][4];
+            for (int h = 0; h < 2; h++) ks[mt][h] = I8 ? scales[16 * mt + 8 * h + gr] : 1.0f;
 #pragma unroll
-                            for (int y = 0; y < 2; y++) {
-                                if constexpr (I8) {
-                                    // word i / 2: four dims; its first two or last two, of two entries each
-                                    const uint32_t sel = y ? 0x7362 : 0x5140;
-                                    const uint32_t a = __byte_perm(v[mt][0][i / 2], v[mt][1][i / 2], sel);
-                                    const uint32_t b = __byte_perm(v[mt][2][i / 2], v[mt][3][i / 2], sel);
-                                    f[y][0] = bytes_to_half2(a, 0x4140), f[y][1] = bytes_to_half2(a, 0x4342);
-                                    f[y][2] = bytes_to_half2(b, 0x4140), f[y][3] = bytes_to_half2(b, 0x4342);
-                                } else {
-                                    f[y][0] = __byte_perm(v[mt][0][i + y], v[mt][1][i + y], 0x5410);
-                                    f[y][1] = __byte_perm(v[mt][0][i + y], v[mt][1][i + y], 0x7632);
-                                    f[y][2] = __byte_perm(v[mt][2][i + y], v[mt][3][i + y], 0x5410);
-                                    f[y][3] = __byte_perm(v[mt][2][i + y], v[mt][3][i + y], 0x7632);
-                                }
-                            }
+        for (int mt = 0; mt < HALVES; mt++)
 #pragma unroll
-                            for (int pl = 0; pl < VP; pl++)
+            for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                                for (int y = 0; y < 2; y++)
+                for (int i = 0; i < 4; i++) s[mt][nt][i] *= unit[nt][i & 1];
+        if (tail) {
 #pragma unroll
-                                    for (int nt = 0; nt < NT; nt++) {
-                                        const uint32_t b0 = pw[mt][nt][pl][0], b1 = pw[mt][nt][pl][1];
-                                        if (mt + pl == 0) mma_first<BF>(acc[y][nt], f[y][0], f[y][1], f[y][2], f[y][3], b0, b1);
-                                        else mma<BF>(acc[y][nt], f[y][0], f[y][1], f[y][2], f[y][3], b0, b1);
-                                    }
-                        }
+            for (int mt = 0; mt < HALVES; mt++)
 #pragma unroll
-                        for (int y = 0; y < 2; y++)
+                for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                            for (int nt = 0; nt < NT; nt++)
+                    for (int i = 0; i < 4; i++) {  // ks may be inf or NaN here: the factor goes in before the mask
+                        const bool seen = e0 + 16 * mt + 8 * (i >> 1) + gr < sees[nt][i & 1];
+                        s[mt][nt][i] = seen ? s[mt][nt][i] * ks[mt][i >> 1] : -INFINITY;
+                    }
 #pragma unroll
-                                for (int e = 0; e < 4; e++) {
-                                    if (!I8 && passes > 1 && sees[nt][e & 1] != upto + e0) continue;  // another token's pass
-                                    float& to = o[gi * PER + i + y][nt][e];
-                                    to = I8 ? fmaf(acc[y][nt][e], back, to) : to + acc[y][nt][e];
-                                }
+            for (int mt = 0; mt < HALVES; mt++) ks[mt][0] = ks[mt][1] = 1.0f;
+        }
+#pragma unroll
+        for (int mt = 0; mt < HALVES; mt++)
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    // (fma(-inf, 1, 0) where there is no maximum yet)
+                    rise |= fmaf(s[mt][nt][i], ks[mt][i >> 1], minus_m[nt][i & 1]) > above[nt][i & 1];
+                }
+        if (__any_sync(0xffffffffu, rise)) {
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int mt = 0; mt < HALVES; mt++)
+                        top = fmaxf(top, fmaxf(s[mt][nt][i] * ks[mt][0], s[mt][nt][2 + i] * ks[mt][1]));
+#pragma unroll
+                    for (int x = 4; x <= 16; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+                    // no other column has a say: a row stays the same whatever its neighbours are
+                    const bool none = above[nt][i] == -INFINITY;
+                    if (none ? top > -INFINITY : top + minus_m[nt][i] > 8.0f) {
+                        const float f = none ? 0.0f : exp2_approx(-minus_m[nt][i] - top);
+                        minus_m[nt][i] = -top;
+                        above[nt][i] = 8.0f;
+                        l[nt][i] *= f;
+                        if (!none)
+#pragma unroll
+                            for (int d = 0; d < MT; d++) o[d][nt][i] *= f, o[d][nt][2 + i] *= f;
+                    }
+                }
+        }
+        // weights
+        // int8: 2^up takes the block's largest finite scale to 1 .. 2^7, so that p v_scale 2^up < 2^15 (p <= 2^8); the one
+        // before is kept while it does.
+        if constexpr (I8) {
+            const float inf = __int_as_float(0x7f800000), vs = fabsf(scales[kBlock + lane]), x = vs * vscale;
+            if (__any_sync(0xffffffffu, x >= 128.0f && vs < inf) || !__any_sync(0xffffffffu, x >= 1.0f && x < inf)) {
+                const unsigned big = __reduce_max_sync(0xffffffffu, vs < inf ? __float_as_uint(vs) : 0u);
+                const int up = min(max(6 - exponent_of(__uint_as_float(big)), -100), 100);
+                vscale = power_of_two(up), back = power_of_two(-up);
+            }
+        }
+        uint32_t pw[HALVES][NT][VP][2];  // [entries 16 mt ..][column tile][plane][first, second 8 entries], transposed
+#pragma unroll
+        for (int mt = 0; mt < HALVES; mt++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int r = 16 * mt + 8 * h + gr;
+                const float vs = I8 ? scales[kBlock + r] * vscale : 1.0f;
+                const bool vs_ok = fabsf(vs) < __int_as_float(0x7f800000);
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    float y[2];
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        const float e = exp2_approx(fmaf(s[mt][nt][2 * h + i], ks[mt][h], minus_m[nt][i]));
+                        l[nt][i] += e;
+                        y[i] = I8 ? e * vs : e;
+                        if (I8 && tail && !vs_ok && e0 + r >= sees[nt][i]) y[i] = 0.0f;  // 0 whatever its scale is
+                    }
+                    if constexpr (VP == 2) {  // (an inf is the largest value and an inf)
+                        const uint32_t hi = pack_finite(y[0], y[1]);
+                        const float2 got = unpack<false>(hi);
+                        pw[mt][nt][0][h] = transpose8x8(hi);
+                        pw[mt][nt][1][h] = transpose8x8(pack<false>(y[0] - got.x, y[1] - got.y));
+                    } else {
+                        pw[mt][nt][0][h] = transpose8x8(pack<BF>(y[0], y[1]));
                     }
                 }
             }
-        }
-        copy_wait<0>();
-
-        // ---- the four warps' shares together ----
-        // smem: [warp][column][HD + 2], a row's last two its maximum and sum
-        constexpr int PITCH = HD + 2, PART = HD + 4;  // here, and in `part` (16-byte loads)
-        float* shared = reinterpret_cast<float*>(smem);
-        static_assert(kWarps * COLS * PITCH * 4 <= R::SMEM && COLS * kMaxCuts * 4 <= R::SMEM, "the shares fit the ring");
-        __syncthreads();  // the rings are empty
+        // values
+        const int passes = !I8 && tail && p.rows > 1 ? p.rows : 1;
+        for (int pass = 0; pass < passes; pass++) {
+            // one pass for all, or one a new token with what it may not see set to 0
+            const int upto = passes == 1 ? INT_MAX : sees_all + pass - e0;
+            constexpr int VB = RB == 64 ? 8 : 16;  // bytes of a row this thread reads at a time
+            constexpr int W = VB / 4, GROUPS = RB / 8 / VB, PER = MT / GROUPS;
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++)
+            for (int gi = 0; gi < GROUPS; gi++) {
+                uint32_t v[HALVES][4][W];  // entries 16 mt + 2t, 2t + 1, 2t + 8, 2t + 9
+#pragma unroll
+                for (int mt = 0; mt < HALVES; mt++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int r = 16 * mt + 2 * t + (e & 1) + 8 * (e >> 1);
+                        if constexpr (W == 2) {
+                            const uint2 x = *reinterpret_cast<const uint2*>(vb + value_at<RB>(r, gr >> 1) + 8 * (gr & 1));
+                            v[mt][e][0] = x.x ^ 0x80808080u, v[mt][e][1] = x.y ^ 0x80808080u;
+                        } else {
+                            uint4 x = *reinterpret_cast<const uint4*>(vb + value_at<RB>(r, 8 * gi + gr));
+                            if (!I8 && r >= upto) x = make_uint4(0, 0, 0, 0);
+                            const uint32_t flip = I8 ? 0x80808080u : 0u;
+                            v[mt][e][0] = x.x ^ flip, v[mt][e][1] = x.y ^ flip, v[mt][e][2] = x.z ^ flip, v[mt][e][3] = x.w ^ flip;
+                        }
+                    }
+#pragma unroll
+                for (int i = 0; i < PER; i += 2) {  // two dim tiles at once, for the same reason
+                    float acc[2][NT][4];
+#pragma unroll
+                    for (int mt = 0; mt < HALVES; mt++) {
+                        uint32_t f[2][4];
+#pragma unroll
+                        for (int y = 0; y < 2; y++) {
+                            if constexpr (I8) {
+                                // word i / 2: four dims; its first two or last two, of two entries each
+                                const uint32_t sel = y ? 0x7362 : 0x5140;
+                                const uint32_t a = __byte_perm(v[mt][0][i / 2], v[mt][1][i / 2], sel);
+                                const uint32_t b = __byte_perm(v[mt][2][i / 2], v[mt][3][i / 2], sel);
+                                f[y][0] = bytes_to_half2(a, 0x4140), f[y][1] = bytes_to_half2(a, 0x4342);
+                                f[y][2] = bytes_to_half2(b, 0x4140), f[y][3] = bytes_to_half2(b, 0x4342);
+                            } else {
+                                f[y][0] = __byte_perm(v[mt][0][i + y], v[mt][1][i + y], 0x5410);
+                                f[y][1] = __byte_perm(v[mt][0][i + y], v[mt][1][i + y], 0x7632);
+                                f[y][2] = __byte_perm(v[mt][2][i + y], v[mt][3][i + y], 0x5410);
+                                f[y][3] = __byte_perm(v[mt][2][i + y], v[mt][3][i + y], 0x7632);
+                            }
+                        }
+#pragma unroll
+                        for (int pl = 0; pl < VP; pl++)
+#pragma unroll
+                            for (int y = 0; y < 2; y++)
+#pragma unroll
+                                for (int nt = 0; nt < NT; nt++) {
+                                    const uint32_t b0 = pw[mt][nt][pl][0], b1 = pw[mt][nt][pl][1];
+                                    if (mt + pl == 0) mma_first<BF>(acc[y][nt], f[y][0], f[y][1], f[y][2], f[y][3], b0, b1);
+                                    else mma<BF>(acc[y][nt], f[y][0], f[y][1], f[y][2], f[y][3], b0, b1);
+                                }
+                    }
+#pragma unroll
+                    for (int y = 0; y < 2; y++)
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                if (!I8 && passes > 1 && sees[nt][e & 1] != upto + e0) continue;  // another token's pass
+                                float& to = o[gi * PER + i + y][nt][e];
+                                to = I8 ? fmaf(acc[y][nt][e], back, to) : to + acc[y][nt][e];
+                            }
+                }
+            }
+        }
+    }
+    copy_wait<0>();
+
+    // ---- the warps' shares together ----
+    // smem: [warp][column][HD + 2], a row's last two its maximum and sum
+    constexpr int PITCH = HD + 2, PART = HD + 4;  // here, and in `part` (16-byte loads)
+    float* shared = reinterpret_cast<float*>(smem);
+    static_assert(kWarps * COLS * PITCH * 4 <= R::SMEM && COLS * kMaxCuts * 4 <= R::SMEM, "the shares fit the ring");
+    __syncthreads();  // the rings are empty
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            float sum = l[nt][i];
+#pragma unroll
+            for (int x = 4; x <= 16; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+            float* to = shared + (warp * COLS + 8 * nt + 2 * t + i) * PITCH;
+            if (gr == 0) to[HD] = above[nt][i] == -INFINITY ? -INFINITY : -minus_m[nt][i], to[HD + 1] = sum;
+#pragma unroll
+            for (int d = 0; d < MT; d++) {
+                // tile d's rows gr and gr + 8 are two neighbouring dims
+                constexpr int VB = RB == 64 ? 8 : 16, PER = MT / (RB / 8 / VB), DIMS = VB / (int)sizeof(CT);
+                const int dim = d / PER * (HD / (MT / PER)) + gr * DIMS + 2 * (d % PER);
+                *reinterpret_cast<float2*>(to + dim) = make_float2(o[d][nt][i], o[d][nt][2 + i]);
+            }
+        }
+    __syncthreads();
+    // A cut segment is longer than P = `most` chunks, so no two have one seg_begin / P, and its pieces fit twice that
+    // many places.
+    const int place = seg_begin / most;
+    float* part = p.part + (int64_t)(2 * place + piece) * COLS * PART;
+    if (threadIdx.x < cols) {  // a column's factors, in the place of the warps' maxima
+        float* at = shared + threadIdx.x * PITCH + HD;
+        float top = -INFINITY, sum = 0.0f, f[kWarps];
+#pragma unroll
+        for (int s = 0; s < kWarps; s++) top = fmaxf(top, at[s * COLS * PITCH]);
+#pragma unroll
+        for (int s = 0; s < kWarps; s++) {
+            const float m = at[s * COLS * PITCH];
+            f[s] = m == -INFINITY ? 1.0f : exp2_approx(m - top);  // no maximum: its shares are zeros, or NaN
+            sum += at[s * COLS * PITCH + 1] * f[s];
+        }
+        if (cuts > 1) __stcg(reinterpret_cast<float2*>(part + threadIdx.x * PART + HD), make_float2(top, sum));
+        const float inv = cuts > 1 ? 1.0f : (sum == 0.0f ? 0.0f : 1.0f / sum);
+#pragma unroll
+        for (int s = 0; s < kWarps; s++) at[s * COLS * PITCH] = f[s] * inv;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < cols * (HD / 2); i += kWarps * 32) {
+        const int x = i / (HD / 2), d = i % (HD / 2) * 2;
+        float2 v = make_float2(0.0f, 0.0f);
+#pragma unroll
+        for (int s = 0; s < kWarps; s++) {
+            const float* from = shared + (s * COLS + x) * PITCH;
+            const float2 y = *reinterpret_cast<const float2*>(from + d);
+            v.x += y.x * from[HD], v.y += y.y * from[HD];
+        }
+        if (cuts == 1) store_out(p, seq, g, x0 + x, d, HD, v);
+        else __stcg(reinterpret_cast<float2*>(part + x * PART + d), v);
+    }
+    if (cuts > 1) {
+        // ---- the segment's pieces together, by the last to come ----
+        __threadfence();
+        __syncthreads();
+        if (threadIdx.x == 0) s_last = atomicAdd(&p.count[place], 1) == cuts - 1;
+        __syncthreads();
+        if (!s_last) return;
+        __threadfence();
+        if (threadIdx.x == 0) p.count[place] = 0;  // as it was found
+        const float* parts = p.part + (int64_t)2 * place * COLS * PART;
+        float* factor = shared;  // [column][kMaxCuts]
+        for (int x = warp; x < cols; x += kWarps) {  // two pieces a lane
+            float2 ms[2];
+            float top = -INFINITY, sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                float sum = l[nt][i];
-#pragma unroll
-                for (int x = 4; x <= 16; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-                float* to = shared + (warp * COLS + 8 * nt + 2 * t + i) * PITCH;
-                if (gr == 0) to[HD] = above[nt][i] == -INFINITY ? -INFINITY : -minus_m[nt][i], to[HD + 1] = sum;
-#pragma unroll
-                for (int d = 0; d < MT; d++) {
-                    // tile d's rows gr and gr + 8 are two neighbouring dims
-                    constexpr int VB = RB == 64 ? 8 : 16, PER = MT / (RB / 8 / VB), DIMS = VB / (int)sizeof(CT);
-                    const int dim = d / PER * (HD / (MT / PER)) + gr * DIMS + 2 * (d % PER);
-                    *reinterpret_cast<float2*>(to + dim) = make_float2(o[d][nt][i], o[d][nt][2 + i]);
-                }
+                const int k = lane + 32 * i;
+                ms[i] = k < cuts ? __ldcg(reinterpret_cast<const float2*>(parts + ((int64_t)k * COLS + x) * PART + HD))
+                                 : make_float2(-INFINITY, 0.0f);
+                top = fmaxf(top, ms[i].x);
             }
-        __syncthreads();
-        // A cut segment is longer than P = `most` chunks, so no two have one seg_begin / P, and its pieces fit twice that
-        // many places.
-        const int place = seg_begin / most;
-        float* part = p.part + (int64_t)(2 * place + piece) * COLS * PART;
-        if (threadIdx.x < cols) {  // a column's factors, in the place of the warps' maxima
-            float* at = shared + threadIdx.x * PITCH + HD;
-            float top = -INFINITY, sum = 0.0f, f[kWarps];
 #pragma unroll
-            for (int s = 0; s < kWarps; s++) top = fmaxf(top, at[s * COLS * PITCH]);
+            for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
 #pragma unroll
-            for (int s = 0; s < kWarps; s++) {
-                const float m = at[s * COLS * PITCH];
-                f[s] = m == -INFINITY ? 1.0f : exp2_approx(m - top);  // no maximum: its shares are zeros, or NaN
-                sum += at[s * COLS * PITCH + 1] * f[s];
+            for (int i = 0; i < 2; i++) {
+                ms[i].x = ms[i].x == -INFINITY ? 1.0f : exp2_approx(ms[i].x - top);
+                sum += ms[i].y * ms[i].x;
             }
-            if (cuts > 1) __stcg(reinterpret_cast<float2*>(part + threadIdx.x * PART + HD), make_float2(top, sum));
-            const float inv = cuts > 1 ? 1.0f : (sum == 0.0f ? 0.0f : 1.0f / sum);
 #pragma unroll
-            for (int s = 0; s < kWarps; s++) at[s * COLS * PITCH] = f[s] * inv;
+            for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+            for (int i = 0; i < 2; i++) factor[x * kMaxCuts + lane + 32 * i] = ms[i].x * inv;
         }
         __syncthreads();
-        for (int i = threadIdx.x; i < cols * (HD / 2); i += kWarps * 32) {
-            const int x = i / (HD / 2), d = i % (HD / 2) * 2;
-            float2 v = make_float2(0.0f, 0.0f);
-#pragma unroll
-            for (int s = 0; s < kWarps; s++) {
-                const float* from = shared + (s * COLS + x) * PITCH;
-                const float2 y = *reinterpret_cast<const float2*>(from + d);
-                v.x += y.x * from[HD], v.y += y.y * from[HD];
-            }
-            if (cuts == 1) store_out(p, seq, g, x0 + x, d, HD, v);
-            else __stcg(reinterpret_cast<float2*>(part + x * PART + d), v);
-        }
-        if (cuts > 1) {
-            // ---- the segment's pieces together, by the last to come ----
-            __threadfence();
-            __syncthreads();
-            if (threadIdx.x == 0) s_last = atomicAdd(&p.count[place], 1) == cuts - 1;
-            __syncthreads();
-            if (!s_last) return;
-            __threadfence();
-            if (threadIdx.x == 0) p.count[place] = 0;  // as it was found
-            const float* parts = p.part + (int64_t)2 * place * COLS * PART;
-            float* factor = shared;  // [column][kMaxCuts]
-            for (int x = warp; x < cols; x += kWarps) {  // two pieces a lane
-                float2 ms[2];
-                float top = -INFINITY, sum = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const int k = lane + 32 * i;
-                    ms[i] = k < cuts ? __ldcg(reinterpret_cast<const float2*>(parts + ((int64_t)k * COLS + x) * PART + HD))
-                                     : make_float2(-INFINITY, 0.0f);
-                    top = fmaxf(top, ms[i].x);
-                }
-#pragma unroll
-                for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    ms[i].x = ms[i].x == -INFINITY ? 1.0f : exp2_approx(ms[i].x - top);
-                    sum += ms[i].y * ms[i].x;
-                }
-#pragma unroll
-                for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-                for (int i = 0; i < 2; i++) factor[x * kMaxCuts + lane + 32 * i] = ms[i].x * inv;
-            }
-            __syncthreads();
-            for (int i = threadIdx.x; i < cols * (HD / 4); i += kWarps * 32) {
-                const int x = i / (HD / 4), d = i % (HD / 4) * 4;
-                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int i = threadIdx.x; i < cols * (HD / 4); i += kWarps * 32) {
+            const int x = i / (HD / 4), d = i % (HD / 4) * 4;
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 8
-                for (int k = 0; k < cuts; k++) {
-                    const float4 y = __ldcg(reinterpret_cast<const float4*>(parts + ((int64_t)k * COLS + x) * PART + d));
-                    const float f = factor[x * kMaxCuts + k];
-                    v.x += y.x * f, v.y += y.y * f, v.z += y.z * f, v.w += y.w * f;
-                }
-                store_out(p, seq, g, x0 + x, d, HD, make_float2(v.x, v.y));
-                store_out(p, seq, g, x0 + x, d + 2, HD, make_float2(v.z, v.w));
+            for (int k = 0; k < cuts; k++) {
+                const float4 y = __ldcg(reinterpret_cast<const float4*>(parts + ((int64_t)k * COLS + x) * PART + d));
+                const float f = factor[x * kMaxCuts + k];
+                v.x += y.x * f, v.y += y.y * f, v.z += y.z * f, v.w += y.w * f;
             }
+            store_out(p, seq, g, x0 + x, d, HD, make_float2(v.x, v.y));
+            store_out(p, seq, g, x0 + x, d + 2, HD, make_float2(v.z, v.w));
         }
+    }
 }
 
 // Column tiles of 8 that a CTA takes: as many as the rows need, up to what the registers hold.

@@ -18,6 +18,25 @@
 //   8         unit list and TMA loads, one lane a 64-column slab
 //   9         issues the tcgen05 products S = Q K^T and O += P V
 //   10        looks through the V block on the diagonal (below)
+// The blocks of all its units are one stream of products.  At head_dim 64 the
+// scores of the next block (or unit) are computed while this block's are
+// exponentiated; at 128 TMEM has no room for that, P overlays the scores it came
+// from and the two tiles take turns at the tensor cores.
+//
+// What bounds it (B200, measured): 8,192 tokens, 32 heads over 8, head_dim 128,
+// bf16: 550 GFLOP in 492 us, 1.12 PFLOP/s, 80% of what cuBLAS sustains under the
+// power cap (the tensor pipe is active in 65% of the cycles at 1.54 GHz: power is
+// part of it).  64 prompts of 33 to 1,024 tokens, head_dim 64: 163 us; half of
+// the products are in blocks on the diagonal or behind the end, the special-
+// function unit takes 2,048 of a block's 3,100 cycles, and each unit of three
+// blocks on average has about 4,000 cycles of its own (first scores, output).
+// Short units run every path of the code once, so its size counts: 84 KB of
+// unrolled code ran 221 us where 60 KB ran 174 (stalls for instructions 1.9 an
+// issue before, 0.2 after).  Measured and not kept: a part of the exponentials by
+// a polynomial on the FMA pipe (498 to 509 us on 8,192 tokens), two threads a row
+// (550), exponents against the last block's maximum while this one's is found
+// (524), turns at the special-function unit (515).
+//
 // The maximum that the exponents refer to rises only when a block exceeds it
 // by 2^8, so O (in TMEM) is rescaled rarely: p stays below 2^8, within fp16,
 // and the row sum takes the same p.
@@ -245,8 +264,7 @@ __device__ __forceinline__ float row_max(const uint32_t* r) {
     return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
 }
 // 16 pairs of scores to p = 2^(c s + off), rounded and packed; sum takes the unrounded ones.  All on the
-// special-function unit: a share of 1/8 or 1/4 by a polynomial on the FMA pipe measured the same to 2% slower (8192
-// tokens 498, 504, 509 us), which the more instructions' power accounts for.
+// special-function unit.
 template <typename T>
 __device__ __forceinline__ void exponentials(const uint32_t* r, float c, float off, float2 (&sum)[2], uint32_t* pk) {
 #pragma unroll
