@@ -24,9 +24,10 @@
 // instructions each on the way to an operand (16 contexts of 8,000, one fp32 row:
 // 139 MB in 37.6 us, 57%); the chain of trips to memory before the first block
 // and the joining for one short context (777 entries: 8.5 us).  64 sequences with
-// 5 fp32 rows, 41 us for 55 MB: 20 rows make 24 columns and two planes of each,
-// 1,150 instructions a warp and 32 entries, issued at 0.4 a clock by the 12 warps
-// that the registers allow, a quarter of a CTA's time before its first block.
+// 5 fp32 rows, 35 us for 55 MB: 20 rows make 24 columns and two planes of each,
+// about 1,100 instructions a warp and 32 entries, issued at 0.4 to 0.5 a clock by
+// the 12 warps that the registers allow, a quarter of a CTA's time before its
+// first block.
 //
 // A CTA's three (64-byte rows) or four warps take blocks of 32 entries (256-byte
 // rows: 16) in turn, each with its own ring of them in flight (cp.async, no
@@ -85,7 +86,7 @@ struct PagedParams {
 // registers, measured no faster: the warps that there are keep the loads going.)
 __host__ __device__ constexpr int ctas_per_sm(int row_bytes) { return row_bytes == 64 ? 4 : 2; }
 
-template <typename CT, int HD>
+template <typename CT, int HD, int NT>
 struct Ring {
     static constexpr int RB = HD * (int)sizeof(CT);                 // bytes of a stored row
     static constexpr int WARPS = RB == 64 ? 3 : 4;
@@ -94,7 +95,7 @@ struct Ring {
     static constexpr int SCALES = sizeof(CT) == 1 ? 2 * BLOCK * 4 : 0;
     static constexpr int BYTES = 2 * BLOCK * RB + SCALES;           // keys, values, scales of a block
     static constexpr int CTAS = ctas_per_sm(RB);
-    static constexpr int STAGES = RB == 64 ? 4 : 3;
+    static constexpr int STAGES = RB == 64 && NT == 1 ? 4 : 3;
     static constexpr int SMEM = WARPS * STAGES * BYTES;
 };
 
@@ -245,14 +246,18 @@ __device__ __forceinline__ void store_out(const PagedParams& p, int seq, int g, 
 }
 
 template <typename CT, int HD, int NT, int PLANES>
-__global__ void __launch_bounds__(Ring<CT, HD>::WARPS * 32, Ring<CT, HD>::CTAS) paged_kernel(const PagedParams p) {
-    using R = Ring<CT, HD>;
+__global__ void __launch_bounds__(Ring<CT, HD, NT>::WARPS * 32, Ring<CT, HD, NT>::CTAS) paged_kernel(const PagedParams p) {
+    using R = Ring<CT, HD, NT>;
     constexpr int RB = R::RB, ST = R::STAGES, kWarps = R::WARPS, kBlock = R::BLOCK, HALVES = kBlock / 16;
     constexpr bool I8 = sizeof(CT) == 1, BF = std::is_same<CT, __nv_bfloat16>::value;
     constexpr int KS = HD / 16;        // products along the dims of a score
     constexpr int MT = HD / 16;        // 16-dim tiles of the output
     constexpr int COLS = 8 * NT;
     constexpr int VP = I8 ? 2 : 1;     // planes of a weight
+    // Queries in shared memory where the registers they would take are the warps' that an SM could hold (64 sequences of 5
+    // fp32 rows: 41.3 us in registers, 35.4; 64 of 5 fp16 rows, head_dim 128: 81 with two tiles and twice the reading, 60
+    // with three).  16-bit ones of two tiles, or at head_dim 64, were 2 to 6% slower so.
+    constexpr bool SHARED_Q = NT > 1 && (I8 || (HD == 128 && NT == 3));
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ int s_before, s_seq, s_piece, s_len, s_cuts, s_most, s_last;
     const pf_paged_cache& c = p.c;
@@ -323,21 +328,24 @@ __global__ void __launch_bounds__(Ring<CT, HD>::WARPS * 32, Ring<CT, HD>::CTAS) 
     const uint32_t ring_u32 = (uint32_t)__cvta_generic_to_shared(ring);
     const int64_t page_slots = (int64_t)c.n_layers * c.n_kv_heads * c.page_size;
     // ---- queries, on their way while the ring is set up ----
-    // int8: piece j of the row's 16-byte ones that this thread reads is dims 64 j + 16 t ..; 16-bit: 32 j + 8 t ..
-    float raw[NT][I8 ? HD / 4 : HD / 8];
+    // int8: piece j of the row's 16-byte ones that this thread reads is dims 64 j + 16 t ..; 16-bit: 32 j + 8 t ..  With one
+    // column tile every warp keeps it in registers; of several each warp prepares its share for all, in shared memory.
+    constexpr int MINE = SHARED_Q ? (NT + kWarps - 1) / kWarps : NT;
+    float raw[MINE][I8 ? HD / 4 : HD / 8];
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-        const int x = 8 * nt + gr, token = token_of(x0 + x, p.group), head = g * p.group + x0 + x - token * p.group;
+    for (int y = 0; y < MINE; y++) {
+        const int nt = SHARED_Q ? warp + y * kWarps : y, x = 8 * nt + gr;
+        const int token = token_of(x0 + x, p.group), head = g * p.group + x0 + x - token * p.group;
         const int64_t at = ((int64_t)seq * p.rows + token) * p.q_stride + head * HD;
         if constexpr (I8) {
 #pragma unroll
-            for (int j = 0; j < HD / 64; j++) load16<PLANES>(p.q, at + 64 * j + 16 * t, p.dtype, x < cols, raw[nt] + 16 * j);
+            for (int j = 0; j < HD / 64; j++) load16<PLANES>(p.q, at + 64 * j + 16 * t, p.dtype, x < cols, raw[y] + 16 * j);
         } else {
 #pragma unroll
             for (int j = 0; j < HD / 32; j++) {
                 float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);  // bits
                 if (x < cols) v = *reinterpret_cast<const float4*>(static_cast<const CT*>(p.q) + at + 32 * j + 8 * t);
-                raw[nt][4 * j] = v.x, raw[nt][4 * j + 1] = v.y, raw[nt][4 * j + 2] = v.z, raw[nt][4 * j + 3] = v.w;
+                raw[y][4 * j] = v.x, raw[y][4 * j + 1] = v.y, raw[y][4 * j + 2] = v.z, raw[y][4 * j + 3] = v.w;
             }
         }
     }
@@ -402,15 +410,20 @@ __global__ void __launch_bounds__(Ring<CT, HD>::WARPS * 32, Ring<CT, HD>::CTAS) 
     }
 
     // ---- queries into operands ----
-    uint32_t q[NT][PLANES][KS][2];
+    // [plane][product][2]; in shared memory two products' four words are one 16-byte piece a lane
+    uint32_t q[SHARED_Q ? 1 : NT][PLANES][KS][2];
     float unit[NT][2];  // score units -> log2 units (log2 e) of this thread's columns 2t, 2t + 1
+    uint4* q_shared = reinterpret_cast<uint4*>(smem + R::SMEM);                              // [tile][plane][KS / 2][lane]
+    float* unit_shared = reinterpret_cast<float*>(q_shared + NT * PLANES * (KS / 2) * 32);  // [column]
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
+    for (int y = 0; y < MINE; y++) {
+        const int nt = SHARED_Q ? warp + y * kWarps : y;
+        uint32_t(&w)[PLANES][KS][2] = q[SHARED_Q ? 0 : y];
         float all = p.scale * 1.4426950408889634f;
         if constexpr (I8) {
             float big = 0.0f;
 #pragma unroll
-            for (int i = 0; i < HD / 4; i++) big = fmaxf(big, fabsf(raw[nt][i]));
+            for (int i = 0; i < HD / 4; i++) big = fmaxf(big, fabsf(raw[y][i]));
             big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
             big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
             const bool finite = big > 0.0f && big < __int_as_float(0x7f800000);
@@ -419,20 +432,37 @@ __global__ void __launch_bounds__(Ring<CT, HD>::WARPS * 32, Ring<CT, HD>::CTAS) 
             all *= power_of_two(-up);
 #pragma unroll
             for (int i = 0; i < HD / 4; i += 2) {
-                const float a = raw[nt][i] * f, b = raw[nt][i + 1] * f;
+                const float a = raw[y][i] * f, b = raw[y][i + 1] * f;
                 const uint32_t hi = pack<false>(a, b);
-                q[nt][0][i / 4][i / 2 % 2] = hi;
+                w[0][i / 4][i / 2 % 2] = hi;
                 if constexpr (PLANES == 2) {
                     const float2 h = unpack<false>(hi);
-                    q[nt][1][i / 4][i / 2 % 2] = pack<false>(a - h.x, b - h.y);
+                    w[1][i / 4][i / 2 % 2] = pack<false>(a - h.x, b - h.y);
                 }
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < HD / 8; i++) q[nt][0][i / 2][i % 2] = __float_as_uint(raw[nt][i]);
+            for (int i = 0; i < HD / 8; i++) w[0][i / 2][i % 2] = __float_as_uint(raw[y][i]);
         }
-        unit[nt][0] = __shfl_sync(0xffffffffu, all, 8 * t);
-        unit[nt][1] = __shfl_sync(0xffffffffu, all, 8 * t + 4);
+        if constexpr (SHARED_Q) {
+            if (nt < NT) {
+#pragma unroll
+                for (int pl = 0; pl < PLANES; pl++)
+#pragma unroll
+                    for (int i = 0; i < KS; i += 2)
+                        q_shared[((nt * PLANES + pl) * (KS / 2) + i / 2) * 32 + lane] =
+                            make_uint4(w[pl][i][0], w[pl][i][1], w[pl][i + 1][0], w[pl][i + 1][1]);
+                if (t == 0) unit_shared[8 * nt + gr] = all;
+            }
+        } else {
+            unit[nt][0] = __shfl_sync(0xffffffffu, all, 8 * t);
+            unit[nt][1] = __shfl_sync(0xffffffffu, all, 8 * t + 4);
+        }
+    }
+    if constexpr (SHARED_Q) {
+        __syncthreads();
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) unit[nt][0] = unit_shared[8 * nt + 2 * t], unit[nt][1] = unit_shared[8 * nt + 2 * t + 1];
     }
     // Entries that this thread's two columns of each tile see.
     int sees[NT][2];
@@ -486,29 +516,46 @@ __global__ void __launch_bounds__(Ring<CT, HD>::WARPS * 32, Ring<CT, HD>::CTAS) 
                     w[mt][h][0] = x.x, w[mt][h][1] = x.y, w[mt][h][2] = x.z, w[mt][h][3] = x.w;
                 }
 #pragma unroll
-            for (int i = 0; i < (I8 ? 4 : 2); i++) {
-                uint32_t f[HALVES][4];
+            for (int i2 = 0; i2 < (I8 ? 4 : 2); i2 += 2) {
+                const int k0 = (I8 ? 4 : 2) * j + i2;  // products k0, k0 + 1 along the dims
+                uint32_t b[NT][PLANES][4];
 #pragma unroll
-                for (int mt = 0; mt < HALVES; mt++) {
-                    if constexpr (I8) {
-                        const uint32_t ua = w[mt][0][i] ^ 0x80808080u, ub = w[mt][1][i] ^ 0x80808080u;
-                        f[mt][0] = bytes_to_half2(ua, 0x4140), f[mt][2] = bytes_to_half2(ua, 0x4342);
-                        f[mt][1] = bytes_to_half2(ub, 0x4140), f[mt][3] = bytes_to_half2(ub, 0x4342);
-                    } else {
-                        f[mt][0] = w[mt][0][2 * i], f[mt][1] = w[mt][1][2 * i];
-                        f[mt][2] = w[mt][0][2 * i + 1], f[mt][3] = w[mt][1][2 * i + 1];
-                    }
-                }
+                for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                for (int pl = 0; pl < PLANES; pl++)
+                    for (int pl = 0; pl < PLANES; pl++) {
+                        if constexpr (SHARED_Q) {
+                            const uint4 x = q_shared[((nt * PLANES + pl) * (KS / 2) + k0 / 2) * 32 + lane];
+                            b[nt][pl][0] = x.x, b[nt][pl][1] = x.y, b[nt][pl][2] = x.z, b[nt][pl][3] = x.w;
+                        } else {
 #pragma unroll
-                    for (int mt = 0; mt < HALVES; mt++)
-#pragma unroll
-                        for (int nt = 0; nt < NT; nt++) {
-                            const uint32_t(&b)[2] = q[nt][pl][(I8 ? 4 : 2) * j + i];
-                            if (i + j + pl == 0) mma_first<BF>(s[mt][nt], f[mt][0], f[mt][1], f[mt][2], f[mt][3], b[0], b[1]);
-                            else mma<BF>(s[mt][nt], f[mt][0], f[mt][1], f[mt][2], f[mt][3], b[0], b[1]);
+                            for (int e = 0; e < 4; e++) b[nt][pl][e] = q[nt][pl][k0 + e / 2][e % 2];
                         }
+                    }
+#pragma unroll
+                for (int i = i2; i < i2 + 2; i++) {
+                    uint32_t f[HALVES][4];
+#pragma unroll
+                    for (int mt = 0; mt < HALVES; mt++) {
+                        if constexpr (I8) {
+                            const uint32_t ua = w[mt][0][i] ^ 0x80808080u, ub = w[mt][1][i] ^ 0x80808080u;
+                            f[mt][0] = bytes_to_half2(ua, 0x4140), f[mt][2] = bytes_to_half2(ua, 0x4342);
+                            f[mt][1] = bytes_to_half2(ub, 0x4140), f[mt][3] = bytes_to_half2(ub, 0x4342);
+                        } else {
+                            f[mt][0] = w[mt][0][2 * i], f[mt][1] = w[mt][1][2 * i];
+                            f[mt][2] = w[mt][0][2 * i + 1], f[mt][3] = w[mt][1][2 * i + 1];
+                        }
+                    }
+#pragma unroll
+                    for (int pl = 0; pl < PLANES; pl++)
+#pragma unroll
+                        for (int mt = 0; mt < HALVES; mt++)
+#pragma unroll
+                            for (int nt = 0; nt < NT; nt++) {
+                                const uint32_t b0 = b[nt][pl][2 * (i - i2)], b1 = b[nt][pl][2 * (i - i2) + 1];
+                                if (i + j + pl == 0) mma_first<BF>(s[mt][nt], f[mt][0], f[mt][1], f[mt][2], f[mt][3], b0, b1);
+                                else mma<BF>(s[mt][nt], f[mt][0], f[mt][1], f[mt][2], f[mt][3], b0, b1);
+                            }
+                }
             }
         }
         // exponents against the maxima so far; does any lie 2^8 above?
@@ -791,14 +838,17 @@ __global__ void __launch_bounds__(Ring<CT, HD>::WARPS * 32, Ring<CT, HD>::CTAS) 
     }
 }
 
-// Column tiles of 8 that a CTA takes: as many as the rows need, up to what the registers hold.
-int tiles_for(int cols, int head_dim) { return std::min(ceil_div(cols, 8), head_dim == 64 ? 4 : 2); }
+// Column tiles of 8 that a CTA takes: the rows' in as few equal groups as the registers allow.
+int tiles_for(int cols, int head_dim) {
+    const int tiles = ceil_div(cols, 8), groups = ceil_div(tiles, head_dim == 64 ? 4 : 3);
+    return ceil_div(tiles, groups);
+}
 
 int cta_limit(const pf_paged_cache& c) { return 148 * ctas_per_sm(c.head_dim * type_bytes(c.dtype)); }
 
 template <typename CT, int HD, int NT, int PLANES>
 pf_status launch_tiles(PagedParams& p, cudaStream_t st) {
-    using R = Ring<CT, HD>;
+    using R = Ring<CT, HD, NT>;
     p.row_groups = ceil_div(p.cols, 8 * NT);
     p.ctas = cta_limit(p.c);
     // segments, and with pieces of total / CTAs chunks or more no more than that many cuts
@@ -806,15 +856,19 @@ pf_status launch_tiles(PagedParams& p, cudaStream_t st) {
     const int64_t chunks = std::max<int64_t>(((int64_t)p.c.max_pages * p.c.page_size + R::CHUNK - 1) / R::CHUNK, 1);
     const int64_t grid = std::min(segments * chunks, segments + p.ctas);
     PF_CHECK(2 * segments * chunks <= INT32_MAX, "pf_paged_attention: too many positions for one call");
+    constexpr int SMEM = R::SMEM + (NT > 1 ? NT * PLANES * (HD / 32) * 512 + 8 * NT * 4 : 0);  // the ring; queries, where they are shared
     static std::atomic<uint64_t> attr{0};
-    PF_TRY(raise_smem_limit(paged_kernel<CT, HD, NT, PLANES>, R::SMEM, attr));
-    return launch_after("paged_attention", paged_kernel<CT, HD, NT, PLANES>, dim3((unsigned)grid), R::WARPS * 32, R::SMEM, st, p);
+    PF_TRY(raise_smem_limit(paged_kernel<CT, HD, NT, PLANES>, SMEM, attr));
+    return launch_after("paged_attention", paged_kernel<CT, HD, NT, PLANES>, dim3((unsigned)grid), R::WARPS * 32, SMEM, st, p);
 }
 
 template <typename CT, int PLANES>
 pf_status launch_paged(PagedParams& p, cudaStream_t st) {
     const int nt = tiles_for(p.cols, p.c.head_dim);
-    if (p.c.head_dim == 128) return nt == 1 ? launch_tiles<CT, 128, 1, PLANES>(p, st) : launch_tiles<CT, 128, 2, PLANES>(p, st);
+    if (p.c.head_dim == 128) {
+        if (nt == 1) return launch_tiles<CT, 128, 1, PLANES>(p, st);
+        return nt == 2 ? launch_tiles<CT, 128, 2, PLANES>(p, st) : launch_tiles<CT, 128, 3, PLANES>(p, st);
+    }
     if (nt == 1) return launch_tiles<CT, 64, 1, PLANES>(p, st);
     if (nt == 2) return launch_tiles<CT, 64, 2, PLANES>(p, st);
     return nt == 3 ? launch_tiles<CT, 64, 3, PLANES>(p, st) : launch_tiles<CT, 64, 4, PLANES>(p, st);
