@@ -6,10 +6,11 @@
 // in one pass over the keys: blocks of 128, the running row maximum m and sum
 // l in fp32, out = O / l at the end.
 //
-// A work unit is two 128-row tiles of queries that read the same keys and
-// values: two heads of one kv head at the same rows (or, with one query head a
-// kv head, two neighbouring row tiles).  Every K and V block is loaded once for
-// both.  One CTA an SM takes unit after unit (clusterlaunchcontrol: a running
+// A query tile's 128 rows are F heads of one kv head at 128 / F tokens, F the
+// largest power of two in the group (up to 32): short sequences and the ends of
+// long ones fill tiles that 128 tokens of one head would leave mostly empty.  A
+// work unit is two such tiles of one kv head; every K and V block is loaded once
+// for both.  One CTA an SM takes unit after unit (clusterlaunchcontrol: a running
 // CTA takes over the launch of the next one, so the units go to whoever is
 // free, longest first within a sequence).  Its warps:
 //   0-3, 4-7  softmax of tile 0 and 1, one row a thread: scores from TMEM,
@@ -24,9 +25,11 @@
 // from and the two tiles take turns at the tensor cores.
 //
 // What bounds it (B200, measured): 8,192 tokens, 32 heads over 8, head_dim 128,
-// bf16: 550 GFLOP in 492 us, 1.12 PFLOP/s, 80% of what cuBLAS sustains under the
+// bf16: 550 GFLOP in 500 us, 1.10 PFLOP/s, 79% of what cuBLAS sustains under the
 // power cap (the tensor pipe is active in 65% of the cycles at 1.54 GHz: power is
-// part of it).  64 prompts of 33 to 1,024 tokens, head_dim 64: 163 us; half of
+// part of it).  64 prompts of 33 to 1,024 tokens, head_dim 64: 153 us (163 with
+// one head a tile; 256 prompts of 5 to 40 tokens, 8 heads a kv head: 84 and 235;
+// 8,192 tokens: 500 and 496); half of
 // the products are in blocks on the diagonal or behind the end, the special-
 // function unit takes 2,048 of a block's 3,100 cycles, and each unit of three
 // blocks on average has about 4,000 cycles of its own (first scores, output).
@@ -80,7 +83,8 @@ struct PromptParams {
     void* out;
     int64_t q_stride, k_stride, v_stride, out_stride;
     const int* offsets;
-    int n_seqs, n_tokens, n_heads, n_kv_heads, group;  // group = n_heads / n_kv_heads
+    int n_seqs, n_tokens, n_heads, n_kv_heads;
+    int pack, packs;  // a tile holds 1 << pack heads; packs of them make the heads of a kv head
     float scale;
     uint32_t* err;
 };
@@ -147,10 +151,10 @@ __device__ __forceinline__ bool mbar_spin(uint32_t bar, uint32_t parity, volatil
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
     return mbar_try_wait(bar, parity) || mbar_spin(bar, parity, abort_flag);
 }
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
     asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
         : "memory");
 }
 // Operand descriptors, 128-byte swizzle (8 rows of 128 bytes = one 1,024-byte
@@ -282,10 +286,11 @@ __device__ __forceinline__ void exponentials(const uint32_t* r, float c, float o
 struct Unit {
     int first, len;   // the sequence's first row and rows
     int g;            // kv head
-    int tile[2];      // row tile of query tile s, -1: none
-    int head[2];
+    int last[2];      // of query tile s: last key block (the one on the diagonal), -1: no such tile
+    int token[2];     // first token
+    int head[2];      // first head
     int bad;          // an inf or NaN in a V block on the diagonal
-    __device__ int blocks() const { return max(tile[0], tile[1]) + 1; }
+    __device__ int blocks() const { return max(last[0], last[1]) + 1; }
 };
 
 // Walks the sequences to unit u; a whole warp, the same in every lane.  Each
@@ -297,7 +302,7 @@ struct UnitList {
     int first = 0, len = 0, pairs = 0;
     __device__ bool find(const PromptParams& p, long long u, Unit& out) {
         if (u < before) seq = 0, before = 0, end_unit = -1;
-        const int lane = threadIdx.x & 31, group = p.group;
+        const int lane = threadIdx.x & 31, tokens = BM >> p.pack;
         while (seq < p.n_seqs) {
             if (end_unit < 0) {
                 first = len = 0;
@@ -308,7 +313,7 @@ struct UnitList {
                     else latch(p.err, ERR_BOUNDS);
                 }
                 // a bad list's sequences may overlap: 64 bits, though a good one's units fit 31
-                const long long two = ((long long)((len + BM - 1) / BM) * group + 1) / 2;
+                const long long two = ((long long)((len + tokens - 1) >> (7 - p.pack)) * p.packs + 1) / 2;
                 pairs = (int)min(two, 0x7fffffffll);
                 end_unit = two * p.n_kv_heads;
                 first_unit = end_unit;
@@ -327,14 +332,12 @@ struct UnitList {
                 out.len = __shfl_sync(0xffffffffu, len, at);
                 const int q = r / p.n_kv_heads, c = 2 * (__shfl_sync(0xffffffffu, pairs, at) - 1 - q);
                 out.g = r - q * p.n_kv_heads;
-                const int tiles = (out.len + BM - 1) / BM;
-                // tiles c and c + 1 of (row tile, head of the group), heads fastest
-                const int t = c / group, h = c - t * group;
-                const bool wraps = h + 1 == group;
-                out.tile[0] = t;
-                out.tile[1] = t + wraps < tiles ? t + wraps : -1;
-                out.head[0] = out.g * group + h;
-                out.head[1] = out.g * group + (wraps ? 0 : h + 1);
+                // tiles c and c + 1 of (tokens, heads), heads fastest
+                const int t = c / p.packs, h = c - t * p.packs, wraps = h + 1 == p.packs;
+                out.token[0] = t * tokens, out.token[1] = (t + wraps) * tokens;
+                out.last[0] = out.token[0] / BM, out.last[1] = out.token[1] < out.len ? out.token[1] / BM : -1;
+                out.head[0] = (out.g * p.packs + h) << p.pack;
+                out.head[1] = (out.g * p.packs + (wraps ? 0 : h + 1)) << p.pack;
                 return true;
             }
             before += __shfl_sync(0xffffffffu, end_unit, 31);
@@ -463,8 +466,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // The unit in the list's slot, as the load warp left it.
     auto take = [&](int i, Unit& u) {
         volatile Unit& v = units[i];
-        u.first = v.first, u.len = v.len, u.g = v.g, u.tile[0] = v.tile[0], u.tile[1] = v.tile[1];
-        u.head[0] = v.head[0], u.head[1] = v.head[1];
+        u.first = v.first, u.len = v.len, u.g = v.g, u.last[0] = v.last[0], u.last[1] = v.last[1];
     };
 
     if (warp >= kSoftmaxWarps) {
@@ -483,7 +485,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (ok) {
                     volatile Unit& v = units[slot];
                     v.first = unit.first, v.len = more ? unit.len : 0, v.g = unit.g;
-                    v.tile[0] = unit.tile[0], v.tile[1] = unit.tile[1], v.head[0] = unit.head[0], v.head[1] = unit.head[1];
+                    v.last[0] = unit.last[0], v.last[1] = unit.last[1], v.token[0] = unit.token[0], v.token[1] = unit.token[1];
+                    v.head[0] = unit.head[0], v.head[1] = unit.head[1];
                     v.bad = 0;
                     mbar_arrive(u_full(slot));
                 }
@@ -509,23 +512,23 @@ __global__ void __launch_bounds__(kThreads, 1)
                     ok = wait(role == 0 ? k_empty(st) : v_empty(st), ((i / ST) & 1) ^ 1);
                     if (!ok) break;
                     mbar_expect_tx(full, Ly::SLAB);
-                    tma_load_2d(tiles + st * Ly::TILE, map, unit.g * HD + c * 64, unit.first + j * BM, full);
+                    tma_load_3d(tiles + st * Ly::TILE, map, c * 64, unit.g, unit.first + j * BM, full);
                     last_bar = full, last_parity = (i / ST) & 1;
                 }
-            } else if (role < 4 && (role == 2 ? unit.tile[0] : unit.tile[1]) >= 0) {
+            } else if (role < 4 && (role == 2 ? unit.last[0] : unit.last[1]) >= 0) {
                 const int s = role - 2;
                 const uint32_t use = s ? taken[1] : taken[0];
                 ok = wait(q_empty(s, use), ((use / QB) & 1) ^ 1);
                 if (ok) {
                     last_bar = q_full(s, use), last_parity = (use / QB) & 1;
                     mbar_expect_tx(last_bar, Ly::SLAB);
-                    tma_load_2d(q_tile(s, use) + c * Ly::SLAB, &map_q, (s ? unit.head[1] : unit.head[0]) * HD + c * 64,
-                                unit.first + (s ? unit.tile[1] : unit.tile[0]) * BM, last_bar);
+                    tma_load_3d(q_tile(s, use) + c * Ly::SLAB, &map_q, c * 64, s ? unit.head[1] : unit.head[0],
+                                unit.first + (s ? unit.token[1] : unit.token[0]), last_bar);
                 }
             }
             it += nb;
 #pragma unroll
-            for (int s = 0; s < 2; s++) taken[s] += unit.tile[s] >= 0;
+            for (int s = 0; s < 2; s++) taken[s] += unit.last[s] >= 0;
             if (!__all_sync(0xffffffffu, ok)) break;
             int got = 0;
             uint32_t x = 0;
@@ -582,7 +585,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!ok) return false;
                 n++;
                 const int len = units[slot].len;
-                next.j = 0, next.n0 = units[slot].tile[0] + 1, next.n1 = units[slot].tile[1] + 1;
+                next.j = 0, next.n0 = units[slot].last[0] + 1, next.n1 = units[slot].last[1] + 1;
                 mbar_arrive(u_empty(slot));
                 return len != 0;
             };
@@ -668,7 +671,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const uint32_t i = it + j, st = i % ST;
                 ok = __all_sync(0xffffffffu, wait(v_full(st), (i / ST) & 1));
                 if (!ok) break;
-                if (j == u.tile[0] || j == u.tile[1]) {
+                if (j == u.last[0] || j == u.last[1]) {
                     const int rows = min(BM, u.len - j * BM);
                     constexpr uint32_t EXP = BF ? 0x7f807f80u : 0x7c007c00u, ONE = BF ? 0x00800080u : 0x04000400u;
                     uint4* tile = reinterpret_cast<uint4*>(smem + Ly::V_OFF + st * Ly::TILE);
@@ -743,8 +746,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int slot = n % kSlots;
             ok = wait_all(u_full(slot), (n / kSlots) & 1);
             if (!ok) break;
-            const int first = units[slot].first, len = units[slot].len, tile = units[slot].tile[s],
-                      head = units[slot].head[s], nb = tile + 1;
+            const int first = units[slot].first, len = units[slot].len, token0 = units[slot].token[s],
+                      head0 = units[slot].head[s], nb = units[slot].last[s] + 1;
             if (len == 0) break;
             m = -INFINITY, off = 0.0f, l = 0.0f;
 #pragma unroll 1
@@ -756,7 +759,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 uint32_t r[128];
                 // r holds the block's quarters in order; on the diagonal from the warp's own quarter on, so that the one to mask
                 // by lane has fixed registers
-                const uint32_t turn = j == nb - 1 ? warp & 3 : 0;
+                // (the warp's 32 rows end in one quarter, as 128 / F tokens and their starts are multiples of each other)
+                const int end = (token0 & (BM - 1)) + ((threadIdx.x & 127) >> p.pack);  // last key that the row sees there
+                const uint32_t turn = j == nb - 1 ? end >> 5 : 0;
 #pragma unroll
                 for (int q = 0; q < 4; q++) tmem_ld32(ts + 32 * ((turn + q) & 3), r + 32 * q);
                 tmem_wait_ld();
@@ -766,14 +771,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                     mbar_arrive_if(s_free(s), lane == 0);
                 }
                 const bool diagonal = j == nb - 1;
-                if (diagonal) {  // row i sees its first i + 1 keys
-                    // r[0 .. 31] are the quarter where this warp's rows end (below); the quarters behind it are not seen at all.
+                if (diagonal) {  // r[0 .. 31] are the quarter where this warp's rows end; those behind it are not seen at all
 #pragma unroll
                     for (int q = 0; q < 32; q++)
-                        if (q > lane) r[q] = 0xff800000u;
+                        if (q > (end & 31)) r[q] = 0xff800000u;
 #pragma unroll
                     for (int q = 32; q < 128; q++)
-                        if ((warp & 3) + q / 32 < 4) r[q] = 0xff800000u;
+                        if ((end >> 5) + q / 32 < 4) r[q] = 0xff800000u;
                 }
                 const float top = row_max<128>(r);
                 const bool rise = (top - m) * c > 8.0f;  // true of a first block that has a score
@@ -807,9 +811,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!ok) break;
                 tc_fence_after();
                 const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-                const int i = tile * BM + (warp & 3) * 32;        // this warp's first row
-                const int rows = bad ? 0 : min(32, len - i);
-                T* out = static_cast<T*>(p.out) + ((int64_t)first + i) * p.out_stride + head * HD;
+                const int row0 = (warp & 3) * 32;  // this warp's first row of the tile
+                const int tokens = bad ? 0 : len - token0, heads = (1 << p.pack) - 1;
+                T* out = static_cast<T*>(p.out) + ((int64_t)first + token0) * p.out_stride + head0 * HD;
                 uint4* stage = reinterpret_cast<uint4*>(smem + Ly::OUT_OFF + warp * 4096);
 #pragma unroll 1
                 for (int q = 0; q < HD; q += 64) {
@@ -835,15 +839,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                     __syncwarp();
 #pragma unroll
                     for (int w = 0; w < 8; w++) {
-                        const int r = 4 * w + (lane >> 3);
-                        if (r < rows)
-                            *reinterpret_cast<uint4*>(out + r * p.out_stride + q + 8 * (lane & 7)) =
+                        const int r = 4 * w + (lane >> 3), token = (row0 + r) >> p.pack, head = (row0 + r) & heads;
+                        if (token < tokens)
+                            *reinterpret_cast<uint4*>(out + token * p.out_stride + head * HD + q + 8 * (lane & 7)) =
                                 stage[r * 8 + ((lane & 7) ^ (r & 7))];
                     }
                     __syncwarp();
                 }
                 if (bad)
-                    for (int w = 0; w < 32 && i + w < len; w++) plain_row<T, HD>(p, first, i + w, head, head / p.group);
+                    for (int w = row0; w < row0 + 32; w++) {
+                        const int token = token0 + (w >> p.pack), head = head0 + (w & heads);
+                        if (token < len) plain_row<T, HD>(p, first, token, head, head / (p.packs << p.pack));
+                    }
             }
             __syncwarp();
             mbar_arrive_if(u_empty(slot), lane == 0);
@@ -881,14 +888,14 @@ pf_status get_encode(EncodeTiled* fn) {
     return PF_OK;
 }
 
-// Boxes of 64 columns x 128 rows of 16-bit values; rows past the end read as zeros.
-pf_status make_map(CUtensorMap* map, const void* at, int64_t width, int64_t rows, int64_t stride) {
+// Boxes of 64 columns x `heads` heads x 128 / heads tokens of 16-bit values; tokens past the end read as zeros.
+pf_status make_map(CUtensorMap* map, const void* at, int hd, int64_t n_heads, int64_t tokens, int64_t stride, int heads) {
     EncodeTiled enc;
     PF_TRY(get_encode(&enc));
-    const cuuint64_t dims[2] = {(cuuint64_t)width, (cuuint64_t)rows};
-    const cuuint64_t strides[1] = {(cuuint64_t)stride * 2};
-    const cuuint32_t box[2] = {64, BM}, estr[2] = {1, 1};
-    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(at), dims, strides, box, estr,
+    const cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)n_heads, (cuuint64_t)tokens};
+    const cuuint64_t strides[2] = {(cuuint64_t)hd * 2, (cuuint64_t)stride * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)heads, (cuuint32_t)(BM / heads)}, estr[3] = {1, 1, 1};
+    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(at), dims, strides, box, estr,
                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     PF_CHECK(r == CUDA_SUCCESS, "pf_prompt_attention: cuTensorMapEncodeTiled failed (%d)", (int)r);
@@ -899,12 +906,12 @@ template <typename T, int HD>
 pf_status launch_prompt(const PromptParams& p, cudaStream_t st) {
     using Ly = Layout<HD>;
     CUtensorMap mq, mk, mv;
-    PF_TRY(make_map(&mq, p.q, (int64_t)p.n_heads * HD, p.n_tokens, p.q_stride));
-    PF_TRY(make_map(&mk, p.k, (int64_t)p.n_kv_heads * HD, p.n_tokens, p.k_stride));
-    PF_TRY(make_map(&mv, p.v, (int64_t)p.n_kv_heads * HD, p.n_tokens, p.v_stride));
-    // row tiles: sum ceil(len / 128) <= (sum len + 127 n_seqs) / 128, and half a pair more a sequence if the group is odd
-    const int64_t group = p.n_heads / p.n_kv_heads, tiles = ((int64_t)p.n_tokens + 127 * (int64_t)p.n_seqs) / BM;
-    const int64_t units = p.n_kv_heads * ((tiles * group + (group % 2 ? p.n_seqs : 0)) / 2);
+    PF_TRY(make_map(&mq, p.q, HD, p.n_heads, p.n_tokens, p.q_stride, 1 << p.pack));
+    PF_TRY(make_map(&mk, p.k, HD, p.n_kv_heads, p.n_tokens, p.k_stride, 1));
+    PF_TRY(make_map(&mv, p.v, HD, p.n_kv_heads, p.n_tokens, p.v_stride, 1));
+    // tiles: sum ceil(len / T) <= (sum len + (T - 1) n_seqs) / T, and half a pair more a sequence if a kv head's are odd
+    const int64_t tokens = BM >> p.pack, tiles = ((int64_t)p.n_tokens + (tokens - 1) * p.n_seqs) / tokens;
+    const int64_t units = p.n_kv_heads * ((tiles * p.packs + (p.packs % 2 ? p.n_seqs : 0)) / 2);
     PF_CHECK(units <= INT32_MAX, "pf_prompt_attention: too many row tiles");
     if (units == 0) return PF_OK;  // not one sequence can hold a row
     static std::atomic<uint64_t> attr{0};
@@ -939,8 +946,11 @@ extern "C" pf_status pf_prompt_attention(const void* q, int64_t q_stride, const 
     PF_TRY(require_device());
     if (n_seqs == 0 || n_tokens == 0) return PF_OK;
     PF_CHECK(q && k && v && out && offsets, "pf_prompt_attention: null argument");
+    const int group = n_heads / n_kv_heads;
+    int pack = 0;
+    while (pack < 5 && group % (2 << pack) == 0) pack++;
     const PromptParams p{q, k, v, out, q_stride, k_stride, v_stride, out_stride, offsets, n_seqs, n_tokens, n_heads,
-                         n_kv_heads, n_heads / n_kv_heads, scale, device_error_flag()};
+                         n_kv_heads, pack, group >> pack, scale, device_error_flag()};
     cudaStream_t st = as_stream(stream);
     if (dtype == PF_BF16)
         return head_dim == 64 ? launch_prompt<__nv_bfloat16, 64>(p, st) : launch_prompt<__nv_bfloat16, 128>(p, st);

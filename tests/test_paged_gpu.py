@@ -625,6 +625,23 @@ def test_prompt_head_layouts(t, dim, heads, kv_heads):
     run_prompt(t, dim, heads, kv_heads, [300, 17])
 
 
+@pytest.mark.parametrize("heads,kv_heads", [(6, 1), (16, 1), (24, 2), (32, 1), (64, 1), (40, 1)])
+@pytest.mark.parametrize("t,dim", [(F16, 64), (BF16, 128)])
+def test_prompt_groups(t, dim, heads, kv_heads):
+    """Tiles of 2 to 32 heads: sequences that end and begin anywhere in them, values that a head's rows may not see."""
+    lens = [1, 3, 4, 5, 31, 33, 63, 65, 130]
+    q, k, v, out = run_prompt(t, dim, heads, kv_heads, lens, fused=True, behind=9)
+    v = v.contiguous()
+    v[sum(lens) - 1] = math.nan  # the last token's
+    again = out.clone()
+    prompt(q, k, v, again, t, ints(offsets_of(lens)), len(lens), q.shape[0], heads, kv_heads, dim)
+    torch.cuda.synchronize()
+    n = sum(lens)
+    want = ph.prompt(q, k, torch.nan_to_num(v, 0), offsets_of(lens), heads, kv_heads, dim, dim ** -0.5)
+    check(again[:n - 1].contiguous(), tuple(x[:n - 1] for x in want), TYPES[t])
+    assert torch.isnan(again[n - 1]).all()
+
+
 @pytest.mark.parametrize("t,dim", [(BF16, 64), (BF16, 128), (F16, 64), (F16, 128)])
 def test_prompt_long(t, dim):
     run_prompt(t, dim, 2, 1, [2500, 4097])
