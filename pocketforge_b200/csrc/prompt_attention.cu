@@ -49,8 +49,10 @@
 //
 // What a row must not see: scores behind the row itself are -inf, their p is 0.
 // But 0 x inf = NaN, so V rows behind the sequence's end (another sequence's)
-// are set to 0 in shared memory, and a diagonal block with an inf or NaN among
-// its own V rows sends its unit's rows through a plain loop, one warp a row.
+// are set to 0 in shared memory, and so is each inf or NaN among the V rows of
+// a block on the diagonal.  The rows that see one have it added to their output
+// again: every weight is positive, so inf x p is inf whatever p is.  That is a
+// walk over at most 256 keys a warp, which no wait of the others can run out on.
 //
 // Every wait is bounded (about a second): a timeout latches ERR_TIMEOUT, the
 // other roles stop waiting, and the CTA lets its copies land and frees its TMEM.
@@ -61,7 +63,6 @@
 #include <type_traits>
 
 #include "paged.cuh"
-#include "row_attention.cuh"
 
 namespace pf {
 
@@ -348,28 +349,29 @@ struct UnitList {
     }
 };
 
-// Row i of a sequence by one warp, from memory.
+// Adds the inf and NaN among the values of keys key .. a token's own to its output, for each head of a kv head's tile and each of
+// a warp's tokens.  What a row has seen its followers see too, so one walk over the keys is enough.
 template <typename T, int HD>
-__device__ __noinline__ void plain_row(const PromptParams& p, int first, int i, int h, int g) {
+__device__ __noinline__ void add_nonfinite(const PromptParams& p, int first, int len, int g, int key, int token, int head0) {
     constexpr int N = HD / 32;
-    const int lane = threadIdx.x & 31;
-    const int64_t at = (int64_t)first + i;
-    float q[N];
+    const int lane = threadIdx.x & 31, end = min(token + (32 >> p.pack), len);
+    float sum[N];
 #pragma unroll
-    for (int d = 0; d < N; d++) q[d] = (float)static_cast<const T*>(p.q)[at * p.q_stride + h * HD + lane + 32 * d] * p.scale;
-    RowSoftmax<HD> s;
-    for (int64_t j = first; j <= at; j++) {
-        float k[N], v[N];
+    for (int d = 0; d < N; d++) sum[d] = 0.0f;
+    for (; token < end; token++) {
+        for (; key <= token; key++)
 #pragma unroll
-        for (int d = 0; d < N; d++) {
-            k[d] = (float)static_cast<const T*>(p.k)[j * p.k_stride + g * HD + lane + 32 * d];
-            v[d] = (float)static_cast<const T*>(p.v)[j * p.v_stride + g * HD + lane + 32 * d];
+            for (int d = 0; d < N; d++) {
+                const float v = (float)static_cast<const T*>(p.v)[((int64_t)first + key) * p.v_stride + g * HD + lane + 32 * d];
+                if (!(fabsf(v) <= 3.402823466e38f)) sum[d] += v;
+            }
+        for (int h = 0; h < 1 << p.pack; h++) {
+            T* out = static_cast<T*>(p.out) + ((int64_t)first + token) * p.out_stride + (head0 + h) * HD + lane;
+#pragma unroll
+            for (int d = 0; d < N; d++)
+                if (sum[d] != 0.0f) out[32 * d] = (T)((float)out[32 * d] + sum[d]);
         }
-        s.add(warp_dot(q, k), v);
     }
-#pragma unroll
-    for (int d = 0; d < N; d++)
-        static_cast<T*>(p.out)[at * p.out_stride + h * HD + lane + 32 * d] = (T)(s.l == 0.0f ? 0.0f : s.o[d] / s.l);
 }
 
 template <typename T, int HD>
@@ -477,8 +479,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         // after another, hence a lane for each.
         const int role = lane / NC, c = lane % NC;
         uint32_t it = 0, taken[2] = {0, 0}, last_bar = 0, last_parity = 0;
-        bool more = true, ok = true;
-        for (uint32_t n = 0;; n++) {
+        bool more = true, ok = true, asked = false;  // asked: for the next unit, without an answer yet
+        uint32_t n = 0;
+        for (;; n++) {
             const int slot = n % kSlots;
             if (lane == 0) {
                 ok = wait(u_empty(slot), ((n / kSlots) & 1) ^ 1);
@@ -491,6 +494,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     mbar_arrive(u_full(slot));
                 }
                 if (ok && more) {  // ask for the next one
+                    asked = true;
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     mbar_expect_tx(next_full, 16);
                     asm volatile(
@@ -534,6 +538,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             uint32_t x = 0;
             if (lane == 0) {
                 ok = wait(next_full, n & 1);
+                asked = !ok;
                 if (ok)
                     asm volatile(
                         "{\n\t.reg .pred q;\n\t.reg .b128 h;\n\t"
@@ -553,10 +558,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             more = got && list.find(p, x, unit);  // the end goes through the list as a unit without rows
         }
         if (!ok) give_up();
-        // given up: let this lane's last copy land before the shared memory is another's
+        // given up: let this lane's last copy, and an answer, land before the shared memory is another's
         if (*abort_flag && last_bar)
             for (uint32_t i = 0; i < 1000u && !mbar_try_wait(last_bar, last_parity); i++) {
             }
+        for (uint32_t i = 0; asked && i < 1000u && !mbar_try_wait(next_full, n & 1); i++) {
+        }
     } else if (warp == 9) {
         // ---------------- products ----------------
         // One lane, chosen by elect.sync: the compiler then knows that the operands are the warp's only ones and takes
@@ -675,18 +682,21 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const int rows = min(BM, u.len - j * BM);
                     constexpr uint32_t EXP = BF ? 0x7f807f80u : 0x7c007c00u, ONE = BF ? 0x00800080u : 0x04000400u;
                     uint4* tile = reinterpret_cast<uint4*>(smem + Ly::V_OFF + st * Ly::TILE);
-                    uint32_t seen = 0;
 #pragma unroll 4
                     for (int x = lane; x < Ly::TILE / 16; x += 32) {
                         if ((x >> 3) % BM < rows) {  // 8 vectors a row, BM rows a slab
                             const uint4 w = tile[x];
                             // an all-ones exponent carries into the sign's place
-                            seen |= ((w.x & EXP) + ONE) | ((w.y & EXP) + ONE) | ((w.z & EXP) + ONE) | ((w.w & EXP) + ONE);
+                            const uint32_t one = ((w.x & EXP) + ONE) | ((w.y & EXP) + ONE) | ((w.z & EXP) + ONE) | ((w.w & EXP) + ONE);
+                            if (one & 0x80008000u) {
+                                auto finite = [&](uint32_t x) { return x & ~(((((x & EXP) + ONE) & 0x80008000u) >> 15) * 0xffffu); };
+                                tile[x] = make_uint4(finite(w.x), finite(w.y), finite(w.z), finite(w.w));
+                                bad = true;
+                            }
                         } else {
                             tile[x] = make_uint4(0, 0, 0, 0);
                         }
                     }
-                    bad |= (seen & 0x80008000u) != 0;
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 }
                 __syncwarp();
@@ -812,7 +822,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tc_fence_after();
                 const float inv = l == 0.0f ? 0.0f : 1.0f / l;
                 const int row0 = (warp & 3) * 32;  // this warp's first row of the tile
-                const int tokens = bad ? 0 : len - token0, heads = (1 << p.pack) - 1;
+                const int tokens = len - token0, heads = (1 << p.pack) - 1;
                 T* out = static_cast<T*>(p.out) + ((int64_t)first + token0) * p.out_stride + head0 * HD;
                 uint4* stage = reinterpret_cast<uint4*>(smem + Ly::OUT_OFF + warp * 4096);
 #pragma unroll 1
@@ -846,11 +856,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     __syncwarp();
                 }
+                // tile 0's diagonal block is the first that the guard changed
                 if (bad)
-                    for (int w = row0; w < row0 + 32; w++) {
-                        const int token = token0 + (w >> p.pack), head = head0 + (w & heads);
-                        if (token < len) plain_row<T, HD>(p, first, token, head, head / (p.packs << p.pack));
-                    }
+                    add_nonfinite<T, HD>(p, first, len, units[slot].g, units[slot].last[0] * BM, token0 + (row0 >> p.pack), head0);
             }
             __syncwarp();
             mbar_arrive_if(u_empty(slot), lane == 0);
@@ -931,7 +939,8 @@ extern "C" pf_status pf_prompt_attention(const void* q, int64_t q_stride, const 
                                          int32_t n_kv_heads, int32_t head_dim, float scale, void* stream) {
     PF_CHECK(dtype == PF_BF16 || dtype == PF_F16, "pf_prompt_attention: dtype %d is neither PF_BF16 nor PF_F16", dtype);
     PF_CHECK(head_dim == 64 || head_dim == 128, "pf_prompt_attention: head_dim %d is neither 64 nor 128", head_dim);
-    PF_CHECK(n_seqs >= 0 && n_tokens >= 0, "pf_prompt_attention: %d sequences, %d tokens", n_seqs, n_tokens);
+    PF_CHECK(n_seqs >= 0 && n_tokens >= 0 && n_seqs <= 1 << 20 && n_tokens <= 1 << 30,
+             "pf_prompt_attention: %d sequences, %d tokens", n_seqs, n_tokens);
     PF_CHECK(n_kv_heads > 0 && n_heads > 0 && n_heads <= 65535 && n_heads % n_kv_heads == 0,
              "pf_prompt_attention: %d heads over %d kv heads", n_heads, n_kv_heads);
     PF_CHECK(scale > 0.0f && scale <= 3.402823466e38f, "pf_prompt_attention: scale must be positive and finite");
