@@ -374,9 +374,11 @@ PF_API pf_status pf_paged_attention(const pf_paged_cache* c, int32_t layer, cons
  * rows will do).  Rows outside [offsets[0], offsets[n_seqs]) of out are left
  * as they were; a sequence whose offsets are out of order or outside
  * [0, n_tokens] latches bit 1 and is left out (where offsets go back, so may be
- * others).  dtype PF_BF16 or PF_F16,
- * head_dim 64 or 128, scale > 0; pointers and the strides' bytes are
- * multiples of 16.  out overlaps none of the inputs. */
+ * others).  An inf among the values is inf, or NaN where its weight rounds to 0,
+ * in the rows that see it, and touches no other.  dtype PF_BF16 or PF_F16,
+ * head_dim 64 or 128, scale > 0; pointers and the strides' bytes are multiples
+ * of 16; 2^20 sequences and 2^30 tokens at most.  out overlaps none of the
+ * inputs. */
 PF_API pf_status pf_prompt_attention(const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
                                      int64_t v_stride, void* out, int64_t out_stride, int32_t dtype,
                                      const int32_t* offsets, int32_t n_seqs, int32_t n_tokens, int32_t n_heads,

@@ -52,7 +52,8 @@
 // are set to 0 in shared memory, and so is each inf or NaN among the V rows of
 // a block on the diagonal.  The rows that see one have it added to their output
 // again: every weight is positive, so inf x p is inf whatever p is.  That is a
-// walk over at most 256 keys a warp, which no wait of the others can run out on.
+// walk over at most 256 keys a row, however long the prompt is.  (One walk for all
+// of a warp's rows came out of the compiler with a block's loop 3% slower.)
 //
 // Every wait is bounded (about a second): a timeout latches ERR_TIMEOUT, the
 // other roles stop waiting, and the CTA lets its copies land and frees its TMEM.
@@ -349,29 +350,26 @@ struct UnitList {
     }
 };
 
-// Adds the inf and NaN among the values of keys key .. a token's own to its output, for each head of a kv head's tile and each of
-// a warp's tokens.  What a row has seen its followers see too, so one walk over the keys is enough.
+// Adds to a row's output the inf and NaN among the values of its tile's first block and the one before it, as far as the row
+// sees them: those that the guard has set to 0, and maybe some that are in the output already, which changes nothing.
 template <typename T, int HD>
-__device__ __noinline__ void add_nonfinite(const PromptParams& p, int first, int len, int g, int key, int token, int head0) {
+__device__ __noinline__ void add_nonfinite(const PromptParams& p, int first, int token, int head, int g, int token0) {
     constexpr int N = HD / 32;
-    const int lane = threadIdx.x & 31, end = min(token + (32 >> p.pack), len);
+    const int lane = threadIdx.x & 31;
     float sum[N];
 #pragma unroll
     for (int d = 0; d < N; d++) sum[d] = 0.0f;
-    for (; token < end; token++) {
-        for (; key <= token; key++)
+#pragma unroll 4
+    for (int key = max(token0 / BM - 1, 0) * BM; key <= token; key++)
 #pragma unroll
-            for (int d = 0; d < N; d++) {
-                const float v = (float)static_cast<const T*>(p.v)[((int64_t)first + key) * p.v_stride + g * HD + lane + 32 * d];
-                if (!(fabsf(v) <= 3.402823466e38f)) sum[d] += v;
-            }
-        for (int h = 0; h < 1 << p.pack; h++) {
-            T* out = static_cast<T*>(p.out) + ((int64_t)first + token) * p.out_stride + (head0 + h) * HD + lane;
-#pragma unroll
-            for (int d = 0; d < N; d++)
-                if (sum[d] != 0.0f) out[32 * d] = (T)((float)out[32 * d] + sum[d]);
+        for (int d = 0; d < N; d++) {
+            const float v = (float)static_cast<const T*>(p.v)[((int64_t)first + key) * p.v_stride + g * HD + lane + 32 * d];
+            if (!(fabsf(v) <= 3.402823466e38f)) sum[d] += v;
         }
-    }
+    T* out = static_cast<T*>(p.out) + ((int64_t)first + token) * p.out_stride + head * HD + lane;
+#pragma unroll
+    for (int d = 0; d < N; d++)
+        if (sum[d] != 0.0f) out[32 * d] = (T)((float)out[32 * d] + sum[d]);
 }
 
 template <typename T, int HD>
@@ -479,7 +477,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // after another, hence a lane for each.
         const int role = lane / NC, c = lane % NC;
         uint32_t it = 0, taken[2] = {0, 0}, last_bar = 0, last_parity = 0;
-        bool more = true, ok = true, asked = false;  // asked: for the next unit, without an answer yet
+        bool more = true, ok = true;
         uint32_t n = 0;
         for (;; n++) {
             const int slot = n % kSlots;
@@ -494,7 +492,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                     mbar_arrive(u_full(slot));
                 }
                 if (ok && more) {  // ask for the next one
-                    asked = true;
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     mbar_expect_tx(next_full, 16);
                     asm volatile(
@@ -538,7 +535,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             uint32_t x = 0;
             if (lane == 0) {
                 ok = wait(next_full, n & 1);
-                asked = !ok;
                 if (ok)
                     asm volatile(
                         "{\n\t.reg .pred q;\n\t.reg .b128 h;\n\t"
@@ -562,8 +558,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (*abort_flag && last_bar)
             for (uint32_t i = 0; i < 1000u && !mbar_try_wait(last_bar, last_parity); i++) {
             }
-        for (uint32_t i = 0; asked && i < 1000u && !mbar_try_wait(next_full, n & 1); i++) {
-        }
+        if (*abort_flag && lane == 0)
+            for (uint32_t i = 0; i < 10u && !mbar_try_wait(next_full, n & 1); i++) {
+            }
     } else if (warp == 9) {
         // ---------------- products ----------------
         // One lane, chosen by elect.sync: the compiler then knows that the operands are the warp's only ones and takes
@@ -682,20 +679,23 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const int rows = min(BM, u.len - j * BM);
                     constexpr uint32_t EXP = BF ? 0x7f807f80u : 0x7c007c00u, ONE = BF ? 0x00800080u : 0x04000400u;
                     uint4* tile = reinterpret_cast<uint4*>(smem + Ly::V_OFF + st * Ly::TILE);
+                    uint32_t seen = 0;
 #pragma unroll 4
                     for (int x = lane; x < Ly::TILE / 16; x += 32) {
                         if ((x >> 3) % BM < rows) {  // 8 vectors a row, BM rows a slab
                             const uint4 w = tile[x];
                             // an all-ones exponent carries into the sign's place
-                            const uint32_t one = ((w.x & EXP) + ONE) | ((w.y & EXP) + ONE) | ((w.z & EXP) + ONE) | ((w.w & EXP) + ONE);
-                            if (one & 0x80008000u) {
-                                auto finite = [&](uint32_t x) { return x & ~(((((x & EXP) + ONE) & 0x80008000u) >> 15) * 0xffffu); };
-                                tile[x] = make_uint4(finite(w.x), finite(w.y), finite(w.z), finite(w.w));
-                                bad = true;
-                            }
+                            seen |= ((w.x & EXP) + ONE) | ((w.y & EXP) + ONE) | ((w.z & EXP) + ONE) | ((w.w & EXP) + ONE);
                         } else {
                             tile[x] = make_uint4(0, 0, 0, 0);
                         }
+                    }
+                    if (seen & 0x80008000u) {
+                        auto finite = [&](uint32_t x) { return x & ~(((((x & EXP) + ONE) & 0x80008000u) >> 15) * 0xffffu); };
+                        bad = true;
+#pragma unroll 1
+                        for (int x = lane; x < Ly::TILE / 16; x += 32)
+                            tile[x] = make_uint4(finite(tile[x].x), finite(tile[x].y), finite(tile[x].z), finite(tile[x].w));
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 }
@@ -856,9 +856,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     __syncwarp();
                 }
-                // tile 0's diagonal block is the first that the guard changed
                 if (bad)
-                    add_nonfinite<T, HD>(p, first, len, units[slot].g, units[slot].last[0] * BM, token0 + (row0 >> p.pack), head0);
+                    for (int w = row0; w < row0 + 32; w++) {
+                        const int token = token0 + (w >> p.pack), head = head0 + (w & heads);
+                        if (token < len) add_nonfinite<T, HD>(p, first, token, head, head / (p.packs << p.pack), token0);
+                    }
             }
             __syncwarp();
             mbar_arrive_if(u_empty(slot), lane == 0);

@@ -690,6 +690,49 @@ def test_prompt_does_not_mix_what_is_masked(t, dim, bad):
     assert torch.isfinite(others).all()
 
 
+@pytest.mark.parametrize("heads,kv_heads", [(2, 2), (4, 2), (8, 1), (6, 1), (33, 1)])
+@pytest.mark.parametrize("t,dim", [(F16, 64), (BF16, 128)])
+def test_prompt_infinities_of_its_own(t, dim, heads, kv_heads):
+    """inf, -inf and NaN among the values of any block: each dim of a row takes what the row has seen of them."""
+    lens, rng = [300, 9, 140], random.Random(heads)
+    q, k, v, ref = run_prompt(t, dim, heads, kv_heads, lens, by=0.25)
+    where = [(r, d) for r in (5, 64, 100, 127, 128, 200, 255, 299, 300, 308, 309, 400, 448)
+             for d in rng.sample(range(kv_heads * dim), 3)] + [(60, 7), (130, 7), (280, 7)]
+    v = v.clone()
+    for i, (r, d) in enumerate(where):
+        v[r, d] = (math.inf, -math.inf, math.nan)[i % 3]
+    out = torch.empty_like(ref)
+    prompt(q, k, v, out, t, ints(offsets_of(lens)), 3, q.shape[0], heads, kv_heads, dim)
+    torch.cuda.synchronize()
+    want, big_v, big_s = ph.prompt(q, k, torch.nan_to_num(v, 0, 0, 0), offsets_of(lens), heads, kv_heads, dim, dim ** -0.5)
+    odd = torch.where(torch.isfinite(v.float()), 0.0, v.float()).view(-1, kv_heads, dim)
+    seen = torch.cat([x.cumsum(0) for x in odd.split(lens)]).repeat_interleave(heads // kv_heads, 1)
+    got, fine = out.view(-1, heads, dim).float(), seen == 0
+    assert torch.equal(torch.isnan(got), torch.isnan(seen))
+    assert torch.equal(got[torch.isinf(seen)], seen[torch.isinf(seen)])
+    check(torch.where(fine, got, 0.0).to(TYPES[t]), (torch.where(fine, want, 0.0), big_v, big_s), TYPES[t])
+
+
+def test_prompt_infinity_at_the_end_of_a_long_one():
+    """An inf among the last tokens' values costs its rows a walk over their own block, not over the whole prompt."""
+    n, dim = 100_000, 64
+    q, k, v = (randn((n, dim), torch.bfloat16, i, 0.5) for i in range(3))
+    v[n - 3, 11] = -math.inf
+    out = torch.empty_like(q)
+    prompt(q, k, v, out, BF16, ints([0, n]), 1, n, 1, 1, dim)
+    torch.cuda.synchronize()
+    assert latched() == 0
+    assert torch.isfinite(out[:n - 3]).all() and (out[n - 3:, 11] == -math.inf).all()
+    few, v0 = [0, 5000, n - 130, n - 3, n - 2, n - 1], torch.nan_to_num(v, 0, 0, 0).double()
+    for i in few:
+        x = q[i].double() @ k[:i + 1].double().T * dim ** -0.5
+        want = ph.softmax_mean(x, v0[:i + 1])
+        got = torch.where(torch.isfinite(out[i].float()), out[i].float(), want.float()).bfloat16()
+        got[11] = want[11] if i >= n - 3 else got[11]
+        check(got, (want.view(1, 1, dim), v0[:i + 1].abs().amax().view(1, 1, 1),
+                    (q[i].double().abs() @ k[:i + 1].double().abs().T * dim ** -0.5).amax().view(1, 1, 1)), torch.bfloat16)
+
+
 def test_prompt_many_sequences():
     rng = random.Random(2)
     run_prompt(BF16, 64, 2, 1, [rng.choice([0, 1, 2, 3, 9]) for _ in range(1500)])
