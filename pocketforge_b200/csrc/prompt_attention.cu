@@ -800,17 +800,30 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 if (any_rise) raise(rise ? top : m, j > 0);
                 uint32_t pk[2][16];
-                exponentials<T>(r, c, off, sum, pk[0]);
-                tmem_st16(tp + 16 * turn, pk[0]);
-                exponentials<T>(r + 32, c, off, sum, pk[1]);
-                tmem_st16(tp + 16 * ((turn + 1) & 3), pk[1]);
-                exponentials<T>(r + 64, c, off, sum, pk[0]);
-                if (!diagonal) publish(p_half(s));  // its stores went on while this quarter was computed
-                tmem_st16(tp + 16 * ((turn + 2) & 3), pk[0]);
-                exponentials<T>(r + 96, c, off, sum, pk[1]);
-                tmem_st16(tp + 16 * ((turn + 3) & 3), pk[1]);
-                publish(p_full(s));
-                if (diagonal) mbar_arrive_if(p_half(s), lane == 0);
+                if (Ly::OWN_P && diagonal && end < 64) {  // nothing behind the block's first half is seen
+                    exponentials<T>(r, c, off, sum, pk[0]);
+                    tmem_st16(tp + 16 * turn, pk[0]);
+#pragma unroll
+                    for (int q = 0; q < 16; q++) pk[0][q] = pk[1][q] = 0;
+                    tmem_st16(tp + 32, pk[0]);
+                    tmem_st16(tp + 48, pk[0]);
+                    if (turn) exponentials<T>(r + 96, c, off, sum, pk[1]);
+                    tmem_st16(tp + 16 * (turn ^ 1), pk[1]);
+                    publish(p_full(s));
+                    mbar_arrive_if(p_half(s), lane == 0);
+                } else {
+                    exponentials<T>(r, c, off, sum, pk[0]);
+                    tmem_st16(tp + 16 * turn, pk[0]);
+                    exponentials<T>(r + 32, c, off, sum, pk[1]);
+                    tmem_st16(tp + 16 * ((turn + 1) & 3), pk[1]);
+                    exponentials<T>(r + 64, c, off, sum, pk[0]);
+                    if (!diagonal) publish(p_half(s));  // its stores went on while this quarter was computed
+                    tmem_st16(tp + 16 * ((turn + 2) & 3), pk[0]);
+                    exponentials<T>(r + 96, c, off, sum, pk[1]);
+                    tmem_st16(tp + 16 * ((turn + 3) & 3), pk[1]);
+                    publish(p_full(s));
+                    if (diagonal) mbar_arrive_if(p_half(s), lane == 0);
+                }
                 l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
             }
             ok = ok && wait_all(u_seen(slot), (n / kSlots) & 1);
