@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(Ring<CT, HD, NT>::WARPS * 32, Ring<CT, HD, NT>
         // pieces that are a little longer): each lane tries one between the share and twice that.
         const int share = (total + p.ctas - 1) / p.ctas;
         int most = 2 * share;
-        if (4 * p.n_seqs * segs < 3 * p.ctas) {
+        if (p.n_seqs * segs < p.ctas / 4 * 3) {
             const int mine = share + lane * ((share + 31) / 32);
             const float inv = 1.0f / (float)mine;
             int pieces = 0;
@@ -427,7 +427,7 @@ __global__ void __launch_bounds__(Ring<CT, HD, NT>::WARPS * 32, Ring<CT, HD, NT>
             big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
             big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
             const bool finite = big > 0.0f && big < __int_as_float(0x7f800000);
-            const int up = finite ? min(max(13 - exponent_of(big), -100), 100) : 0;
+            const int up = finite ? min(13 - exponent_of(big), 100) : 0;  // -114 at least
             const float f = power_of_two(up);
             all *= power_of_two(-up);
 #pragma unroll
@@ -625,7 +625,7 @@ __global__ void __launch_bounds__(Ring<CT, HD, NT>::WARPS * 32, Ring<CT, HD, NT>
             const float inf = __int_as_float(0x7f800000), vs = fabsf(scales[kBlock + lane]), x = vs * vscale;
             if (__any_sync(0xffffffffu, x >= 128.0f && vs < inf) || !__any_sync(0xffffffffu, x >= 1.0f && x < inf)) {
                 const unsigned big = __reduce_max_sync(0xffffffffu, vs < inf ? __float_as_uint(vs) : 0u);
-                const int up = min(max(6 - exponent_of(__uint_as_float(big)), -100), 100);
+                const int up = min(6 - exponent_of(__uint_as_float(big)), 100);  // -121 at least
                 vscale = power_of_two(up), back = power_of_two(-up);
             }
         }

@@ -409,6 +409,19 @@ def test_attention_scores_of_all_sizes():
             attend(c, t, 2, 3, 4, by=by)
 
 
+@pytest.mark.parametrize("rows", [1, 4])
+def test_attention_numbers_near_the_largest(rows):
+    """fp32 queries and int8 scales of 2^112 and more: the powers of two that take them into fp16's range reach there."""
+    c = Cache(I8, 1, 1, 64, 16, 40, 2, 30).place([12, 37])
+    c.ks *= 2.0 ** 6
+    c.vs *= 2.0 ** 118
+    q = randn((2 * rows, 4 * 64), torch.float32, 3, 2.0 ** 118)
+    out = torch.empty_like(q)
+    c.attend(0, q, out, F32, 2, rows, 4, 2.0 ** -125)
+    torch.cuda.synchronize()
+    check(out, c.attention(0, q, 2, rows, 4, 2.0 ** -125), torch.float32)
+
+
 @pytest.mark.parametrize("cache,t", [(I8, F32), (I8, BF16), (BF16, BF16), (F16, F16)])
 def test_attention_rows_of_unlike_sizes(cache, t):
     """A head whose queries are large, small or no numbers leaves the heads beside it as they are."""
