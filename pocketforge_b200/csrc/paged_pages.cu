@@ -21,6 +21,7 @@ namespace {
 constexpr int kDecide = 1024;   // threads of the deciding CTA
 constexpr int kPerThread = 64;  // pages a thread takes at once at most (one bit each)
 constexpr int kCopy = 256;      // threads of a copying CTA
+constexpr int kMaxPages = 1 << 28, kMaxSeqs = 1 << 20;
 constexpr int kVecs = 4;        // 16-byte vectors a thread has in flight
 
 // Exclusive prefix sum over the CTA's 1,024 threads, and the total.
@@ -169,7 +170,7 @@ __global__ void free_kernel(const pf_paged_cache c, const int* seqs, uint32_t* e
     if (threadIdx.x == 0) s_len = atomicExch(&c.lens[s], 0);
     __syncthreads();
     if (s_len < 0 || s_len > (int64_t)c.max_pages * c.page_size) {
-        if (threadIdx.x == 0) latch(err, ERR_BOUNDS);
+        if (threadIdx.x == 0) c.lens[s] = s_len, latch(err, ERR_BOUNDS);  // left as it is
         return;
     }
     const int pages = (int)(((int64_t)s_len + c.page_size - 1) / c.page_size);
@@ -406,7 +407,7 @@ pf_status check_paged_cache(const pf_paged_cache* c, const char* where, bool nee
              "%s: page_size %d is not 16, 32, 64 or 128", where, c->page_size);
     PF_CHECK(c->n_layers > 0 && c->n_kv_heads > 0 && c->n_pages > 0 && c->max_seqs > 0 && c->max_pages > 0,
              "%s: a size is not positive", where);
-    PF_CHECK((int64_t)c->n_layers * c->n_kv_heads <= 65536 && c->n_pages <= (1 << 28) && c->max_seqs <= (1 << 20) &&
+    PF_CHECK((int64_t)c->n_layers * c->n_kv_heads <= 65536 && c->n_pages <= kMaxPages && c->max_seqs <= kMaxSeqs &&
                  (int64_t)c->max_pages * c->page_size <= 1 << 30,
              "%s: a size is too large", where);
     PF_CHECK(c->k && c->v && c->table && c->lens && c->refs, "%s: null pointer in the cache", where);
@@ -425,7 +426,7 @@ using namespace pf;
 extern "C" {
 
 size_t pf_paged_work_bytes(const pf_paged_cache* c) {
-    if (!c || c->n_pages <= 0 || c->max_seqs <= 0) return 0;
+    if (!c || c->n_pages <= 0 || c->max_seqs <= 0 || c->n_pages > kMaxPages || c->max_seqs > kMaxSeqs) return 0;
     return page_work_bytes(*c);
 }
 

@@ -223,6 +223,17 @@ def test_pages_lists_that_are_wrong():
         ok("pf_paged_copy", c.ref, None, None, n, None)
 
 
+def test_pages_free_leaves_a_length_that_is_none():
+    c = Cache(I8, 1, 1, 64, 16, 12, 4, 4).place([20, 5, 64, 1])
+    c.lens[0], c.lens[2] = -7, 65
+    refs, table = c.refs.tolist(), c.table.tolist()
+    c.free([0, 1, 2, 0])
+    assert latched() == 1
+    refs[table[1][0]] = 0
+    table[1][0] = -1
+    assert c.lens.tolist() == [-7, 0, 65, 1] and c.refs.tolist() == refs and c.table.tolist() == table
+
+
 # ---------------------------------------------------------------------------
 # Store
 # ---------------------------------------------------------------------------
