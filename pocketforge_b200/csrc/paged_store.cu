@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(kThreads) store_kernel(const pf_paged_cache c,
             const int t = t0 + lane;
             while (b < n_seqs && offsets[b + 1] <= t) b++;  // (b = -1: offsets[0] > t0)
             int page = -1, slot = 0;
-            if (b >= 0 && b < n_seqs) {
+            if (b >= 0 && b < n_seqs && offsets[b] <= t) {
                 const int n = seq_len(c, b, err);
                 const int64_t pos = (int64_t)n - ((int64_t)offsets[b + 1] - t);
                 if (n >= 0 && pos >= 0 && pos < n) {
@@ -176,6 +176,9 @@ __global__ void __launch_bounds__(kThreads) store_kernel(const pf_paged_cache c,
             }
             s_page[lane] = page, s_slot[lane] = slot;
         }
+    } else if (blockIdx.x == 0) {  // meanwhile one CTA looks at the offsets' order
+        for (int j = threadIdx.x - 32; j < n_seqs; j += kThreads - 32)
+            if (offsets[j] > offsets[j + 1]) latch(err, ERR_BOUNDS);
     }
     __syncthreads();
     while (u < rows) {
@@ -217,7 +220,7 @@ extern "C" pf_status pf_paged_store(const pf_paged_cache* c, int32_t layer, cons
                                     int32_t n_seqs, int32_t n_tokens, void* stream) {
     PF_TRY(check_paged_cache(c, "pf_paged_store", false));
     PF_CHECK(layer >= 0 && layer < c->n_layers, "pf_paged_store: layer %d of %d", layer, c->n_layers);
-    PF_CHECK(n_seqs >= 0 && n_seqs <= c->max_seqs && n_tokens >= 0, "pf_paged_store: %d sequences of %d, %d tokens",
+    PF_CHECK(n_seqs >= 0 && n_seqs <= c->max_seqs && n_tokens >= 0 && n_tokens <= 1 << 30, "pf_paged_store: %d sequences of %d, %d tokens",
              n_seqs, c->max_seqs, n_tokens);
     PF_CHECK(dtype == PF_F32 || (c->dtype == PF_I8 ? dtype == PF_BF16 || dtype == PF_F16 : dtype == c->dtype),
              "pf_paged_store: rows of dtype %d into a cache of dtype %d", dtype, c->dtype);

@@ -127,6 +127,14 @@ def test_a_good_call_needs_a_device():
     assert L.pf_prompt_attention(A, 256, A, 128, A, 128, A, 256, _lib.PF_BF16, A, 1, 5, 4, 2, 64, 0.125, None) == none
 
 
+def test_calls_too_large_to_count():
+    refused("pf_paged_store", C.byref(cache()), 0, A, 128, A, 128, _lib.PF_F32, A, 1, (1 << 30) + 1, None)
+    for seqs, tokens in (((1 << 20) + 1, 5), (1, (1 << 30) + 1)):
+        refused("pf_prompt_attention", A, 256, A, 128, A, 128, A, 256, _lib.PF_BF16, A, seqs, tokens, 4, 2, 64, 0.125, None)
+    assert _lib.lib().pf_paged_work_bytes(C.byref(cache(n_pages=(1 << 28) + 1))) == 0
+    assert _lib.lib().pf_paged_work_bytes(C.byref(cache(max_seqs=(1 << 20) + 1))) == 0
+
+
 def test_work_sizes():
     L = _lib.lib()
     assert L.pf_paged_work_bytes(C.byref(cache())) >= 4 * (3 * 32 + 2 * 4)

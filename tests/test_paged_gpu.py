@@ -332,6 +332,21 @@ def test_store_leaves_out_what_has_no_place():
     ok("pf_paged_store", c.ref, 0, None, 64, None, 64, F16, None, 0, 0, None)
 
 
+def test_store_offsets_that_go_back():
+    """Bit 1; the rows of sequences whose offsets are in order are where they belong, the others nowhere else."""
+    c = Cache(F16, 1, 1, 64, 16, 8, 4, 2).place([8, 8, 8, 8])
+    want = c.k.clone()
+    x = randn((8, 64), torch.float16, 3)
+    c.store(0, x, x, [0, 6, 4, 4, 8], F16)
+    assert latched() == 1
+    torch.cuda.synchronize()
+    page = [int(p) for p in c.table[:, 0]]
+    want[page[3], 0, 0, 4:8] = x[4:8]
+    free = torch.ones_like(c.k, dtype=torch.bool)
+    free[page[0], 0, 0, 2:8] = free[page[3], 0, 0, 4:6] = False  # (rows 4 and 5 are named by two)
+    assert torch.equal(c.k[free], want[free])
+
+
 def test_store_many_sequences():
     """Sequence search over 3,000 offsets, most of them of empty sequences."""
     rng = random.Random(1)
