@@ -53,6 +53,34 @@ __device__ __forceinline__ int seq_len(const pf_paged_cache& c, int b, uint32_t*
     return -1;
 }
 
+constexpr int kDecide = 1024;  // threads of a CTA that decides for the others
+// Exclusive prefix sum over the CTA's 1,024 threads, and the total.
+__device__ __forceinline__ long long block_scan(long long v, long long* total, long long* s_warp) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    long long x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    if (lane == 31) s_warp[warp] = x;
+    __syncthreads();
+    if (warp == 0) {
+        long long w = s_warp[lane];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long y = __shfl_up_sync(0xffffffffu, w, o);
+            if (lane >= o) w += y;
+        }
+        s_warp[lane] = w;
+    }
+    __syncthreads();
+    const long long before = warp ? s_warp[warp - 1] : 0;
+    *total = s_warp[31];
+    __syncthreads();  // s_warp is free for the next scan
+    return before + x - v;
+}
+
 // A launch that may begin while the one before it in the stream still runs: the
 // kernel waits for that one's end itself (after_previous) before it reads or
 // writes anything, so only the way to its first instruction overlaps.

@@ -66,6 +66,10 @@ namespace pf {
 namespace {
 
 constexpr int kMaxCuts = 64;     // pieces of a segment: as many as one CTA joins in about a microsecond
+// Sequences from which on a launch of one CTA plans the pieces for all: its 2 us are less than what every CTA would take to
+// look through them (bf16: 1,000 sequences of 50 to 200 tokens 314 and 121 us, 250 of them 49 and 35, 128 36.0 and 36.9; one kv
+// head's 128 of 500 to 1,500, where the pieces are tried out, 22.6 and 20.0, 64 of them 16.5 and 18.0).
+constexpr int kPlanned = 160, kPlannedFew = 96;
 constexpr int kCounters = 1024;  // at the start of `work`: seg_begin / P is below the CTAs that fit
 
 struct PagedParams {
@@ -78,6 +82,7 @@ struct PagedParams {
     float scale;
     int ctas;      // that fit the GPU
     int* count;    // [kCounters] pieces of a cut segment that have ended
+    int2* plan;    // of many sequences: {pieces, most}, then each one's {pieces, chunks} before it; else null
     float* part;   // [piece of a cut segment][columns a row group][head_dim + 4]
     uint32_t* err;
 };
@@ -227,6 +232,23 @@ __device__ __forceinline__ int cuts_of(int n, int most, float inv) {
     return min(k + (k * most < n), kMaxCuts);
 }
 
+// Chunks a piece.  With nearly as many segments as CTAs fit, only what is twice as long as the share is cut.  With fewer, the
+// least with which all pieces are there at once (a second, nearly empty round of CTAs costs more than pieces that are a little
+// longer), of 32 between the share and twice that: pieces_at(most, 1 / most) says how many there are, fewer of longer ones.
+__host__ __device__ constexpr int few_segments(int ctas) { return ctas / 4 * 3; }
+template <typename F>
+__device__ __forceinline__ int piece_limit(int total, int segments, int ctas, const F& pieces_at) {
+    const int share = (total + ctas - 1) / ctas, step = (share + 31) / 32;
+    if (segments >= few_segments(ctas)) return 2 * share;
+    int i = 0;
+#pragma unroll 1
+    for (int by = 16; by; by >>= 1) {
+        const int mine = share + (i + by - 1) * step;
+        if (pieces_at(mine, 1.0f / (float)mine) > ctas) i += by;
+    }
+    return share + i * step;
+}
+
 // x / group for a column x of at most eight tokens.
 __device__ __forceinline__ int token_of(int x, int group) {
     int t = 0;
@@ -243,6 +265,45 @@ __device__ __forceinline__ void store_out(const PagedParams& p, int seq, int g, 
     else
         *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + at) =
             p.dtype == PF_BF16 ? pack<true>(v.x, v.y) : pack<false>(v.x, v.y);
+}
+
+// Sum over the CTA's threads, in all of them.
+__device__ __forceinline__ int block_sum(int v, int* s_warp) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    v = __reduce_add_sync(0xffffffffu, v);
+    if (lane == 0) s_warp[warp] = v;
+    __syncthreads();
+    v = __reduce_add_sync(0xffffffffu, s_warp[lane]);
+    __syncthreads();
+    return v;
+}
+
+// The plan of many sequences, which every CTA of the attention would take longer to make than to look up.
+__global__ void __launch_bounds__(kDecide) plan_kernel(const PagedParams p, int chunk) {
+    after_previous();
+    __shared__ int s_sum[32];
+    __shared__ long long s_scan[32];
+    const int segs = p.c.n_kv_heads * p.row_groups;
+    auto chunks = [&](int b, uint32_t* err) { return max((length_of(p, b, err) + chunk - 1) / chunk, 1); };
+    int total = 0;
+    for (int b = threadIdx.x; b < p.n_seqs; b += kDecide) total += chunks(b, p.err);
+    total = block_sum(total, s_sum) * segs;
+    const int most = piece_limit(total, p.n_seqs * segs, p.ctas, [&](int mine, float inv) {
+        int pieces = 0;
+        for (int b = threadIdx.x; b < p.n_seqs; b += kDecide) pieces += cuts_of(chunks(b, nullptr), mine, inv);
+        return block_sum(pieces, s_sum) * segs;
+    });
+    const float inv = 1.0f / (float)most;
+    long long before = 0;  // pieces and chunks, 32 bits each
+    for (int b0 = 0; b0 < p.n_seqs; b0 += kDecide) {
+        const int b = b0 + threadIdx.x, n = b < p.n_seqs ? chunks(b, nullptr) : 0;
+        long long all;
+        const long long mine = n ? (((long long)cuts_of(n, most, inv) << 32) | n) * segs : 0;
+        const long long x = before + block_scan(mine, &all, s_scan);
+        if (n) p.plan[1 + b] = make_int2((int)(x >> 32), (int)x);
+        before += all;
+    }
+    if (threadIdx.x == 0) p.plan[0] = make_int2((int)(before >> 32), most);
 }
 
 template <typename CT, int HD, int NT, int PLANES>
@@ -266,16 +327,32 @@ __global__ void __launch_bounds__(Ring<CT, HD, NT>::WARPS * 32, Ring<CT, HD, NT>
 
     after_previous();
     // ---- this CTA's piece ----  (the host has seen to it that all chunks count in 31 bits)
-    if (warp == 0) {
+    if (warp == 0 && p.plan) {
+        const int2 all = p.plan[0];
+        const int x = (int)blockIdx.x;
+        int at = 0;
+        for (int n = x < all.x ? p.n_seqs : 0; n > 1;) {  // among n from `at` on: 32 at a time
+            const int step = (n + 31) / 32;
+            const bool le = lane * step < n && p.plan[1 + at + lane * step].x <= x;
+            const int k = __popc(__ballot_sync(0xffffffffu, le)) - 1;
+            at += k * step;
+            n = min(step, n - k * step);
+        }
+        if (lane == 0) {
+            s_seq = x < all.x ? at : -1;
+            s_piece = x - p.plan[1 + at].x;
+            s_before = p.plan[1 + at].y;
+            s_len = length_of(p, at, nullptr);
+            s_cuts = cuts_of(chunks_of<R::CHUNK>(s_len), all.y, 1.0f / (float)all.y);
+            s_most = all.y;
+        }
+    } else if (warp == 0) {
         int total = 0;
         for (int b = lane; b < p.n_seqs; b += 32) total += chunks_of<R::CHUNK>(length_of(p, b, blockIdx.x == 0 ? p.err : nullptr));
         total = __reduce_add_sync(0xffffffffu, total) * segs;
-        // Chunks a piece.  With nearly as many segments as CTAs fit, only what is twice as long as the share is cut.  With
-        // fewer, the least with which all pieces are there at once (a second, nearly empty round of CTAs costs more than
-        // pieces that are a little longer): each lane tries one between the share and twice that.
         const int share = (total + p.ctas - 1) / p.ctas;
         int most = 2 * share;
-        if (p.n_seqs * segs < p.ctas / 4 * 3) {
+        if (p.n_seqs * segs < few_segments(p.ctas)) {  // as piece_limit, each lane trying one
             const int mine = share + lane * ((share + 31) / 32);
             const float inv = 1.0f / (float)mine;
             int pieces = 0;
@@ -846,6 +923,11 @@ int tiles_for(int cols, int head_dim) {
 
 int cta_limit(const pf_paged_cache& c) { return 148 * ctas_per_sm(c.head_dim * type_bytes(c.dtype)); }
 
+// Of `work`: the counters, the pieces of cut segments, the plan.
+size_t part_bytes(const pf_paged_cache& c, int tiles) {
+    return (size_t)(cta_limit(c) + 1) * 2 * 8 * tiles * (c.head_dim + 4) * sizeof(float);
+}
+
 template <typename CT, int HD, int NT, int PLANES>
 pf_status launch_tiles(PagedParams& p, cudaStream_t st) {
     using R = Ring<CT, HD, NT>;
@@ -856,7 +938,10 @@ pf_status launch_tiles(PagedParams& p, cudaStream_t st) {
     const int64_t chunks = std::max<int64_t>(((int64_t)p.c.max_pages * p.c.page_size + R::CHUNK - 1) / R::CHUNK, 1);
     const int64_t grid = std::min(segments * chunks, segments + p.ctas);
     PF_CHECK(2 * segments * chunks <= INT32_MAX, "pf_paged_attention: too many positions for one call");
+    if (p.n_seqs >= (segments < few_segments(p.ctas) ? kPlannedFew : kPlanned))
+        p.plan = reinterpret_cast<int2*>(reinterpret_cast<char*>(p.part) + part_bytes(p.c, NT));
     constexpr int SMEM = R::SMEM + (NT > 1 ? NT * PLANES * (HD / 32) * 512 + 8 * NT * 4 : 0);  // the ring; queries, where they are shared
+    if (p.plan) PF_TRY(launch_after("paged_attention_plan", plan_kernel, dim3(1), kDecide, 0, st, p, R::CHUNK));
     static std::atomic<uint64_t> attr{0};
     PF_TRY(raise_smem_limit(paged_kernel<CT, HD, NT, PLANES>, SMEM, attr));
     return launch_after("paged_attention", paged_kernel<CT, HD, NT, PLANES>, dim3((unsigned)grid), R::WARPS * 32, SMEM, st, p);
@@ -886,8 +971,7 @@ size_t pf_paged_attention_work_bytes(const pf_paged_cache* c, int32_t n_seqs, in
     if (!c || n_seqs < 0 || rows < 1 || rows > 8 || n_heads < 1 || c->n_kv_heads < 1 || n_heads % c->n_kv_heads) return 0;
     if (c->head_dim != 64 && c->head_dim != 128) return 0;
     const int nt = tiles_for(n_heads / c->n_kv_heads * rows, c->head_dim);
-    // counters, then the pieces of cut segments
-    return kCounters * sizeof(int) + (size_t)(cta_limit(*c) + 1) * 2 * 8 * nt * (c->head_dim + 4) * sizeof(float);
+    return kCounters * sizeof(int) + part_bytes(*c, nt) + (n_seqs < kPlannedFew ? 0 : (size_t)(n_seqs + 1) * sizeof(int2));
 }
 
 pf_status pf_paged_attention(const pf_paged_cache* c, int32_t layer, const void* q, int64_t q_stride, void* out,

@@ -18,38 +18,10 @@ namespace pf {
 
 namespace {
 
-constexpr int kDecide = 1024;   // threads of the deciding CTA
 constexpr int kPerThread = 64;  // pages a thread takes at once at most (one bit each)
 constexpr int kCopy = 256;      // threads of a copying CTA
 constexpr int kMaxPages = 1 << 28, kMaxSeqs = 1 << 20;
 constexpr int kVecs = 4;        // 16-byte vectors a thread has in flight
-
-// Exclusive prefix sum over the CTA's 1,024 threads, and the total.
-__device__ __forceinline__ long long block_scan(long long v, long long* total, long long* s_warp) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    long long x = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-    }
-    if (lane == 31) s_warp[warp] = x;
-    __syncthreads();
-    if (warp == 0) {
-        long long w = s_warp[lane];
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long y = __shfl_up_sync(0xffffffffu, w, o);
-            if (lane >= o) w += y;
-        }
-        s_warp[lane] = w;
-    }
-    __syncthreads();
-    const long long before = warp ? s_warp[warp - 1] : 0;
-    *total = s_warp[31];
-    __syncthreads();  // s_warp is free for the next scan
-    return before + x - v;
-}
 
 // This thread's pages [first, first + count) of the chunk at `base`, as a mask
 // of those in use.

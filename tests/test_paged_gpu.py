@@ -435,6 +435,29 @@ def test_attention_scores_of_all_sizes():
             attend(c, t, 2, 3, 4, by=by)
 
 
+@pytest.mark.parametrize("n_seqs,heads,kv_heads,rows", [(95, 2, 1, 1), (96, 2, 1, 1), (159, 2, 2, 1), (160, 4, 4, 1), (500, 1, 1, 2),
+                                                        (1030, 1, 1, 1)])
+@pytest.mark.parametrize("cache,t", [(I8, F32), (BF16, BF16)])
+def test_attention_many_sequences(cache, t, n_seqs, heads, kv_heads, rows):
+    """As many as have their pieces planned by a launch of its own, and a few less; empty ones, long ones, one that is none."""
+    rng = random.Random(n_seqs)
+    lens = [rng.choice([0, 1, rng.randint(2, 60), rng.randint(60, 130)]) for _ in range(n_seqs)]
+    lens[0], lens[n_seqs // 2], lens[-1] = 3000, 700, 1900
+    c = Cache(cache, 1, kv_heads, 64, 16, sum(-(-n // 16) for n in lens), n_seqs, 200).place(lens)
+    work = c.work_for(n_seqs, 8, heads)
+    attend(c, t, n_seqs, rows, heads, work=work)
+    attend(c, t, 5, rows, heads, work=work)  # the same work for a few
+    attend(c, t, n_seqs, rows, heads, work=work, seed=9)
+    assert latched() == 0
+    c.lens[7] = 200 * 16 + 1
+    q = randn((n_seqs * rows, heads * 64), TYPES[t], 3)
+    out = torch.empty_like(q)
+    c.attend(0, q, out, t, n_seqs, rows, heads, 0.125, work)
+    assert latched() == 1
+    c.lens[7] = 0
+    check(out, c.attention(0, q, n_seqs, rows, heads, 0.125), TYPES[t])
+
+
 @pytest.mark.parametrize("rows", [1, 4])
 def test_attention_numbers_near_the_largest(rows):
     """fp32 queries and int8 scales of 2^112 and more: the powers of two that take them into fp16's range reach there."""
