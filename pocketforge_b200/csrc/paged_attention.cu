@@ -82,7 +82,7 @@ struct PagedParams {
     float scale;
     int ctas;      // that fit the GPU
     int* count;    // [kCounters] pieces of a cut segment that have ended
-    int2* plan;    // of many sequences: {pieces, most}, then each one's {pieces, chunks} before it; else null
+    int4* plan;    // of many sequences: {pieces, most}, then each piece's {sequence, which of its pieces, chunks before it, length}
     float* part;   // [piece of a cut segment][columns a row group][head_dim + 4]
     uint32_t* err;
 };
@@ -298,12 +298,13 @@ __global__ void __launch_bounds__(kDecide) plan_kernel(const PagedParams p, int 
     for (int b0 = 0; b0 < p.n_seqs; b0 += kDecide) {
         const int b = b0 + threadIdx.x, n = b < p.n_seqs ? chunks(b, nullptr) : 0;
         long long all;
-        const long long mine = n ? (((long long)cuts_of(n, most, inv) << 32) | n) * segs : 0;
-        const long long x = before + block_scan(mine, &all, s_scan);
-        if (n) p.plan[1 + b] = make_int2((int)(x >> 32), (int)x);
+        const int my_pieces = n ? cuts_of(n, most, inv) * segs : 0;
+        const long long x = before + block_scan(((long long)my_pieces << 32) | (n * segs), &all, s_scan);
+        const int len = n ? length_of(p, b, nullptr) : 0;
+        for (int i = 0; i < my_pieces; i++) p.plan[1 + (x >> 32) + i] = make_int4(b, i, (int)x, len);
         before += all;
     }
-    if (threadIdx.x == 0) p.plan[0] = make_int2((int)(before >> 32), most);
+    if (threadIdx.x == 0) p.plan[0] = make_int4((int)(before >> 32), most, 0, 0);
 }
 
 template <typename CT, int HD, int NT, int PLANES>
@@ -328,23 +329,11 @@ __global__ void __launch_bounds__(Ring<CT, HD, NT>::WARPS * 32, Ring<CT, HD, NT>
     after_previous();
     // ---- this CTA's piece ----  (the host has seen to it that all chunks count in 31 bits)
     if (warp == 0 && p.plan) {
-        const int2 all = p.plan[0];
-        const int x = (int)blockIdx.x;
-        int at = 0;
-        for (int n = x < all.x ? p.n_seqs : 0; n > 1;) {  // among n from `at` on: 32 at a time
-            const int step = (n + 31) / 32;
-            const bool le = lane * step < n && p.plan[1 + at + lane * step].x <= x;
-            const int k = __popc(__ballot_sync(0xffffffffu, le)) - 1;
-            at += k * step;
-            n = min(step, n - k * step);
-        }
         if (lane == 0) {
-            s_seq = x < all.x ? at : -1;
-            s_piece = x - p.plan[1 + at].x;
-            s_before = p.plan[1 + at].y;
-            s_len = length_of(p, at, nullptr);
-            s_cuts = cuts_of(chunks_of<R::CHUNK>(s_len), all.y, 1.0f / (float)all.y);
-            s_most = all.y;
+            const int4 all = p.plan[0], mine = p.plan[1 + blockIdx.x];  // (there is room for one a CTA)
+            s_seq = (int)blockIdx.x < all.x ? mine.x : -1;
+            s_piece = mine.y, s_before = mine.z, s_len = mine.w, s_most = all.y;
+            s_cuts = cuts_of(chunks_of<R::CHUNK>(mine.w), all.y, 1.0f / (float)all.y);
         }
     } else if (warp == 0) {
         int total = 0;
@@ -928,6 +917,11 @@ size_t part_bytes(const pf_paged_cache& c, int tiles) {
     return (size_t)(cta_limit(c) + 1) * 2 * 8 * tiles * (c.head_dim + 4) * sizeof(float);
 }
 
+size_t plan_bytes(const pf_paged_cache& c, int tiles, int n_seqs, int cols) {
+    const size_t segments = (size_t)n_seqs * c.n_kv_heads * ceil_div(cols, 8 * tiles);
+    return (1 + segments + cta_limit(c)) * sizeof(int4);
+}
+
 template <typename CT, int HD, int NT, int PLANES>
 pf_status launch_tiles(PagedParams& p, cudaStream_t st) {
     using R = Ring<CT, HD, NT>;
@@ -939,7 +933,7 @@ pf_status launch_tiles(PagedParams& p, cudaStream_t st) {
     const int64_t grid = std::min(segments * chunks, segments + p.ctas);
     PF_CHECK(2 * segments * chunks <= INT32_MAX, "pf_paged_attention: too many positions for one call");
     if (p.n_seqs >= (segments < few_segments(p.ctas) ? kPlannedFew : kPlanned))
-        p.plan = reinterpret_cast<int2*>(reinterpret_cast<char*>(p.part) + part_bytes(p.c, NT));
+        p.plan = reinterpret_cast<int4*>(reinterpret_cast<char*>(p.part) + part_bytes(p.c, NT));
     constexpr int SMEM = R::SMEM + (NT > 1 ? NT * PLANES * (HD / 32) * 512 + 8 * NT * 4 : 0);  // the ring; queries, where they are shared
     if (p.plan) PF_TRY(launch_after("paged_attention_plan", plan_kernel, dim3(1), kDecide, 0, st, p, R::CHUNK));
     static std::atomic<uint64_t> attr{0};
@@ -971,7 +965,7 @@ size_t pf_paged_attention_work_bytes(const pf_paged_cache* c, int32_t n_seqs, in
     if (!c || n_seqs < 0 || rows < 1 || rows > 8 || n_heads < 1 || c->n_kv_heads < 1 || n_heads % c->n_kv_heads) return 0;
     if (c->head_dim != 64 && c->head_dim != 128) return 0;
     const int nt = tiles_for(n_heads / c->n_kv_heads * rows, c->head_dim);
-    return kCounters * sizeof(int) + part_bytes(*c, nt) + (n_seqs < kPlannedFew ? 0 : (size_t)(n_seqs + 1) * sizeof(int2));
+    return kCounters * sizeof(int) + part_bytes(*c, nt) + (n_seqs < kPlannedFew ? 0 : plan_bytes(*c, nt, n_seqs, n_heads / c->n_kv_heads * rows));
 }
 
 pf_status pf_paged_attention(const pf_paged_cache* c, int32_t layer, const void* q, int64_t q_stride, void* out,
