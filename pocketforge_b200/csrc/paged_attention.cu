@@ -70,6 +70,7 @@ constexpr int kMaxCuts = 64;     // pieces of a segment: as many as one CTA join
 // look through them (bf16: 1,000 sequences of 50 to 200 tokens 314 and 121 us, 250 of them 49 and 35, 128 36.0 and 36.9; one kv
 // head's 128 of 500 to 1,500, where the pieces are tried out, 22.6 and 20.0, 64 of them 16.5 and 18.0).
 constexpr int kPlanned = 160, kPlannedFew = 96;
+constexpr int kWhole = 4;        // chunks that are not cut if no sequence has more: joining costs 2 us (4 x 300 entries: 5.5 and 7.2 us)
 constexpr int kCounters = 1024;  // at the start of `work`: seg_begin / P is below the CTAs that fit
 
 struct PagedParams {
@@ -87,9 +88,11 @@ struct PagedParams {
     uint32_t* err;
 };
 
-// CTAs that fit an SM, by the bytes of a stored row.  (More of them with shorter rings, where one column tile leaves the
-// registers, measured no faster: the warps that there are keep the loads going.)
-__host__ __device__ constexpr int ctas_per_sm(int row_bytes) { return row_bytes == 64 ? 4 : 2; }
+// CTAs that fit an SM, by the bytes of a stored row, its type and the column tiles.  (Three with rings of two blocks instead of
+// two of three, where the registers allow it: 1,000 sequences of 50 to 200 tokens 114 to 86 us, 16 of 8,000 49.1 to 48.2.)
+__host__ __device__ constexpr int ctas_per_sm(int row_bytes, bool i8, int tiles) {
+    return row_bytes == 64 ? 4 : (row_bytes == 128 && !i8 && tiles == 1 ? 3 : 2);
+}
 
 template <typename CT, int HD, int NT>
 struct Ring {
@@ -99,8 +102,8 @@ struct Ring {
     static constexpr int CHUNK = WARPS * BLOCK;                     // entries the CTA takes at a time
     static constexpr int SCALES = sizeof(CT) == 1 ? 2 * BLOCK * 4 : 0;
     static constexpr int BYTES = 2 * BLOCK * RB + SCALES;           // keys, values, scales of a block
-    static constexpr int CTAS = ctas_per_sm(RB);
-    static constexpr int STAGES = RB == 64 && NT == 1 ? 4 : 3;
+    static constexpr int CTAS = ctas_per_sm(RB, sizeof(CT) == 1, NT);
+    static constexpr int STAGES = RB == 64 && NT == 1 ? 4 : (CTAS == 3 ? 2 : 3);
     static constexpr int SMEM = WARPS * STAGES * BYTES;
 };
 
@@ -286,9 +289,14 @@ __global__ void __launch_bounds__(kDecide) plan_kernel(const PagedParams p, int 
     const int segs = p.c.n_kv_heads * p.row_groups;
     auto chunks = [&](int b, uint32_t* err) { return max((length_of(p, b, err) + chunk - 1) / chunk, 1); };
     int total = 0;
-    for (int b = threadIdx.x; b < p.n_seqs; b += kDecide) total += chunks(b, p.err);
+    bool long_one = false;
+    for (int b = threadIdx.x; b < p.n_seqs; b += kDecide) {
+        const int n = chunks(b, p.err);
+        total += n;
+        long_one |= n > kWhole;
+    }
     total = block_sum(total, s_sum) * segs;
-    const int most = piece_limit(total, p.n_seqs * segs, p.ctas, [&](int mine, float inv) {
+    const int most = !__syncthreads_or(long_one) ? kWhole : piece_limit(total, p.n_seqs * segs, p.ctas, [&](int mine, float inv) {
         int pieces = 0;
         for (int b = threadIdx.x; b < p.n_seqs; b += kDecide) pieces += cuts_of(chunks(b, nullptr), mine, inv);
         return block_sum(pieces, s_sum) * segs;
@@ -337,11 +345,18 @@ __global__ void __launch_bounds__(Ring<CT, HD, NT>::WARPS * 32, Ring<CT, HD, NT>
         }
     } else if (warp == 0) {
         int total = 0;
-        for (int b = lane; b < p.n_seqs; b += 32) total += chunks_of<R::CHUNK>(length_of(p, b, blockIdx.x == 0 ? p.err : nullptr));
+        bool long_one = false;
+        for (int b = lane; b < p.n_seqs; b += 32) {
+            const int n = chunks_of<R::CHUNK>(length_of(p, b, blockIdx.x == 0 ? p.err : nullptr));
+            total += n;
+            long_one |= n > kWhole;
+        }
         total = __reduce_add_sync(0xffffffffu, total) * segs;
         const int share = (total + p.ctas - 1) / p.ctas;
         int most = 2 * share;
-        if (p.n_seqs * segs < few_segments(p.ctas)) {  // as piece_limit, each lane trying one
+        if (!__any_sync(0xffffffffu, long_one)) {
+            most = kWhole;
+        } else if (p.n_seqs * segs < few_segments(p.ctas)) {  // as piece_limit, each lane trying one
             const int mine = share + lane * ((share + 31) / 32);
             const float inv = 1.0f / (float)mine;
             int pieces = 0;
@@ -910,23 +925,25 @@ int tiles_for(int cols, int head_dim) {
     return ceil_div(tiles, groups);
 }
 
-int cta_limit(const pf_paged_cache& c) { return 148 * ctas_per_sm(c.head_dim * type_bytes(c.dtype)); }
+int cta_limit(const pf_paged_cache& c, int tiles) {
+    return 148 * ctas_per_sm(c.head_dim * type_bytes(c.dtype), c.dtype == PF_I8, tiles);
+}
 
 // Of `work`: the counters, the pieces of cut segments, the plan.
 size_t part_bytes(const pf_paged_cache& c, int tiles) {
-    return (size_t)(cta_limit(c) + 1) * 2 * 8 * tiles * (c.head_dim + 4) * sizeof(float);
+    return (size_t)(cta_limit(c, tiles) + 1) * 2 * 8 * tiles * (c.head_dim + 4) * sizeof(float);
 }
 
 size_t plan_bytes(const pf_paged_cache& c, int tiles, int n_seqs, int cols) {
     const size_t segments = (size_t)n_seqs * c.n_kv_heads * ceil_div(cols, 8 * tiles);
-    return (1 + segments + cta_limit(c)) * sizeof(int4);
+    return (1 + segments + cta_limit(c, tiles)) * sizeof(int4);
 }
 
 template <typename CT, int HD, int NT, int PLANES>
 pf_status launch_tiles(PagedParams& p, cudaStream_t st) {
     using R = Ring<CT, HD, NT>;
     p.row_groups = ceil_div(p.cols, 8 * NT);
-    p.ctas = cta_limit(p.c);
+    p.ctas = cta_limit(p.c, NT);
     // segments, and with pieces of total / CTAs chunks or more no more than that many cuts
     const int64_t segments = (int64_t)p.n_seqs * p.c.n_kv_heads * p.row_groups;
     const int64_t chunks = std::max<int64_t>(((int64_t)p.c.max_pages * p.c.page_size + R::CHUNK - 1) / R::CHUNK, 1);
