@@ -280,8 +280,11 @@ PF_API pf_status pf_check_ordered_scan(const float* terms, int32_t rows, int32_t
  * copies a last, partly filled one.  A page id outside [0, n_pages), a length
  * outside [0, max_pages * page_size] or an offset out of order is not
  * followed: it latches bit 1 of pf_read_device_error and its row, entry or
- * page is left out.  k, v and work are 16-byte aligned.  Calls on one cache
- * are ordered by the caller (one stream, or events between streams). */
+ * page is left out (pf_paged_attention takes the positions of a page that is
+ * none as zeros).  k, v, the scales and work are 16-byte aligned.  Calls on one
+ * cache are ordered by the caller (one stream, or events between streams).  The
+ * first call on a device allocates the word that pf_read_device_error reads:
+ * make it before any stream capture. */
 enum { PF_F32 = 0, PF_BF16 = 1, PF_F16 = 2, PF_I8 = 3 };
 
 typedef struct pf_paged_cache {
@@ -323,7 +326,7 @@ PF_API pf_status pf_paged_free(const pf_paged_cache* c, const int32_t* seqs, int
  * copied, every layer, into the lowest free page.  A parent may be named many
  * times.  Children are empty, distinct, and no parents of the same call: one
  * that is not latches bit 1 and is left as it is; one for which no page is
- * free latches bit 8 and stays empty. */
+ * free latches bit 8 and stays empty.  65,535 children at most. */
 PF_API pf_status pf_paged_fork(const pf_paged_cache* c, const int32_t* parents, const int32_t* children, int32_t n,
                                void* stream);
 /* Copies n pages, every layer, with their scales: src[i] -> dst[i] (device
@@ -339,8 +342,10 @@ PF_API pf_status pf_paged_compact(const pf_paged_cache* c, void* stream);
  * (device array of n_seqs + 1, not decreasing) of k and v, each row
  * [n_kv_heads][head_dim] of `dtype` at k_stride / v_stride elements, are the
  * last positions of sequence b, whose length counts them already
- * (pf_paged_reserve).  n_tokens rows are there at all; those outside
- * [offsets[0], offsets[n_seqs]) are left out.  dtype: any of PF_F32, PF_BF16,
+ * (pf_paged_reserve).  n_tokens rows (2^30 at most) are there at all; those
+ * outside [offsets[0], offsets[n_seqs]) are left out.  Offsets that go back
+ * latch bit 1; the rows around them may be left out, or stand in places of
+ * their sequences that others belong in.  dtype: any of PF_F32, PF_BF16,
  * PF_F16 for a PF_I8 cache; PF_F32 or the cache's own for the others.  A row
  * with an infinity or NaN is stored in a PF_I8 cache with a NaN scale.  k, v
  * and the strides' bytes are multiples of 16. */

@@ -27,8 +27,8 @@
 // What bounds it (B200, measured): 8,192 tokens, 32 heads over 8, head_dim 128,
 // bf16: 550 GFLOP in 500 us, 1.10 PFLOP/s, 79% of what cuBLAS sustains under the
 // power cap (the tensor pipe is active in 65% of the cycles at 1.54 GHz: power is
-// part of it).  64 prompts of 33 to 1,024 tokens, head_dim 64: 153 us (163 with
-// one head a tile; 256 prompts of 5 to 40 tokens, 8 heads a kv head: 84 and 235;
+// part of it).  64 prompts of 33 to 1,024 tokens, head_dim 64: 151 us (163 with
+// one head a tile; 256 prompts of 5 to 40 tokens, 8 heads a kv head: 82 and 235;
 // 8,192 tokens: 500 and 496); half of
 // the products are in blocks on the diagonal or behind the end, the special-
 // function unit takes 2,048 of a block's 3,100 cycles, and each unit of three
