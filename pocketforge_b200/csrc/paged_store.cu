@@ -1,8 +1,8 @@
 // paged_store.cu — new keys and values into the pages of the paged cache.
 //
 // A row (token, kv head) is read once and written once: bound by HBM and the
-// quantising for a prompt (23,000 tokens of 8 heads, fp32 to int8: 140 MB in 34
-// us, 63% of the measured copy rate; bf16 to bf16 74%), by the chain of trips to
+// quantising for a prompt (23,000 tokens of 8 heads, fp32 to int8: 140 MB in 33
+// us, 65% of the measured copy rate; bf16 to bf16 74%), by the chain of trips to
 // memory (offsets, length, table, row) for a step (320 tokens: 3.3 us).  A CTA takes TOKENS tokens, as few as still fill the GPU; its warps
 // first find each one's sequence (a 32-way search of the offsets: two rounds up
 // to 1,024 sequences) and leave its place in shared memory, while the first

@@ -458,6 +458,27 @@ def test_attention_many_sequences(cache, t, n_seqs, heads, kv_heads, rows):
     check(out, c.attention(0, q, n_seqs, rows, heads, 0.125), TYPES[t])
 
 
+def test_attention_many_sequences_in_a_graph():
+    """The plan is made anew at every replay, on lengths that have changed, and again on another stream."""
+    n = 170
+    c = Cache(BF16, 1, 2, 64, 16, n * 12, n, 12).place([12 * 16] * n)
+    q = randn((n, 4 * 64), torch.bfloat16, 5)
+    out, work = torch.empty_like(q), c.work_for(n, 1, 4)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.attend(0, q, out, BF16, n, 1, 4, 0.125, work)
+    rng, other = random.Random(3), torch.cuda.Stream()
+    for most in (1, 60, 12 * 16):
+        c.lens.copy_(ints([rng.randint(0, most) for _ in range(n - 1)] + [12 * 16]))
+        out.fill_(7)
+        other.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(other if most == 60 else torch.cuda.current_stream()):
+            for _ in range(3):
+                graph.replay()
+        torch.cuda.synchronize()
+        check(out, c.attention(0, q, n, 1, 4, 0.125), torch.bfloat16)
+
+
 @pytest.mark.parametrize("rows", [1, 4])
 def test_attention_numbers_near_the_largest(rows):
     """fp32 queries and int8 scales of 2^112 and more: the powers of two that take them into fp16's range reach there."""
