@@ -44,12 +44,21 @@
 // Accuracy.  int8 codes are exact in fp16, and fp32 queries are split into two
 // fp16 planes (22 bits) after a power of two takes the row's largest value to
 // 2^13..2^14.  Over an int8 cache weights are two fp16 planes as well; they take
-// the entry's scale, and a power of two that keeps a block's largest below 2^15.
+// the entry's scale, and a power of two that keeps a block's largest at or below 2^15.
 // Over a 16-bit cache weights are rounded to its type (both operands of a
 // product have one type), an error like the output's own rounding; a second
-// plane would turn an inf among the values into NaN.  A block's products
-// start from zero and are added to O in fp32 with rounding, as the tensor cores
-// cut sums off instead, which would add up over a long cache.
+// plane would turn an inf among the values into NaN.  fp16 ends at 2^-24, and a
+// long row's many weights below that can be its answer where the largest ones
+// meet small values.  So the largest weights are taken to the end of fp16's range
+// (LIFT, or the scales' power of two), and the maximum that exponents refer to
+// rises as soon as it is exceeded by 2^6: a weight is off by 2^-34 of the row's
+// largest at most beside its rounding, over an int8 cache by 2^-33 of the largest
+// times its block's largest scale (2^-26 where that has come down to 2^-7 of an
+// earlier block's).  Rising from 2^2 on keeps four bits more but took 64 sequences
+// with 5 rows from 35.2 to 38.8 us (int8) and 51.1 to 58.7 (fp16, head_dim 128);
+// 2^6: 35.5 and 51.2.  bf16 has fp32's range: 2^8.  A block's products start from
+// zero and are added to O in fp32 with rounding, as the tensor cores cut sums off
+// instead, which would add up over a long cache.
 //
 // A row sees nothing behind its own position: those entries' weights are 0 by
 // selection, entries behind the sequence's end are zeros in shared memory, and
@@ -324,6 +333,8 @@ __global__ void __launch_bounds__(Ring<CT, HD, NT>::WARPS * 32, Ring<CT, HD, NT>
     constexpr int MT = HD / 16;        // 16-dim tiles of the output
     constexpr int COLS = 8 * NT;
     constexpr int VP = I8 ? 2 : 1;     // planes of a weight
+    // Weights are 2^(LIFT + x) with x <= RISE; at most 2^15 in fp16, where int8 rows' scales take what a LIFT would.
+    constexpr int RISE = BF ? 8 : 6, LIFT = BF || I8 ? 0 : 15 - RISE, TOP_SCALE = 15 - RISE;
     // Queries in shared memory where the registers they would take are the warps' that an SM could hold (64 sequences of 5
     // fp32 rows: 41.3 us in registers, 35.4; 64 of 5 fp16 rows, head_dim 128: 81 with two tiles and twice the reading, 60
     // with three).  16-bit ones of two tiles, or at head_dim 64, were 2 to 6% slower so.
@@ -556,7 +567,7 @@ __global__ void __launch_bounds__(Ring<CT, HD, NT>::WARPS * 32, Ring<CT, HD, NT>
         }
 
     // ---- running softmax ----
-    // Maxima as their negatives, 0 as long as there is none (`above`, the exponent that calls for a new one, is -inf then).
+    // LIFT minus the maxima, 0 as long as there is none (`above`, the exponent that calls for a new one, is -inf then).
     float o[MT][NT][4], minus_m[NT][2], above[NT][2], l[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
@@ -639,7 +650,7 @@ __global__ void __launch_bounds__(Ring<CT, HD, NT>::WARPS * 32, Ring<CT, HD, NT>
                 }
             }
         }
-        // exponents against the maxima so far; does any lie 2^8 above?
+        // exponents against the maxima so far; does any lie RISE above?
         const bool tail = e0 + kBlock > sees_all;  // some entry is not seen by every column
         bool rise = false;
         float ks[HALVES][2];
@@ -688,10 +699,10 @@ __global__ void __launch_bounds__(Ring<CT, HD, NT>::WARPS * 32, Ring<CT, HD, NT>
                     for (int x = 4; x <= 16; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
                     // no other column has a say: a row stays the same whatever its neighbours are
                     const bool none = above[nt][i] == -INFINITY;
-                    if (none ? top > -INFINITY : top + minus_m[nt][i] > 8.0f) {
-                        const float f = none ? 0.0f : exp2_approx(-minus_m[nt][i] - top);
-                        minus_m[nt][i] = -top;
-                        above[nt][i] = 8.0f;
+                    if (none ? top > -INFINITY : top + minus_m[nt][i] > LIFT + RISE) {
+                        const float f = none ? 0.0f : exp2_approx(LIFT - minus_m[nt][i] - top);
+                        minus_m[nt][i] = LIFT - top;
+                        above[nt][i] = LIFT + RISE;
                         l[nt][i] *= f;
                         if (!none)
 #pragma unroll
@@ -700,13 +711,14 @@ __global__ void __launch_bounds__(Ring<CT, HD, NT>::WARPS * 32, Ring<CT, HD, NT>
                 }
         }
         // weights
-        // int8: 2^up takes the block's largest finite scale to 1 .. 2^7, so that p v_scale 2^up < 2^15 (p <= 2^8); the one
-        // before is kept while it does.
+        // int8: 2^up takes the block's largest finite scale to 2^(TOP_SCALE - 1) .., so that p v_scale 2^up < 2^15 (p <= 2^RISE);
+        // the one before is kept while it is below 2^TOP_SCALE and not below 2^-7 of that.
         if constexpr (I8) {
             const float inf = __int_as_float(0x7f800000), vs = fabsf(scales[kBlock + lane]), x = vs * vscale;
-            if (__any_sync(0xffffffffu, x >= 128.0f && vs < inf) || !__any_sync(0xffffffffu, x >= 1.0f && x < inf)) {
+            constexpr float TOP = 1 << TOP_SCALE, LOW = TOP / 128;
+            if (__any_sync(0xffffffffu, x >= TOP && vs < inf) || !__any_sync(0xffffffffu, x >= LOW && x < inf)) {
                 const unsigned big = __reduce_max_sync(0xffffffffu, vs < inf ? __float_as_uint(vs) : 0u);
-                const int up = min(6 - exponent_of(__uint_as_float(big)), 100);  // -121 at least
+                const int up = min(TOP_SCALE - 1 - exponent_of(__uint_as_float(big)), 100);  // -121 at least
                 vscale = power_of_two(up), back = power_of_two(-up);
             }
         }

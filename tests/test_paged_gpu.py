@@ -665,6 +665,89 @@ def test_attention_answers_do_not_depend_on_the_run():
         assert torch.equal(out, first)
 
 
+def one_dim_keys(c, n, nats):
+    """Sequence 0's keys have one dim other than 0, and queries of 8 there score `nats[j]` over key j at scale 1/8."""
+    page, slot = c.table[0, torch.arange(n, device="cuda") // c.page].long(), torch.arange(n, device="cuda") % c.page
+    c.k.zero_()
+    if c.ks is None:
+        c.k[page, 0, :, slot, 0] = nats.to(c.k.dtype)[:, None]
+        return page, slot, c.k[page, 0, 0, slot, 0].double()
+    c.k[page, 0, :, slot, 0] = (127 * nats.sign()).to(torch.int8)[:, None]
+    c.ks[page, 0, :, slot] = (nats.abs() / 127)[:, None]
+    return page, slot, c.ks[page, 0, 0, slot].double() * c.k[page, 0, 0, slot, 0].double()
+
+
+@pytest.mark.parametrize("dim,rows", [(64, 1), (64, 3), (128, 1), (128, 5)])
+@pytest.mark.parametrize("cache", [F16, BF16])
+@pytest.mark.parametrize("at,nats", [(0, 17.4), (0, 18.0), (40_000, 17.4), (65_529, 21.0), (0, 4.0)])
+def test_attention_one_key_takes_nearly_all(cache, dim, rows, at, nats):
+    """A key far above 65,535 others whose values are all that comes out: each weight is far below fp16's range beside the
+    largest one, and together they are the answer."""
+    n = 65_536
+    c = Cache(cache, 1, 1, dim, 64, 1024, 1, 1024).place([n])
+    scores = torch.zeros(n, device="cuda")
+    scores[at] = nats
+    page, slot, s = one_dim_keys(c, n, scores)
+    c.v.copy_(torch.rand(c.v.shape, generator=torch.Generator("cuda").manual_seed(5), device="cuda") * 0.5 + 0.5)
+    c.v[page[at], 0, 0, slot[at]] = 0
+    q = torch.zeros(rows, 2 * dim, dtype=TYPES[cache], device="cuda")
+    q[:, 0] = q[:, dim] = 8
+    out = torch.empty_like(q)
+    c.attend(0, q, out, cache, 1, rows, 2, 0.125)
+    torch.cuda.synchronize()
+    v = c.v[page, 0, 0, slot].double()
+    # a weight and the output are rounded to the type (eps / 2 each; fp16 weights are 2^9 times what they are to the largest, so
+    # those too small for its normal numbers are off by 2^-34 of it); 2^-16 of a weight for its score, which has one product
+    # (31 x 2^-24 in each of four roundings at most), the exponential and the sums; fp16 outputs below 2^-14 are off by 2^-25
+    half = torch.finfo(TYPES[cache]).eps / 2
+    for r in range(rows):
+        m = n - rows + 1 + r
+        want = ph.softmax_mean(s[:m], v[:m])
+        for h in range(2):
+            got = out[r, h * dim:(h + 1) * dim].double()
+            tol = (2 * half + 2.0 ** -16) * want + (2.0 ** -25 + m * 2.0 ** -34 if cache == F16 else 0.0)
+            assert ((got - want).abs() <= tol).all(), ((got - want).abs() / want).max()
+
+
+@pytest.mark.parametrize("cache,t,dim", [(F16, F16, 64), (F16, F16, 128), (BF16, BF16, 64), (I8, F32, 64), (I8, F32, 128),
+                                         (I8, F16, 64)])
+@pytest.mark.parametrize("rows", [1, 3])
+@pytest.mark.parametrize("nats", [16.4, 21.2])
+def test_attention_a_few_keys_take_nearly_all_of_long_ones(cache, t, dim, rows, nats):
+    """The same where a warp walks over a third or a quarter of a whole sequence: as many segments as CTAs, none of them cut,
+    and keys far above the others among the first ones of every warp."""
+    n, seqs, kv_heads = 65_536, 64, 8
+    c = Cache(cache, 1, kv_heads, dim, 64, 1024, seqs, 1024).place([n])
+    c.table.copy_(c.table[:1].expand(seqs, 1024).contiguous())  # every sequence has the same pages
+    c.lens.fill_(n)
+    scores, high = torch.full((n,), -1.0, device="cuda"), torch.tensor([0, 16, 32, 48, 64, 96], device="cuda")
+    scores[high] = nats
+    page, slot, s = one_dim_keys(c, n, scores)
+    if cache == I8:
+        c.v.fill_(100)
+        c.vs.fill_(0.0123)
+    else:
+        c.v.fill_(0.75)
+    c.v[page[high], 0, :, slot[high]] = 0
+    q = torch.zeros(seqs * rows, kv_heads * dim, dtype=TYPES[t], device="cuda")
+    q[:, ::dim] = 8
+    out = torch.empty_like(q)
+    c.attend(0, q, out, t, seqs, rows, kv_heads, 0.125)
+    torch.cuda.synchronize()
+    v = c.v[page, 0, 0, slot, 0].double() * (c.vs[page, 0, 0, slot].double() if cache == I8 else 1)
+    # beside the weights' and the output's rounding: fp16 weights too small for its normal numbers are off by 2^-34 of the
+    # largest, int8 ones (with their scales, all alike) by 2^-33, and there are six of the largest.  2^-15 of a weight for its
+    # score (23 x 1.44 x 2^-24 in each of four roundings), exponential and sums
+    half = torch.finfo(TYPES[t]).eps / 2
+    for r in range(rows):
+        m = n - rows + 1 + r
+        want = ph.softmax_mean(s[:m], v[:m, None])
+        got = out.view(seqs, rows, -1)[:, r].double()
+        tol = (2.0 ** -15 + half) * want + (2.0 ** -25 if t == F16 else 0.0)
+        tol += m / 6 * v.max() * {I8: 2.0 ** -33, F16: 2.0 ** -34, BF16: 0.0}[cache] + (half * want if cache != I8 else 0.0)
+        assert ((got - want).abs() <= tol).all(), ((got - want).abs() / tol).max()
+
+
 # ---------------------------------------------------------------------------
 # Prompt attention
 # ---------------------------------------------------------------------------
