@@ -41,11 +41,15 @@
 // (524), turns at the special-function unit (515).
 //
 // The maximum that the exponents refer to rises only when a block exceeds it
-// by 2^8, so O (in TMEM) is rescaled rarely: p stays below 2^8, within fp16,
-// and the row sum takes the same p.
+// by 2^8 (fp16: 2^6), so O (in TMEM) is rescaled rarely, and the row sum takes the
+// same p.
 //
 // Rounding: scores, maxima, sums and O are fp32.  P is rounded to the inputs'
-// 16-bit type, which the tensor core asks for (both operands of one type).
+// 16-bit type, which the tensor core asks for (both operands of one type).  fp16
+// ends at 2^-24, and a long row's many p below that can be its answer where the
+// largest ones meet small values: p is taken 2^9 times, so that the largest are at
+// the end of fp16's range (2^15), and is off by 2^-34 of the row's largest at most
+// beside its rounding.
 //
 // What a row must not see: scores behind the row itself are -inf, their p is 0.
 // But 0 x inf = NaN, so V rows behind the sequence's end (another sequence's)
@@ -724,14 +728,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t ts = tmem + lanes + Ly::S + s * 128, tp = tmem + lanes + Ly::P + s * Ly::P_STEP,
                        to = tmem + lanes + Ly::O + s * HD;
         const float c = p.scale * 1.4426950408889634f;  // log2 e
+        constexpr float RISE = BF ? 8.0f : 6.0f, LIFT = BF ? 0.0f : 15.0f - RISE;  // p = 2^(LIFT + x) with x <= RISE
         uint32_t cs = 0;  // blocks of this side
-        float m = -INFINITY, off = 0.0f, l = 0.0f;  // maximum that exponents refer to, -c m, row sum
+        float m = -INFINITY, off = 0.0f, l = 0.0f;  // maximum that exponents refer to, LIFT - c m, row sum
         auto wait_all = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
         // A higher maximum: l and, where there is one, O scaled down to it.
         auto raise = [&](float to_m, bool scale_o) {
             const float f = to_m == m ? 1.0f : ex2((m - to_m) * c);
             m = to_m;
-            off = m == -INFINITY ? 0.0f : -m * c;
+            off = m == -INFINITY ? 0.0f : BF ? -m * c : fmaf(-m, c, LIFT);
             l *= f;
             if (!scale_o) return;
 #pragma unroll 1
@@ -790,7 +795,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if ((end >> 5) + q / 32 < 4) r[q] = 0xff800000u;
                 }
                 const float top = row_max<128>(r);
-                const bool rise = (top - m) * c > 8.0f;  // true of a first block that has a score
+                const bool rise = (top - m) * c > RISE;  // true of a first block that has a score
                 const bool any_rise = __any_sync(0xffffffffu, rise);
                 // P's columns (head_dim 64) and O are free once the product before is done
                 if (j > 0 && (Ly::OWN_P || any_rise)) {

@@ -899,6 +899,32 @@ def test_prompt_infinity_at_the_end_of_a_long_one():
                     (q[i].double().abs() @ k[:i + 1].double().abs().T * dim ** -0.5).amax().view(1, 1, 1)), torch.bfloat16)
 
 
+@pytest.mark.parametrize("t,dim,heads", [(F16, 64, 1), (F16, 64, 2), (F16, 128, 1), (BF16, 64, 1), (BF16, 128, 2)])
+@pytest.mark.parametrize("at,nats", [(0, 17.4), (200, 18.0), (0, 4.0)])
+def test_prompt_one_key_takes_nearly_all(t, dim, heads, at, nats):
+    """A key far above all others whose values are all that comes out of the rows that see it."""
+    n = 65_536
+    q = torch.zeros(n, heads * dim, dtype=TYPES[t], device="cuda")
+    q.view(n, heads, dim)[:, :, 0] = 8
+    k = torch.zeros(n, dim, dtype=TYPES[t], device="cuda")
+    k[at, 0] = nats
+    v = (torch.rand(n, dim, generator=torch.Generator("cuda").manual_seed(5), device="cuda") * 0.5 + 0.5).to(TYPES[t])
+    v[at] = 0
+    out = torch.empty_like(q)
+    ok("pf_prompt_attention", q.data_ptr(), q.stride(0), k.data_ptr(), dim, v.data_ptr(), dim, out.data_ptr(), out.stride(0),
+       t, ints([0, n]).data_ptr(), 1, n, heads, 1, dim, 0.125, ph.stream())
+    torch.cuda.synchronize()
+    # a weight and the output are rounded to the type, and each of a row's products of 16 keys is added to 24 bits and may be
+    # cut there (4,096 x 2^-23); scores and exponentials, and what is below fp16's normal numbers, as in the paged attention's
+    half = torch.finfo(TYPES[t]).eps / 2
+    for i in (300, 5_000, 33_333, n - 1):
+        want = ph.softmax_mean(k[:i + 1, 0].double(), v[:i + 1].double())
+        for h in range(heads):
+            got = out[i, h * dim:(h + 1) * dim].double()
+            tol = (2 * half + 2.0 ** -11 + 2.0 ** -16) * want + (2.0 ** -25 + i * 2.0 ** -34 if t == F16 else 0.0)
+            assert ((got - want).abs() <= tol).all(), (i, ((got - want).abs() / want).max())
+
+
 def test_prompt_many_sequences():
     rng = random.Random(2)
     run_prompt(BF16, 64, 2, 1, [rng.choice([0, 1, 2, 3, 9]) for _ in range(1500)])
