@@ -276,15 +276,20 @@ PF_API pf_status pf_check_ordered_scan(const float* terms, int32_t rows, int32_t
  *
  * To begin with, refs and lens are zero (the table's contents do not matter).
  * Position p of sequence b is slot p % page_size of page
- * table[b][p / page_size].  Only full pages are ever shared: pf_paged_fork
- * copies a last, partly filled one.  A page id outside [0, n_pages), a length
- * outside [0, max_pages * page_size] or an offset out of order is not
- * followed: it latches bit 1 of pf_read_device_error and its row, entry or
- * page is left out (pf_paged_attention takes the positions of a page that is
- * none as zeros).  k, v, the scales and work are 16-byte aligned.  Calls on one
- * cache are ordered by the caller (one stream, or events between streams).  The
- * first call on a device allocates the word that pf_read_device_error reads:
- * make it before any stream capture. */
+ * table[b][p / page_size]; -1 stands behind its last page.  Only full pages are
+ * ever shared: pf_paged_fork copies a last, partly filled one.  The caller may
+ * lower a length between calls, to 1 at least, and so give back tokens (a verify
+ * step's rejected drafts): the sequence keeps its pages, pf_paged_reserve fills
+ * them again before it takes others, and pf_paged_free frees them all.  lens,
+ * table and refs are otherwise the operations' own.
+ * A page id outside [0, n_pages), a length outside [0, max_pages * page_size] or
+ * an offset out of order is not followed: it latches bit 1 of
+ * pf_read_device_error and its row, entry or page is left out
+ * (pf_paged_attention takes the positions of a page that is none as zeros).  k,
+ * v, the scales and work are 16-byte aligned.  Calls on one cache are ordered by
+ * the caller (one stream, or events between streams).  The first call on a
+ * device allocates the word that pf_read_device_error reads: make it before any
+ * stream capture. */
 enum { PF_F32 = 0, PF_BF16 = 1, PF_F16 = 2, PF_I8 = 3 };
 
 typedef struct pf_paged_cache {

@@ -19,7 +19,7 @@ struct PageWork {
     int* dst;      // [n_pages]
     int* remap;    // [n_pages] new place of a moved page
     int* mark;     // [max_seqs] first list index that names the sequence
-    int4* plan;    // [max_seqs] per list index: pages asked for before it; of a fork, {fresh page, parent's page, length}
+    int4* plan;    // [max_seqs] per list index: {pages asked for before it, its own, held}; of a fork, {fresh page, parent's page, length}
 };
 __host__ __device__ inline PageWork page_work(const pf_paged_cache& c) {
     int* w = reinterpret_cast<int*>(c.work);

@@ -73,22 +73,33 @@ __device__ __forceinline__ void mark_first(const pf_paged_cache& c, const int* l
     __syncthreads();
 }
 
-// Pages that entry i of a reserve asks for; -1: refused (bit latched by the caller's second look).
-__device__ __forceinline__ int reserve_need(const pf_paged_cache& c, const PageWork& w, const int* seqs,
-                                            const int* counts, int i, uint32_t* err) {
+// Pages that sequence s of length n holds: those its length asks for, and behind them what it has taken for tokens that its
+// owner has given back since by a lower length.  Every operation that adds pages leaves -1 behind the last one.
+__device__ __forceinline__ int held_pages(const pf_paged_cache& c, int s, int n) {
+    int held = (int)(((int64_t)n + c.page_size - 1) / c.page_size);
+    if (n)
+        while (held < c.max_pages && in_range(c.table[(int64_t)s * c.max_pages + held], c.n_pages)) held++;
+    return held;
+}
+
+// {pages that entry i of a reserve asks for, pages that its sequence holds}; -1: refused (bit latched by the caller's second
+// look).
+__device__ __forceinline__ int2 reserve_need(const pf_paged_cache& c, const PageWork& w, const int* seqs,
+                                             const int* counts, int i, uint32_t* err) {
     const int s = seqs[i];
     if (!in_range(s, c.max_seqs) || w.mark[s] != i || counts[i] < 0) {
         latch(err, ERR_BOUNDS);
-        return -1;
+        return make_int2(-1, 0);
     }
     const int n = seq_len(c, s, err);
-    if (n < 0) return -1;
+    if (n < 0) return make_int2(-1, 0);
     const int64_t pages = ((int64_t)n + counts[i] + c.page_size - 1) / c.page_size;
     if (pages > c.max_pages) {
         latch(err, ERR_CONTEXT);
-        return -1;
+        return make_int2(-1, 0);
     }
-    return (int)(pages - (n + (int64_t)c.page_size - 1) / c.page_size);
+    const int held = held_pages(c, s, n);
+    return make_int2(max((int)pages - held, 0), held);
 }
 
 __global__ void __launch_bounds__(kDecide) reserve_kernel(const pf_paged_cache c, const int* seqs, const int* counts,
@@ -100,10 +111,10 @@ __global__ void __launch_bounds__(kDecide) reserve_kernel(const pf_paged_cache c
     long long want = 0;
     for (int base = 0; base < n; base += kDecide) {
         const int i = base + threadIdx.x;
-        const int need = i < n ? reserve_need(c, w, seqs, counts, i, err) : 0;
+        const int2 need = i < n ? reserve_need(c, w, seqs, counts, i, err) : make_int2(0, 0);
         long long total;
-        const long long before = want + block_scan(max(need, 0), &total, s_warp);
-        if (i < n) w.plan[i].x = need < 0 ? -1 : (int)min(before, (long long)INT_MAX);
+        const long long before = want + block_scan(max(need.x, 0), &total, s_warp);
+        if (i < n) w.plan[i] = make_int4(need.x < 0 ? -1 : (int)min(before, (long long)INT_MAX), need.x, need.y, 0);
         want += total;
     }
     const int found = want > 0 ? list_free(c, min(want, (long long)c.n_pages), w.src, s_warp) : 0;
@@ -111,21 +122,23 @@ __global__ void __launch_bounds__(kDecide) reserve_kernel(const pf_paged_cache c
     // one warp an entry: its pages are w.src[before .. before + need)
     const int lane = threadIdx.x & 31;
     for (int i = threadIdx.x >> 5; i < n; i += kDecide / 32) {
-        const int before = w.plan[i].x;
+        const int4 plan = w.plan[i];
+        const int before = plan.x, need = plan.y, held = plan.z;
         if (before < 0) continue;
-        const int s = seqs[i], len = c.lens[s], old = (len + c.page_size - 1) / c.page_size;
-        const int need = (int)(((int64_t)len + counts[i] + c.page_size - 1) / c.page_size) - old;
-        __syncwarp();  // every lane has read the length
+        const int s = seqs[i];
         if (need && (int64_t)before + need > found) {
             if (lane == 0) latch(err, ERR_CONTEXT);
             continue;
         }
         for (int j = lane; j < need; j += 32) {
             const int p = w.src[before + j];
-            c.table[(int64_t)s * c.max_pages + old + j] = p;
+            c.table[(int64_t)s * c.max_pages + held + j] = p;
             c.refs[p] = 1;
         }
-        if (lane == 0) c.lens[s] = len + counts[i];
+        if (lane == 0) {
+            if (need && held + need < c.max_pages) c.table[(int64_t)s * c.max_pages + held + need] = -1;
+            c.lens[s] += counts[i];
+        }
     }
 }
 
@@ -133,25 +146,34 @@ __global__ void __launch_bounds__(kDecide) reserve_kernel(const pf_paged_cache c
 // twice is freed once.
 __global__ void free_kernel(const pf_paged_cache c, const int* seqs, uint32_t* err) {
     after_previous();
-    __shared__ int s_len;
+    __shared__ int s_len, s_end;
     const int s = seqs[blockIdx.x];
     if (!in_range(s, c.max_seqs)) {
         if (threadIdx.x == 0) latch(err, ERR_BOUNDS);
         return;
     }
-    if (threadIdx.x == 0) s_len = atomicExch(&c.lens[s], 0);
+    if (threadIdx.x == 0) s_len = atomicExch(&c.lens[s], 0), s_end = INT_MAX;
     __syncthreads();
     if (s_len < 0 || s_len > (int64_t)c.max_pages * c.page_size) {
         if (threadIdx.x == 0) c.lens[s] = s_len, latch(err, ERR_BOUNDS);  // left as it is
         return;
     }
+    if (s_len == 0) return;
     const int pages = (int)(((int64_t)s_len + c.page_size - 1) / c.page_size);
-    for (int j = threadIdx.x; j < pages; j += blockDim.x) {
+    for (int j0 = 0;; j0 += blockDim.x) {  // up to the first entry behind the length that is no page (held_pages)
+        const int j = j0 + threadIdx.x;
         int* at = c.table + (int64_t)s * c.max_pages + j;
-        const int p = *at;
-        *at = -1;
-        if (in_range(p, c.n_pages)) atomicSub(&c.refs[p], 1);
-        else latch(err, ERR_BOUNDS);
+        const int p = j < c.max_pages ? *at : -1;
+        if (j >= pages && !in_range(p, c.n_pages)) atomicMin(&s_end, j);
+        __syncthreads();
+        const int end = s_end;
+        if (j < end) {
+            *at = -1;
+            if (in_range(p, c.n_pages)) atomicSub(&c.refs[p], 1);
+            else latch(err, ERR_BOUNDS);
+        }
+        if (end <= j0 + (int)blockDim.x) break;
+        __syncthreads();  // s_end has been read
     }
 }
 
@@ -226,6 +248,7 @@ __global__ void __launch_bounds__(kCopy) fork_copy_kernel(const pf_paged_cache c
         }
         if (threadIdx.x == 0) {
             if (rest) to[full] = fresh;
+            if (full + (rest > 0) < c.max_pages) to[full + (rest > 0)] = -1;
             c.lens[k] = len;
         }
     }
@@ -357,9 +380,12 @@ __global__ void __launch_bounds__(kCopy) compact_move_kernel(const pf_paged_cach
     for (int s = (int)(blockIdx.x * (kCopy / 32) + (threadIdx.x >> 5)); s < c.max_seqs; s += gridDim.x * (kCopy / 32)) {
         const int len = seq_len(c, s, err);
         const int pages = (int)(((int64_t)max(len, 0) + c.page_size - 1) / c.page_size);
-        for (int j = threadIdx.x & 31; j < pages; j += 32) {
+        for (int j = threadIdx.x & 31, end = 0; pages && !end; j += 32) {  // (and those held behind the length)
             int* at = c.table + (int64_t)s * c.max_pages + j;
-            const int p = *at;
+            const int p = j < c.max_pages ? *at : -1;
+            const unsigned ends = __ballot_sync(0xffffffffu, j >= pages && !in_range(p, c.n_pages));
+            end = ends != 0;
+            if (end && (threadIdx.x & 31) >= __ffs((int)ends) - 1) continue;
             if (!in_range(p, c.n_pages)) latch(err, ERR_BOUNDS);
             else if (p >= n_live) *at = w.remap[p];
         }

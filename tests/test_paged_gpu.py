@@ -234,6 +234,111 @@ def test_pages_free_leaves_a_length_that_is_none():
     assert c.lens.tolist() == [-7, 0, 65, 1] and c.refs.tolist() == refs and c.table.tolist() == table
 
 
+def test_pages_lengths_that_the_caller_lowers():
+    """Rejected tokens are given back by a lower length: the sequence keeps its pages for the next ones."""
+    c = Cache(I8, 1, 1, 64, 16, 12, 4, 4)
+    c.table.copy_(ints([[3, 7, 1, 9], [0, 0, 0, 0], [11, 10, 9, 8], [2, 4, 6, 8]]))  # contents do not matter
+    c.reserve([0], [14])
+    for _ in range(9):  # 5 tokens into the second page and 4 of them back
+        c.reserve([0], [5])
+        assert c.table[0, :2].tolist() == [0, 1] and int(c.refs.sum()) == 2
+        c.lens[0] -= 5
+        c.reserve([0], [1])
+        c.lens[0] -= 1
+    assert c.lens.tolist() == [14, 0, 0, 0] and c.refs.tolist() == [1, 1] + [0] * 10
+    c.reserve([0], [40])  # 54 tokens: two pages held, two more
+    assert c.table[0].tolist() == [0, 1, 2, 3]
+    c.lens[0] = 20  # pages 2 and 3 held behind the length, in a row that is full
+    c.fork([0], [1])  # the child has what the length counts
+    assert c.lens.tolist() == [20, 20, 0, 0] and c.refs.tolist() == [2, 1, 1, 1, 1] + [0] * 7
+    assert c.table[1, :2].tolist() == [0, 4]
+    c.free([1])
+    assert c.refs.tolist() == [1, 1, 1, 1] + [0] * 8
+    c.reserve([2, 3], [16, 17])  # pages 4, 5 and 6
+    c.free([2])
+    c.lens[3] = 3
+    c.compact()  # the page behind a length moves with the others
+    assert c.refs.tolist() == [1] * 6 + [0] * 6
+    assert c.table[0].tolist() == [0, 1, 2, 3] and c.table[3, :2].tolist() == [5, 4]
+    c.reserve([3], [20])
+    assert c.lens[3] == 23 and c.refs.tolist() == [1] * 6 + [0] * 6
+    c.free([0, 3])
+    assert c.lens.tolist() == [0, 0, 0, 0] and not c.refs.any()
+    assert c.table[0].tolist() == [-1] * 4 and c.table[3, :2].tolist() == [-1, -1]
+    assert latched() == 0
+
+
+class Held(Model):
+    """The model where a sequence may hold more pages than its length asks for."""
+
+    def reserve(self, seqs, counts):
+        asked, free, flags = 0, [i for i, r in enumerate(self.refs) if r == 0], 0
+        for s, n in zip(seqs, counts):
+            total = -(-(self.lens[s] + n) // self.c.page)
+            if total > self.c.max_pages:
+                flags |= 8
+                continue
+            need = max(total - len(self.table[s]), 0)
+            mine = free[asked:asked + need]
+            asked += need
+            if len(mine) < need:
+                flags |= 8
+                continue
+            for p in mine:
+                self.refs[p] = 1
+            self.table[s] += mine
+            self.lens[s] += n
+        return flags
+
+    def fork(self, parents, children):
+        held = {p: self.table[p] for p in parents}
+        for p in held:
+            self.table[p] = held[p][:-(-self.lens[p] // self.c.page)]
+        flags = super().fork(parents, children)
+        for p in held:
+            self.table[p] = held[p]
+        return flags
+
+
+@pytest.mark.parametrize("dtype,layers,kv_heads,page,pages,seqs,max_pages", [(I8, 2, 2, 16, 60, 9, 7), (F16, 1, 1, 32, 900, 40, 300)])
+def test_pages_follow_the_model_with_lengths_lowered(dtype, layers, kv_heads, page, pages, seqs, max_pages):
+    """Random operations, some lengths lowered between them (never into a page that a fork has shared)."""
+    c = Cache(dtype, layers, kv_heads, 64, page, pages, seqs, max_pages)
+    m, rng = Held(c), random.Random(pages)
+    c.table.copy_(ints([[rng.randrange(pages) for _ in range(max_pages)] for _ in range(seqs)]))
+    for step in range(150):
+        used = [s for s in range(seqs) if m.lens[s]]
+        empty = [s for s in range(seqs) if not m.lens[s]]
+        op = rng.choice(["reserve", "reserve", "reserve", "lower", "lower", "fork", "fork", "free", "compact"])
+        flags = 0
+        if op == "reserve":
+            some = rng.sample(range(seqs), rng.randint(1, seqs))
+            counts = [rng.choice([0, 1, 5, page, rng.randint(0, 4 * page), rng.randint(0, max_pages * page)]) for _ in some]
+            c.reserve(some, counts)
+            flags = m.reserve(some, counts)
+        elif op == "lower" and used:
+            for s in rng.sample(used, rng.randint(1, len(used))):
+                shared = sum(m.refs[p] > 1 for p in m.table[s])
+                m.lens[s] = rng.randint(min(max(1, shared * page), m.lens[s]), m.lens[s])
+            c.lens.copy_(ints(m.lens))
+        elif op == "fork" and used and empty:
+            kids = rng.sample(empty, rng.randint(1, len(empty)))
+            par = [rng.choice(used) for _ in kids]
+            c.fork(par, kids)
+            flags = m.fork(par, kids)
+        elif op == "free" and used:
+            some = rng.sample(used, rng.randint(1, max(1, len(used) // 2)))
+            c.free(some)
+            m.free(some)
+        elif op == "compact":
+            c.compact()
+            m.compact()
+        m.same()
+        assert latched() == flags, (step, op)
+    c.free(list(range(seqs)))
+    assert not c.refs.any() and latched() == 0
+
+
 # ---------------------------------------------------------------------------
 # Store
 # ---------------------------------------------------------------------------
@@ -1056,3 +1161,48 @@ def test_a_run_of_them_together(cache, t, dim, page):
     feed([2, 3], [2 * page + 3, 1], 600)
     agree(3, 700)
     assert latched() == 0
+
+
+@pytest.mark.parametrize("cache,t", [(I8, F32), (BF16, BF16)])
+def test_verify_steps_that_give_tokens_back(cache, t):
+    """Steps of five tokens, captured once, of which the host takes back 0 to 4: the cache holds what was kept, attention is the
+    definition's, and no page is lost."""
+    heads, kv_heads, dim, page, n = 8, 2, 64, 16, 3
+    c = Cache(cache, 1, kv_heads, dim, page, 40, n + 1, 12)
+    c.table.fill_(3)
+    c.reserve([0, 1, 2], [30, 1, 16])
+    first = randn((47, kv_heads * dim), TYPES[t], 1)
+    c.store(0, first, first, [0, 30, 31, 47], t)
+    fed = [x.clone() for x in first.split([30, 1, 16])]
+    new, q = randn((5 * n, kv_heads * dim), TYPES[t], 2), randn((5 * n, heads * dim), TYPES[t], 3)
+    out, work, back = torch.empty_like(q), c.work_for(n, 5, heads), ints([0] * (n + 1))
+    seqs, five, off = ints([0, 1, 2]), ints([5] * n), ints([0, 5, 10, 15])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.lens.sub_(back)
+        ok("pf_paged_reserve", c.ref, seqs.data_ptr(), five.data_ptr(), n, ph.stream())
+        ok("pf_paged_store", c.ref, 0, new.data_ptr(), kv_heads * dim, new.data_ptr(), kv_heads * dim, t, off.data_ptr(), n, 5 * n,
+           ph.stream())
+        c.attend(0, q, out, t, n, 5, heads, 0.125, work)
+    rng = random.Random(4)
+    for step in range(25):
+        new.copy_(randn(new.shape, TYPES[t], 100 + step))
+        q.copy_(randn(q.shape, TYPES[t], 200 + step))
+        graph.replay()
+        torch.cuda.synchronize()
+        check(out, c.attention(0, q, n, 5, heads, 0.125), TYPES[t])
+        less = [rng.randint(0, 4) for _ in range(n)]
+        back.copy_(ints(less + [0]))
+        for b in range(n):
+            fed[b] = torch.cat([fed[b], new[5 * b:5 * b + 5]])
+            have = torch.cat([c.history(b, 0, g)[0] for g in range(kv_heads)], 1)
+            want = fed[b].double().view(-1, kv_heads, dim)
+            # int8: half a code of the row's largest value / 127, and the scale's and product's roundings
+            off_by = want.abs().amax(2, keepdim=True) / 127 * (0.5 + 2.0 ** -15) if cache == I8 else 0.0
+            assert ((have.view_as(want) - want).abs() <= off_by).all(), (step, b)
+            fed[b] = fed[b][:fed[b].shape[0] - less[b]]
+    most = c.lens.tolist()  # each step's last length is at least any before it
+    assert int(c.refs.sum()) == sum(-(-x // page) for x in most[:n])
+    c.free([0, 1, 2])
+    assert not c.refs.any() and latched() == 0
