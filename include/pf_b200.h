@@ -280,8 +280,9 @@ PF_API pf_status pf_check_ordered_scan(const float* terms, int32_t rows, int32_t
  * ever shared: pf_paged_fork copies a last, partly filled one.  The caller may
  * lower a length between calls, to 1 at least, and so give back tokens (a verify
  * step's rejected drafts): the sequence keeps its pages, pf_paged_reserve fills
- * them again before it takes others, and pf_paged_free frees them all.  lens,
- * table and refs are otherwise the operations' own.
+ * them again before it takes others, and pf_paged_free frees them all.  (Not
+ * into a page that a fork has shared: pf_paged_store does not write those.)
+ * lens, table and refs are otherwise the operations' own.
  * A page id outside [0, n_pages), a length outside [0, max_pages * page_size] or
  * an offset out of order is not followed: it latches bit 1 of
  * pf_read_device_error and its row, entry or page is left out
@@ -348,8 +349,12 @@ PF_API pf_status pf_paged_compact(const pf_paged_cache* c, void* stream);
  * [n_kv_heads][head_dim] of `dtype` at k_stride / v_stride elements, are the
  * last positions of sequence b, whose length counts them already
  * (pf_paged_reserve).  n_tokens rows (2^30 at most) are there at all; those
- * outside [offsets[0], offsets[n_seqs]) are left out.  Offsets that go back
- * latch bit 1; the rows around them may be left out, or stand in places of
+ * outside [offsets[0], offsets[n_seqs]) are left out.  A page that more than
+ * one sequence holds is never written: a row that would stand in one (its
+ * sequence was refused room, or its length lowered into a shared page) latches
+ * bit 1 and is left out.  After a refused reserve the caller leaves the sequence
+ * out: rows given for it would take the places of its last ones.  Offsets that
+ * go back latch bit 1; the rows around them may be left out, or stand in places of
  * their sequences that others belong in.  dtype: any of PF_F32, PF_BF16,
  * PF_F16 for a PF_I8 cache; PF_F32 or the cache's own for the others.  A row
  * with an infinity or NaN is stored in a PF_I8 cache with a NaN scale.  k, v

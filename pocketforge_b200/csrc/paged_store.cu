@@ -2,8 +2,9 @@
 //
 // A row (token, kv head) is read once and written once: bound by HBM and the
 // quantising for a prompt (23,000 tokens of 8 heads, fp32 to int8: 140 MB in 33
-// us, 65% of the measured copy rate; bf16 to bf16 74%), by the chain of trips to
-// memory (offsets, length, table, row) for a step (320 tokens: 3.3 us).  A CTA takes TOKENS tokens, as few as still fill the GPU; its warps
+// us, 65% of the measured copy rate; bf16 to bf16 73%), by the chain of trips to
+// memory (offsets, length, table, holders, row) for a step (320 tokens: 3.45 us).
+// A CTA takes TOKENS tokens, as few as still fill the GPU; its warps
 // first find each one's sequence (a 32-way search of the offsets: two rounds up
 // to 1,024 sequences) and leave its place in shared memory, while the first
 // rows are on their way.  Every group of head_dim / 8 lanes moves one row's key
@@ -169,7 +170,8 @@ __global__ void __launch_bounds__(kThreads) store_kernel(const pf_paged_cache c,
                     page = c.table[(int64_t)b * c.max_pages + pos / c.page_size];
                     slot = (int)(pos % c.page_size);
                 }
-                if ((unsigned)page >= (unsigned)c.n_pages) {
+                // (a page that others hold too is theirs as it is: the sequence got no room, or its length was lowered into it)
+                if ((unsigned)page >= (unsigned)c.n_pages || c.refs[page] > 1) {
                     page = -1;
                     latch(err, ERR_BOUNDS);
                 }

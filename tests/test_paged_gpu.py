@@ -339,6 +339,36 @@ def test_pages_follow_the_model_with_lengths_lowered(dtype, layers, kv_heads, pa
     assert not c.refs.any() and latched() == 0
 
 
+def test_store_does_not_write_a_shared_page():
+    """A sequence that got no room, or whose length was lowered into a page that a fork shares: bit 1, the page stays."""
+    for cache in (I8, F16):
+        c = Cache(cache, 1, 2, 64, 16, 4, 3, 4)
+        c.reserve([0, 1], [32, 32])
+        c.free([1])
+        c.fork([0], [1])
+        c.reserve([2], [32])
+        c.reserve([1], [1])
+        assert latched() == 8 and c.lens.tolist() == [32, 32, 32]
+        x = randn((2, 128), TYPES[F32], 3)
+        want = [t.clone() for t in (c.k, c.v)]
+        c.store(0, x, x, [0, 0, 1], F32)  # position 31 of a page that sequence 0 holds as well
+        assert latched() == 1
+        assert torch.equal(c.k, want[0]) and torch.equal(c.v, want[1])
+        c.lens[1] = 20
+        c.store(0, x, x, [0, 0, 2], F32)
+        assert latched() == 1
+        assert torch.equal(c.k, want[0]) and torch.equal(c.v, want[1])
+        c.free([0])  # now the pages are sequence 1's alone
+        c.store(0, x, x, [0, 0, 2], F32)
+        assert latched() == 0
+        page = int(c.table[1, 1])
+        if cache == F16:
+            assert torch.equal(c.k[page, 0, :, 2:4], x.half().view(2, 2, 64).transpose(0, 1))
+        else:
+            assert not torch.equal(c.k[page, 0, :, 2:4], want[0][page, 0, :, 2:4])
+        assert torch.equal(c.k[page, 0, :, 4:], want[0][page, 0, :, 4:])
+
+
 # ---------------------------------------------------------------------------
 # Store
 # ---------------------------------------------------------------------------
