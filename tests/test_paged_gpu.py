@@ -223,6 +223,18 @@ def test_pages_lists_that_are_wrong():
         ok("pf_paged_copy", c.ref, None, None, n, None)
 
 
+def test_pages_a_request_too_large():
+    """Pages are given out in the list's order: behind an entry for which they run out, only entries that need none are served."""
+    c = Cache(I8, 1, 1, 64, 16, 10, 5, 12)
+    c.reserve([4], [10])
+    c.reserve([0, 1, 4, 2], [10 * 16, 1, 6, 1])  # nine are free, the first asks for ten
+    assert latched() == 8
+    assert c.lens.tolist() == [0, 0, 0, 0, 16] and c.refs.tolist() == [1] + [0] * 9
+    c.reserve([0, 1, 2], [13 * 16, 1, 1])  # more than a sequence holds: takes no one's place
+    assert latched() == 8
+    assert c.lens.tolist() == [0, 1, 1, 0, 16] and c.table[1, 0] == 1 and c.table[2, 0] == 2
+
+
 def test_pages_free_leaves_a_length_that_is_none():
     c = Cache(I8, 1, 1, 64, 16, 12, 4, 4).place([20, 5, 64, 1])
     c.lens[0], c.lens[2] = -7, 65
