@@ -463,6 +463,26 @@ def test_store_halves_and_extremes():
     assert c.k[int(c.table[0, 0]), 0, 0, 0, :8].tolist() == [127, 1, -1, 2, -3, 127, 0, -127]
 
 
+@pytest.mark.parametrize("big", [5e-37, 2.0 ** -121, 1e-38, 3e-41, 1e-45])
+def test_store_rows_of_tiny_values(big):
+    """Rows whose 127 / largest passes fp32's range: the codes are those of the row times 2^64, the scale its own."""
+    one = np.float32(big)
+    parts = np.array([1, -1, 0, 0.5, -0.25, 0.9, -0.3, 0.004, 0.0039, -0.0], np.float32)
+    row = np.resize(parts, 64) * one
+    k = torch.from_numpy(np.stack([row, -row[::-1]])).cuda().contiguous()
+    c = Cache(I8, 1, 1, 64, 16, 2, 1, 2).place([2])
+    c.store(0, k, k, [0, 2], F32)
+    torch.cuda.synchronize()
+    page = int(c.table[0, 0])
+    for t in range(2):
+        x = k[t].cpu().numpy()
+        code, _ = store_codes(torch.from_numpy(x * np.float32(2.0 ** 64)))
+        assert np.abs(code).max() == 127
+        for codes, scales in ((c.k, c.ks), (c.v, c.vs)):
+            assert torch.equal(codes[page, 0, 0, t].cpu(), torch.from_numpy(code))
+            assert scales[page, 0, 0, t].cpu() == torch.tensor(np.abs(x).max() / np.float32(127))
+
+
 def test_store_leaves_out_what_has_no_place():
     c = Cache(F16, 1, 1, 64, 16, 8, 3, 2).place([16, 20, 4])
     c.table[1, 1] = 99  # no such page
