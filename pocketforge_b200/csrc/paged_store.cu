@@ -4,9 +4,11 @@
 // quantising for a prompt (23,000 tokens of 8 heads, fp32 to int8: 140 MB in 33
 // us, 65% of the measured copy rate; bf16 to bf16 73%), by the chain of trips to
 // memory (offsets, length, table, holders, row) for a step (320 tokens: 3.45 us).
-// A CTA takes TOKENS tokens, as few as still fill the GPU; its warps
-// first find each one's sequence (a 32-way search of the offsets: two rounds up
-// to 1,024 sequences) and leave its place in shared memory, while the first
+// A CTA takes TOKENS tokens, as few as still fill the GPU; one of its warps finds
+// their sequences (a 32-way search of the offsets for the first: two rounds up to
+// 1,024 sequences; each of the others from there in doubling steps, which a
+// million empty sequences between two tokens make 40 trips) and leaves their
+// places in shared memory, while the others look at the offsets and the first
 // rows are on their way.  Every group of head_dim / 8 lanes moves one row's key
 // and value, 8 elements a lane of each (two contiguous runs of 4 if they are fp32), the
 // row's largest value found by shuffles.  One row in flight a lane and more CTAs
@@ -20,6 +22,8 @@
 // step rounded to fp32; scale 1 for a row of zeros.  A row that holds an
 // infinity or NaN has no such scale: its scale is NaN, so that whatever reads
 // it is NaN too, and its codes are zero.
+#include <algorithm>
+
 #include "paged.cuh"
 
 namespace pf {
@@ -28,6 +32,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kElems = 8;  // elements a lane
+constexpr int kLook = kThreads - 32;  // threads of a CTA that look at the offsets' order
 
 // Number of entries of off[0 .. n) that are <= x (they do not decrease), by a whole warp.
 __device__ __forceinline__ int count_le(const int* off, int n, int x) {
@@ -157,11 +162,15 @@ __global__ void __launch_bounds__(kThreads) store_kernel(const pf_paged_cache c,
         }
     };
     if (u < rows) load();
-    if (threadIdx.x < 32) {  // one search for the first token; the others' sequences are close behind
-        int b = count_le(offsets, n_seqs + 1, t0) - 1;
+    if (threadIdx.x < 32) {  // one search for the first token; the others' sequences are close behind, or far behind empty ones
+        int b = tokens > 0 ? count_le(offsets, n_seqs + 1, t0) - 1 : 0;
         if (lane < tokens) {
             const int t = t0 + lane;
-            while (b < n_seqs && offsets[b + 1] <= t) b++;  // (b = -1: offsets[0] > t0)
+            auto begun = [&](int i) { return i <= n_seqs && offsets[i] <= t; };  // (b = -1: offsets[0] > t0)
+            int step = 1;
+            for (; begun(b + step); step *= 2) b += step;
+            while (step /= 2)
+                if (begun(b + step)) b += step;
             int page = -1, slot = 0;
             if (b >= 0 && b < n_seqs && offsets[b] <= t) {
                 const int n = seq_len(c, b, err);
@@ -178,8 +187,8 @@ __global__ void __launch_bounds__(kThreads) store_kernel(const pf_paged_cache c,
             }
             s_page[lane] = page, s_slot[lane] = slot;
         }
-    } else if (blockIdx.x == 0) {  // meanwhile one CTA looks at the offsets' order
-        for (int j = threadIdx.x - 32; j < n_seqs; j += kThreads - 32)
+    } else {  // meanwhile the other warps look at a share of the offsets' order
+        for (int64_t j = (int64_t)blockIdx.x * kLook + threadIdx.x - 32; j < n_seqs; j += (int64_t)gridDim.x * kLook)
             if (offsets[j] > offsets[j + 1]) latch(err, ERR_BOUNDS);
     }
     __syncthreads();
@@ -196,12 +205,14 @@ pf_status launch_store(const pf_paged_cache& c, int layer, const void* k, int64_
                        const int* offsets, int n_seqs, int n_tokens, cudaStream_t st) {
     uint32_t* err = device_error_flag();
     const ST *kp = static_cast<const ST*>(k), *vp = static_cast<const ST*>(v);
+    // CTAs behind the tokens', if there are very many sequences, only look at offsets: eight a thread
+    const int look = ceil_div(n_seqs, 8 * kLook);
     // 16 tokens a CTA share one round of searches; below four CTAs an SM the chain of a single round is what counts
     if (n_tokens >= 16 * 4 * 148)
-        return launch_after("paged_store", store_kernel<ST, CT, HD, 16>, dim3(ceil_div(n_tokens, 16)), kThreads, 0, st, c, layer, kp, ks,
-                            vp, vs, offsets, n_seqs, n_tokens, err);
-    return launch_after("paged_store", store_kernel<ST, CT, HD, 2>, dim3(ceil_div(n_tokens, 2)), kThreads, 0, st, c, layer, kp, ks, vp,
-                        vs, offsets, n_seqs, n_tokens, err);
+        return launch_after("paged_store", store_kernel<ST, CT, HD, 16>, dim3(std::max(ceil_div(n_tokens, 16), look)), kThreads, 0, st, c,
+                            layer, kp, ks, vp, vs, offsets, n_seqs, n_tokens, err);
+    return launch_after("paged_store", store_kernel<ST, CT, HD, 2>, dim3(std::max(ceil_div(n_tokens, 2), look)), kThreads, 0, st, c, layer,
+                        kp, ks, vp, vs, offsets, n_seqs, n_tokens, err);
 }
 
 template <typename ST, typename CT>

@@ -529,6 +529,44 @@ def test_store_many_sequences():
         at += n
 
 
+def elapsed(f):
+    f()
+    a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    a.record()
+    f()
+    b.record()
+    torch.cuda.synchronize()
+    return a.elapsed_time(b)
+
+
+def test_store_among_very_many_empty_sequences():
+    """Two tokens a million sequences apart: found by halving, not by a walk past each of them (30 ms)."""
+    n = 1 << 20
+    c = Cache(F16, 1, 1, 64, 16, 4, n, 1)
+    busy = [0, 5, n // 2, n - 1]
+    for i, b in enumerate(busy):
+        c.table[b, 0] = i
+        c.lens[b] = 3
+    c.refs.fill_(1)
+    new = torch.zeros(n + 1, dtype=torch.int32, device="cuda")
+    for b in busy:
+        new[b + 1:] += 1
+    x = randn((6, 64), torch.float16, 3)  # (rows behind the last sequence's stay out)
+    want = c.k.clone()
+    for i in range(4):
+        want[i, 0, 0, 2] = x[i]
+
+    def call():
+        ok("pf_paged_store", c.ref, 0, x.data_ptr(), 64, x.data_ptr(), 64, F16, new.data_ptr(), n, 6, ph.stream())
+
+    ms = elapsed(call)
+    assert torch.equal(c.k, want)
+    assert ms < 2.0, ms
+    new[n // 2 + 7] = 1  # goes back, far from any CTA's own tokens
+    call()
+    assert latched() == 1
+
+
 # ---------------------------------------------------------------------------
 # Attention over the cache
 # ---------------------------------------------------------------------------
