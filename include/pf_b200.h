@@ -343,7 +343,9 @@ PF_API pf_status pf_paged_copy(const pf_paged_cache* c, const int32_t* src, cons
                                void* stream);
 /* Moves the pages in use to the front of the cache: with n_live of them, the
  * i-th one (by index) at or behind n_live goes to the i-th free page before
- * it.  Tables and refs follow; the moved pages' old places are free. */
+ * it.  Tables and refs follow; the moved pages' old places are free.  Where
+ * pages move, a table entry that names a free page at or behind n_live latches
+ * bit 1 and stays. */
 PF_API pf_status pf_paged_compact(const pf_paged_cache* c, void* stream);
 
 /* Stores new keys and values of one layer.  Rows offsets[b] to offsets[b+1]

@@ -17,7 +17,7 @@ struct PageWork {
     int* n_live;   // pages in use (compaction)
     int* src;      // [n_pages]
     int* dst;      // [n_pages]
-    int* remap;    // [n_pages] new place of a moved page
+    int* remap;    // [n_pages] of those at n_live and behind: new place of a page in use, -1 of a free one
     int* mark;     // [max_seqs] first list index that names the sequence
     int4* plan;    // [max_seqs] per list index: {pages asked for before it, its own, held}; of a fork, {fresh page, parent's page, length}
 };

@@ -352,6 +352,8 @@ __global__ void __launch_bounds__(kDecide) compact_decide_kernel(const pf_paged_
         // pages before n_live count if free, those behind it if in use
         const int front = min(max(n_live - s.first, 0), s.count);
         unsigned long long hole = ~s.live & ones(front), mover = s.live & ~ones(front);
+        for (unsigned long long dead = ~s.live & ~ones(front) & ones(s.count); dead; dead &= dead - 1)
+            w.remap[s.first + __ffsll((long long)dead) - 1] = -1;  // a table that names it is wrong
         long long total;
         const long long before =
             block_scan(((long long)__popcll(hole) << 32) | __popcll(mover), &total, s_warp);
@@ -386,8 +388,9 @@ __global__ void __launch_bounds__(kCopy) compact_move_kernel(const pf_paged_cach
             const unsigned ends = __ballot_sync(0xffffffffu, j >= pages && !in_range(p, c.n_pages));
             end = ends != 0;
             if (end && (threadIdx.x & 31) >= __ffs((int)ends) - 1) continue;
-            if (!in_range(p, c.n_pages)) latch(err, ERR_BOUNDS);
-            else if (p >= n_live) *at = w.remap[p];
+            const int to = !in_range(p, c.n_pages) ? -1 : p < n_live ? p : w.remap[p];
+            if (to < 0) latch(err, ERR_BOUNDS);
+            else if (to != p) *at = to;
         }
     }
     copy_pages(c, w.src, w.dst, n, err);

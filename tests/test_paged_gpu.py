@@ -381,6 +381,18 @@ def test_store_does_not_write_a_shared_page():
         assert torch.equal(c.k[page, 0, :, 4:], want[0][page, 0, :, 4:])
 
 
+def test_pages_compact_and_a_page_that_no_one_holds():
+    """A table that names a free page behind those in use: bit 1, and the entry stays."""
+    c = Cache(I8, 1, 1, 64, 16, 12, 3, 4)
+    c.work.fill_(7)
+    c.reserve([0, 1, 2], [32, 32, 32])
+    c.free([0])
+    c.table[1, 1] = 9
+    c.compact()
+    assert latched() == 1
+    assert c.table[1, :2].tolist() == [2, 9] and c.table[2, :2].tolist() == [0, 1]
+
+
 # ---------------------------------------------------------------------------
 # Store
 # ---------------------------------------------------------------------------
