@@ -287,10 +287,10 @@ PF_API pf_status pf_check_ordered_scan(const float* terms, int32_t rows, int32_t
  * an offset out of order is not followed: it latches bit 1 of
  * pf_read_device_error and its row, entry or page is left out
  * (pf_paged_attention takes the positions of a page that is none as zeros).  k,
- * v, the scales and work are 16-byte aligned.  Calls on one cache are ordered by
- * the caller (one stream, or events between streams).  The first call on a
- * device allocates the word that pf_read_device_error reads: make it before any
- * stream capture. */
+ * v, the scales and work are 16-byte aligned, arrays of int32_t 4-byte aligned.
+ * Calls on one cache are ordered by the caller (one stream, or events between
+ * streams).  The first call on a device allocates the word that
+ * pf_read_device_error reads: make it before any stream capture. */
 enum { PF_F32 = 0, PF_BF16 = 1, PF_F16 = 2, PF_I8 = 3 };
 
 typedef struct pf_paged_cache {

@@ -417,6 +417,8 @@ pf_status check_paged_cache(const pf_paged_cache* c, const char* where, bool nee
     const uintptr_t all = (uintptr_t)c->k | (uintptr_t)c->v | (need_work ? (uintptr_t)c->work : 0) |
                           (c->dtype == PF_I8 ? (uintptr_t)c->k_scale | (uintptr_t)c->v_scale : 0);
     PF_CHECK(all % 16 == 0, "%s: k, v, scales and work must be 16-byte aligned", where);
+    PF_CHECK(((uintptr_t)c->table | (uintptr_t)c->lens | (uintptr_t)c->refs) % 4 == 0,
+             "%s: table, lens and refs must be 4-byte aligned", where);
     return PF_OK;
 }
 
@@ -435,6 +437,7 @@ pf_status pf_paged_reserve(const pf_paged_cache* c, const int32_t* seqs, const i
                            void* stream) {
     PF_TRY(check_paged_cache(c, "pf_paged_reserve", true));
     PF_CHECK(n >= 0 && n <= c->max_seqs, "pf_paged_reserve: %d sequences of %d", n, c->max_seqs);
+    PF_CHECK(((uintptr_t)seqs | (uintptr_t)counts) % 4 == 0, "pf_paged_reserve: seqs and counts must be 4-byte aligned");
     PF_TRY(require_device());
     if (n == 0) return PF_OK;
     PF_CHECK(seqs && counts, "pf_paged_reserve: null argument");
@@ -444,6 +447,7 @@ pf_status pf_paged_reserve(const pf_paged_cache* c, const int32_t* seqs, const i
 pf_status pf_paged_free(const pf_paged_cache* c, const int32_t* seqs, int32_t n, void* stream) {
     PF_TRY(check_paged_cache(c, "pf_paged_free", false));
     PF_CHECK(n >= 0 && n <= c->max_seqs, "pf_paged_free: %d sequences of %d", n, c->max_seqs);
+    PF_CHECK((uintptr_t)seqs % 4 == 0, "pf_paged_free: seqs must be 4-byte aligned");
     PF_TRY(require_device());
     if (n == 0) return PF_OK;
     PF_CHECK(seqs, "pf_paged_free: null argument");
@@ -454,6 +458,7 @@ pf_status pf_paged_fork(const pf_paged_cache* c, const int32_t* parents, const i
                         void* stream) {
     PF_TRY(check_paged_cache(c, "pf_paged_fork", true));
     PF_CHECK(n >= 0 && n <= c->max_seqs && n <= 65535, "pf_paged_fork: %d children of %d sequences", n, c->max_seqs);
+    PF_CHECK(((uintptr_t)parents | (uintptr_t)children) % 4 == 0, "pf_paged_fork: parents and children must be 4-byte aligned");
     PF_TRY(require_device());
     if (n == 0) return PF_OK;
     PF_CHECK(parents && children, "pf_paged_fork: null argument");
@@ -466,6 +471,7 @@ pf_status pf_paged_fork(const pf_paged_cache* c, const int32_t* parents, const i
 pf_status pf_paged_copy(const pf_paged_cache* c, const int32_t* src, const int32_t* dst, int32_t n, void* stream) {
     PF_TRY(check_paged_cache(c, "pf_paged_copy", false));
     PF_CHECK(n >= 0 && n <= c->n_pages, "pf_paged_copy: %d pages of %d", n, c->n_pages);
+    PF_CHECK(((uintptr_t)src | (uintptr_t)dst) % 4 == 0, "pf_paged_copy: src and dst must be 4-byte aligned");
     PF_TRY(require_device());
     if (n == 0) return PF_OK;
     PF_CHECK(src && dst, "pf_paged_copy: null argument");

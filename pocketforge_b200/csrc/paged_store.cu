@@ -241,6 +241,7 @@ extern "C" pf_status pf_paged_store(const pf_paged_cache* c, int32_t layer, cons
     PF_CHECK(k_stride >= width && v_stride >= width && k_stride * es % 16 == 0 && v_stride * es % 16 == 0 &&
                  (uintptr_t)k % 16 == 0 && (uintptr_t)v % 16 == 0,
              "pf_paged_store: rows are narrower than the heads or not 16-byte aligned");
+    PF_CHECK((uintptr_t)offsets % 4 == 0, "pf_paged_store: offsets must be 4-byte aligned");
     PF_TRY(require_device());
     if (n_seqs == 0 || n_tokens == 0) return PF_OK;
     PF_CHECK(k && v && offsets, "pf_paged_store: null argument");

@@ -972,6 +972,7 @@ extern "C" pf_status pf_prompt_attention(const void* q, int64_t q_stride, const 
              "pf_prompt_attention: pointers and strides must be multiples of 16 bytes");
     PF_CHECK(std::max(std::max(q_stride, out_stride), std::max(k_stride, v_stride)) < (int64_t)1 << 38,
              "pf_prompt_attention: a stride is too large");  // a tensor map's strides end at 2^40 bytes
+    PF_CHECK((uintptr_t)offsets % 4 == 0, "pf_prompt_attention: offsets must be 4-byte aligned");
     PF_TRY(require_device());
     if (n_seqs == 0 || n_tokens == 0) return PF_OK;
     PF_CHECK(q && k && v && out && offsets, "pf_prompt_attention: null argument");

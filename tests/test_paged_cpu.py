@@ -142,3 +142,25 @@ def test_work_sizes():
     assert L.pf_paged_attention_work_bytes(C.byref(cache()), 4, 8, 4) > 0
     for bad in ((-1, 1, 4), (1, 0, 4), (1, 9, 4), (1, 1, 0), (1, 1, 3)):
         assert L.pf_paged_attention_work_bytes(C.byref(cache()), *bad) == 0
+
+
+@pytest.mark.parametrize("off", [1, 2, 3])
+def test_lists_that_are_not_aligned(off):
+    """Arrays of 32-bit integers begin at a multiple of 4 bytes."""
+    for name in ("table", "lens", "refs"):
+        c = C.byref(cache(**{name: A + off}))
+        refused("pf_paged_reserve", c, A, A, 1, None)
+        refused("pf_paged_free", c, A, 1, None)
+        refused("pf_paged_fork", c, A, A, 1, None)
+        refused("pf_paged_copy", c, A, A, 1, None)
+        refused("pf_paged_compact", c, None)
+        refused("pf_paged_store", c, 0, A, 128, A, 128, _lib.PF_F32, A, 1, 1, None)
+        refused("pf_paged_attention", c, 0, A, 256, A, 256, _lib.PF_F32, 1, 1, 4, 0.125, A, 1 << 30, None)
+    c = C.byref(cache())
+    for a, b in ((A + off, A), (A, A + off)):
+        refused("pf_paged_reserve", c, a, b, 1, None)
+        refused("pf_paged_fork", c, a, b, 1, None)
+        refused("pf_paged_copy", c, a, b, 1, None)
+    refused("pf_paged_free", c, A + off, 1, None)
+    refused("pf_paged_store", c, 0, A, 128, A, 128, _lib.PF_F32, A + off, 1, 1, None)
+    refused("pf_prompt_attention", A, 256, A, 128, A, 128, A, 256, _lib.PF_BF16, A + off, 1, 5, 4, 2, 64, 0.125, None)
