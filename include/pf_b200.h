@@ -374,7 +374,7 @@ PF_API pf_status pf_paged_store(const pf_paged_cache* c, int32_t layer, const vo
  * its first n - rows + 1 + r positions; a row that sees none gives zeros.
  *   out = sum_j softmax_j(scale * (q . k_j)) v_j
  * dtype: PF_F32, PF_BF16 or PF_F16 for a PF_I8 cache (PF_F32 keeps 32-bit
- * accuracy), the cache's own for the others.  scale > 0.  `work`:
+ * accuracy), the cache's own for the others.  0 < scale <= 2.3e38.  `work`:
  * pf_paged_attention_work_bytes() bytes, 16-byte aligned, zero before the
  * first call that uses it (every call leaves its counters zero); calls that
  * may run at the same time need one each.  q, out and the strides' bytes are
@@ -395,7 +395,7 @@ PF_API pf_status pf_paged_attention(const pf_paged_cache* c, int32_t layer, cons
  * [0, n_tokens] latches bit 1 and is left out (where offsets go back, so may be
  * others).  An inf among the values is inf, or NaN where its weight rounds to 0,
  * in the rows that see it, and touches no other.  dtype PF_BF16 or PF_F16,
- * head_dim 64 or 128, scale > 0; pointers and the strides' bytes are multiples
+ * head_dim 64 or 128, 0 < scale <= 2.3e38; pointers and the strides' bytes are multiples
  * of 16; 2^20 sequences and 2^30 tokens at most.  out overlaps none of the
  * inputs. */
 PF_API pf_status pf_prompt_attention(const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,

@@ -53,6 +53,8 @@ __device__ __forceinline__ int seq_len(const pf_paged_cache& c, int b, uint32_t*
     return -1;
 }
 
+constexpr float kMaxScale = 2.3e38f;  // of scores: times log2 e it is still finite
+
 constexpr int kDecide = 1024;  // threads of a CTA that decides for the others
 // Exclusive prefix sum over the CTA's 1,024 threads, and the total.
 __device__ __forceinline__ long long block_scan(long long v, long long* total, long long* s_warp) {

@@ -1008,7 +1008,7 @@ pf_status pf_paged_attention(const pf_paged_cache* c, int32_t layer, const void*
              "pf_paged_attention: %d heads over %d kv heads", n_heads, c->n_kv_heads);
     PF_CHECK(c->dtype == PF_I8 ? dtype == PF_F32 || dtype == PF_BF16 || dtype == PF_F16 : dtype == c->dtype,
              "pf_paged_attention: rows of dtype %d over a cache of dtype %d", dtype, c->dtype);
-    PF_CHECK(scale > 0.0f && scale <= 3.402823466e38f, "pf_paged_attention: scale must be positive and finite");
+    PF_CHECK(scale > 0.0f && scale <= kMaxScale, "pf_paged_attention: scale must be positive and at most 2.3e38");
     const int64_t width = (int64_t)n_heads * c->head_dim, es = type_bytes(dtype);
     PF_CHECK(q_stride >= width && out_stride >= width && q_stride * es % 16 == 0 && out_stride * es % 16 == 0 &&
                  (uintptr_t)q % 16 == 0 && (uintptr_t)out % 16 == 0,

@@ -963,7 +963,7 @@ extern "C" pf_status pf_prompt_attention(const void* q, int64_t q_stride, const 
              "pf_prompt_attention: %d sequences, %d tokens", n_seqs, n_tokens);
     PF_CHECK(n_kv_heads > 0 && n_heads > 0 && n_heads <= 65535 && n_heads % n_kv_heads == 0,
              "pf_prompt_attention: %d heads over %d kv heads", n_heads, n_kv_heads);
-    PF_CHECK(scale > 0.0f && scale <= 3.402823466e38f, "pf_prompt_attention: scale must be positive and finite");
+    PF_CHECK(scale > 0.0f && scale <= kMaxScale, "pf_prompt_attention: scale must be positive and at most 2.3e38");
     const int64_t wq = (int64_t)n_heads * head_dim, wk = (int64_t)n_kv_heads * head_dim;
     PF_CHECK(q_stride >= wq && out_stride >= wq && k_stride >= wk && v_stride >= wk,
              "pf_prompt_attention: a stride is smaller than its row");

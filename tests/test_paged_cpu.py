@@ -164,3 +164,10 @@ def test_lists_that_are_not_aligned(off):
     refused("pf_paged_free", c, A + off, 1, None)
     refused("pf_paged_store", c, 0, A, 128, A, 128, _lib.PF_F32, A + off, 1, 1, None)
     refused("pf_prompt_attention", A, 256, A, 128, A, 128, A, 256, _lib.PF_BF16, A + off, 1, 5, 4, 2, 64, 0.125, None)
+
+
+def test_scales_whose_log2_units_are_no_number():
+    """Scores are taken to log2 units by scale * log2 e: a scale that has none there is refused."""
+    for scale in (2.4e38, 3.4e38):
+        refused("pf_paged_attention", C.byref(cache()), 0, A, 256, A, 256, _lib.PF_F32, 1, 1, 4, scale, A, 1 << 30, None)
+        refused("pf_prompt_attention", A, 256, A, 128, A, 128, A, 256, _lib.PF_BF16, A, 1, 5, 4, 2, 64, scale, None)
