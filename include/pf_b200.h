@@ -377,8 +377,8 @@ PF_API pf_status pf_paged_store(const pf_paged_cache* c, int32_t layer, const vo
  * accuracy), the cache's own for the others.  0 < scale <= 2.3e38.  `work`:
  * pf_paged_attention_work_bytes() bytes, 16-byte aligned, zero before the
  * first call that uses it (every call leaves its counters zero); calls that
- * may run at the same time need one each.  q, out and the strides' bytes are
- * multiples of 16. */
+ * may run at the same time need one each.  (A size of 0: the sizes are refused.)
+ * q, out and the strides' bytes are multiples of 16. */
 PF_API size_t pf_paged_attention_work_bytes(const pf_paged_cache* c, int32_t n_seqs, int32_t rows, int32_t n_heads);
 PF_API pf_status pf_paged_attention(const pf_paged_cache* c, int32_t layer, const void* q, int64_t q_stride,
                                     void* out, int64_t out_stride, int32_t dtype, int32_t n_seqs, int32_t rows,

@@ -7,8 +7,9 @@
 
 namespace pf {
 
-// Checks a cache's sizes and pointers (the page operations' `work` included
-// with `need_work`); the message names the calling entry point.
+// Checks a cache's sizes, and its pointers as well (the page operations' `work`
+// included with `need_work`); the message names the calling entry point.
+pf_status check_paged_sizes(const pf_paged_cache* c, const char* where);
 pf_status check_paged_cache(const pf_paged_cache* c, const char* where, bool need_work);
 
 // What two launches of a page operation pass on, in the cache's `work`.

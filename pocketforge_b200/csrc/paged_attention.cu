@@ -74,6 +74,7 @@ namespace pf {
 
 namespace {
 
+constexpr int kMaxHeads = 65535;
 constexpr int kMaxCuts = 64;     // pieces of a segment: as many as one CTA joins in about a microsecond
 // Sequences from which on a launch of one CTA plans the pieces for all: its 2 us are less than what every CTA would take to
 // look through them (bf16: 1,000 sequences of 50 to 200 tokens 314 and 121 us, 250 of them 49 and 35, 128 36.0 and 36.9; one kv
@@ -991,8 +992,9 @@ using namespace pf;
 extern "C" {
 
 size_t pf_paged_attention_work_bytes(const pf_paged_cache* c, int32_t n_seqs, int32_t rows, int32_t n_heads) {
-    if (!c || n_seqs < 0 || rows < 1 || rows > 8 || n_heads < 1 || c->n_kv_heads < 1 || n_heads % c->n_kv_heads) return 0;
-    if (c->head_dim != 64 && c->head_dim != 128) return 0;
+    if (check_paged_sizes(c, "pf_paged_attention_work_bytes") != PF_OK || n_seqs < 0 || n_seqs > 1 << 20 || rows < 1 || rows > 8 ||
+        n_heads < 1 || n_heads > kMaxHeads || n_heads % c->n_kv_heads)
+        return 0;
     const int nt = tiles_for(n_heads / c->n_kv_heads * rows, c->head_dim);
     return kCounters * sizeof(int) + part_bytes(*c, nt) + (n_seqs < kPlannedFew ? 0 : plan_bytes(*c, nt, n_seqs, n_heads / c->n_kv_heads * rows));
 }
@@ -1004,7 +1006,7 @@ pf_status pf_paged_attention(const pf_paged_cache* c, int32_t layer, const void*
     PF_CHECK(layer >= 0 && layer < c->n_layers, "pf_paged_attention: layer %d of %d", layer, c->n_layers);
     PF_CHECK(n_seqs >= 0 && n_seqs <= c->max_seqs, "pf_paged_attention: %d sequences of %d", n_seqs, c->max_seqs);
     PF_CHECK(rows >= 1 && rows <= 8, "pf_paged_attention: %d rows are not 1 to 8", rows);
-    PF_CHECK(n_heads > 0 && n_heads <= 65535 && n_heads % c->n_kv_heads == 0,
+    PF_CHECK(n_heads > 0 && n_heads <= kMaxHeads && n_heads % c->n_kv_heads == 0,
              "pf_paged_attention: %d heads over %d kv heads", n_heads, c->n_kv_heads);
     PF_CHECK(c->dtype == PF_I8 ? dtype == PF_F32 || dtype == PF_BF16 || dtype == PF_F16 : dtype == c->dtype,
              "pf_paged_attention: rows of dtype %d over a cache of dtype %d", dtype, c->dtype);

@@ -400,7 +400,7 @@ constexpr int kCopyCtas = 148 * 8;  // all SMs full of copying CTAs
 
 }  // namespace
 
-pf_status check_paged_cache(const pf_paged_cache* c, const char* where, bool need_work) {
+pf_status check_paged_sizes(const pf_paged_cache* c, const char* where) {
     PF_CHECK(c, "%s: null cache", where);
     PF_CHECK(c->dtype == PF_I8 || c->dtype == PF_BF16 || c->dtype == PF_F16, "%s: cache dtype %d", where, c->dtype);
     PF_CHECK(c->head_dim == 64 || c->head_dim == 128, "%s: head_dim %d is neither 64 nor 128", where, c->head_dim);
@@ -411,6 +411,11 @@ pf_status check_paged_cache(const pf_paged_cache* c, const char* where, bool nee
     PF_CHECK((int64_t)c->n_layers * c->n_kv_heads <= 65536 && c->n_pages <= kMaxPages && c->max_seqs <= kMaxSeqs &&
                  (int64_t)c->max_pages * c->page_size <= 1 << 30,
              "%s: a size is too large", where);
+    return PF_OK;
+}
+
+pf_status check_paged_cache(const pf_paged_cache* c, const char* where, bool need_work) {
+    PF_TRY(check_paged_sizes(c, where));
     PF_CHECK(c->k && c->v && c->table && c->lens && c->refs, "%s: null pointer in the cache", where);
     PF_CHECK(c->dtype != PF_I8 || (c->k_scale && c->v_scale), "%s: an int8 cache needs scales", where);
     PF_CHECK(!need_work || c->work, "%s: null work in the cache", where);
@@ -429,8 +434,7 @@ using namespace pf;
 extern "C" {
 
 size_t pf_paged_work_bytes(const pf_paged_cache* c) {
-    if (!c || c->n_pages <= 0 || c->max_seqs <= 0 || c->n_pages > kMaxPages || c->max_seqs > kMaxSeqs) return 0;
-    return page_work_bytes(*c);
+    return check_paged_sizes(c, "pf_paged_work_bytes") == PF_OK ? page_work_bytes(*c) : 0;
 }
 
 pf_status pf_paged_reserve(const pf_paged_cache* c, const int32_t* seqs, const int32_t* counts, int32_t n,

@@ -171,3 +171,29 @@ def test_scales_whose_log2_units_are_no_number():
     for scale in (2.4e38, 3.4e38):
         refused("pf_paged_attention", C.byref(cache()), 0, A, 256, A, 256, _lib.PF_F32, 1, 1, 4, scale, A, 1 << 30, None)
         refused("pf_prompt_attention", A, 256, A, 128, A, 128, A, 256, _lib.PF_BF16, A, 1, 5, 4, 2, 64, scale, None)
+
+
+SIZES = [dict(dtype=_lib.PF_F32), dict(dtype=7), dict(head_dim=96), dict(page_size=48), dict(n_layers=0), dict(n_kv_heads=0),
+         dict(n_pages=-3), dict(max_seqs=0), dict(max_pages=0), dict(max_pages=1 << 30, page_size=128),
+         dict(n_layers=1 << 20, n_kv_heads=1 << 14)]
+
+
+@pytest.mark.parametrize("bad", SIZES, ids=str)
+def test_no_work_size_for_sizes_that_are_refused(bad):
+    c = C.byref(cache(**bad))
+    assert _lib.lib().pf_paged_work_bytes(c) == 0
+    assert _lib.lib().pf_paged_attention_work_bytes(c, 2, 1, 4) == 0
+
+
+def test_no_work_size_for_heads_that_are_refused():
+    """65,536 heads and more; the columns of 2^31 - 2 of them, 8 rows each, would pass 32 bits."""
+    for heads in (65_536, (1 << 31) - 2):
+        assert _lib.lib().pf_paged_attention_work_bytes(C.byref(cache()), 2, 8, heads) == 0
+    assert _lib.lib().pf_paged_attention_work_bytes(C.byref(cache(n_kv_heads=1)), 2, 8, 65_535) > 0
+
+
+def test_work_sizes_need_no_pointers():
+    """The size is asked for before there is a cache."""
+    c = cache(k=None, v=None, k_scale=None, v_scale=None, table=None, lens=None, refs=None, work=None)
+    assert _lib.lib().pf_paged_work_bytes(C.byref(c)) == _lib.lib().pf_paged_work_bytes(C.byref(cache())) > 0
+    assert _lib.lib().pf_paged_attention_work_bytes(C.byref(c), 2, 1, 4) > 0
