@@ -207,8 +207,10 @@ pf_status launch_store(const pf_paged_cache& c, int layer, const void* k, int64_
     const ST *kp = static_cast<const ST*>(k), *vp = static_cast<const ST*>(v);
     // CTAs behind the tokens', if there are very many sequences, only look at offsets: eight a thread
     const int look = ceil_div(n_seqs, 8 * kLook);
-    // 16 tokens a CTA share one round of searches; below four CTAs an SM the chain of a single round is what counts
-    if (n_tokens >= 16 * 4 * 148)
+    // 16 tokens a CTA share one round of searches, from one CTA an SM on; below that the chain of a single round is what counts
+    // (fp32 to int8, 8 kv heads, us with 2 and with 16: 640 tokens 3.6 and 6.3, 2,560 6.9 and 7.4, 3,840 9.5 and 8.2, 9,472
+    // 21.6 and 15.6; 2 kv heads: 640 3.5 and 3.8, 2,560 6.2 and 4.0, 9,472 18.1 and 5.8)
+    if (n_tokens >= 16 * 148)
         return launch_after("paged_store", store_kernel<ST, CT, HD, 16>, dim3(std::max(ceil_div(n_tokens, 16), look)), kThreads, 0, st, c,
                             layer, kp, ks, vp, vs, offsets, n_seqs, n_tokens, err);
     return launch_after("paged_store", store_kernel<ST, CT, HD, 2>, dim3(std::max(ceil_div(n_tokens, 2), look)), kThreads, 0, st, c, layer,
