@@ -541,6 +541,35 @@ def test_store_many_sequences():
         at += n
 
 
+@pytest.mark.parametrize("cache,rows,dim,kv_heads", [(I8, F32, 64, 8), (I8, BF16, 128, 3), (I8, F16, 64, 1), (BF16, F32, 64, 2), (F16, F16, 128, 5)])
+def test_store_many_tokens(cache, rows, dim, kv_heads):
+    """A whole batch's prompts, for which a CTA takes more tokens: empty sequences, ends inside a CTA's tokens."""
+    rng = random.Random(dim + kv_heads)
+    new = [rng.choice([0, 0, 1, 7, 16, rng.randint(1, 90)]) for _ in range(320)]
+    before = [rng.randint(0, 40) if n else 0 for n in new]
+    total = [a + b for a, b in zip(before, new)]
+    c = Cache(cache, 2, kv_heads, dim, 16, sum(-(-x // 16) for x in total) + 3, 320, 9).place(total)
+    off, tokens = offsets_of(new), sum(new)
+    assert tokens > 2368
+    k, v = (randn((tokens, kv_heads * dim), TYPES[rows], i) for i in (1, 2))
+    want = [x.clone() for x in (c.k, c.v) + ((c.ks, c.vs) if cache == I8 else ())]
+    seq = torch.repeat_interleave(torch.arange(320), torch.tensor(new)).cuda()
+    pos = torch.cat([torch.arange(b, b + n) for b, n in zip(before, new)]).cuda()
+    page, slot = c.table[seq, pos // 16].long(), pos % 16
+    for i, x in enumerate((k, v)):
+        row = x.view(tokens, kv_heads, dim)
+        if cache == I8:
+            code, scale = store_codes(row)
+            want[i][page, 1, :, slot] = torch.from_numpy(code).cuda()
+            want[2 + i][page, 1, :, slot] = torch.from_numpy(scale).cuda()
+        else:
+            want[i][page, 1, :, slot] = row.to(TYPES[cache])
+    c.store(1, k, v, off, rows)
+    torch.cuda.synchronize()
+    for x, y in zip((c.k, c.v, c.ks, c.vs), want):
+        assert torch.equal(x, y)
+
+
 def elapsed(f):
     f()
     a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
@@ -880,6 +909,29 @@ def test_attention_answers_do_not_depend_on_the_run():
         c.attend(0, q, out, F32, 3, 2, 16, 0.125, work)
         torch.cuda.synchronize()
         assert torch.equal(out, first)
+
+
+@pytest.mark.parametrize("cache,t", [(I8, F32), (BF16, BF16)])
+@pytest.mark.parametrize("rows", [1, 5])
+def test_attention_a_real_step(cache, t, rows):
+    """64 sequences, 32 heads over 8, one token and a verify step's five."""
+    rng = random.Random(rows)
+    lens = [rng.randint(512, 1024) for _ in range(64)]
+    c = Cache(cache, 1, 8, 64, 64, sum(-(-n // 64) for n in lens), 64, 16).place(lens)
+    q = randn((64 * rows, 32 * 64), TYPES[t], 3, 1.5)
+    out = torch.empty_like(q)
+    c.attend(0, q, out, t, 64, rows, 32, 0.125)
+    torch.cuda.synchronize()
+    for b in range(64):
+        for g in range(8):
+            k, v = c.history(b, 0, g)
+            at = (slice(b * rows, (b + 1) * rows), slice(4 * g, 4 * g + 4))
+            x = q.view(-1, 32, 64)[at].double() @ k.T * 0.125  # [row][head][entry]
+            seen = torch.arange(lens[b], device="cuda") < (lens[b] - rows + 1 + torch.arange(rows, device="cuda"))[:, None, None]
+            p = torch.softmax(torch.where(seen, x, -math.inf), -1)
+            big_s = (q.view(-1, 32, 64)[at].double().abs() @ k.abs().T * 0.125).amax(-1, keepdim=True)
+            big_v = v.abs().max().expand(rows, 4, 1)
+            check(out.view(-1, 32, 64)[at].contiguous(), (p @ v, big_v, big_s), TYPES[t])
 
 
 def one_dim_keys(c, n, nats):
