@@ -45,9 +45,13 @@
 // fp16 planes (22 bits) after a power of two takes the row's largest value to
 // 2^13..2^14.  Over an int8 cache weights are two fp16 planes as well; they take
 // the entry's scale, and a power of two that keeps a block's largest at or below 2^15.
-// Over a 16-bit cache weights are rounded to its type (both operands of a
-// product have one type), an error like the output's own rounding; a second
-// plane would turn an inf among the values into NaN.  fp16 ends at 2^-24, and a
+// Over a 16-bit cache both operands of a product have its type.  With one column
+// tile, where HBM is waited for, weights are two planes of it (64 x 1 rows at
+// head_dim 128 38.1 and 38.6 us, 8 long contexts 124.5 and 125.6): the first is
+// cut, not rounded, so that the second is above 0 as well and an inf among the
+// values stays one.  With more tiles they are rounded to one plane, an error like
+// the output's own rounding; a second one took 64 x 5 rows from 31.6 to 36.4 us
+// (head_dim 64) and from 49.7 to 56.1 (128).  fp16 ends at 2^-24, and a
 // long row's many weights below that can be its answer where the largest ones
 // meet small values.  So the largest weights are taken to the end of fp16's range
 // (LIFT, or the scales' power of two), and the maximum that exponents refer to
@@ -185,6 +189,14 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     uint32_t r;
     if constexpr (BF) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+// The same, cut off instead of rounded.
+template <bool BF>
+__device__ __forceinline__ uint32_t pack_cut(float lo, float hi) {
+    if constexpr (BF) return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632);
+    uint32_t r;
+    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
 // The same to fp16 with an inf taken down to the largest value.
@@ -333,7 +345,7 @@ __global__ void __launch_bounds__(Ring<CT, HD, NT>::WARPS * 32, Ring<CT, HD, NT>
     constexpr int KS = HD / 16;        // products along the dims of a score
     constexpr int MT = HD / 16;        // 16-dim tiles of the output
     constexpr int COLS = 8 * NT;
-    constexpr int VP = I8 ? 2 : 1;     // planes of a weight
+    constexpr int VP = I8 || NT == 1 ? 2 : 1;  // planes of a weight
     // Weights are 2^(LIFT + x) with x <= RISE; at most 2^15 in fp16, where int8 rows' scales take what a LIFT would.
     constexpr int RISE = BF ? 8 : 6, LIFT = BF || I8 ? 0 : 15 - RISE, TOP_SCALE = 15 - RISE;
     // Queries in shared memory where the registers they would take are the warps' that an SM could hold (64 sequences of 5
@@ -741,11 +753,19 @@ __global__ void __launch_bounds__(Ring<CT, HD, NT>::WARPS * 32, Ring<CT, HD, NT>
                         y[i] = I8 ? e * vs : e;
                         if (I8 && tail && !vs_ok && e0 + r >= sees[nt][i]) y[i] = 0.0f;  // 0 whatever its scale is
                     }
-                    if constexpr (VP == 2) {  // (an inf is the largest value and an inf)
+                    if constexpr (I8) {  // (an inf is the largest value and an inf)
                         const uint32_t hi = pack_finite(y[0], y[1]);
                         const float2 got = unpack<false>(hi);
                         pw[mt][nt][0][h] = transpose8x8(hi);
                         pw[mt][nt][1][h] = transpose8x8(pack<false>(y[0] - got.x, y[1] - got.y));
+                    } else if constexpr (VP == 2) {
+                        // y cut to the type, and what is left of y (1 + 2^-23), which is above 0 (fp16: 2^-24 at least) if y is
+                        const uint32_t hi = pack_cut<BF>(y[0], y[1]);
+                        const float2 got = unpack<BF>(hi);
+                        float lo[2] = {fmaf(y[0], 1.00000012f, -got.x), fmaf(y[1], 1.00000012f, -got.y)};
+                        if constexpr (!BF) lo[0] = fmaxf(lo[0], fminf(y[0], 0x1p-24f)), lo[1] = fmaxf(lo[1], fminf(y[1], 0x1p-24f));
+                        pw[mt][nt][0][h] = transpose8x8(hi);
+                        pw[mt][nt][1][h] = transpose8x8(pack<BF>(lo[0], lo[1]));
                     } else {
                         pw[mt][nt][0][h] = transpose8x8(pack<BF>(y[0], y[1]));
                     }

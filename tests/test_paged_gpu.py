@@ -1017,6 +1017,48 @@ def test_attention_a_few_keys_take_nearly_all_of_long_ones(cache, t, dim, rows, 
         assert ((got - want).abs() <= tol).all(), ((got - want).abs() / tol).max()
 
 
+@pytest.mark.parametrize("cache", [BF16, F16])
+@pytest.mark.parametrize("dim,rows,group", [(64, 1, 4), (128, 1, 8), (64, 2, 4), (128, 2, 3), (64, 8, 1)])
+def test_attention_weights_keep_more_than_16_bits(cache, dim, rows, group):
+    """Up to eight rows a kv head over a 16-bit cache: the output's rounding is the only one to 16 bits."""
+    c = Cache(cache, 1, 2, dim, 16, 400, 5, 200).place([40, 333, 7, 2900, 90])
+    t, heads = TYPES[cache], 2 * group
+    q = randn((5 * rows, heads * dim), t, 3)
+    out = torch.empty_like(q)
+    c.attend(0, q, out, cache, 5, rows, heads, dim ** -0.5)
+    torch.cuda.synchronize()
+    want, big_v, big_s = c.attention(0, q, 5, rows, heads, dim ** -0.5)
+    # a weight's second plane is rounded to 16 bits: 2^-16 of the weight in bf16, 2^-21 in fp16, or 2^-24 of what is 2^9 for the
+    # largest; scores, sums and exponentials as in tolerance()
+    half = torch.finfo(t).eps / 2
+    tol = (2.0 ** -17 * big_s + 2.0 ** -18 + 2.0 ** -16) * big_v + half * want.abs()
+    d = (out.double().view_as(want) - want).abs()
+    assert (d <= tol).all(), (d / tol).max()
+
+
+@pytest.mark.parametrize("cache", [BF16, F16])
+@pytest.mark.parametrize("dim,rows", [(64, 1), (128, 1), (64, 2), (128, 2), (64, 5)])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf])
+def test_attention_an_infinity_stays_one(cache, dim, rows, bad):
+    """An inf among the values of any entry, whatever part of its weight a plane holds: that dim of the rows that see it."""
+    n, heads = 150, 4
+    c = Cache(cache, 1, 1, dim, 16, 40, 1, 20).place([n])
+    q = randn((rows, heads * dim), TYPES[cache], 3, 0.5)
+    q[:, :dim] = 0  # weights that are powers of two: nothing is left for a second plane
+    for at in range(0, n, 7):
+        page, slot = int(c.table[0, at // 16]), at % 16
+        c.v[page, 0, 0, slot, at % dim] = bad
+    out = torch.empty_like(q)
+    c.attend(0, q, out, cache, 1, rows, heads, dim ** -0.5)
+    torch.cuda.synchronize()
+    got = out.view(rows, heads, dim)
+    for r in range(rows):
+        hit = sorted({at % dim for at in range(0, n, 7) if at < n - rows + 1 + r})
+        assert (got[r][:, hit] == bad).all()
+        rest = [d for d in range(dim) if d not in hit]
+        assert torch.isfinite(got[r][:, rest]).all()
+
+
 # ---------------------------------------------------------------------------
 # Prompt attention
 # ---------------------------------------------------------------------------
