@@ -373,6 +373,13 @@ PF_API pf_status pf_paged_store(const pf_paged_cache* c, int32_t layer, const vo
  * kv head h / (n_heads / n_kv_heads).  Row r of a sequence of length n sees
  * its first n - rows + 1 + r positions; a row that sees none gives zeros.
  *   out = sum_j softmax_j(scale * (q . k_j)) v_j
+ * Scores, maxima, sums and output sums are fp32.  A weight is held in 22 bits or
+ * more over a PF_I8 cache (two fp16 planes), in two planes of the cache's type
+ * over the others where rows * n_heads / n_kv_heads is 8 at most, and else
+ * rounded to it: off by half a step of the type, which moves the output by half a
+ * step of the largest value at most.  Beside that fp16 planes lose 2^-33 of the
+ * row's largest weight.  An inf among the values is inf in the rows that see it,
+ * or NaN where its weight is 0 in the type.
  * dtype: PF_F32, PF_BF16 or PF_F16 for a PF_I8 cache (PF_F32 keeps 32-bit
  * accuracy), the cache's own for the others.  0 < scale <= 2.3e38.  `work`:
  * pf_paged_attention_work_bytes() bytes, 16-byte aligned, zero before the
@@ -394,7 +401,9 @@ PF_API pf_status pf_paged_attention(const pf_paged_cache* c, int32_t layer, cons
  * as they were; a sequence whose offsets are out of order or outside
  * [0, n_tokens] latches bit 1 and is left out (where offsets go back, so may be
  * others).  An inf among the values is inf, or NaN where its weight rounds to 0,
- * in the rows that see it, and touches no other.  dtype PF_BF16 or PF_F16,
+ * in the rows that see it, and touches no other.  Weights are rounded to the
+ * type before they meet the values (half a step, and beside that 2^-34 of a row's
+ * largest in fp16); all else is fp32 but for the output's own rounding.  dtype PF_BF16 or PF_F16,
  * head_dim 64 or 128, 0 < scale <= 2.3e38; pointers and the strides' bytes are multiples
  * of 16; 2^20 sequences and 2^30 tokens at most.  out overlaps none of the
  * inputs. */

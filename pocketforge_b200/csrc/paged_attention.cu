@@ -22,11 +22,12 @@
 // 65,536 entries, head_dim 128: 713 MB in 124 us, 5.7 TB/s, 88% of the measured
 // copy rate); instruction issue for int8 ones, whose codes take one and a half
 // instructions each on the way to an operand (16 contexts of 8,000, one fp32 row:
-// 139 MB in 37.6 us, 57%); the chain of trips to memory before the first block
+// 139 MB in 40.6 us, 53%); the chain of trips to memory before the first block
 // and the joining for one short context (777 entries: 8.5 us).  64 sequences with
 // 5 fp32 rows, 35 us for 55 MB: 20 rows make 24 columns and two planes of each,
-// about 1,100 instructions a warp and 32 entries, issued at 0.4 to 0.5 a clock by
-// the 12 warps that the registers allow, a quarter of a CTA's time before its
+// about 1,100 instructions a warp and 32 entries, issued at 0.44 a clock by the 10
+// of 12 warps that are there on average (ncu; the tensor pipe is active in 29% of
+// the cycles), a quarter of a CTA's time before its
 // first block.
 //
 // A CTA's three (64-byte rows) or four warps take blocks of 32 entries (256-byte
@@ -44,7 +45,7 @@
 // Accuracy.  int8 codes are exact in fp16, and fp32 queries are split into two
 // fp16 planes (22 bits) after a power of two takes the row's largest value to
 // 2^13..2^14.  Over an int8 cache weights are two fp16 planes as well; they take
-// the entry's scale, and a power of two that keeps a block's largest at or below 2^15.
+// the entry's scale, and a power of two that keeps a block's largest below 2^15.
 // Over a 16-bit cache both operands of a product have its type.  With one column
 // tile, where HBM is waited for, weights are two planes of it (64 x 1 rows at
 // head_dim 128 38.1 and 38.6 us, 8 long contexts 124.5 and 125.6): the first is
@@ -56,9 +57,9 @@
 // meet small values.  So the largest weights are taken to the end of fp16's range
 // (LIFT, or the scales' power of two), and the maximum that exponents refer to
 // rises as soon as it is exceeded by 2^6: a weight is off by 2^-34 of the row's
-// largest at most beside its rounding, over an int8 cache by 2^-33 of the largest
-// times its block's largest scale (2^-26 where that has come down to 2^-7 of an
-// earlier block's).  Rising from 2^2 on keeps four bits more but took 64 sequences
+// largest at most beside its rounding (2^-33 where its second plane is kept above
+// 0), over an int8 cache by 2^-33 of the largest weight times the largest scale of
+// its block or of one before.  Rising from 2^2 on keeps four bits more but took 64 sequences
 // with 5 rows from 35.2 to 38.8 us (int8) and 51.1 to 58.7 (fp16, head_dim 128);
 // 2^6: 35.5 and 51.2.  bf16 has fp32's range: 2^8.  A block's products start from
 // zero and are added to O in fp32 with rounding, as the tensor cores cut sums off
@@ -260,6 +261,9 @@ __device__ __forceinline__ int cuts_of(int n, int most, float inv) {
 // Chunks a piece.  With nearly as many segments as CTAs fit, only what is twice as long as the share is cut.  With fewer, the
 // least with which all pieces are there at once (a second, nearly empty round of CTAs costs more than pieces that are a little
 // longer), of 32 between the share and twice that: pieces_at(most, 1 / most) says how many there are, fewer of longer ones.
+// (int8, one fp32 row, 592 places; us with the border at 1/2, 3/4 and 1 of them: 320 segments of 500 to 1,500 entries 21.5, 22.0 and
+// 22.0, 384: 23.7, 22.9 and 22.9, 512: 26.8, 26.8 and 27.6, 576: 28.0, 28.0 and 31.7; 384 of 4,000 63.5, 65.3 and 65.0, 576: 68.5, 68.5
+// and 72.8.)
 __host__ __device__ constexpr int few_segments(int ctas) { return ctas / 4 * 3; }
 template <typename F>
 __device__ __forceinline__ int piece_limit(int total, int segments, int ctas, const F& pieces_at) {
@@ -952,7 +956,10 @@ __global__ void __launch_bounds__(Ring<CT, HD, NT>::WARPS * 32, Ring<CT, HD, NT>
     }
 }
 
-// Column tiles of 8 that a CTA takes: the rows' in as few equal groups as the registers allow.
+// Column tiles of 8 that a CTA takes: the rows' in as few equal groups as the registers allow, as each group reads the cache
+// anew.  (Four tiles or two groups of two, head_dim 64, 64 sequences of 7,000 to 8,000 entries: bf16 208 and 286 us, int8 with
+// fp16 rows 272 and 295, with fp32 rows 310 and 317.  Short contexts of int8 rows, where four tiles spill and the half as many
+// segments are cut, lose by it: 512 to 1,024 entries of 4 kv heads 41 and 27 us; of 8 kv heads 48 and 46.)
 int tiles_for(int cols, int head_dim) {
     const int tiles = ceil_div(cols, 8), groups = ceil_div(tiles, head_dim == 64 ? 4 : 3);
     return ceil_div(tiles, groups);

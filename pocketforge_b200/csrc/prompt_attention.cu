@@ -26,13 +26,16 @@
 //
 // What bounds it (B200, measured): 8,192 tokens, 32 heads over 8, head_dim 128,
 // bf16: 550 GFLOP in 500 us, 1.10 PFLOP/s, 79% of what cuBLAS sustains under the
-// power cap (the tensor pipe is active in 65% of the cycles at 1.54 GHz: power is
-// part of it).  64 prompts of 33 to 1,024 tokens, head_dim 64: 151 us (163 with
-// one head a tile; 256 prompts of 5 to 40 tokens, 8 heads a kv head: 82 and 235;
-// 8,192 tokens: 500 and 496); half of
-// the products are in blocks on the diagonal or behind the end, the special-
-// function unit takes 2,048 of a block's 3,100 cycles, and each unit of three
-// blocks on average has about 4,000 cycles of its own (first scores, output).
+// power cap (ncu: tensor pipe and special-function unit are each active in 64% of
+// the cycles at 1.6 GHz; the two tiles wait for both in turn, and the clock is
+// the power cap's).  64 prompts of 33 to 1,024 tokens, head_dim 64: 151 us (163
+// with one head a tile; 256 prompts of 5 to 40 tokens, 8 heads a kv head: 80 and
+// 235; 8,192 tokens: 500 and 496); half of the products are in blocks on the
+// diagonal or behind the end, the special-function unit takes 2,048 of a full
+// block's 3,100 cycles, and each unit of three blocks on average has about 4,000
+// cycles of its own (first scores, output): 280,000 cycles for an SM's 63 blocks
+// and 21 units, where 267,000 are counted (special-function unit active in 41% of
+// them, tensor pipe in 23%).
 // Short units run every path of the code once, so its size counts: 84 KB of
 // unrolled code ran 221 us where 60 KB ran 174 (stalls for instructions 1.9 an
 // issue before, 0.2 after).  Measured and not kept: a part of the exponentials by
