@@ -73,12 +73,12 @@ __device__ __forceinline__ void mark_first(const pf_paged_cache& c, const int* l
     __syncthreads();
 }
 
-// Pages that sequence s of length n holds: those its length asks for, and behind them what it has taken for tokens that its
-// owner has given back since by a lower length.  Every operation that adds pages leaves -1 behind the last one.
-__device__ __forceinline__ int held_pages(const pf_paged_cache& c, int s, int n) {
+// Pages that sequence s of length n holds, `most` at most: those its length asks for, and behind them what it has taken for
+// tokens that its owner has given back since by a lower length.  Every operation that adds pages leaves -1 behind the last one.
+__device__ __forceinline__ int held_pages(const pf_paged_cache& c, int s, int n, int most) {
     int held = (int)(((int64_t)n + c.page_size - 1) / c.page_size);
     if (n)
-        while (held < c.max_pages && in_range(c.table[(int64_t)s * c.max_pages + held], c.n_pages)) held++;
+        while (held < most && in_range(c.table[(int64_t)s * c.max_pages + held], c.n_pages)) held++;
     return held;
 }
 
@@ -98,8 +98,8 @@ __device__ __forceinline__ int2 reserve_need(const pf_paged_cache& c, const Page
         latch(err, ERR_CONTEXT);
         return make_int2(-1, 0);
     }
-    const int held = held_pages(c, s, n);
-    return make_int2(max((int)pages - held, 0), held);
+    const int held = held_pages(c, s, n, (int)pages);
+    return make_int2((int)pages - held, held);
 }
 
 __global__ void __launch_bounds__(kDecide) reserve_kernel(const pf_paged_cache c, const int* seqs, const int* counts,

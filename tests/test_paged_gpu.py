@@ -351,6 +351,27 @@ def test_pages_follow_the_model_with_lengths_lowered(dtype, layers, kv_heads, pa
     assert not c.refs.any() and latched() == 0
 
 
+def test_pages_many_held_behind_a_length():
+    """A whole context reserved at once and given back: the next tokens' room does not take a walk past all of its pages."""
+    c = Cache(I8, 1, 1, 64, 16, 90_000, 2, 88_000, fill=False)
+    c.reserve([0, 1], [85_000 * 16, 5])
+    c.lens[0] = 1
+    seqs, counts = ints([0, 1]), ints([0, 1])
+
+    def call():
+        ok("pf_paged_reserve", c.ref, seqs.data_ptr(), counts.data_ptr(), 2, ph.stream())
+
+    ms = elapsed(call)
+    assert ms < 0.5, ms
+    c.reserve([0], [32])
+    assert c.lens.tolist() == [33, 7] and int(c.refs.sum()) == 85_001
+    c.reserve([0], [85_000 * 16])  # three pages more than it holds
+    assert int(c.lens[0]) == 85_000 * 16 + 33 and int(c.refs.sum()) == 85_004
+    assert c.table[0, 85_000:85_004].tolist() == [85_001, 85_002, 85_003, -1]
+    c.free([0, 1])
+    assert not c.refs.any() and latched() == 0
+
+
 def test_store_does_not_write_a_shared_page():
     """A sequence that got no room, or whose length was lowered into a page that a fork shares: bit 1, the page stays."""
     for cache in (I8, F16):
