@@ -160,18 +160,20 @@ __global__ void free_kernel(const pf_paged_cache c, const int* seqs, uint32_t* e
     }
     if (s_len == 0) return;
     const int pages = (int)(((int64_t)s_len + c.page_size - 1) / c.page_size);
-    for (int j0 = 0;; j0 += blockDim.x) {  // up to the first entry behind the length that is no page (held_pages)
-        const int j = j0 + threadIdx.x;
-        int* at = c.table + (int64_t)s * c.max_pages + j;
-        const int p = j < c.max_pages ? *at : -1;
+    int* row = c.table + (int64_t)s * c.max_pages;
+    auto give = [&](int j, int p) {
+        row[j] = -1;
+        if (in_range(p, c.n_pages)) atomicSub(&c.refs[p], 1);
+        else latch(err, ERR_BOUNDS);
+    };
+    const int whole = pages / (int)blockDim.x * blockDim.x;
+    for (int j = threadIdx.x; j < whole; j += blockDim.x) give(j, row[j]);
+    for (int j0 = whole;; j0 += blockDim.x) {  // up to the first entry behind the length that is no page (held_pages)
+        const int j = j0 + threadIdx.x, p = j < c.max_pages ? row[j] : -1;
         if (j >= pages && !in_range(p, c.n_pages)) atomicMin(&s_end, j);
         __syncthreads();
         const int end = s_end;
-        if (j < end) {
-            *at = -1;
-            if (in_range(p, c.n_pages)) atomicSub(&c.refs[p], 1);
-            else latch(err, ERR_BOUNDS);
-        }
+        if (j < end) give(j, p);
         if (end <= j0 + (int)blockDim.x) break;
         __syncthreads();  // s_end has been read
     }
@@ -382,15 +384,20 @@ __global__ void __launch_bounds__(kCopy) compact_move_kernel(const pf_paged_cach
     for (int s = (int)(blockIdx.x * (kCopy / 32) + (threadIdx.x >> 5)); s < c.max_seqs; s += gridDim.x * (kCopy / 32)) {
         const int len = seq_len(c, s, err);
         const int pages = (int)(((int64_t)max(len, 0) + c.page_size - 1) / c.page_size);
-        for (int j = threadIdx.x & 31, end = 0; pages && !end; j += 32) {  // (and those held behind the length)
-            int* at = c.table + (int64_t)s * c.max_pages + j;
-            const int p = j < c.max_pages ? *at : -1;
-            const unsigned ends = __ballot_sync(0xffffffffu, j >= pages && !in_range(p, c.n_pages));
-            end = ends != 0;
-            if (end && (threadIdx.x & 31) >= __ffs((int)ends) - 1) continue;
+        int* row = c.table + (int64_t)s * c.max_pages;
+        auto follow = [&](int j, int p) {
             const int to = !in_range(p, c.n_pages) ? -1 : p < n_live ? p : w.remap[p];
             if (to < 0) latch(err, ERR_BOUNDS);
-            else if (to != p) *at = to;
+            else if (to != p) row[j] = to;
+        };
+        const int whole = pages & ~31;
+        int j = threadIdx.x & 31;
+        for (; j < whole; j += 32) follow(j, row[j]);
+        for (bool more = pages > 0; more; j += 32) {  // the last ones, and those held behind the length
+            const int p = j < c.max_pages ? row[j] : -1;
+            const unsigned ends = __ballot_sync(0xffffffffu, j >= pages && !in_range(p, c.n_pages));
+            more = ends == 0;
+            if (more || (threadIdx.x & 31) < __ffs((int)ends) - 1) follow(j, p);
         }
     }
     copy_pages(c, w.src, w.dst, n, err);
