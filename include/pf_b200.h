@@ -321,8 +321,9 @@ PF_API size_t pf_paged_work_bytes(const pf_paged_cache* c);
  * sequence would pass max_pages, the sequence keeps its length and pages and
  * bit 8 is latched.  Pages are given out in the list's order: behind an entry
  * for which they run out no other takes one, and only entries that need none
- * are served; an entry that would pass max_pages takes no one's place.  A sequence named again, or out of range, and a count
- * below zero latch bit 1 and are left out. */
+ * are served; an entry that would pass max_pages takes no one's place.  A
+ * sequence named again, or out of range, and a count below zero latch bit 1 and
+ * are left out. */
 PF_API pf_status pf_paged_reserve(const pf_paged_cache* c, const int32_t* seqs, const int32_t* counts, int32_t n,
                                   void* stream);
 /* Gives up n sequences (device array): their length becomes 0, their table
